@@ -29,6 +29,7 @@ extern "C" {
 
 #define XSPMM_F32 0
 #define XSPMM_F16 1
+#define XSPMM_BF16 2 /* the feed-forward layer and the norm only */
 #define XSPMM_I32 0
 #define XSPMM_I64 1
 
@@ -390,6 +391,98 @@ int xspmm_mtx_info(xspmm_mtx_t m, int64_t* rows, int64_t* cols, int64_t* nnz);
 int xspmm_mtx_export(xspmm_mtx_t m, int itype, int vtype, void* row_ptr, void* col_ind,
                      void* values);
 int xspmm_mtx_free(xspmm_mtx_t m);
+
+/*
+ * The feed-forward layer of a model on block-sparse weights, with its backward
+ * pass.  No counterpart in the reference, whose one operator is the product.
+ *
+ * Activations are features x tokens, row-major, ld = N tokens.  Every array is
+ * of one value type (XSPMM_F32, XSPMM_F16 or XSPMM_BF16); sums are fp32 and are
+ * rounded once, when they are stored.  Block values, activations and gradients
+ * start on a 16-byte boundary (biases and per-feature arrays need not).  The
+ * results may not overlap the operands.  N = 0 is allowed: sums over no tokens
+ * are zero.  Asynchronous on `stream`; nothing is allocated.
+ */
+#define XSPMM_ACT_NONE 0
+#define XSPMM_ACT_RELU 1
+#define XSPMM_ACT_SILU 2      /* z / (1 + exp(-z)) */
+#define XSPMM_ACT_GELU 3      /* z (1 + erf(z / sqrt 2)) / 2 */
+#define XSPMM_ACT_GELU_TANH 4 /* its form with tanh */
+
+/*
+ * What the operators need to know of a weight's blocks, laid out once: the BCSR
+ * arrays (16x16 blocks, block columns strictly ascending within a row, as
+ * csr_to_bcsr makes them) and the same blocks by block-column.  The arrays are
+ * not referenced afterwards; the values are passed to every call, so they may
+ * change between calls.  Arrays that are no such matrix fail with
+ * XSPMM_ERR_INVALID.  Synchronizes `stream`.
+ */
+typedef struct xspmm_weight_s* xspmm_weight_t;
+int xspmm_weight_create(int itype, int64_t M, int64_t K, int64_t Mb, int64_t Kb, int64_t nnzb, const void* brp,
+                        const void* bci, void* stream, xspmm_weight_t* weight_out);
+int xspmm_weight_destroy(xspmm_weight_t weight);
+
+/*
+ * y = act(A x + bias) + residual, A M x K, x K x N, y and residual M x N, bias
+ * M.  bias, residual and keep may be NULL; keep receives A x + bias, which the
+ * backward pass takes where there is an activation.
+ */
+int xspmm_linear(xspmm_weight_t weight, int vtype, int act, const void* vals, const void* x, const void* bias,
+                 const void* residual, void* y, void* keep, int64_t N, void* stream);
+
+/*
+ * Its backward pass from dy: dz = dy act'(keep), rounded to the value type
+ * before the products; dx = A^T dz (K x N), dvals = the stored blocks of
+ * dz x^T (zero past the edges of A), dbias = sums of dz over the tokens.  Each
+ * result may be NULL.  The residual's gradient is dy itself.  keep is not read
+ * with XSPMM_ACT_NONE.  scratch (256-byte aligned) holds dz: as many bytes as
+ * xspmm_linear_backward_scratch says.
+ */
+int xspmm_linear_backward_scratch(xspmm_weight_t weight, int vtype, int act, int64_t N, int64_t* bytes);
+int xspmm_linear_backward(xspmm_weight_t weight, int vtype, int act, const void* vals, const void* x,
+                          const void* keep, const void* dy, void* dx, void* dvals, void* dbias, int64_t N,
+                          void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
+ * h = act(G x + gate_bias) * (U x + up_bias), G and U M x K with blocks of
+ * their own.  The biases may be NULL, and so may keep_gate and keep_up, which
+ * receive the two sums for the backward pass.
+ */
+int xspmm_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act, const void* gate_vals,
+                const void* up_vals, const void* x, const void* gate_bias, const void* up_bias, void* h,
+                void* keep_gate, void* keep_up, int64_t N, void* stream);
+
+/*
+ * Its backward pass from dh: dg = dh keep_up act'(keep_gate) and
+ * du = dh act(keep_gate), rounded to the value type before the products;
+ * dx = G^T dg + U^T du, the stored blocks of dg x^T and du x^T, the sums of dg
+ * and du over the tokens.  Each result may be NULL.  scratch (256-byte aligned)
+ * holds dg and du: as many bytes as xspmm_gated_backward_scratch says.
+ */
+int xspmm_gated_backward_scratch(xspmm_weight_t gate, int vtype, int64_t N, int64_t* bytes);
+int xspmm_gated_backward(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act, const void* gate_vals,
+                         const void* up_vals, const void* x, const void* keep_gate, const void* keep_up,
+                         const void* dh, void* dx, void* dgate_vals, void* dup_vals, void* dgate_bias, void* dup_bias,
+                         int64_t N, void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
+ * Layer norm over the K features of every token: y = (x - mean) rstd weight +
+ * bias, rstd = 1 / sqrt(variance + eps), the variance over K.  x and y are
+ * K x N, weight and bias K (NULL: ones, zeros).  mean and rstd (fp32, N) are
+ * kept for the backward pass, or both NULL.  scratch (256-byte aligned) has as
+ * many bytes as xspmm_layer_norm_scratch says (backward = 0).
+ */
+int xspmm_layer_norm_scratch(int64_t K, int64_t N, int backward, int64_t* bytes);
+int xspmm_layer_norm(int vtype, int64_t K, int64_t N, const void* x, const void* weight, const void* bias, float eps,
+                     void* y, float* mean, float* rstd, void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
+ * Its backward pass: dx (K x N), dweight and dbias (K, summed over the tokens);
+ * each may be NULL.  scratch as above, with backward = 1.
+ */
+int xspmm_layer_norm_backward(int vtype, int64_t K, int64_t N, const void* dy, const void* x, const void* weight,
+                              const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                              void* scratch, int64_t scratch_bytes, void* stream);
 
 #ifdef __cplusplus
 }

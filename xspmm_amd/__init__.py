@@ -628,3 +628,18 @@ class SpMMPlan:
         except Exception:
             pass
 
+
+
+# The feed-forward layer's operators need torch, which the module loads on the
+# first use of one.
+_FEED_FORWARD = ("SparseWeight", "sparse_linear", "sparse_linear_backward", "sparse_gated", "sparse_gated_backward",
+                 "layer_norm", "layer_norm_backward")
+
+
+def __getattr__(name):
+    if name in _FEED_FORWARD:
+        from . import feed_forward
+        for n in _FEED_FORWARD:
+            globals()[n] = getattr(feed_forward, n)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

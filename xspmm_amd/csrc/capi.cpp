@@ -5,9 +5,11 @@
 #include <hip/hip_fp16.h>
 
 #include <cstring>
+#include <memory>
 #include <string>
 #include <utility>
 
+#include "feed_forward.hpp"
 #include "internal.hpp"
 #include "xspmm_capi.h"
 
@@ -19,6 +21,9 @@ struct xspmm_plan_s {
 };
 struct xspmm_mtx_s {
     MtxData data;
+};
+struct xspmm_weight_s {
+    BlockIndex index;
 };
 
 namespace {
@@ -73,11 +78,60 @@ void with_index(int itype, F&& f)
     else throw std::invalid_argument("unknown index type code");
 }
 
+// Calls f(Tag<value>) for the value types of the feed-forward layer.
+template <typename F>
+void with_layer_type(int vtype, F&& f)
+{
+    if (vtype == XSPMM_F32) f(Tag<float>{});
+    else if (vtype == XSPMM_F16) f(Tag<_Float16>{});
+    else if (vtype == XSPMM_BF16) f(Tag<__bf16>{});
+    else throw std::invalid_argument("unknown value type code");
+}
+
 hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 void require(bool ok, const char* what)
 {
     if (!ok) throw std::invalid_argument(what);
+}
+
+// A dense operand of the feed-forward layer: there unless it is empty, and on
+// a 16-byte boundary.
+template <typename T>
+const T* operand(const void* p, bool needed, const char* what)
+{
+    if (p == nullptr && needed) throw std::invalid_argument(std::string("xSpMM: ") + what + " is null.");
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
+        throw std::invalid_argument(std::string("xSpMM: ") + what + " must start on a 16-byte boundary.");
+    return static_cast<const T*>(p);
+}
+
+template <typename T>
+T* result(void* p, bool needed, const char* what)
+{
+    return const_cast<T*>(operand<T>(p, needed, what));
+}
+
+void require_layer(const BlockIndex& w, int act, int64_t N)
+{
+    require(act >= XSPMM_ACT_NONE && act <= XSPMM_ACT_GELU_TANH, "unknown activation code");
+    require(N >= 0, "xSpMM: negative N.");
+    // products of element counts stay below 2^62
+    require(N <= (int64_t(1) << 30), "xSpMM: at most 2^30 tokens.");
+    (void)w;
+}
+
+// 256-byte aligned bytes of one M x N array of a backward pass
+int64_t layer_array(int vtype, int64_t M, int64_t N)
+{
+    const int64_t size = vtype == XSPMM_F32 ? 4 : 2;
+    return (M * N * size + 255) / 256 * 256;
+}
+
+void require_scratch(const void* p, int64_t have, int64_t need)
+{
+    require(have >= need && (need == 0 || p != nullptr), "xSpMM: the scratch is smaller than its query says.");
+    require(reinterpret_cast<uintptr_t>(p) % 256 == 0 || need == 0, "xSpMM: scratch must start on a 256-byte boundary.");
 }
 
 }  // namespace
@@ -469,6 +523,236 @@ int xspmm_mtx_export(xspmm_mtx_t m, int itype, int vtype, void* row_ptr, void* c
 int xspmm_mtx_free(xspmm_mtx_t m)
 {
     return guarded([&] { delete m; });
+}
+
+int xspmm_weight_create(int itype, int64_t M, int64_t K, int64_t Mb, int64_t Kb, int64_t nnzb, const void* brp,
+                        const void* bci, void* stream, xspmm_weight_t* weight_out)
+{
+    return guarded([&] {
+        require(weight_out != nullptr, "xspmm_weight_create: weight_out is null.");
+        *weight_out = nullptr;
+        with_index(itype, [&](auto ti) {
+            using I = typename decltype(ti)::type;
+            auto w = std::make_unique<xspmm_weight_s>();
+            build_block_index<I>(w->index, M, K, Mb, Kb, nnzb, static_cast<const I*>(brp),
+                                 static_cast<const I*>(bci), as_stream(stream));
+            *weight_out = w.release();
+        });
+    });
+}
+
+int xspmm_weight_destroy(xspmm_weight_t weight)
+{
+    return guarded([&] { delete weight; });
+}
+
+int xspmm_linear(xspmm_weight_t weight, int vtype, int act, const void* vals, const void* x, const void* bias,
+                 const void* residual, void* y, void* keep, int64_t N, void* stream)
+{
+    return guarded([&] {
+        require(weight != nullptr, "xspmm_linear: null weight.");
+        const BlockIndex& w = weight->index;
+        require_layer(w, act, N);
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = w.M > 0 && N > 0;
+            ForwardArgs<T> a{};
+            a.weight[0] = &w;
+            a.vals[0] = operand<T>(vals, any && w.nnzb > 0, "vals");
+            a.x = operand<T>(x, any && w.nnzb > 0, "x");
+            a.bias[0] = static_cast<const T*>(bias);
+            a.residual = operand<T>(residual, false, "residual");
+            a.y = result<T>(y, any, "y");
+            a.keep[0] = result<T>(keep, false, "keep");
+            a.N = N;
+            a.act = act;
+            if (any) feed_forward<T>(a, 1, as_stream(stream));
+        });
+    });
+}
+
+int xspmm_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act, const void* gate_vals,
+                const void* up_vals, const void* x, const void* gate_bias, const void* up_bias, void* h,
+                void* keep_gate, void* keep_up, int64_t N, void* stream)
+{
+    return guarded([&] {
+        require(gate != nullptr && up != nullptr, "xspmm_gated: null weight.");
+        const BlockIndex &g = gate->index, &u = up->index;
+        require(g.M == u.M && g.K == u.K, "xspmm_gated: gate and up differ in shape.");
+        require_layer(g, act, N);
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = g.M > 0 && N > 0;
+            ForwardArgs<T> a{};
+            a.weight[0] = &g;
+            a.weight[1] = &u;
+            a.vals[0] = operand<T>(gate_vals, any && g.nnzb > 0, "gate_vals");
+            a.vals[1] = operand<T>(up_vals, any && u.nnzb > 0, "up_vals");
+            a.x = operand<T>(x, any && g.nnzb + u.nnzb > 0, "x");
+            a.bias[0] = static_cast<const T*>(gate_bias);
+            a.bias[1] = static_cast<const T*>(up_bias);
+            a.y = result<T>(h, any, "h");
+            a.keep[0] = result<T>(keep_gate, false, "keep_gate");
+            a.keep[1] = result<T>(keep_up, false, "keep_up");
+            a.N = N;
+            a.act = act;
+            if (any) feed_forward<T>(a, 2, as_stream(stream));
+        });
+    });
+}
+
+int xspmm_linear_backward_scratch(xspmm_weight_t weight, int vtype, int act, int64_t N, int64_t* bytes)
+{
+    return guarded([&] {
+        require(weight != nullptr && bytes != nullptr, "xspmm_linear_backward_scratch: null argument.");
+        require_layer(weight->index, act, N);
+        with_layer_type(vtype, [](auto) {});
+        *bytes = act == XSPMM_ACT_NONE ? 0 : layer_array(vtype, weight->index.M, N);
+    });
+}
+
+int xspmm_linear_backward(xspmm_weight_t weight, int vtype, int act, const void* vals, const void* x,
+                          const void* keep, const void* dy, void* dx, void* dvals, void* dbias, int64_t N,
+                          void* scratch, int64_t scratch_bytes, void* stream)
+{
+    return guarded([&] {
+        require(weight != nullptr, "xspmm_linear_backward: null weight.");
+        const BlockIndex& w = weight->index;
+        require_layer(w, act, N);
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = w.M > 0 && N > 0, act_too = act != XSPMM_ACT_NONE;
+            require_scratch(scratch, scratch_bytes, any && act_too ? layer_array(vtype, w.M, N) : 0);
+            const T* z = operand<T>(keep, any && act_too, "keep");
+            const T* g = operand<T>(dy, any, "dy");
+            const T* v = operand<T>(vals, any && dx != nullptr && w.nnzb > 0, "vals");
+            const T* xs = operand<T>(x, any && dvals != nullptr && w.nnzb > 0, "x");
+            T* out_x = result<T>(dx, false, "dx");
+            T* out_v = result<T>(dvals, false, "dvals");
+            T* out_b = static_cast<T*>(dbias);
+            const hipStream_t s = as_stream(stream);
+            T* dz = act_too ? static_cast<T*>(scratch) : nullptr;
+            if (act_too || out_b) activation_backward<T>(z, nullptr, g, dz, nullptr, out_b, nullptr, act, w.M, N, s);
+            const T* d = act_too ? dz : g;
+            if (out_x && w.K > 0 && N > 0) {
+                TransposedArgs<T> t{};
+                t.weight[0] = &w;
+                t.vals[0] = v;
+                t.dz[0] = d;
+                t.dx = out_x;
+                t.N = N;
+                transposed_product<T>(t, 1, s);
+            }
+            if (out_v) sampled_product<T>(w, d, xs, out_v, N, s);
+        });
+    });
+}
+
+int xspmm_gated_backward_scratch(xspmm_weight_t gate, int vtype, int64_t N, int64_t* bytes)
+{
+    return guarded([&] {
+        require(gate != nullptr && bytes != nullptr, "xspmm_gated_backward_scratch: null argument.");
+        require_layer(gate->index, XSPMM_ACT_NONE, N);
+        with_layer_type(vtype, [](auto) {});
+        *bytes = 2 * layer_array(vtype, gate->index.M, N);
+    });
+}
+
+int xspmm_gated_backward(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act, const void* gate_vals,
+                         const void* up_vals, const void* x, const void* keep_gate, const void* keep_up,
+                         const void* dh, void* dx, void* dgate_vals, void* dup_vals, void* dgate_bias, void* dup_bias,
+                         int64_t N, void* scratch, int64_t scratch_bytes, void* stream)
+{
+    return guarded([&] {
+        require(gate != nullptr && up != nullptr, "xspmm_gated_backward: null weight.");
+        const BlockIndex &wg = gate->index, &wu = up->index;
+        require(wg.M == wu.M && wg.K == wu.K, "xspmm_gated_backward: gate and up differ in shape.");
+        require_layer(wg, act, N);
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = wg.M > 0 && N > 0;
+            const int64_t each = layer_array(vtype, wg.M, N);
+            require_scratch(scratch, scratch_bytes, any ? 2 * each : 0);
+            const T* zg = operand<T>(keep_gate, any, "keep_gate");
+            const T* zu = operand<T>(keep_up, any, "keep_up");
+            const T* g = operand<T>(dh, any, "dh");
+            const T* vg = operand<T>(gate_vals, any && dx != nullptr && wg.nnzb > 0, "gate_vals");
+            const T* vu = operand<T>(up_vals, any && dx != nullptr && wu.nnzb > 0, "up_vals");
+            const T* xs = operand<T>(x, any && ((dgate_vals && wg.nnzb > 0) || (dup_vals && wu.nnzb > 0)), "x");
+            T* out_x = result<T>(dx, false, "dx");
+            T* out_g = result<T>(dgate_vals, false, "dgate_vals");
+            T* out_u = result<T>(dup_vals, false, "dup_vals");
+            const hipStream_t s = as_stream(stream);
+            T* dg = static_cast<T*>(scratch);
+            T* du = any ? reinterpret_cast<T*>(static_cast<char*>(scratch) + each) : nullptr;
+            if (any)
+                activation_backward<T>(zg, zu, g, dg, du, static_cast<T*>(dgate_bias), static_cast<T*>(dup_bias), act,
+                                       wg.M, N, s);
+            else  // sums over no tokens
+                for (void* b : {dgate_bias, dup_bias})
+                    if (b)
+                        activation_backward<T>(nullptr, nullptr, nullptr, nullptr, nullptr, static_cast<T*>(b),
+                                               nullptr, XSPMM_ACT_NONE, wg.M, N, s);
+            if (out_x && wg.K > 0 && N > 0) {
+                TransposedArgs<T> t{};
+                t.weight[0] = &wg;
+                t.weight[1] = &wu;
+                t.vals[0] = vg;
+                t.vals[1] = vu;
+                t.dz[0] = dg;
+                t.dz[1] = du;
+                t.dx = out_x;
+                t.N = N;
+                transposed_product<T>(t, 2, s);
+            }
+            if (out_g) sampled_product<T>(wg, dg, xs, out_g, N, s);
+            if (out_u) sampled_product<T>(wu, du, xs, out_u, N, s);
+        });
+    });
+}
+
+int xspmm_layer_norm_scratch(int64_t K, int64_t N, int backward, int64_t* bytes)
+{
+    return guarded([&] {
+        require(bytes != nullptr, "xspmm_layer_norm_scratch: bytes is null.");
+        require(K >= 0 && N >= 0 && K <= 0x7fffffffLL && N <= (int64_t(1) << 30), "xSpMM: bad size of a norm.");
+        *bytes = layer_norm_scratch(K, N, backward);
+    });
+}
+
+int xspmm_layer_norm(int vtype, int64_t K, int64_t N, const void* x, const void* weight, const void* bias, float eps,
+                     void* y, float* mean, float* rstd, void* scratch, int64_t scratch_bytes, void* stream)
+{
+    return guarded([&] {
+        require(K >= 0 && N >= 0 && K <= 0x7fffffffLL && N <= (int64_t(1) << 30), "xSpMM: bad size of a norm.");
+        require(eps >= 0.f, "xSpMM: a norm's eps is not negative.");
+        require((mean == nullptr) == (rstd == nullptr), "xSpMM: a norm keeps both statistics or none.");
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = K > 0 && N > 0;
+            require_scratch(scratch, scratch_bytes, layer_norm_scratch(K, N, 0));
+            layer_norm<T>(operand<T>(x, any, "x"), static_cast<const T*>(weight), static_cast<const T*>(bias), eps,
+                          result<T>(y, any, "y"), mean, rstd, K, N, scratch, as_stream(stream));
+        });
+    });
+}
+
+int xspmm_layer_norm_backward(int vtype, int64_t K, int64_t N, const void* dy, const void* x, const void* weight,
+                              const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                              void* scratch, int64_t scratch_bytes, void* stream)
+{
+    return guarded([&] {
+        require(K >= 0 && N >= 0 && K <= 0x7fffffffLL && N <= (int64_t(1) << 30), "xSpMM: bad size of a norm.");
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = K > 0 && N > 0;
+            require(!any || (mean != nullptr && rstd != nullptr), "xSpMM: a norm's gradient needs its statistics.");
+            require_scratch(scratch, scratch_bytes, layer_norm_scratch(K, N, 1));
+            layer_norm_backward<T>(operand<T>(dy, any, "dy"), operand<T>(x, any, "x"), static_cast<const T*>(weight),
+                                   mean, rstd, result<T>(dx, false, "dx"), static_cast<T*>(dweight),
+                                   static_cast<T*>(dbias), K, N, scratch, as_stream(stream));
+        });
+    });
 }
 
 }  // extern "C"

@@ -1,0 +1,183 @@
+// feed_forward_device.hpp -- device code that the feed-forward kernels share:
+// value types, loads, matrix instructions, activations.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "feed_forward.hpp"
+
+namespace xspmm {
+namespace detail {
+namespace ff {
+
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kXcds = 8;  // accelerator dies of an MI355X, each with its own L2
+
+template <typename T>
+constexpr bool is_f32 = sizeof(T) == 4;
+
+// VEC consecutive elements at any element's address (the GPU reads and writes
+// vectors off their alignment; aligned ones are no slower for this type).
+template <typename T, int VEC>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+    T v[VEC];
+};
+
+// The same as dwords, for the operands of matrix instructions; one 16-bit
+// element takes a dword of its own.
+template <typename T, int VEC>
+constexpr int kDwords = VEC * (int)sizeof(T) < 4 ? 1 : VEC * (int)sizeof(T) / 4;
+
+template <int D>
+struct Dwords {
+    uint32_t d[D];
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_buffer(const void* base, uint32_t bytes)
+{
+    // raw dword access; a load past `bytes` gives zeros and touches no memory
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ Dwords<kDwords<T, VEC>> buffer_load(__amdgpu_buffer_rsrc_t r, uint32_t off)
+{
+    Dwords<kDwords<T, VEC>> o;
+    constexpr int bytes = VEC * (int)sizeof(T);
+    if constexpr (bytes == 2) {
+        o.d[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)off, 0, 0);
+    } else if constexpr (bytes == 4) {
+        o.d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0);
+    } else if constexpr (bytes == 8) {
+        const u32x2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0);
+        o.d[0] = v.x;
+        o.d[1] = v.y;
+    } else {
+        static_assert(bytes == 16);
+        const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.d[i] = v[i];
+    }
+    return o;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ Dwords<kDwords<T, VEC>> global_load(const T* p)
+{
+    Dwords<kDwords<T, VEC>> o;
+    if constexpr (VEC * sizeof(T) == 2) {
+        o.d[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else {
+        struct __attribute__((packed, aligned(sizeof(T)))) P {
+            uint32_t d[kDwords<T, VEC>];
+        };
+        const P v = *reinterpret_cast<const P*>(p);
+#pragma unroll
+        for (int i = 0; i < kDwords<T, VEC>; ++i) o.d[i] = v.d[i];
+    }
+    return o;
+}
+
+// D += A B of 16x16x32 16-bit values: lane l holds row (column) l % 16 of A
+// (B) at k = 8 (l / 16) .. + 7, and column l % 16 of D at rows 4 (l / 16) .. + 3.
+template <typename T>
+__device__ __forceinline__ float4_t mfma16(u32x4_t a, u32x4_t b, float4_t c)
+{
+    if constexpr (__is_same(T, _Float16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b),
+                                                      c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// D += A B of 16x16x4 fp32 values: lane l holds row (column) l % 16 at k = l / 16.
+__device__ __forceinline__ float4_t mfma32(uint32_t a, uint32_t b, float4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b), c, 0, 0,
+                                                0);
+}
+
+// ---------------------------------------------------------------------------
+// activations, in fp32.  Every form takes its sigmoid or error function from
+// values that neither overflow nor cancel: infinite sums give the limits.
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
+
+constexpr float kGeluA = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kGeluB = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float z)
+{
+    if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;  // a NaN stays
+    if constexpr (ACT == kActSilu) return z / (1.f + expf(-z));
+    if constexpr (ACT == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    // 0.5 (1 + tanh u) = sigmoid(2u)
+    if constexpr (ACT == kActGeluTanh) return z / (1.f + expf(-kGeluA * (z + kGeluB * z * z * z)));
+    return z;
+}
+
+// value and slope
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z, float* value)
+{
+    if constexpr (ACT == kActRelu) {
+        *value = z < 0.f ? 0.f : z;
+        return z > 0.f ? 1.f : z == z ? 0.f : z;
+    }
+    if constexpr (ACT == kActSilu) {
+        const float p = sigmoid(z);
+        *value = z * p;
+        return p * (1.f + z * (1.f - p));
+    }
+    if constexpr (ACT == kActGelu) {
+        const float p = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+        *value = z * p;
+        return p + 0.3989422804014327f * z * expf(-0.5f * z * z);
+    }
+    if constexpr (ACT == kActGeluTanh) {
+        // beyond |z| = 16 the sigmoid is 0 or 1 in fp32 and the slope with it;
+        // the clamp keeps z^3 finite there
+        const float c = fminf(fmaxf(z, -16.f), 16.f);
+        const float p = sigmoid(kGeluA * (c + kGeluB * c * c * c));
+        *value = z * p;
+        return z == z ? p + c * p * (1.f - p) * kGeluA * (1.f + 3.f * kGeluB * c * c) : z;
+    }
+    *value = z;
+    return 1.f;
+}
+
+// f(constant activation)
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& f)
+{
+    switch (act) {
+    case kActRelu: f(std::integral_constant<int, kActRelu>{}); break;
+    case kActSilu: f(std::integral_constant<int, kActSilu>{}); break;
+    case kActGelu: f(std::integral_constant<int, kActGelu>{}); break;
+    case kActGeluTanh: f(std::integral_constant<int, kActGeluTanh>{}); break;
+    default: f(std::integral_constant<int, kActNone>{}); break;
+    }
+}
+
+// Work item of workgroup w in a grid of 8 * xcd_chunk(total): each XCD takes a
+// contiguous range of items, so that neighbours share its L2.  -1: padding.
+__host__ __device__ __forceinline__ int64_t xcd_chunk(int64_t total) { return (total + kXcds - 1) / kXcds; }
+__device__ __forceinline__ int64_t xcd_item(int64_t w, int64_t total)
+{
+    const int64_t i = (w % kXcds) * xcd_chunk(total) + w / kXcds;
+    return i < total ? i : -1;
+}
+
+}  // namespace ff
+}  // namespace detail
+}  // namespace xspmm

@@ -1,0 +1,354 @@
+"""The feed-forward layer of a model on block-sparse weights, and layer norm.
+
+Activations are features x tokens, contiguous, as the B and C of ``spmm``; a
+weight is a ``BCSRMatrix`` of 16x16 blocks (``csr_to_bcsr``) whose block
+positions a ``SparseWeight`` lays out once.  Every array of a call has the
+weight's value type: float16, float32, or bfloat16, which the operators here
+take besides the framework's two.  Sums are fp32, rounded once.
+
+  sparse_linear            y = act(A x + bias) + residual
+  sparse_gated             h = act(G x + bias_gate) * (U x + bias_up)
+  layer_norm               over the features of every token
+  *_backward               their gradients
+
+The operators run on torch's current stream and allocate their results and
+scratch with torch.  ``FeedForward`` puts them together as a module with
+gradients.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+import xspmm_amd as X
+
+BF16 = 2
+ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+_TYPES = {torch.float32: X.F32, torch.float16: X.F16, torch.bfloat16: BF16}
+
+
+def _prototypes(L):
+    p, i64, i32, f32 = C.c_void_p, C.c_int64, C.c_int, C.c_float
+    out = C.POINTER(C.c_int64)
+    for name, args in {
+        "xspmm_weight_create": [i32, i64, i64, i64, i64, i64, p, p, p, C.POINTER(C.c_void_p)],
+        "xspmm_weight_destroy": [p],
+        "xspmm_linear": [p, i32, i32, p, p, p, p, p, p, i64, p],
+        "xspmm_gated": [p, p, i32, i32, p, p, p, p, p, p, p, p, i64, p],
+        "xspmm_linear_backward_scratch": [p, i32, i32, i64, out],
+        "xspmm_linear_backward": [p, i32, i32, p, p, p, p, p, p, p, i64, p, i64, p],
+        "xspmm_gated_backward_scratch": [p, i32, i64, out],
+        "xspmm_gated_backward": [p, p, i32, i32, p, p, p, p, p, p, p, p, p, p, p, i64, p, i64, p],
+        "xspmm_layer_norm_scratch": [i64, i64, i32, out],
+        "xspmm_layer_norm": [i32, i64, i64, p, p, p, f32, p, p, p, p, i64, p],
+        "xspmm_layer_norm_backward": [i32, i64, i64, p, p, p, p, p, p, p, p, p, i64, p],
+    }.items():
+        f = getattr(L, name)
+        f.restype, f.argtypes = i32, args
+    return L
+
+
+_lib = None
+
+
+def _load():
+    global _lib
+    if _lib is None:
+        _lib = _prototypes(X.load())
+    return _lib
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+class _Here:
+    """The device of a call's operands as the current one."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _check(t, name, shape, dtype, device, aligned=True):
+    if type(t) is not torch.Tensor and not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    at = t.data_ptr()
+    if aligned and at % 16:
+        raise ValueError(f"{name} must start on a 16-byte boundary")
+    return at or None
+
+
+def _activation(name):
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown activation {name!r}: one of {', '.join(k for k in ACTIVATIONS if k)}") from None
+
+
+def _scratch(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+class SparseWeight:
+    """Where the 16x16 blocks of a BCSR matrix stand, laid out once for products
+    with the matrix and with its transpose.  The block values stay the matrix's
+    own (``values``, num_blocks * 256 of them) and may change between calls; the
+    positions are read once, here, and synchronize torch's current stream."""
+
+    def __init__(self, A):
+        self._h = None
+        if A.r_block != 16 or A.c_block != 16:
+            raise ValueError("a weight has 16x16 blocks")
+        if A.values.dtype not in _TYPES:
+            raise TypeError(f"unsupported value dtype {A.values.dtype}")
+        rp, ci = A.row_ptr, A.col_ind
+        device = rp.device
+        if device.type != "cuda":
+            raise ValueError("a weight's arrays are on the GPU")
+        X.icode(rp.dtype)
+        _check(rp, "row_ptr", (int(A.num_block_rows) + 1,), rp.dtype, device, aligned=False)
+        _check(ci, "col_ind", (int(ci.numel()),), rp.dtype, device, aligned=False)
+        self.device = device
+        self.shape = (int(A.num_rows), int(A.num_cols))
+        self.num_blocks = int(ci.numel())
+        self.dtype = A.values.dtype
+        self.code = _TYPES[self.dtype]
+        self.matrix = A
+        _check(A.values, "values", (self.num_blocks * 256,), self.dtype, device)
+        h = C.c_void_p()
+        self._L = _load()
+        with _Here(device) as stream:
+            X._check(self._L.xspmm_weight_create(X.icode(rp.dtype), *self.shape, int(A.num_block_rows),
+                                                 int(A.num_block_cols), self.num_blocks, X._ptr(rp), X._ptr(ci),
+                                                 stream, C.byref(h)))
+        self._h = h
+
+    @property
+    def values(self):
+        return self.matrix.values
+
+    @values.setter
+    def values(self, v):
+        _check(v, "values", (self.num_blocks * 256,), self.dtype, self.device)
+        self.matrix.values = v
+
+    def _values(self):
+        if self._h is None:
+            raise RuntimeError("SparseWeight is closed")
+        return _check(self.matrix.values, "values", (self.num_blocks * 256,), self.dtype, self.device)
+
+    def close(self):
+        if self._h is not None:
+            self._L.xspmm_weight_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _tokens(x, name="x"):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if x.dim() != 2:
+        raise ValueError(f"{name} must be features x tokens, got {x.dim()} dimensions")
+    return x.shape[1]
+
+
+def _optional(t, name, shape, dtype, device, aligned=True):
+    return None if t is None else _check(t, name, shape, dtype, device, aligned)
+
+
+def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, out=None):
+    """act(W x + bias) + residual, M x N; with keep also W x + bias, which
+    ``sparse_linear_backward`` takes where there is an activation."""
+    act = _activation(activation)
+    (M, K), N, dt, dev = W.shape, _tokens(x), W.dtype, W.device
+    vals = W._values()
+    xp = _check(x, "x", (K, N), dt, dev)
+    bp = _optional(bias, "bias", (M,), dt, dev, aligned=False)
+    rp = _optional(residual, "residual", (M, N), dt, dev)
+    y = torch.empty((M, N), dtype=dt, device=dev) if out is None else out
+    yp = _check(y, "out", (M, N), dt, dev)
+    z = torch.empty((M, N), dtype=dt, device=dev) if keep else None
+    with _Here(dev) as stream:
+        rc = W._L.xspmm_linear(W._h, W.code, act, vals, xp, bp, rp, yp, z.data_ptr() or None if keep else None, N,
+                               stream)
+    if rc:
+        X._check(rc)
+    return (y, z) if keep else y
+
+
+def sparse_linear_backward(W, x, kept, dy, activation=None, bias=False, need=(True, True)):
+    """(dx, dvalues, dbias) from dy = the gradient of ``sparse_linear``'s result
+    and `kept` = W x + bias (not read, and may be None, without an activation).
+    bias: whether the layer has one (dbias is None otherwise); need: whether dx
+    and dvalues are wanted (None otherwise).  The residual's gradient is dy."""
+    act = _activation(activation)
+    (M, K), N, dt, dev = W.shape, _tokens(dy, "dy"), W.dtype, W.device
+    vals = W._values()
+    xp = _check(x, "x", (K, N), dt, dev)
+    zp = _check(kept, "kept", (M, N), dt, dev) if act else None
+    gp = _check(dy, "dy", (M, N), dt, dev)
+    dx = torch.empty((K, N), dtype=dt, device=dev) if need[0] else None
+    dv = torch.empty(W.num_blocks * 256, dtype=dt, device=dev) if need[1] else None
+    db = torch.empty(M, dtype=dt, device=dev) if bias else None
+    n = C.c_int64(0)
+    L = W._L
+    with _Here(dev) as stream:
+        rc = L.xspmm_linear_backward_scratch(W._h, W.code, act, N, C.byref(n))
+        if rc:
+            X._check(rc)
+        ws = _scratch(n.value, dev)
+        rc = L.xspmm_linear_backward(W._h, W.code, act, vals, xp, zp, gp, _at(dx), _at(dv), _at(db), N, _at(ws),
+                                     n.value, stream)
+    if rc:
+        X._check(rc)
+    return dx, dv, db
+
+
+def _at(t):
+    return None if t is None else t.data_ptr() or None
+
+
+def _pair(G, U):
+    if G.shape != U.shape or G.dtype != U.dtype or G.device != U.device:
+        raise ValueError(f"gate ({G.shape}, {G.dtype}, {G.device}) and up ({U.shape}, {U.dtype}, {U.device}) differ")
+    return G.shape
+
+
+def sparse_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", keep=False, out=None):
+    """act(G x + bias_gate) * (U x + bias_up), M x N; with keep also the two
+    sums, which ``sparse_gated_backward`` takes.  G and U have blocks of their
+    own."""
+    act = _activation(activation)
+    (M, K), N, dt, dev = _pair(G, U), _tokens(x), G.dtype, G.device
+    gv, uv = G._values(), U._values()
+    xp = _check(x, "x", (K, N), dt, dev)
+    gb = _optional(bias_gate, "bias_gate", (M,), dt, dev, aligned=False)
+    ub = _optional(bias_up, "bias_up", (M,), dt, dev, aligned=False)
+    h = torch.empty((M, N), dtype=dt, device=dev) if out is None else out
+    hp = _check(h, "out", (M, N), dt, dev)
+    zg = torch.empty((M, N), dtype=dt, device=dev) if keep else None
+    zu = torch.empty((M, N), dtype=dt, device=dev) if keep else None
+    with _Here(dev) as stream:
+        rc = G._L.xspmm_gated(G._h, U._h, G.code, act, gv, uv, xp, gb, ub, hp, _at(zg), _at(zu), N, stream)
+    if rc:
+        X._check(rc)
+    return (h, zg, zu) if keep else h
+
+
+def sparse_gated_backward(G, U, x, kept_gate, kept_up, dh, activation="silu", bias=False, need=(True, True, True)):
+    """(dx, dvalues of G, dvalues of U, dbias_gate, dbias_up) from dh = the
+    gradient of ``sparse_gated``'s result and the two sums it kept.  bias:
+    whether the biases' gradients are wanted; need: whether the first three are
+    (None otherwise)."""
+    act = _activation(activation)
+    (M, K), N, dt, dev = _pair(G, U), _tokens(dh, "dh"), G.dtype, G.device
+    gv, uv = G._values(), U._values()
+    xp = _check(x, "x", (K, N), dt, dev)
+    zg = _check(kept_gate, "kept_gate", (M, N), dt, dev)
+    zu = _check(kept_up, "kept_up", (M, N), dt, dev)
+    hp = _check(dh, "dh", (M, N), dt, dev)
+    dx = torch.empty((K, N), dtype=dt, device=dev) if need[0] else None
+    dg = torch.empty(G.num_blocks * 256, dtype=dt, device=dev) if need[1] else None
+    du = torch.empty(U.num_blocks * 256, dtype=dt, device=dev) if need[2] else None
+    bg = torch.empty(M, dtype=dt, device=dev) if bias else None
+    bu = torch.empty(M, dtype=dt, device=dev) if bias else None
+    n = C.c_int64(0)
+    L = G._L
+    with _Here(dev) as stream:
+        rc = L.xspmm_gated_backward_scratch(G._h, G.code, N, C.byref(n))
+        if rc:
+            X._check(rc)
+        ws = _scratch(n.value, dev)
+        rc = L.xspmm_gated_backward(G._h, U._h, G.code, act, gv, uv, xp, zg, zu, hp, _at(dx), _at(dg), _at(du),
+                                    _at(bg), _at(bu), N, _at(ws), n.value, stream)
+    if rc:
+        X._check(rc)
+    return dx, dg, du, bg, bu
+
+
+def _norm_operands(x, weight, bias):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch tensor")
+    if x.dim() != 2:
+        raise ValueError(f"x must be features x tokens, got {x.dim()} dimensions")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if x.device.type != "cuda":
+        raise ValueError("x is not on the GPU")
+    K, N = x.shape
+    if K == 0:
+        raise ValueError("a norm needs at least one feature")
+    dt, dev = x.dtype, x.device
+    return (K, N, dt, dev, _check(x, "x", (K, N), dt, dev), _optional(weight, "weight", (K,), dt, dev, aligned=False),
+            _optional(bias, "bias", (K,), dt, dev, aligned=False))
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, keep=False, out=None):
+    """Layer norm over the features (rows) of every token (column) of x; with
+    keep also the tokens' mean and 1 / sqrt(variance + eps) in fp32, which
+    ``layer_norm_backward`` takes."""
+    K, N, dt, dev, xp, wp, bp = _norm_operands(x, weight, bias)
+    L = _load()
+    y = torch.empty((K, N), dtype=dt, device=dev) if out is None else out
+    yp = _check(y, "out", (K, N), dt, dev)
+    mean = torch.empty(N, dtype=torch.float32, device=dev) if keep else None
+    rstd = torch.empty(N, dtype=torch.float32, device=dev) if keep else None
+    n = C.c_int64(0)
+    with _Here(dev) as stream:
+        rc = L.xspmm_layer_norm_scratch(K, N, 0, C.byref(n))
+        if rc:
+            X._check(rc)
+        ws = _scratch(n.value, dev)
+        rc = L.xspmm_layer_norm(_TYPES[dt], K, N, xp, wp, bp, eps, yp, _at(mean), _at(rstd), _at(ws), n.value, stream)
+    if rc:
+        X._check(rc)
+    return (y, mean, rstd) if keep else y
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, need=(True, True, True)):
+    """(dx, dweight, dbias) of ``layer_norm`` from dy and the statistics it
+    kept; weight may be None (ones).  need: which of them are wanted (None
+    otherwise)."""
+    K, N, dt, dev, xp, wp, _ = _norm_operands(x, weight, None)
+    L = _load()
+    gp = _check(dy, "dy", (K, N), dt, dev)
+    mp = _check(mean, "mean", (N,), torch.float32, dev, aligned=False)
+    sp = _check(rstd, "rstd", (N,), torch.float32, dev, aligned=False)
+    dx = torch.empty((K, N), dtype=dt, device=dev) if need[0] else None
+    dw = torch.empty(K, dtype=dt, device=dev) if need[1] else None
+    db = torch.empty(K, dtype=dt, device=dev) if need[2] else None
+    n = C.c_int64(0)
+    with _Here(dev) as stream:
+        rc = L.xspmm_layer_norm_scratch(K, N, 1, C.byref(n))
+        if rc:
+            X._check(rc)
+        ws = _scratch(n.value, dev)
+        rc = L.xspmm_layer_norm_backward(_TYPES[dt], K, N, gp, xp, wp, mp, sp, _at(dx), _at(dw), _at(db), _at(ws),
+                                         n.value, stream)
+    if rc:
+        X._check(rc)
+    return dx, dw, db
