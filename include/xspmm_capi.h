@@ -472,7 +472,7 @@ int xspmm_gated_backward(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int 
  * kept for the backward pass, or both NULL.  scratch (256-byte aligned) has as
  * many bytes as xspmm_layer_norm_scratch says (backward = 0).
  */
-int xspmm_layer_norm_scratch(int64_t K, int64_t N, int backward, int64_t* bytes);
+int xspmm_layer_norm_scratch(int vtype, int64_t K, int64_t N, int backward, int64_t* bytes);
 int xspmm_layer_norm(int vtype, int64_t K, int64_t N, const void* x, const void* weight, const void* bias, float eps,
                      void* y, float* mean, float* rstd, void* scratch, int64_t scratch_bytes, void* stream);
 

@@ -325,7 +325,7 @@ def test_other_stream_and_repeats():
 # ---------------------------------------------------------------------------
 
 NORM_SIZES = [(1, 1), (1, 40), (64, 1), (100, 3), (4096, 1), (777, 17), (64, 64), (500, 130), (130, 1000), (2000, 257),
-              (16, 5000), (4096, 33)]
+              (16, 5000), (4096, 33), (1000, 9), (300, 70), (5000, 40), (9000, 21), (20000, 19), (20000, 300)]
 
 
 def norm64(x, w, b, eps):

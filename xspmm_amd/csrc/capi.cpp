@@ -711,12 +711,14 @@ int xspmm_gated_backward(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int 
     });
 }
 
-int xspmm_layer_norm_scratch(int64_t K, int64_t N, int backward, int64_t* bytes)
+int xspmm_layer_norm_scratch(int vtype, int64_t K, int64_t N, int backward, int64_t* bytes)
 {
     return guarded([&] {
         require(bytes != nullptr, "xspmm_layer_norm_scratch: bytes is null.");
         require(K >= 0 && N >= 0 && K <= 0x7fffffffLL && N <= (int64_t(1) << 30), "xSpMM: bad size of a norm.");
-        *bytes = layer_norm_scratch(K, N, backward);
+        with_layer_type(vtype, [&](auto tv) {
+            *bytes = layer_norm_scratch(K, N, sizeof(typename decltype(tv)::type), backward);
+        });
     });
 }
 
@@ -730,7 +732,7 @@ int xspmm_layer_norm(int vtype, int64_t K, int64_t N, const void* x, const void*
         with_layer_type(vtype, [&](auto tv) {
             using T = typename decltype(tv)::type;
             const bool any = K > 0 && N > 0;
-            require_scratch(scratch, scratch_bytes, layer_norm_scratch(K, N, 0));
+            require_scratch(scratch, scratch_bytes, layer_norm_scratch(K, N, sizeof(T), 0));
             layer_norm<T>(operand<T>(x, any, "x"), static_cast<const T*>(weight), static_cast<const T*>(bias), eps,
                           result<T>(y, any, "y"), mean, rstd, K, N, scratch, as_stream(stream));
         });
@@ -747,7 +749,7 @@ int xspmm_layer_norm_backward(int vtype, int64_t K, int64_t N, const void* dy, c
             using T = typename decltype(tv)::type;
             const bool any = K > 0 && N > 0;
             require(!any || (mean != nullptr && rstd != nullptr), "xSpMM: a norm's gradient needs its statistics.");
-            require_scratch(scratch, scratch_bytes, layer_norm_scratch(K, N, 1));
+            require_scratch(scratch, scratch_bytes, layer_norm_scratch(K, N, sizeof(T), 1));
             layer_norm_backward<T>(operand<T>(dy, any, "dy"), operand<T>(x, any, "x"), static_cast<const T*>(weight),
                                    mean, rstd, result<T>(dx, false, "dx"), static_cast<T*>(dweight),
                                    static_cast<T*>(dbias), K, N, scratch, as_stream(stream));

@@ -81,7 +81,8 @@ template <typename T>
 void activation_backward(const T* z, const T* up, const T* dy, T* dz, T* dup, T* dbias, T* dbias_up, int act,
                          int64_t M, int64_t N, hipStream_t s);
 
-int64_t layer_norm_scratch(int64_t K, int64_t N, int backward);
+// size: bytes of a value
+int64_t layer_norm_scratch(int64_t K, int64_t N, int64_t size, int backward);
 template <typename T>
 void layer_norm(const T* x, const T* weight, const T* bias, float eps, T* y, float* mean, float* rstd, int64_t K,
                 int64_t N, void* scratch, hipStream_t s);

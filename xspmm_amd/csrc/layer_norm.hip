@@ -27,273 +27,399 @@ struct NormShape {
     int64_t len;      // rows per slice
 };
 
-constexpr int kNormWaves = 4;
+constexpr int kForwardWaves = 8, kBackwardWaves = 4;
 
+// count (the same for all V columns), means, sums of squared deviations
+template <int V>
 struct Moments {
-    float n, m, s;  // count, mean, sum of squared deviations
+    float n, m[V], s[V];
 };
 
-__device__ __forceinline__ Moments join(Moments a, Moments b)
+template <int V>
+__device__ __forceinline__ void join(Moments<V>& a, const Moments<V>& b)
 {
     const float n = a.n + b.n;
-    if (n == 0.f) return a;
-    const float d = b.m - a.m, share = b.n / n;
-    return {n, a.m + d * share, a.s + b.s + d * d * a.n * share};
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void load_tokens(float (&v)[V], const T* p, int64_t n, int64_t N)
-{
-    if (n + V <= N) {
-        const auto q = *reinterpret_cast<const Pack<T, V>*>(p + n);
+    const float share = n > 0.f ? b.n / n : 0.f, weight = a.n * share;
+    a.n = n;
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (float)q.v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = n + i < N ? (float)p[n + i] : 0.f;
+    for (int i = 0; i < V; ++i) {
+        const float d = b.m[i] - a.m[i];
+        a.m[i] += d * share;
+        a.s[i] += b.s[i] + d * d * weight;
     }
 }
 
+// A lane's V tokens start at min(n, N - V): no load or store needs a condition
+// (one on a load makes the wave wait for it before the next), and the lanes at
+// the end do the same work for the same tokens.  Where they would count twice,
+// own() leaves a lane its tokens from n on.
 template <typename T, int V>
-__device__ __forceinline__ void store_tokens(T* p, const float (&v)[V], int64_t n, int64_t N)
+__device__ __forceinline__ Pack<T, V> load_tokens(const T* p)
 {
-    if (n + V <= N) {
-        Pack<T, V> q;
-#pragma unroll
-        for (int i = 0; i < V; ++i) q.v[i] = (T)v[i];
-        *reinterpret_cast<Pack<T, V>*>(p + n) = q;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (n + i < N) p[n + i] = (T)v[i];
-    }
+    return *reinterpret_cast<const Pack<T, V>*>(p);
 }
 
-// Moments of rows [k0 + sub, k1) step `step` of the lane's columns, kU rows at
-// a time: mean and deviations of those first, then joined.
 template <typename T, int V>
-__device__ __forceinline__ void column_moments(Moments (&mo)[V], const T* x, int64_t k0, int64_t k1, int64_t step,
-                                               int64_t n, int64_t N)
+__device__ __forceinline__ void store_tokens(T* p, const float (&v)[V])
 {
-    constexpr int kU = 8;
+    Pack<T, V> q;
 #pragma unroll
-    for (int i = 0; i < V; ++i) mo[i] = {0.f, 0.f, 0.f};
-    if (n >= N) return;
+    for (int i = 0; i < V; ++i) q.v[i] = (T)v[i];
+    *reinterpret_cast<Pack<T, V>*>(p) = q;
+}
+
+__device__ __forceinline__ bool own(int64_t n, int64_t at, int64_t N, int i) { return at + i >= n && at + i < N; }
+
+// Moments of rows [k0, k1) step `step` of the lane's columns, kU rows at a
+// time: mean and deviations of those first, then joined.  x is at the lane's
+// first token.
+template <typename T, int V>
+__device__ __forceinline__ Moments<V> column_moments(const T* x, int64_t k0, int64_t k1, int64_t step, int64_t N)
+{
+    constexpr int kU = V >= 4 ? 8 : 16;
+    Moments<V> all;
+    all.n = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) all.m[i] = all.s[i] = 0.f;
     for (int64_t k = k0; k < k1; k += kU * step) {
-        float v[kU][V];
-        float count = 0.f;
+        Pack<T, V> raw[kU];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int64_t r = k + u * step;
-            if (r < k1) {
-                load_tokens<T, V>(v[u], x + r * N, n, N);
-                count += 1.f;
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[u][i] = 0.f;
-            }
-        }
+        for (int u = 0; u < kU; ++u) raw[u] = load_tokens<T, V>(x + min(k + u * step, k1 - 1) * N);
+        const int64_t left = (k1 - k + step - 1) / step;
+        Moments<V> mo;
+        mo.n = left < kU ? (float)left : (float)kU;
+        const float inv = 1.f / mo.n;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float sum = 0.f;
 #pragma unroll
-            for (int u = 0; u < kU; ++u) sum += v[u][i];
-            const float m = sum / count;
-            float s = 0.f;
+            for (int u = 0; u < kU; ++u) sum += u < left ? (float)raw[u].v[i] : 0.f;
+            mo.m[i] = sum * inv;
+            mo.s[i] = 0.f;
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
-                const float d = k + u * step < k1 ? v[u][i] - m : 0.f;
-                s += d * d;
+                const float d = u < left ? (float)raw[u].v[i] - mo.m[i] : 0.f;
+                mo.s[i] += d * d;
             }
-            mo[i] = join(mo[i], {count, m, s});
         }
+        join(all, mo);
     }
+    return all;
 }
 
 // Joins the lanes of a wave that hold the same columns, then the waves (LDS:
-// [waves][np * V]); the first wave's first np lanes have the result.
+// [waves][np]); the first wave's first np lanes have the result.
 template <int V, int WAVES>
-__device__ __forceinline__ void join_workgroup(Moments (&mo)[V], int np, Moments* red)
+__device__ __forceinline__ void join_workgroup(Moments<V>& mo, int np, Moments<V>* red)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int d = np; d < 64; d <<= 1) {
+        Moments<V> o;
+        o.n = __shfl_down(mo.n, d, 64);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const Moments o = {__shfl_down(mo[i].n, d, 64), __shfl_down(mo[i].m, d, 64), __shfl_down(mo[i].s, d, 64)};
-            mo[i] = join(mo[i], o);
+            o.m[i] = __shfl_down(mo.m[i], d, 64);
+            o.s[i] = __shfl_down(mo.s[i], d, 64);
         }
+        join(mo, o);
     }
-    if (lane < np)
-#pragma unroll
-        for (int i = 0; i < V; ++i) red[(wave * np + lane) * V + i] = mo[i];
+    if (lane < np) red[wave * np + lane] = mo;
     __syncthreads();
     if (wave == 0 && lane < np)
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w)
-#pragma unroll
-            for (int i = 0; i < V; ++i) mo[i] = join(mo[i], red[(w * np + lane) * V + i]);
-}
-
-template <typename T, int V>
-__global__ __launch_bounds__(64 * kNormWaves) void ln_stats_kernel(const T* __restrict__ x, float2* __restrict__ part,
-                                                                   int64_t K, int64_t N, NormShape h)
-{
-    __shared__ Moments red[kNormWaves * 64 * V];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t tile = blockIdx.x % h.tiles, slice = blockIdx.x / h.tiles;
-    const int64_t n = (tile * h.np + lane % h.np) * V;
-    const int64_t k0 = slice * h.len, k1 = min(K, k0 + h.len);
-    const int per = 64 / h.np;
-    Moments mo[V];
-    column_moments<T, V>(mo, x, k0 + wave * per + lane / h.np, k1, kNormWaves * per, n, N);
-    join_workgroup<V, kNormWaves>(mo, h.np, red);
-    if (wave == 0 && lane < h.np)
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (n + i < N) part[slice * N + n + i] = float2{mo[i].m, mo[i].s};
+        for (int w = 1; w < WAVES; ++w) join(mo, red[w * np + lane]);
 }
 
 __device__ __forceinline__ float rstd_of(float s, float K, float eps) { return 1.f / sqrtf(s / K + eps); }
 
-__global__ __launch_bounds__(256) void ln_join_kernel(const float2* __restrict__ part, float* __restrict__ mean,
-                                                      float* __restrict__ rstd, int64_t K, int64_t N, NormShape h,
-                                                      float eps)
-{
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
-    Moments mo = {0.f, 0.f, 0.f};
-    for (int64_t s = 0; s < h.slices; ++s) {
-        const float2 p = part[s * N + n];
-        mo = join(mo, {(float)(min(K, (s + 1) * h.len) - s * h.len), p.x, p.y});
-    }
-    mean[n] = mo.m;
-    rstd[n] = rstd_of(mo.s, (float)K, eps);
-}
-
 template <typename T, int V>
-__device__ __forceinline__ void normalize(const T* x, const T* w, const T* b, T* y, const float (&m)[V],
-                                          const float (&r)[V], int64_t k0, int64_t k1, int64_t step, int64_t n,
-                                          int64_t N)
-{
-    if (n >= N) return;
-#pragma unroll 4
-    for (int64_t k = k0; k < k1; k += step) {
-        float v[V];
-        load_tokens<T, V>(v, x + k * N, n, N);
-        const float wk = w ? (float)w[k] : 1.f, bk = b ? (float)b[k] : 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (v[i] - m[i]) * r[i] * wk + bk;
-        store_tokens<T, V>(y + k * N, v, n, N);
-    }
-}
-
-template <typename T, int V>
-__global__ __launch_bounds__(64 * kNormWaves) void ln_apply_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                                                                   const T* __restrict__ b,
-                                                                   const float* __restrict__ mean,
-                                                                   const float* __restrict__ rstd, T* __restrict__ y,
+__global__ __launch_bounds__(64 * kForwardWaves) void ln_stats_kernel(const T* __restrict__ x, float2* __restrict__ part,
                                                                    int64_t K, int64_t N, NormShape h)
 {
+    __shared__ Moments<V> red[kForwardWaves * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t tile = blockIdx.x % h.tiles, slice = blockIdx.x / h.tiles;
-    const int64_t n = (tile * h.np + lane % h.np) * V;
+    const int64_t tile = blockIdx.x / h.slices, slice = blockIdx.x % h.slices;
+    const int64_t at = min((tile * h.np + lane % h.np) * V, N - V);
     const int64_t k0 = slice * h.len, k1 = min(K, k0 + h.len);
     const int per = 64 / h.np;
-    float m[V], r[V];
-    load_tokens<float, V>(m, mean, n, N);
-    load_tokens<float, V>(r, rstd, n, N);
-    normalize<T, V>(x, w, b, y, m, r, k0 + wave * per + lane / h.np, k1, kNormWaves * per, n, N);
+    Moments<V> mo = column_moments<T, V>(x + at, k0 + wave * per + lane / h.np, k1, kForwardWaves * per, N);
+    join_workgroup<V, kForwardWaves>(mo, h.np, red);
+    if (wave == 0 && lane < h.np)
+#pragma unroll
+        for (int i = 0; i < V; ++i) part[slice * N + at + i] = float2{mo.m[i], mo.s[i]};
 }
 
-// Few tokens: a workgroup takes all rows of a tile, twice.
-constexpr int kSmallWaves = 16;
+// U rows of a lane on their way: its tokens, weight and bias
+template <typename T, int V, int U>
+struct Rows {
+    Pack<T, V> raw[U];
+    T w[U], b[U];
+
+    // x at the lane's first token
+    __device__ __forceinline__ void load(const T* x, const T* wp, const T* bp, int64_t k, int64_t k1, int64_t step,
+                                         int64_t N)
+    {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t q = min(k + u * step, k1 - 1);
+            raw[u] = load_tokens<T, V>(x + q * N);
+            w[u] = wp ? wp[q] : (T)1.f;
+            b[u] = bp ? bp[q] : (T)0.f;
+        }
+    }
+    __device__ __forceinline__ void store(T* y, const float (&m)[V], const float (&r)[V], int64_t k, int64_t k1,
+                                          int64_t step, int64_t N) const
+    {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k + u * step >= k1) break;
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = ((float)raw[u].v[i] - m[i]) * r[i] * (float)w[u] + (float)b[u];
+            store_tokens<T, V>(y + (k + u * step) * N, v);
+        }
+    }
+};
+
+// Every workgroup joins the slices' moments of its columns (a few KB that its
+// XCD's L2 holds) rather than waiting for a launch of its own to do it.
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kSmallWaves) void ln_small_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                                                                    const T* __restrict__ b, float eps,
-                                                                    T* __restrict__ y, float* __restrict__ mean,
-                                                                    float* __restrict__ rstd, int64_t K, int64_t N,
-                                                                    int np)
+__global__ __launch_bounds__(64 * kForwardWaves) void ln_apply_kernel(const T* __restrict__ x, const T* __restrict__ w,
+                                                                   const T* __restrict__ b,
+                                                                   const float2* __restrict__ part, float eps,
+                                                                   float* __restrict__ mean, float* __restrict__ rstd,
+                                                                   T* __restrict__ y, int64_t K, int64_t N, NormShape h)
 {
-    __shared__ Moments red[kSmallWaves * 64 * V];
+    constexpr int kThreads = 64 * kForwardWaves;
+    __shared__ Moments<1> red[kThreads];
     __shared__ float2 stats[64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t n = ((int64_t)blockIdx.x * np + lane % np) * V;
-    const int per = 64 / np;
-    const int64_t k0 = wave * per + lane / np, step = kSmallWaves * per;
-    Moments mo[V];
-    column_moments<T, V>(mo, x, k0, K, step, n, N);
-    join_workgroup<V, kSmallWaves>(mo, np, red);
-    if (wave == 0 && lane < np)
+    const int64_t tile = blockIdx.x / h.slices, slice = blockIdx.x % h.slices;
+    const int per = 64 / h.np;
+    const int64_t at = min((tile * h.np + lane % h.np) * V, N - V);
+    const int64_t k1 = min(K, (slice + 1) * h.len), step = kForwardWaves * per;
+    int64_t k = slice * h.len + wave * per + lane / h.np;
+    constexpr int U = V >= 4 ? 8 : 16;
+    Rows<T, V, U> rows;
+    if (k < k1) rows.load(x + at, w, b, k, k1, step, N);  // under way while the moments are joined
+    const int cols = h.np * V, shares = kThreads / cols;
+    const int64_t base = max(min(tile * cols, N - cols), (int64_t)0);  // the last tile moves back
+    {
+        const int c = threadIdx.x % cols, share = threadIdx.x / cols;
+        const int64_t col = base + c;
+        Moments<1> mo = {0.f, {0.f}, {0.f}};
+        if (col < N) {
+            for (int64_t s0 = share; s0 < h.slices; s0 += 4 * shares) {
+                float2 p[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float r = rstd_of(mo[i].s, (float)K, eps);
-            stats[lane * V + i] = float2{mo[i].m, r};
-            if (mean && n + i < N) {
-                mean[n + i] = mo[i].m;
-                rstd[n + i] = r;
+                for (int u = 0; u < 4; ++u) p[u] = part[min(s0 + u * shares, h.slices - 1) * N + col];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int64_t s = s0 + u * shares;
+                    if (s < h.slices)
+                        join(mo, Moments<1>{(float)(min(K, (s + 1) * h.len) - s * h.len), {p[u].x}, {p[u].y}});
+                }
             }
         }
-    __syncthreads();
+        red[threadIdx.x] = mo;
+        __syncthreads();
+        if (share == 0) {
+            for (int q = 1; q < shares; ++q) join(mo, red[q * cols + c]);
+            const float r = rstd_of(mo.s[0], (float)K, eps);
+            stats[c] = float2{mo.m[0], r};
+            if (slice == 0 && mean && col < N) {
+                mean[col] = mo.m[0];
+                rstd[col] = r;
+            }
+        }
+        __syncthreads();
+    }
     float m[V], r[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float2 q = stats[(lane % np) * V + i];
+        const float2 q = stats[at - base + i];
         m[i] = q.x;
         r[i] = q.y;
     }
-    normalize<T, V>(x, w, b, y, m, r, k0, K, step, n, N);
+    while (k < k1) {
+        rows.store(y + at, m, r, k, k1, step, N);
+        k += U * step;
+        if (k < k1) rows.load(x + at, w, b, k, k1, step, N);
+    }
+}
+
+// Few tokens: a workgroup takes all rows of np columns.  Up to kHeld values a
+// thread stay in registers between the mean, the deviations and the result;
+// beyond that the rows are read again.
+constexpr int kSmallWaves = 16;
+constexpr int kHeld = 16;
+
+// sums of v over the lanes and waves with the same lane % np, for all of them
+__device__ __forceinline__ float sum_workgroup(float v, int np, float* red)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = 32; d >= np; d >>= 1) v += __shfl_xor(v, d, 64);
+    if (lane < np) red[wave * np + lane] = v;
+    __syncthreads();
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSmallWaves; ++w) all += red[w * np + lane % np];
+    __syncthreads();
+    return all;
+}
+
+template <typename T>
+__global__ __launch_bounds__(64 * kSmallWaves) void ln_small_kernel(const T* __restrict__ x, const T* __restrict__ w,
+                                                                    const T* __restrict__ b, float eps,
+                                                                    T* __restrict__ y, float* __restrict__ mean,
+                                                                    float* __restrict__ rstd, int32_t K, int64_t N,
+                                                                    int np)
+{
+    __shared__ float red[kSmallWaves * 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t n = (int64_t)blockIdx.x * np + lane % np;
+    const int32_t per = 64 / np, k0 = wave * per + lane / np, step = kSmallWaves * per;
+    const bool there = n < N;
+    float v[kHeld];
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+        const int64_t k = k0 + (int64_t)u * step;
+        v[u] = there && k < K ? (float)x[k * N + n] : 0.f;
+        sum += v[u];
+    }
+    const int64_t rest = k0 + (int64_t)kHeld * step;
+    if (there)
+        for (int64_t k = rest; k < K; k += step) sum += (float)x[k * N + n];
+    const float m = sum_workgroup(sum, np, red) / (float)K;
+    sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+        const float d = k0 + (int64_t)u * step < K ? v[u] - m : 0.f;
+        sum += d * d;
+    }
+    if (there)
+        for (int64_t k = rest; k < K; k += step) {
+            const float d = (float)x[k * N + n] - m;
+            sum += d * d;
+        }
+    const float r = rstd_of(sum_workgroup(sum, np, red), (float)K, eps);
+    if (!there) return;
+    if (mean && threadIdx.x < np) {
+        mean[n] = m;
+        rstd[n] = r;
+    }
+    auto put = [&](int64_t k, float xv) {
+        const float wk = w ? (float)w[k] : 1.f, bk = b ? (float)b[k] : 0.f;
+        y[k * N + n] = (T)((xv - m) * r * wk + bk);
+    };
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+        const int64_t k = k0 + (int64_t)u * step;
+        if (k < K) put(k, v[u]);
+    }
+    for (int64_t k = rest; k < K; k += step) put(k, (float)x[k * N + n]);
 }
 
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
 
+// The sums over a wave of eight values a lane: lane l returns sum l / 8.
+__device__ __forceinline__ float reduce_eight(const float (&q)[8], int lane)
+{
+    float h4[4], h2[2];
+    const bool b5 = lane & 32, b4 = lane & 16, b3 = lane & 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float mine = b5 ? q[4 + i] : q[i], give = b5 ? q[i] : q[4 + i];
+        h4[i] = mine + __shfl_xor(give, 32, 64);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float mine = b4 ? h4[2 + i] : h4[i], give = b4 ? h4[i] : h4[2 + i];
+        h2[i] = mine + __shfl_xor(give, 16, 64);
+    }
+    float v = (b3 ? h2[1] : h2[0]) + __shfl_xor(b3 ? h2[0] : h2[1], 8, 64);
+#pragma unroll
+    for (int d = 4; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
 // Sums of a slice and a tile: down the columns of g and g h (colpart
 // [slices][N]), along the rows of dy h and dy (rowpart [tiles][K]).
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kNormWaves) void ln_backward_sums_kernel(
+__global__ __launch_bounds__(64 * kBackwardWaves) void ln_backward_sums_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ w, const float* __restrict__ mean,
     const float* __restrict__ rstd, float2* __restrict__ colpart, float2* __restrict__ rowpart, int64_t K, int64_t N,
     NormShape h)
 {
-    __shared__ float2 red[kNormWaves * 64 * V];
+    __shared__ float2 red[kBackwardWaves * 64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t tile = blockIdx.x % h.tiles, slice = blockIdx.x / h.tiles;
-    const int64_t n = (tile * h.np + lane % h.np) * V;
+    const int64_t tile = blockIdx.x / h.slices, slice = blockIdx.x % h.slices;
+    const int64_t n = (tile * h.np + lane % h.np) * V, at = min(n, N - V);
     const int64_t k1 = min(K, (slice + 1) * h.len);
     const int per = 64 / h.np;
-    float m[V], r[V], c1[V], c2[V];
+    const auto m = load_tokens<float, V>(mean + at), r = load_tokens<float, V>(rstd + at);
+    float c1[V], c2[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) c1[i] = c2[i] = m[i] = r[i] = 0.f;
-    if (n < N) {
-        load_tokens<float, V>(m, mean, n, N);
-        load_tokens<float, V>(r, rstd, n, N);
-    }
-    // every lane of a wave makes the same rounds: rows are reduced across lanes
+    for (int i = 0; i < V; ++i) c1[i] = c2[i] = 0.f;
+    // whether every lane of the wave owns all its tokens
+    const bool whole = (tile + 1) * h.np * V <= N;
+    // Four rows at a time: their eight row sums are reduced across the np lanes
+    // together, lanes taking half of the remaining sums each (10 exchanges for
+    // np = 64 rather than 48).  Every lane of a wave makes the same rounds.
     const int64_t first = slice * h.len + wave * per;
-    for (int64_t kb = first; kb < k1; kb += kNormWaves * per) {
-        const int64_t k = kb + lane / h.np;
-        float a = 0.f, b = 0.f;
-        if (k < k1 && n < N) {
-            float g[V], v[V];
-            load_tokens<T, V>(g, dy + k * N, n, N);
-            load_tokens<T, V>(v, x + k * N, n, N);
-            const float wk = w ? (float)w[k] : 1.f;
+    const int64_t step = kBackwardWaves * per;
+    for (int64_t kb = first; kb < k1; kb += 4 * step) {
+        float q[8];  // sums of dy h of the four rows, then of dy
+        Pack<T, V> g[4], v[4];
+        T wt[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t k = min(kb + lane / h.np + u * step, k1 - 1);
+            g[u] = load_tokens<T, V>(dy + k * N + at);
+            v[u] = load_tokens<T, V>(x + k * N + at);
+            if (w) wt[u] = w[k];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool in = kb + lane / h.np + u * step < k1;
+            const float wk = !in ? 0.f : w ? (float)wt[u] : 1.f;
+            float a = 0.f, b = 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float hv = (v[i] - m[i]) * r[i];  // a token past the last has rstd 0 and dy 0
-                const float gh = g[i] * hv;
+                float gv = (float)g[u].v[i], gh = gv * ((float)v[u].v[i] - m.v[i]) * r.v[i];
+                if (!whole && !own(n, at, N, i)) gv = gh = 0.f;
                 a += gh;
-                b += g[i];
-                c1[i] += g[i] * wk;
-                c2[i] += gh * wk;
+                b += gv;
+                c1[i] += in ? gv * wk : 0.f;
+                c2[i] += in ? gh * wk : 0.f;
+            }
+            q[u] = a;
+            q[4 + u] = b;
+        }
+        if (h.np == 64) {
+            const float total = reduce_eight(q, lane);
+            // lane 8 i (bits 5, 4, 3 of the lane choose the sum) holds sum i
+            const int which = lane >> 3, u = which & 3;
+            const int64_t k = kb + u * step;
+            if ((lane & 7) == 0 && k < k1) {
+                float* o = reinterpret_cast<float*>(rowpart + tile * K + k);
+                o[which >> 2] = total;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float a = q[u], b = q[4 + u];
+                for (int d = h.np / 2; d > 0; d >>= 1) {
+                    a += __shfl_down(a, d, 64);
+                    b += __shfl_down(b, d, 64);
+                }
+                const int64_t k = kb + lane / h.np + u * step;
+                if (k < k1 && lane % h.np == 0) rowpart[tile * K + k] = float2{a, b};
             }
         }
-        for (int d = h.np / 2; d > 0; d >>= 1) {
-            a += __shfl_down(a, d, 64);
-            b += __shfl_down(b, d, 64);
-        }
-        if (k < k1 && lane % h.np == 0) rowpart[tile * K + k] = float2{a, b};
     }
     for (int d = h.np; d < 64; d <<= 1)
 #pragma unroll
@@ -308,77 +434,95 @@ __global__ __launch_bounds__(64 * kNormWaves) void ln_backward_sums_kernel(
     if (wave == 0 && lane < h.np)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            for (int q = 1; q < kNormWaves; ++q) {
+            for (int q = 1; q < kBackwardWaves; ++q) {
                 const float2 o = red[(q * h.np + lane) * V + i];
                 c1[i] += o.x;
                 c2[i] += o.y;
             }
-            if (n + i < N) colpart[slice * N + n + i] = float2{c1[i], c2[i]};
+            if (own(n, at, N, i)) colpart[slice * N + at + i] = float2{c1[i], c2[i]};
         }
 }
 
-// workgroups [0, ceil(N / 256)): a column's means; the rest: a row's sums
+// sum of p[i * ld], i < n, in order, eight loads at a time
+__device__ __forceinline__ float2 sum_strided(const float2* p, int64_t n, int64_t ld)
+{
+    float a = 0.f, b = 0.f;
+    for (int64_t i = 0; i < n; i += 8) {
+        float2 q[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) q[u] = p[min(i + u, n - 1) * ld];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            a += i + u < n ? q[u].x : 0.f;
+            b += i + u < n ? q[u].y : 0.f;
+        }
+    }
+    return {a, b};
+}
+
+// workgroups [0, ceil(N / 64)): a column's means; the rest: a row's sums
 template <typename T>
-__global__ __launch_bounds__(256) void ln_backward_join_kernel(const float2* __restrict__ colpart,
+__global__ __launch_bounds__(64) void ln_backward_join_kernel(const float2* __restrict__ colpart,
                                                                const float2* __restrict__ rowpart,
                                                                float2* __restrict__ means, T* __restrict__ dw,
                                                                T* __restrict__ db, int64_t K, int64_t N, NormShape h)
 {
-    const int64_t cols = (N + 255) / 256;
+    const int64_t cols = (N + 63) / 64;
     if (blockIdx.x < cols) {
-        const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        const int64_t n = (int64_t)blockIdx.x * 64 + threadIdx.x;
         if (n >= N) return;
-        float a = 0.f, b = 0.f;
-        for (int64_t s = 0; s < h.slices; ++s) {
-            const float2 p = colpart[s * N + n];
-            a += p.x;
-            b += p.y;
-        }
-        means[n] = float2{a / (float)K, b / (float)K};
+        const float2 p = sum_strided(colpart + n, h.slices, N);
+        means[n] = float2{p.x / (float)K, p.y / (float)K};
     } else {
-        const int64_t k = ((int64_t)blockIdx.x - cols) * 256 + threadIdx.x;
+        const int64_t k = ((int64_t)blockIdx.x - cols) * 64 + threadIdx.x;
         if (k >= K) return;
-        float a = 0.f, b = 0.f;
-        for (int64_t t = 0; t < h.tiles; ++t) {
-            const float2 p = rowpart[t * K + k];
-            a += p.x;
-            b += p.y;
-        }
-        if (dw) dw[k] = (T)a;
-        if (db) db[k] = (T)b;
+        const float2 p = sum_strided(rowpart + k, h.tiles, K);
+        if (dw) dw[k] = (T)p.x;
+        if (db) db[k] = (T)p.y;
     }
 }
 
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kNormWaves) void ln_backward_apply_kernel(
+__global__ __launch_bounds__(64 * kBackwardWaves) void ln_backward_apply_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ w, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float2* __restrict__ means, T* __restrict__ dx, int64_t K, int64_t N,
     NormShape h)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t tile = blockIdx.x % h.tiles, slice = blockIdx.x / h.tiles;
-    const int64_t n = (tile * h.np + lane % h.np) * V;
-    if (n >= N) return;
+    const int64_t tile = blockIdx.x / h.slices, slice = blockIdx.x % h.slices;
+    const int64_t at = min((tile * h.np + lane % h.np) * V, N - V);
     const int64_t k1 = min(K, (slice + 1) * h.len);
     const int per = 64 / h.np;
-    float m[V], r[V], c1[V], c2[V];
-    load_tokens<float, V>(m, mean, n, N);
-    load_tokens<float, V>(r, rstd, n, N);
+    const auto m = load_tokens<float, V>(mean + at), r = load_tokens<float, V>(rstd + at);
+    float c1[V], c2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float2 p = n + i < N ? means[n + i] : float2{0.f, 0.f};
+        const float2 p = means[at + i];
         c1[i] = p.x;
         c2[i] = p.y;
     }
-#pragma unroll 2
-    for (int64_t k = slice * h.len + wave * per + lane / h.np; k < k1; k += kNormWaves * per) {
-        float g[V], v[V];
-        load_tokens<T, V>(g, dy + k * N, n, N);
-        load_tokens<T, V>(v, x + k * N, n, N);
-        const float wk = w ? (float)w[k] : 1.f;
+    constexpr int U = 4;
+    const int64_t step = kBackwardWaves * per;
+    for (int64_t k = slice * h.len + wave * per + lane / h.np; k < k1; k += U * step) {
+        Pack<T, V> g[U], v[U];
+        T wt[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (g[i] * wk - c1[i] - (v[i] - m[i]) * r[i] * c2[i]) * r[i];
-        store_tokens<T, V>(dx + k * N, v, n, N);
+        for (int u = 0; u < U; ++u) {
+            const int64_t q = min(k + u * step, k1 - 1);
+            g[u] = load_tokens<T, V>(dy + q * N + at);
+            v[u] = load_tokens<T, V>(x + q * N + at);
+            if (w) wt[u] = w[q];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k + u * step >= k1) break;
+            const float wk = w ? (float)wt[u] : 1.f;
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                o[i] = ((float)g[u].v[i] * wk - c1[i] - ((float)v[u].v[i] - m.v[i]) * r.v[i] * c2[i]) * r.v[i];
+            store_tokens<T, V>(dx + (k + u * step) * N + at, o);
+        }
     }
 }
 
@@ -390,15 +534,15 @@ int pow2_at_least(int64_t n, int most)
 }
 
 // size: bytes of an element
-NormShape norm_shape(int64_t K, int64_t N, int v)
+NormShape norm_shape(int64_t K, int64_t N, int v, int np, int waves, int64_t groups)
 {
     NormShape h{1, v, 0, 0, 0};
     if (N == 0) return h;
-    h.np = pow2_at_least((N + v - 1) / v, 64);
+    h.np = pow2_at_least((N + v - 1) / v, np);
     h.tiles = (N + h.np * v - 1) / (h.np * v);
-    const int64_t rows = kNormWaves * (64 / h.np);  // a workgroup's rows at a time
-    // about 1024 workgroups of at least 8 rounds
-    int64_t slices = (1024 + h.tiles - 1) / h.tiles;
+    const int64_t rows = waves * (64 / h.np);  // a workgroup's rows at a time
+    // about `groups` workgroups of at least 8 rounds
+    int64_t slices = (groups + h.tiles - 1) / h.tiles;
     const int64_t most = (K + 8 * rows - 1) / (8 * rows);
     if (slices > most) slices = most;
     if (slices < 1) slices = 1;
@@ -407,8 +551,11 @@ NormShape norm_shape(int64_t K, int64_t N, int v)
     return h;
 }
 
-int forward_v(int64_t N) { return N >= 128 ? 2 : 1; }
-int backward_v(int64_t N) { return N >= 256 ? 4 : 1; }
+NormShape forward_shape(int64_t K, int64_t N, int64_t size) { return N < 64 ? norm_shape(K, N, 1, 64, kForwardWaves, 256) : norm_shape(K, N, (int)(16 / size), 16, kForwardWaves, 256); }
+NormShape backward_shape(int64_t K, int64_t N, int64_t size)
+{
+    return norm_shape(K, N, N < 256 ? 1 : (int)(16 / size), 64, kBackwardWaves, 512);
+}
 bool small_norm(int64_t K, int64_t N) { return K * N <= 65536 || N <= 16; }
 
 dim3 norm_grid(const NormShape& h)
@@ -420,22 +567,20 @@ dim3 norm_grid(const NormShape& h)
 
 }  // namespace ff
 
-int64_t layer_norm_scratch(int64_t K, int64_t N, int backward)
+int64_t layer_norm_scratch(int64_t K, int64_t N, int64_t size, int backward)
 {
     using namespace ff;
     if (K <= 0 || N <= 0) return 0;
     Carve c;
     if (backward) {
-        const NormShape h = norm_shape(K, N, backward_v(N));
+        const NormShape h = backward_shape(K, N, size);
         c.take((size_t)(h.slices * N) * 8);
         c.take((size_t)(h.tiles * K) * 8);
         c.take((size_t)N * 8);
     } else {
         if (small_norm(K, N)) return 0;
-        const NormShape h = norm_shape(K, N, forward_v(N));
+        const NormShape h = forward_shape(K, N, size);
         c.take((size_t)(h.slices * N) * 8);
-        c.take((size_t)N * 4);
-        c.take((size_t)N * 4);
     }
     return (int64_t)c.end;
 }
@@ -448,29 +593,22 @@ void layer_norm(const T* x, const T* weight, const T* bias, float eps, T* y, flo
     if (K == 0 || N == 0) return;
     if (small_norm(K, N)) {
         const int np = pow2_at_least(N, 8);
-        hipLaunchKernelGGL((ln_small_kernel<T, 1>), dim3((unsigned)((N + np - 1) / np)), dim3(64 * kSmallWaves), 0, s,
-                           x, weight, bias, eps, y, mean, rstd, K, N, np);
+        hipLaunchKernelGGL((ln_small_kernel<T>), dim3((unsigned)((N + np - 1) / np)), dim3(64 * kSmallWaves), 0, s, x,
+                           weight, bias, eps, y, mean, rstd, (int32_t)K, N, np);
         XSPMM_LAUNCH_CHECK();
         return;
     }
-    const NormShape h = norm_shape(K, N, forward_v(N));
-    char* p = static_cast<char*>(scratch);
-    Carve c;
-    float2* part = reinterpret_cast<float2*>(p + c.take((size_t)(h.slices * N) * 8));
-    float* m = reinterpret_cast<float*>(p + c.take((size_t)N * 4));
-    float* r = reinterpret_cast<float*>(p + c.take((size_t)N * 4));
-    if (mean) m = mean;
-    if (rstd) r = rstd;
+    const NormShape h = forward_shape(K, N, sizeof(T));
+    float2* part = static_cast<float2*>(scratch);
     auto go = [&](auto v) {
         constexpr int V = decltype(v)::value;
-        hipLaunchKernelGGL((ln_stats_kernel<T, V>), norm_grid(h), dim3(64 * kNormWaves), 0, s, x, part, K, N, h);
-        hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, part, m, r, K, N, h,
-                           eps);
-        hipLaunchKernelGGL((ln_apply_kernel<T, V>), norm_grid(h), dim3(64 * kNormWaves), 0, s, x, weight, bias, m, r,
-                           y, K, N, h);
+        hipLaunchKernelGGL((ln_stats_kernel<T, V>), norm_grid(h), dim3(64 * kForwardWaves), 0, s, x, part, K, N, h);
+        hipLaunchKernelGGL((ln_apply_kernel<T, V>), norm_grid(h), dim3(64 * kForwardWaves), 0, s, x, weight, bias, part,
+                           eps, mean, rstd, y, K, N, h);
     };
-    if (h.v == 2)
-        go(std::integral_constant<int, 2>{});
+    constexpr int most = 16 / sizeof(T);
+    if (h.v == most)
+        go(std::integral_constant<int, most>{});
     else
         go(std::integral_constant<int, 1>{});
     XSPMM_LAUNCH_CHECK();
@@ -482,7 +620,7 @@ void layer_norm_backward(const T* dy, const T* x, const T* weight, const float* 
 {
     using namespace ff;
     if (K == 0) return;
-    const NormShape h = norm_shape(K, N, backward_v(N));
+    const NormShape h = backward_shape(K, N, sizeof(T));
     char* p = static_cast<char*>(scratch);
     Carve c;
     float2* colpart = reinterpret_cast<float2*>(p + c.take((size_t)(h.slices * N) * 8));
@@ -491,16 +629,17 @@ void layer_norm_backward(const T* dy, const T* x, const T* weight, const float* 
     auto go = [&](auto v) {
         constexpr int V = decltype(v)::value;
         if (N > 0)
-            hipLaunchKernelGGL((ln_backward_sums_kernel<T, V>), norm_grid(h), dim3(64 * kNormWaves), 0, s, dy, x,
+            hipLaunchKernelGGL((ln_backward_sums_kernel<T, V>), norm_grid(h), dim3(64 * kBackwardWaves), 0, s, dy, x,
                                weight, mean, rstd, colpart, rowpart, K, N, h);
-        hipLaunchKernelGGL((ln_backward_join_kernel<T>), dim3((unsigned)((N + 255) / 256 + (K + 255) / 256)),
-                           dim3(256), 0, s, colpart, rowpart, means, dweight, dbias, K, N, h);
+        hipLaunchKernelGGL((ln_backward_join_kernel<T>), dim3((unsigned)((N + 63) / 64 + (K + 63) / 64)),
+                           dim3(64), 0, s, colpart, rowpart, means, dweight, dbias, K, N, h);
         if (N > 0 && dx)
-            hipLaunchKernelGGL((ln_backward_apply_kernel<T, V>), norm_grid(h), dim3(64 * kNormWaves), 0, s, dy, x,
+            hipLaunchKernelGGL((ln_backward_apply_kernel<T, V>), norm_grid(h), dim3(64 * kBackwardWaves), 0, s, dy, x,
                                weight, mean, rstd, means, dx, K, N, h);
     };
-    if (h.v == 4)
-        go(std::integral_constant<int, 4>{});
+    constexpr int most = 16 / sizeof(T);
+    if (h.v == most)
+        go(std::integral_constant<int, most>{});
     else
         go(std::integral_constant<int, 1>{});
     XSPMM_LAUNCH_CHECK();

@@ -40,7 +40,7 @@ def _prototypes(L):
         "xspmm_linear_backward": [p, i32, i32, p, p, p, p, p, p, p, i64, p, i64, p],
         "xspmm_gated_backward_scratch": [p, i32, i64, out],
         "xspmm_gated_backward": [p, p, i32, i32, p, p, p, p, p, p, p, p, p, p, p, i64, p, i64, p],
-        "xspmm_layer_norm_scratch": [i64, i64, i32, out],
+        "xspmm_layer_norm_scratch": [i32, i64, i64, i32, out],
         "xspmm_layer_norm": [i32, i64, i64, p, p, p, f32, p, p, p, p, i64, p],
         "xspmm_layer_norm_backward": [i32, i64, i64, p, p, p, p, p, p, p, p, p, i64, p],
     }.items():
@@ -319,7 +319,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, keep=False, out=None):
     rstd = torch.empty(N, dtype=torch.float32, device=dev) if keep else None
     n = C.c_int64(0)
     with _Here(dev) as stream:
-        rc = L.xspmm_layer_norm_scratch(K, N, 0, C.byref(n))
+        rc = L.xspmm_layer_norm_scratch(_TYPES[dt], K, N, 0, C.byref(n))
         if rc:
             X._check(rc)
         ws = _scratch(n.value, dev)
@@ -343,7 +343,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, need=(True, True, True)):
     db = torch.empty(K, dtype=dt, device=dev) if need[2] else None
     n = C.c_int64(0)
     with _Here(dev) as stream:
-        rc = L.xspmm_layer_norm_scratch(K, N, 1, C.byref(n))
+        rc = L.xspmm_layer_norm_scratch(_TYPES[dt], K, N, 1, C.byref(n))
         if rc:
             X._check(rc)
         ws = _scratch(n.value, dev)
