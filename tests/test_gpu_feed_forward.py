@@ -194,6 +194,22 @@ def test_gated_backward(kind, N, act):
         close(got, d.sum(1), (N + 2) * EPS32 * d.abs().sum(1) + o.sum(1) + u * d.sum(1).abs() + TINY, name)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(300, 290, 72), (300, 290, 67), (257, 600, 64), (600, 257, 200), (2100, 2060, 136),
+                                   (2100, 2060, 75), (3000, 1400, 8)])
+@pytest.mark.parametrize("density", [0.02, 0.3])
+def test_weight_gradient_tiles(kind, M, K, N, density):
+    """Several tiles of either size, ragged edges, tokens in whole chunks and not, sparse and denser tiles."""
+    dtype, u = TYPES[kind]
+    W, A, where = weight(M, K, density, dtype, N, empty_rows=(1,))
+    x, dy = normal((K, N), dtype, 1), normal((M, N), dtype, 2)
+    _, dv, _ = X.sparse_linear_backward(W, x, None, dy, need=(False, True))
+    want = at_blocks(f64(dy) @ f64(x).t(), where)
+    S = at_blocks(f64(dy).abs() @ f64(x).abs().t(), where)
+    close(dv, want, (N + 2) * EPS32 * S + u * want.abs() * 1.01 + TINY, "dvalues")
+    assert not dv.cpu()[~where[2].reshape(-1)].any()
+
+
 def test_wanted_gradients_only():
     W, _, _ = weight(64, 64, 0.5, torch.float16, 1)
     x, z, dy = (normal((64, 20), torch.float16, s) for s in (1, 2, 3))

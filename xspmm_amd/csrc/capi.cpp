@@ -643,7 +643,15 @@ int xspmm_linear_backward(xspmm_weight_t weight, int vtype, int act, const void*
                 t.N = N;
                 transposed_product<T>(t, 1, s);
             }
-            if (out_v) sampled_product<T>(w, d, xs, out_v, N, s);
+            if (out_v) {
+                SampledArgs<T> t{};
+                t.weight[0] = &w;
+                t.dz[0] = d;
+                t.x = xs;
+                t.dvals[0] = out_v;
+                t.N = N;
+                sampled_product<T>(t, 1, s);
+            }
         });
     });
 }
@@ -705,8 +713,18 @@ int xspmm_gated_backward(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int 
                 t.N = N;
                 transposed_product<T>(t, 2, s);
             }
-            if (out_g) sampled_product<T>(wg, dg, xs, out_g, N, s);
-            if (out_u) sampled_product<T>(wu, du, xs, out_u, N, s);
+            if (out_g || out_u) {
+                SampledArgs<T> t{};
+                t.weight[0] = &wg;
+                t.weight[1] = &wu;
+                t.dz[0] = dg;
+                t.dz[1] = du;
+                t.x = xs;
+                t.dvals[0] = out_g;
+                t.dvals[1] = out_u;
+                t.N = N;
+                sampled_product<T>(t, 2, s);
+            }
         });
     });
 }

@@ -24,6 +24,7 @@ struct BlockIndex {
     int32_t* tptr = nullptr;  // [Kb + 1]
     int32_t* trow = nullptr;  // [nnzb] block-rows by block-column, ascending
     int32_t* tblk = nullptr;  // [nnzb] and their positions in the BCSR order
+    int32_t* map = nullptr;   // [Mb * Kb] position of each block, or -1; null on large grids of few blocks
     void* memory = nullptr;   // the one allocation behind them
 
     BlockIndex() = default;
@@ -71,9 +72,26 @@ struct TransposedArgs {
 template <typename T>
 void transposed_product(const TransposedArgs<T>& a, int weights, hipStream_t s);
 
-// dvals = (dz x^T) at the stored blocks, zero past the edges of A
+// dvals_i = (dz_i x^T) at the stored blocks, zero past the edges of A_i; a null
+// dvals is not wanted
 template <typename T>
-void sampled_product(const BlockIndex& w, const T* dz, const T* x, T* dvals, int64_t N, hipStream_t s);
+struct SampledArgs {
+    const BlockIndex* weight[2];
+    const T* dz[2];
+    const T* x;
+    T* dvals[2];
+    int64_t N;
+};
+template <typename T>
+void sampled_product(const SampledArgs<T>& a, int weights, hipStream_t s);
+
+// Bytes of `rows` rows of N elements where those of whole blocks of rows stay
+// below 2^31, else -1.
+inline int64_t narrow_bytes(int64_t rows, int64_t N, int64_t size)
+{
+    const __int128 b = (__int128)((rows + 15) / 16 * 16) * N * size;
+    return b < ((int64_t)1 << 31) ? rows * N * size : -1;
+}
 
 // linear (up null): dz = dy act'(z);  gated: dz = dy up act'(z), dup = dy act(z).
 // dz / dup may be null (sums only).  bias sums over the tokens where not null.

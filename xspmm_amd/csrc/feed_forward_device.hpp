@@ -18,6 +18,11 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
+// Offset of what is not there: past the end of every buffer, and still so with
+// the offset of a row within a block added (operands of kernels that use it have
+// less than 2^31 bytes, rows past the last included).
+constexpr uint32_t kNone = 0x80000000u;
+
 constexpr int kXcds = 8;  // accelerator dies of an MI355X, each with its own L2
 
 template <typename T>
@@ -83,6 +88,34 @@ __device__ __forceinline__ Dwords<kDwords<T, VEC>> global_load(const T* p)
         for (int i = 0; i < kDwords<T, VEC>; ++i) o.d[i] = v.d[i];
     }
     return o;
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p)
+{
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// A load straight into LDS: lane l's 16 bytes at byte `off` of the buffer land at
+// LDS address lds + 16 l (zeros past its end).  The compiler does not see it:
+// dma_wait() before the barrier that lets the others read.
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4_t dma_buffer(const void* base, uint32_t bytes)
+{
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return i32x4_t{(int)(uint32_t)a, (int)(uint32_t)((a >> 32) & 0xffffu), (int)bytes, 0x00020000};
+}
+__device__ __forceinline__ void dma_to_lds(uint32_t lds, uint32_t off, i32x4_t buffer)
+{
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(off), "s"(buffer)
+                 : "memory", "m0");
+}
+// Until at most LEFT of this wave's loads, the latest ones, are under way.
+template <int LEFT>
+__device__ __forceinline__ void dma_wait()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
 }
 
 // D += A B of 16x16x32 16-bit values: lane l holds row (column) l % 16 of A

@@ -24,11 +24,6 @@ namespace detail {
 namespace ff {
 
 constexpr int kWaves = 4;
-// Offset of what is not there: past the end of every buffer, and still so
-// with the offset of a row within a block added (operands of narrow kernels
-// have less than 2^31 bytes, rows past the last included).
-constexpr uint32_t kNone = 0x80000000u;
-
 template <typename T>
 struct Side {
     const int32_t* ptr;
@@ -359,14 +354,6 @@ void launch_product(const ProductArgs<T>& a, int64_t blocks, bool wide, hipStrea
     }
 }
 
-// Bytes of `rows` rows of N elements, rows past the last of a block included;
-// -1 from 2^31 on.
-int64_t narrow_bytes(int64_t rows, int64_t N, int64_t size)
-{
-    const __int128 b = (__int128)((rows + 15) / 16 * 16) * N * size;
-    return b < ((int64_t)1 << 31) ? (int64_t)(rows * N * size) : -1;
-}
-
 }  // namespace ff
 
 template <typename T>
@@ -379,12 +366,12 @@ void feed_forward(const ForwardArgs<T>& f, int weights, hipStream_t s)
     for (int l = 0; l < weights; ++l) {
         const BlockIndex& wl = *f.weight[l];
         a.side[l] = {wl.ptr, wl.col, nullptr, f.vals[l], f.x, f.bias[l], f.keep[l]};
-        const int64_t vb = ff::narrow_bytes(wl.nnzb, 256, sizeof(T));
+        const int64_t vb = narrow_bytes(wl.nnzb, 256, sizeof(T));
         wide |= vb < 0;
         a.vals_bytes[l] = (uint32_t)vb;
         blocks += wl.nnzb;
     }
-    const int64_t xb = ff::narrow_bytes(w.K, f.N, sizeof(T));
+    const int64_t xb = narrow_bytes(w.K, f.N, sizeof(T));
     wide |= xb < 0;
     a.x_bytes = (uint32_t)xb;
     a.residual = f.residual;
@@ -411,12 +398,12 @@ void transposed_product(const TransposedArgs<T>& t, int weights, hipStream_t s)
     for (int l = 0; l < weights; ++l) {
         const BlockIndex& wl = *t.weight[l];
         a.side[l] = {wl.tptr, wl.trow, wl.tblk, t.vals[l], t.dz[l], nullptr, nullptr};
-        const int64_t vb = ff::narrow_bytes(wl.nnzb, 256, sizeof(T));
+        const int64_t vb = narrow_bytes(wl.nnzb, 256, sizeof(T));
         wide |= vb < 0;
         a.vals_bytes[l] = (uint32_t)vb;
         blocks += wl.nnzb;
     }
-    const int64_t xb = ff::narrow_bytes(w.M, t.N, sizeof(T));
+    const int64_t xb = narrow_bytes(w.M, t.N, sizeof(T));
     wide |= xb < 0;
     a.x_bytes = (uint32_t)xb;
     a.y = t.dx;

@@ -37,7 +37,7 @@ template <typename I>
 __global__ __launch_bounds__(256) void ff_check_col_kernel(const int32_t* __restrict__ ptr, const I* __restrict__ bci,
                                                            int64_t Mb, int64_t Kb, const int* bad_in,
                                                            int32_t* __restrict__ col, int32_t* __restrict__ row,
-                                                           int* bad)
+                                                           int32_t* __restrict__ map, int* bad)
 {
     if (*bad_in & kBadPtr) return;
     const int64_t br = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
@@ -49,6 +49,7 @@ __global__ __launch_bounds__(256) void ff_check_col_kernel(const int32_t* __rest
         if (!ok) atomicOr(bad, kBadCol);
         col[b] = ok ? (int32_t)c : 0;
         row[b] = (int32_t)br;
+        if (map && ok) map[br * Kb + c] = b;
     }
 }
 
@@ -112,7 +113,14 @@ __global__ __launch_bounds__(kScanThreads) void ff_scan_kernel(int32_t* __restri
     }
 }
 
-__global__ void ff_clear_kernel(int* p) { *p = 0; }
+__global__ __launch_bounds__(256) void ff_fill_kernel(int32_t* __restrict__ p, int64_t n, int32_t v)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = v;
+}
+
+// The tile kernels' map costs 4 bytes for every block of the grid, stored or
+// not: worth it up to 64 MB where at least one block in 64 is stored.
+bool wants_map(int64_t Mb, int64_t Kb, int64_t nnzb) { return Mb * Kb <= (1 << 24) && nnzb * 64 >= Mb * Kb && nnzb > 0; }
 
 }  // namespace
 
@@ -138,6 +146,8 @@ void build_block_index(BlockIndex& out, int64_t M, int64_t K, int64_t Mb, int64_
     const size_t o_col = c.take((size_t)nnzb * 4), o_row = c.take((size_t)nnzb * 4);
     const size_t o_trow = c.take((size_t)nnzb * 4), o_tblk = c.take((size_t)nnzb * 4);
     const size_t o_bad = c.take(4);
+    const bool map = wants_map(Mb, Kb, nnzb);
+    const size_t o_map = c.take(map ? (size_t)(Mb * Kb) * 4 : 0);
     XSPMM_HIP_CHECK(hipMalloc(&out.memory, c.end));
     char* p = static_cast<char*>(out.memory);
     out.ptr = reinterpret_cast<int32_t*>(p + o_ptr);
@@ -146,14 +156,17 @@ void build_block_index(BlockIndex& out, int64_t M, int64_t K, int64_t Mb, int64_
     out.row = reinterpret_cast<int32_t*>(p + o_row);
     out.trow = reinterpret_cast<int32_t*>(p + o_trow);
     out.tblk = reinterpret_cast<int32_t*>(p + o_tblk);
+    if (map) out.map = reinterpret_cast<int32_t*>(p + o_map);
     int* bad = reinterpret_cast<int*>(p + o_bad);
 
     auto groups = [](int64_t n, int64_t per) { return dim3((unsigned)((n + per - 1) / per)); };
-    hipLaunchKernelGGL(ff_clear_kernel, dim3(1), dim3(1), 0, s, bad);
+    hipLaunchKernelGGL(ff_fill_kernel, dim3(1), dim3(256), 0, s, bad, (int64_t)1, 0);
+    if (map)
+        hipLaunchKernelGGL(ff_fill_kernel, dim3(1024), dim3(256), 0, s, out.map, Mb * Kb, -1);
     hipLaunchKernelGGL((ff_check_ptr_kernel<I>), groups(Mb + 1, 256), dim3(256), 0, s, brp, Mb, nnzb, out.ptr, bad);
     if (Mb > 0)
         hipLaunchKernelGGL((ff_check_col_kernel<I>), groups(Mb, 4), dim3(256), 0, s, out.ptr, bci, Mb, Kb, bad,
-                           out.col, out.row, bad);
+                           out.col, out.row, out.map, bad);
     if (Kb > 0)
         hipLaunchKernelGGL((ff_transpose_kernel<false>), groups(Kb, 4), dim3(256), 0, s, out.ptr, out.col, Mb, Kb,
                            bad, out.tptr, nullptr, nullptr, nullptr);
