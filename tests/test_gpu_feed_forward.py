@@ -169,7 +169,7 @@ def test_linear_backward(kind, N, act):
 
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("N", [1, 40, 131])
-@pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu_tanh"])
 def test_gated_backward(kind, N, act):
     dtype, u = TYPES[kind]
     M, K = 101, 140
@@ -208,6 +208,40 @@ def test_weight_gradient_tiles(kind, M, K, N, density):
     S = at_blocks(f64(dy).abs() @ f64(x).abs().t(), where)
     close(dv, want, (N + 2) * EPS32 * S + u * want.abs() * 1.01 + TINY, "dvalues")
     assert not dv.cpu()[~where[2].reshape(-1)].any()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(300, 290, 136), (290, 300, 131), (64, 2100, 128), (2100, 64, 264), (1100, 1300, 200),
+                                   (700, 90, 257)])
+@pytest.mark.parametrize("density", [0.2, 0.6, 1.0])
+def test_product_tiles(kind, M, K, N, density):
+    """Sizes at which several tiles meet: more block-columns than a window of positions, one and two of a pair of
+    blocks stored, ragged edges, tokens in whole chunks and not."""
+    dtype, u = TYPES[kind]
+    G, Ga, _ = weight(M, K, density, dtype, N, empty_rows=(1,))
+    U, Ua, _ = weight(M, K, density / 2, dtype, N + 1, empty_rows=(0,))
+    x, dy, b, r = normal((K, N), dtype, 1), normal((M, N), dtype, 2), normal((M,), dtype, 3), normal((M, N), dtype, 4)
+    y, z = X.sparse_linear(G, x, bias=b, activation="relu", residual=r, keep=True)
+    z64 = Ga @ f64(x) + f64(b)[:, None]
+    err = (K + 2) * EPS32 * (Ga.abs() @ f64(x).abs() + f64(b).abs()[:, None])
+    close(z, z64, err + u * z64.abs() + TINY, "kept")
+    y64 = z64.clamp(min=0) + f64(r)
+    close(y, y64, err + 4 * EPS32 * f64(r).abs() + u * y64.abs() * 1.01 + TINY, "y")
+    h, zg, zu = X.sparse_gated(G, U, x, None, b, activation="none", keep=True)
+    g64, u64 = Ga @ f64(x), Ua @ f64(x) + f64(b)[:, None]
+    eu = (K + 2) * EPS32 * (Ua.abs() @ f64(x).abs() + f64(b).abs()[:, None])
+    close(zg, g64, err + u * g64.abs() + TINY, "gate")
+    close(zu, u64, eu + u * u64.abs() + TINY, "up")
+    close(h, g64 * u64, err * (u64.abs() + eu) + g64.abs() * eu + u * (g64 * u64).abs() * 1.01 + TINY, "h")
+    dx, _, _ = X.sparse_linear_backward(G, x, None, dy, need=(True, False))
+    want = Ga.t() @ f64(dy)
+    close(dx, want, (M + 2) * EPS32 * (Ga.abs().t() @ f64(dy).abs()) + u * want.abs() * 1.01 + TINY, "dx")
+    one = torch.ones_like(dy)
+    dx = X.sparse_gated_backward(G, U, x, one, dy, dy, activation="none", need=(True, False, False))[0]
+    g = (f64(dy) ** 2).to(dtype).double()
+    want = Ga.t() @ g + Ua.t() @ f64(dy)
+    S = Ga.abs().t() @ g + Ua.abs().t() @ f64(dy).abs()
+    close(dx, want, (2 * M + 2) * EPS32 * S + 2 * u * (Ga.abs().t() @ g) + u * want.abs() * 1.01 + TINY, "gated dx")
 
 
 def test_wanted_gradients_only():
@@ -277,7 +311,7 @@ def test_no_blocks_and_no_tokens(kind):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("N", [1, 5, 33, 140])
+@pytest.mark.parametrize("N", [1, 5, 33, 136, 141])
 def test_what_is_not_finite_stays_in_its_token(kind, N):
     """Inf and NaN reach the results of their own token and of the rows whose blocks read them, no others;
     rows past the last of a ragged weight read nothing."""

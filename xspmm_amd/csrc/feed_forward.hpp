@@ -72,6 +72,12 @@ struct TransposedArgs {
 template <typename T>
 void transposed_product(const TransposedArgs<T>& a, int weights, hipStream_t s);
 
+// The same by tiles, for 16-bit values: false where that does not apply or pay.
+template <typename T>
+bool feed_forward_tiles(const ForwardArgs<T>& a, int weights, hipStream_t s);
+template <typename T>
+bool transposed_tiles(const TransposedArgs<T>& a, int weights, hipStream_t s);
+
 // dvals_i = (dz_i x^T) at the stored blocks, zero past the edges of A_i; a null
 // dvals is not wanted
 template <typename T>

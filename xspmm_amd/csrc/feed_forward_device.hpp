@@ -15,6 +15,8 @@ namespace ff {
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
@@ -129,6 +131,18 @@ __device__ __forceinline__ float4_t mfma16(u32x4_t a, u32x4_t b, float4_t c)
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                        __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// D += A B of 16x16x16 16-bit values: as above, at k = 4 (l / 16) .. + 3.
+template <typename T>
+__device__ __forceinline__ float4_t mfma16_half(u32x2_t a, u32x2_t b, float4_t c)
+{
+    if constexpr (__is_same(T, _Float16))
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4_t, a), __builtin_bit_cast(half4_t, b), c,
+                                                     0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_t, a),
+                                                         __builtin_bit_cast(short4_t, b), c, 0, 0, 0);
 }
 
 // D += A B of 16x16x4 fp32 values: lane l holds row (column) l % 16 at k = l / 16.

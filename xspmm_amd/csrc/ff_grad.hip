@@ -25,6 +25,7 @@ __global__ __launch_bounds__(256) void ff_act_backward_kernel(const T* __restric
                                                               T* __restrict__ dbias_up, int64_t M, int64_t N)
 {
     constexpr int V = 16 / sizeof(T);
+    constexpr bool kReads = GATED || ACT != kActNone;  // z
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
     if (row >= M) return;
@@ -42,12 +43,12 @@ __global__ __launch_bounds__(256) void ff_act_backward_kernel(const T* __restric
         if (n + V <= N) {
             const auto g = *reinterpret_cast<const Pack<T, V>*>(dy + at + n);
             Pack<T, V> zz, uu, o, ou;
-            if (ACT != kActNone) zz = *reinterpret_cast<const Pack<T, V>*>(z + at + n);
+            if (kReads) zz = *reinterpret_cast<const Pack<T, V>*>(z + at + n);
             if (GATED) uu = *reinterpret_cast<const Pack<T, V>*>(up + at + n);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float a, b;
-                one(ACT != kActNone ? (float)zz.v[i] : 0.f, GATED ? (float)uu.v[i] : 0.f, (float)g.v[i], a, b);
+                one(kReads ? (float)zz.v[i] : 0.f, GATED ? (float)uu.v[i] : 0.f, (float)g.v[i], a, b);
                 o.v[i] = (T)a;
                 ou.v[i] = (T)b;
             }
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(256) void ff_act_backward_kernel(const T* __restric
         } else {
             for (int64_t m = n; m < N; ++m) {
                 float a, b;
-                one(ACT != kActNone ? (float)z[at + m] : 0.f, GATED ? (float)up[at + m] : 0.f, (float)dy[at + m], a, b);
+                one(kReads ? (float)z[at + m] : 0.f, GATED ? (float)up[at + m] : 0.f, (float)dy[at + m], a, b);
                 if (dz) dz[at + m] = (T)a;
                 if (GATED) dup[at + m] = (T)b;
             }

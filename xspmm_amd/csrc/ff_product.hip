@@ -359,6 +359,8 @@ void launch_product(const ProductArgs<T>& a, int64_t blocks, bool wide, hipStrea
 template <typename T>
 void feed_forward(const ForwardArgs<T>& f, int weights, hipStream_t s)
 {
+    if constexpr (!ff::is_f32<T>)
+        if (feed_forward_tiles<T>(f, weights, s)) return;
     const BlockIndex& w = *f.weight[0];
     ff::ProductArgs<T> a{};
     int64_t blocks = 0;
@@ -391,6 +393,8 @@ void feed_forward(const ForwardArgs<T>& f, int weights, hipStream_t s)
 template <typename T>
 void transposed_product(const TransposedArgs<T>& t, int weights, hipStream_t s)
 {
+    if constexpr (!ff::is_f32<T>)
+        if (transposed_tiles<T>(t, weights, s)) return;
     const BlockIndex& w = *t.weight[0];
     ff::ProductArgs<T> a{};
     int64_t blocks = 0;
