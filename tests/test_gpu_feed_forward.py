@@ -194,7 +194,7 @@ def test_gated_backward(kind, N, act):
         close(got, d.sum(1), (N + 2) * EPS32 * d.abs().sum(1) + o.sum(1) + u * d.sum(1).abs() + TINY, name)
 
 
-@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("M,K,N", [(300, 290, 72), (300, 290, 67), (257, 600, 64), (600, 257, 200), (2100, 2060, 136),
                                    (2100, 2060, 75), (3000, 1400, 8)])
 @pytest.mark.parametrize("density", [0.02, 0.3])

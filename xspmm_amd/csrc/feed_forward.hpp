@@ -21,6 +21,8 @@ struct BlockIndex {
     int32_t* ptr = nullptr;   // [Mb + 1]
     int32_t* col = nullptr;   // [nnzb]
     int32_t* row = nullptr;   // [nnzb] block-row of each block
+    int64_t groups = 0;
+    int32_t* group = nullptr; // [groups] first blocks of runs of up to 4 within a block-row
     int32_t* tptr = nullptr;  // [Kb + 1]
     int32_t* trow = nullptr;  // [nnzb] block-rows by block-column, ascending
     int32_t* tblk = nullptr;  // [nnzb] and their positions in the BCSR order
@@ -34,6 +36,8 @@ struct BlockIndex {
         if (memory) (void)hipFree(memory);
     }
 };
+
+constexpr int kGroupBlocks = 4;
 
 // Fills `out` from BCSR arrays on the device; synchronizes `s`.  Throws
 // std::invalid_argument where they are no BCSR matrix with strictly ascending

@@ -57,7 +57,9 @@ struct Step {
     Dwords<kDwords<T, VEC>> b[kRows];
 };
 
-template <typename T, int VEC, bool TR, bool WIDE>
+// ONE: a single token, whose rows of x are consecutive: one load has them all, and
+// the 16 columns of the instruction compute the same.
+template <typename T, int VEC, bool TR, bool WIDE, bool ONE>
 struct Walk {
     static constexpr int kRows = Step<T, VEC>::kRows;
     static constexpr int kPer = is_f32<T> ? 1 : 2;  // blocks per step
@@ -109,6 +111,10 @@ struct Walk {
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) put(st, i, buffer_load<T, 1>(vr, a0 + (uint32_t)((sub + i) * 16 + li) * (uint32_t)sizeof(T)).d[0]);
             }
+            if constexpr (ONE) {
+                load_one(st, row, absent);
+                return;
+            }
             const uint32_t ld = (uint32_t)N * (uint32_t)sizeof(T);
             const uint32_t x0 = absent ? kNone : (uint32_t)row * ld + (uint32_t)n * (uint32_t)sizeof(T);
             if (!cut) {
@@ -145,6 +151,30 @@ struct Walk {
         }
     }
 
+    // x has one column: the lane's rows in one load (in parts at the edge, as a
+    // load past the end gives whole dwords of zeros)
+    __device__ __forceinline__ void load_one(Step<T, VEC>& st, int32_t row, bool absent) const
+    {
+        uint32_t d[4] = {0u, 0u, 0u, 0u};
+        if (row + kRows <= in_rows || absent) {
+            const auto v = buffer_load<float, 4>(xr, absent ? kNone : (uint32_t)row * (uint32_t)sizeof(T));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] = v.d[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const uint32_t v =
+                    buffer_load<T, 1>(xr, row + i < in_rows ? (uint32_t)(row + i) * (uint32_t)sizeof(T) : kNone).d[0];
+                if constexpr (is_f32<T>)
+                    d[i] = v;
+                else
+                    d[i / 2] |= v << (16 * (i % 2));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.b[i].d[0] = d[i];
+    }
+
     // element i of a lane's values of A
     static __device__ __forceinline__ void put(Step<T, VEC>& st, int i, uint32_t v)
     {
@@ -163,6 +193,10 @@ struct Walk {
                 for (int i = 0; i < 4; ++i) acc[c] = mfma32(st.a[i], st.b[i].d[c], acc[c]);
         } else {
             const u32x4_t a = {st.a[0], st.a[1], st.a[2], st.a[3]};
+            if constexpr (ONE) {
+                acc[0] = mfma16<T>(a, u32x4_t{st.b[0].d[0], st.b[1].d[0], st.b[2].d[0], st.b[3].d[0]}, acc[0]);
+                return;
+            }
 #pragma unroll
             for (int c = 0; c < VEC; ++c) {
                 u32x4_t v;
@@ -175,31 +209,90 @@ struct Walk {
         }
     }
 
-    // acc += blocks [b, end) times x: the loads of a step run ahead of the
+    // acc += blocks [b, end) times x: the loads of kAhead steps run ahead of the
     // instructions of the step before
+    static constexpr int kAhead = ONE ? 4 : VEC <= 2 ? 3 : 2;
     __device__ __forceinline__ void run(float4_t (&acc)[VEC], int32_t b, int32_t end) const
     {
         if (b >= end) return;
         const int32_t last = end - 1 - (kPer == 2 ? (end - 1 - b) % 2 : 0);
-        Step<T, VEC> s0, s1;
-        load(s0, b, end);
-        for (; b < end; b += 2 * kPer) {
-            load(s1, b + kPer < last ? b + kPer : last, end);
-            multiply(acc, s0);
-            if (b + kPer >= end) break;
-            load(s0, b + 2 * kPer < last ? b + 2 * kPer : last, end);
-            multiply(acc, s1);
+        Step<T, VEC> s[kAhead];
+#pragma unroll
+        for (int p = 0; p + 1 < kAhead; ++p) load(s[p], b + p * kPer < last ? b + p * kPer : last, end);
+        for (; b < end; b += kAhead * kPer) {
+#pragma unroll
+            for (int p = 0; p < kAhead; ++p) {
+                const int32_t next = b + (p + kAhead - 1) * kPer;
+                load(s[(p + kAhead - 1) % kAhead], next < last ? next : last, end);
+                multiply(acc, s[p]);
+                if (b + (p + 1) * kPer >= end) return;
+            }
         }
     }
 };
 
-// NACC accumulators: 2 for the gated forward product.  SPLIT waves share a
-// block-row's blocks and add up in LDS, in their order.
-template <typename T, int VEC, int NACC, bool TR, int SPLIT, bool WIDE>
-__global__ __launch_bounds__(64 * kWaves) void ff_product_kernel(const ProductArgs<T> a)
+// The result's rows 4 (l / 16) + q of a wave's block-row and the lane's VEC tokens
+template <typename T, int VEC, int NACC, bool TR>
+__device__ __forceinline__ void finish(const ProductArgs<T>& a, float (&z)[NACC][VEC], int64_t row, int64_t n,
+                                       int64_t first, int64_t end)
 {
-    constexpr int kRowsPerGroup = kWaves / SPLIT;
-    constexpr int kTile = 16 * VEC;
+    const bool whole = n >= first && n + VEC <= end;
+    auto store = [&](T* p, const float(&v)[VEC]) {
+        if (whole) {
+            Pack<T, VEC> o;
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) o.v[c] = (T)v[c];
+            *reinterpret_cast<Pack<T, VEC>*>(p + row * a.N + n) = o;
+        } else {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c)
+                if (n + c >= first && n + c < end) p[row * a.N + n + c] = (T)v[c];
+        }
+    };
+    if constexpr (!TR) {
+        float r[VEC];
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) r[c] = 0.f;
+        if (a.residual) {
+            if (whole) {
+                const Pack<T, VEC> k = *reinterpret_cast<const Pack<T, VEC>*>(a.residual + row * a.N + n);
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) r[c] = (float)k.v[c];
+            } else {
+#pragma unroll
+                for (int c = 0; c < VEC; ++c)
+                    if (n + c >= first && n + c < end) r[c] = (float)a.residual[row * a.N + n + c];
+            }
+        }
+#pragma unroll
+        for (int l = 0; l < NACC; ++l) {
+            const float bias = a.side[l].bias ? (float)a.side[l].bias[row] : 0.f;
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) z[l][c] += bias;
+            if (a.side[l].keep) store(a.side[l].keep, z[l]);
+        }
+        with_act(a.act, [&](auto act) {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) z[0][c] = act_value<decltype(act)::value>(z[0][c]);
+        });
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+            if constexpr (NACC == 2) z[0][c] *= z[1][c];
+            z[0][c] += r[c];
+        }
+    }
+    store(a.y, z[0]);
+}
+
+// NACC accumulators: 2 for the gated forward product.  SPLIT waves share a
+// block-row's blocks and add up in LDS, in their order; four of them then finish
+// a quarter of its rows each.
+template <typename T, int VEC, int NACC, bool TR, int SPLIT, bool WIDE, bool ONE>
+__global__ __launch_bounds__(64 * (SPLIT > kWaves ? SPLIT : kWaves)) void ff_product_kernel(const ProductArgs<T> a)
+{
+    constexpr int kRowsPerGroup = SPLIT > kWaves ? 1 : kWaves / SPLIT;
+    constexpr int kTile = ONE ? 1 : 16 * VEC;
+    using W = Walk<T, VEC, TR, WIDE, ONE>;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t groups = (a.block_rows + kRowsPerGroup - 1) / kRowsPerGroup;
@@ -211,7 +304,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_product_kernel(const ProductAr
     const int64_t first = item / groups * kTile;  // the tile's first token
     // the last tile moves back into the matrix (and stores its own tokens only)
     const int64_t n0 = first + kTile > a.N && a.N >= kTile ? a.N - kTile : first;
-    const int64_t n = n0 + VEC * (lane & 15);
+    const int64_t n = ONE ? lane & 15 : n0 + VEC * (lane & 15);
 
     float4_t acc[NACC][VEC];
 #pragma unroll
@@ -220,9 +313,9 @@ __global__ __launch_bounds__(64 * kWaves) void ff_product_kernel(const ProductAr
         for (int c = 0; c < VEC; ++c) acc[l][c] = float4_t{0.f, 0.f, 0.f, 0.f};
     if (br < a.block_rows) {
         auto side = [&](int l, float4_t(&to)[VEC]) {
-            const Walk<T, VEC, TR, WIDE> w(a, l, n, lane);
+            const W w(a, l, n, lane);
             const int32_t b = a.side[l].ptr[br], e = a.side[l].ptr[br + 1];
-            constexpr int per = Walk<T, VEC, TR, WIDE>::kPer;
+            constexpr int per = W::kPer;
             const int32_t steps = (e - b + per - 1) / per;
             const int32_t lo = b + per * (int32_t)((int64_t)steps * part / SPLIT);
             const int32_t hi = b + per * (int32_t)((int64_t)steps * (part + 1) / SPLIT);
@@ -234,95 +327,64 @@ __global__ __launch_bounds__(64 * kWaves) void ff_product_kernel(const ProductAr
         else if (a.sides == 2)
             side(1, acc[0]);
     }
+    const int64_t row0 = 16 * (int64_t)br + 4 * (lane >> 4);
+    float z[NACC][VEC];
     if constexpr (SPLIT > 1) {
-        __shared__ float4_t red[kRowsPerGroup][SPLIT - 1][NACC][VEC][64];
-        if (part > 0) {
+        __shared__ float red[kRowsPerGroup][SPLIT][NACC][VEC][4][64];
 #pragma unroll
-            for (int l = 0; l < NACC; ++l)
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) red[wave / SPLIT][part - 1][l][c][lane] = acc[l][c];
-        }
-        __syncthreads();
-        if (part > 0) return;
-        for (int p = 0; p < SPLIT - 1; ++p)
-#pragma unroll
-            for (int l = 0; l < NACC; ++l)
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) acc[l][c] += red[wave / SPLIT][p][l][c][lane];
-    }
-    if (br >= a.block_rows) return;
-
-    // lane l: rows 4 (l / 16) + q of the block-row, its VEC tokens
-    const bool whole = n >= first && n + VEC <= a.N;
-    const bool any = n + VEC > first && n < a.N;
-    if (!any) return;
-    auto store = [&](T* p, const float(&v)[VEC], int64_t row) {
-        if (whole) {
-            Pack<T, VEC> o;
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) o.v[c] = (T)v[c];
-            *reinterpret_cast<Pack<T, VEC>*>(p + row * a.N + n) = o;
-        } else {
+        for (int l = 0; l < NACC; ++l)
 #pragma unroll
             for (int c = 0; c < VEC; ++c)
-                if (n + c >= first && n + c < a.N) p[row * a.N + n + c] = (T)v[c];
-        }
-    };
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int64_t row = 16 * (int64_t)br + 4 * (lane >> 4) + q;
-        if (row >= a.rows) continue;
-        float z[NACC][VEC];
+                for (int q = 0; q < 4; ++q) red[wave / SPLIT][part][l][c][q][lane] = acc[l][c][q];
+        __syncthreads();
+        if (part >= 4) return;
 #pragma unroll
-        for (int l = 0; l < NACC; ++l) {
-            const float bias = !TR && a.side[l].bias ? (float)a.side[l].bias[row] : 0.f;
+        for (int l = 0; l < NACC; ++l)
 #pragma unroll
-            for (int c = 0; c < VEC; ++c) z[l][c] = TR ? acc[l][c][q] : acc[l][c][q] + bias;
-            if (!TR && a.side[l].keep) store(a.side[l].keep, z[l], row);
-        }
-        if constexpr (!TR) {
-            with_act(a.act, [&](auto act) {
+            for (int c = 0; c < VEC; ++c) {
+                z[l][c] = 0.f;
 #pragma unroll
-                for (int c = 0; c < VEC; ++c) z[0][c] = act_value<decltype(act)::value>(z[0][c]);
-            });
-            if constexpr (NACC == 2)
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) z[0][c] *= z[1][c];
-            if (a.residual) {
-                if (whole) {
-                    const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(a.residual + row * a.N + n);
-#pragma unroll
-                    for (int c = 0; c < VEC; ++c) z[0][c] += (float)r.v[c];
-                } else {
-#pragma unroll
-                    for (int c = 0; c < VEC; ++c)
-                        if (n + c >= first && n + c < a.N) z[0][c] += (float)a.residual[row * a.N + n + c];
-                }
+                for (int p = 0; p < SPLIT; ++p) z[l][c] += red[wave / SPLIT][p][l][c][part][lane];
             }
+        if (row0 + part < a.rows && n + VEC > first && n < a.N)
+            finish<T, VEC, NACC, TR>(a, z, row0 + part, n, first, a.N);
+    } else {
+        if (n + VEC <= first || n >= a.N) return;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (row0 + q >= a.rows) break;
+#pragma unroll
+            for (int l = 0; l < NACC; ++l)
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) z[l][c] = acc[l][c][q];
+            finish<T, VEC, NACC, TR>(a, z, row0 + q, n, first, a.N);
         }
-        store(a.y, z[0], row);
     }
 }
 
-template <typename T, int VEC, int NACC, bool TR, int SPLIT, bool WIDE>
+template <typename T, int VEC, int NACC, bool TR, int SPLIT, bool WIDE, bool ONE = false>
 void launch(const ProductArgs<T>& a, hipStream_t s)
 {
-    constexpr int rows = kWaves / SPLIT;
-    const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + 16 * VEC - 1) / (16 * VEC));
+    constexpr int rows = SPLIT > kWaves ? 1 : kWaves / SPLIT, threads = 64 * (SPLIT > kWaves ? SPLIT : kWaves);
+    constexpr int tile = ONE ? 1 : 16 * VEC;
+    const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + tile - 1) / tile);
     const int64_t grid = kXcds * xcd_chunk(items);
     if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many tokens for one launch.");
-    hipLaunchKernelGGL((ff_product_kernel<T, VEC, NACC, TR, SPLIT, WIDE>), dim3((unsigned)grid), dim3(64 * kWaves), 0,
+    hipLaunchKernelGGL((ff_product_kernel<T, VEC, NACC, TR, SPLIT, WIDE, ONE>), dim3((unsigned)grid), dim3(threads), 0,
                        s, a);
     XSPMM_LAUNCH_CHECK();
 }
 
-template <typename T, int VEC, int NACC, bool TR, bool WIDE>
+template <typename T, int VEC, int NACC, bool TR>
 void launch_split(const ProductArgs<T>& a, int split, hipStream_t s)
 {
-    if (split == 4)
-        launch<T, VEC, NACC, TR, 4, WIDE>(a, s);
-    else
-        launch<T, VEC, NACC, TR, 1, WIDE>(a, s);
+    if (split == 1)
+        launch<T, VEC, NACC, TR, 1, false>(a, s);
+    else if (split == 4 || VEC > 2)
+        launch<T, VEC, NACC, TR, 4, false>(a, s);
+    else if constexpr (VEC <= 2)
+        launch<T, VEC, NACC, TR, 16, false>(a, s);
 }
 
 template <typename T, int NACC, bool TR>
@@ -332,25 +394,38 @@ void launch_product(const ProductArgs<T>& a, int64_t blocks, bool wide, hipStrea
     constexpr int most = is_f32<T> ? 4 : 8;
     int vec = most;
     while (vec > 1 && 16 * vec > a.N) vec /= 2;
-    auto waves = [&](int v) { return (int64_t)a.block_rows * ((a.N + 16 * v - 1) / (16 * v)); };
-    while (vec > 4 && waves(vec) < 2048) vec /= 2;
-    const int split = waves(vec) < 2048 && blocks >= 8 * a.block_rows ? 4 : 1;
     if (wide) {
         if (vec == 1)
-            launch_split<T, 1, NACC, TR, true>(a, split, s);
+            launch<T, 1, NACC, TR, 4, true>(a, s);
         else if (a.N >= 64)
-            launch_split<T, 4, NACC, TR, true>(a, split, s);
+            launch<T, 4, NACC, TR, 1, true>(a, s);
         else
-            launch_split<T, 2, NACC, TR, true>(a, split, s);
+            launch<T, 2, NACC, TR, 4, true>(a, s);
+        return;
+    }
+    // Wide tiles while they leave enough waves for the chip, with four waves to a
+    // block-row if need be (8192 x 8192, 5 % of the blocks, 256 tokens: 14.1 us with
+    // 8 x 16 tokens a wave, 16.8 with 4 x 16); narrow ones where even those are few
+    // (1024 x 1024, 20 %, 64 tokens: 5.6 us with 16 tokens a wave, 6.5 with 64).
+    auto waves = [&](int v) { return (int64_t)a.block_rows * ((a.N + 16 * v - 1) / (16 * v)); };
+    while (vec > 4 && waves(vec) < 1024) vec /= 2;
+    while (vec > 1 && waves(vec) < 256) vec /= 2;
+    const int64_t each = blocks / a.block_rows;  // blocks of a wave without a split
+    const int split = waves(vec) <= 512 && each >= 64 ? 16 : waves(vec) < 4096 && each >= 8 ? 4 : 1;
+    if (a.N == 1) {
+        if (split == 16)
+            launch<T, 1, NACC, TR, 16, false, true>(a, s);
+        else
+            launch<T, 1, NACC, TR, 4, false, true>(a, s);
         return;
     }
     switch (vec) {
     case 8:
-        if constexpr (!is_f32<T>) launch_split<T, 8, NACC, TR, false>(a, split, s);
+        if constexpr (!is_f32<T>) launch_split<T, 8, NACC, TR>(a, split, s);
         break;
-    case 4: launch_split<T, 4, NACC, TR, false>(a, split, s); break;
-    case 2: launch_split<T, 2, NACC, TR, false>(a, split, s); break;
-    default: launch_split<T, 1, NACC, TR, false>(a, split, s); break;
+    case 4: launch_split<T, 4, NACC, TR>(a, split, s); break;
+    case 2: launch_split<T, 2, NACC, TR>(a, split, s); break;
+    default: launch_split<T, 1, NACC, TR>(a, split, s); break;
     }
 }
 

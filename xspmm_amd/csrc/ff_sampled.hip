@@ -12,9 +12,17 @@ namespace detail {
 namespace ff {
 
 // ---------------------------------------------------------------------------
-// One wave per stored block (SPLIT waves share its tokens), operands straight
-// from memory: for 32-bit values, few blocks, and operands of any size.
+// One wave per four consecutive blocks (SPLIT waves share their tokens), operands
+// straight from memory: for few blocks and operands of any size.
 // ---------------------------------------------------------------------------
+
+constexpr int kGroup = kGroupBlocks;  // stored blocks of a wave
+
+// One step's operands: V tokens of a row per lane
+template <typename T, int ROWS>
+struct SampledStep {
+    u32x4_t d[ROWS], x[kGroup];
+};
 
 template <typename T, int SPLIT>
 __global__ __launch_bounds__(256) void ff_sampled_kernel(const int32_t* __restrict__ row, const int32_t* __restrict__ col,
@@ -26,64 +34,264 @@ __global__ __launch_bounds__(256) void ff_sampled_kernel(const int32_t* __restri
     constexpr int kStep = 4 * V;
     constexpr int kPer = 4 / SPLIT;
     const int lane = threadIdx.x & 63;
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g = lane >> 4;
-    const int64_t b = (int64_t)blockIdx.x * kPer + wave / SPLIT;
+    const int64_t b0 = ((int64_t)blockIdx.x * kPer + wave / SPLIT) * kGroup;
     const int part = wave % SPLIT;
-    float4_t acc = {0.f, 0.f, 0.f, 0.f};
-    int32_t r0 = 0, c0 = 0;
-    if (b < nnzb) {
-        r0 = 16 * row[b];
-        c0 = 16 * col[b];
+    float4_t acc[kGroup];
+    int32_t r0[kGroup], c0[kGroup];
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+        acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+        const int64_t b = min(b0 + i, nnzb - 1);  // past the last block: the last one again, not stored
+        r0[i] = 16 * row[b];
+        c0[i] = 16 * col[b];
+    }
+    // whole: all lanes' tokens are there, without a condition around the load (one
+    // makes the wave wait for it before the next)
+    auto tokens = [&](const T* p, int64_t n, auto whole) {
+        u32x4_t v = {0u, 0u, 0u, 0u};
+        if (decltype(whole)::value || n + V <= N) {
+            const auto q = global_load<T, V>(p + n);
+            v = u32x4_t{q.d[0], q.d[1], q.d[2], q.d[3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (n + i < N) {
+                    const uint32_t q = global_load<T, 1>(p + n + i).d[0];
+                    if constexpr (is_f32<T>)
+                        v[i] = q;
+                    else
+                        v[i / 2] |= q << (16 * (i % 2));
+                }
+        }
+        return v;
+    };
+    // ROWS: 1 where the blocks stand in one block-row, else one operand each
+    auto run = [&](auto rows) {
+        constexpr int ROWS = decltype(rows)::value;
         // rows past the edge read the last one; their results are not kept
-        const T* pd = dz + (int64_t)min(r0 + li, M - 1) * N;
-        const T* px = x + (int64_t)min(c0 + li, K - 1) * N;
-        const int64_t steps = (N + kStep - 1) / kStep;
-        const int64_t lo = steps * part / SPLIT, hi = steps * (part + 1) / SPLIT;
-        for (int64_t st = lo; st < hi; ++st) {
+        const T *pd[ROWS], *px[kGroup];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) pd[i] = dz + (int64_t)min(r0[i] + li, M - 1) * N;
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) px[i] = x + (int64_t)min(c0[i] + li, K - 1) * N;
+        auto load = [&](SampledStep<T, ROWS>& s, int64_t st, auto whole) {
             const int64_t n = st * kStep + V * g;
-            uint32_t a[4] = {0, 0, 0, 0}, d[4] = {0, 0, 0, 0};
-            if (n + V <= N) {
-                const auto va = global_load<T, V>(px + n), vd = global_load<T, V>(pd + n);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = va.d[i], d[i] = vd.d[i];
-            } else {
+            for (int i = 0; i < ROWS; ++i) s.d[i] = tokens(pd[i], n, whole);
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (n + i < N) {
-                        const uint32_t ua = global_load<T, 1>(px + n + i).d[0], ud = global_load<T, 1>(pd + n + i).d[0];
-                        if constexpr (is_f32<T>) {
-                            a[i] = ua, d[i] = ud;
-                        } else {
-                            a[i / 2] |= ua << (16 * (i % 2)), d[i / 2] |= ud << (16 * (i % 2));
-                        }
-                    }
+            for (int i = 0; i < kGroup; ++i) s.x[i] = tokens(px[i], n, whole);
+        };
+        auto multiply = [&](const SampledStep<T, ROWS>& s) {
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i) {
+                const u32x4_t d = s.d[ROWS == 1 ? 0 : i];
+                if constexpr (is_f32<T>) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[i] = mfma32(s.x[i][q], d[q], acc[i]);
+                } else {
+                    acc[i] = mfma16<T>(s.x[i], d, acc[i]);
+                }
             }
-            if constexpr (is_f32<T>) {
+        };
+        const int64_t steps = (N + kStep - 1) / kStep;
+        int64_t st = steps * part / SPLIT;
+        const int64_t hi = steps * (part + 1) / SPLIT, full = min(hi, N / kStep);
+        const std::true_type yes{};
+        // whole steps: the loads of one run ahead of the instructions of the last
+        if (st < full) {
+            SampledStep<T, ROWS> a, b;
+            load(a, st, yes);
+            for (;; st += 2) {
+                load(b, min(st + 1, full - 1), yes);
+                multiply(a);
+                if (st + 1 >= full) break;
+                load(a, min(st + 2, full - 1), yes);
+                multiply(b);
+                if (st + 2 >= full) break;
+            }
+            st = full;
+        }
+        if (st < hi) {
+            SampledStep<T, ROWS> a;
+            load(a, st, std::false_type{});
+            multiply(a);
+        }
+    };
+    if (b0 < nnzb && N > 0) {
+        if (r0[0] == r0[kGroup - 1])
+            run(std::integral_constant<int, 1>{});
+        else
+            run(std::integral_constant<int, kGroup>{});
+    }
+    if constexpr (SPLIT > 1) {
+        __shared__ float4_t red[kPer][SPLIT][kGroup][64];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc = mfma32(a[i], d[i], acc);
+        for (int i = 0; i < kGroup; ++i) red[wave / SPLIT][part][i][lane] = acc[i];
+        __syncthreads();
+        static_assert(SPLIT == kGroup);  // each wave finishes a block
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+            if (i != part) continue;
+            acc[i] = red[wave / SPLIT][0][i][lane];
+            for (int p = 1; p < SPLIT; ++p) acc[i] += red[wave / SPLIT][p][i][lane];
+        }
+    }
+    // lane: row li of the block, columns 4 g .. + 3
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+        if (b0 + i >= nnzb || (SPLIT > 1 && i != part)) continue;
+        Pack<T, 4> o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o.v[q] = (T)(r0[i] + li < M && c0[i] + 4 * g + q < K ? acc[i][q] : 0.f);
+        *reinterpret_cast<Pack<T, 4>*>(dvals + (b0 + i) * 256 + li * 16 + 4 * g) = o;
+    }
+}
+
+// The same for blocks of one block-row, where rows are on 16-byte boundaries: a
+// wave moves 128 bytes of its rows of dz and x at a time into LDS of its own, in
+// whole lines (the operands themselves are 16 bytes of 16 rows, and memory serves
+// one line at a time), one stage ahead of the one that it multiplies.  It waits
+// for nothing but its own loads.
+template <typename T>
+struct SampledWave {
+    const int32_t* group;
+    const int32_t* ptr;
+    const int32_t* row;
+    const int32_t* col;
+    const T* dz;
+    const T* x;
+    T* dvals;
+    int64_t groups;
+    int32_t M, K;
+    int64_t N;
+    uint32_t dz_bytes, x_bytes;
+};
+
+template <typename T, int SPLIT>
+__global__ __launch_bounds__(256, 2) void ff_sampled_wave_kernel(const SampledWave<T> a)
+{
+    constexpr int V = 16 / sizeof(T), kTokens = 128 / (int)sizeof(T);
+    constexpr int kUnits = 1 + kGroup, kStage = kUnits * 16 * 128, kLoads = 2 * kUnits;
+    constexpr int kPer = 4 / SPLIT;
+    __shared__ __align__(16) unsigned char smem[4][2][kStage];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, g = lane >> 4;
+    const int64_t item = xcd_item(blockIdx.x, (a.groups + kPer - 1) / kPer);
+    if (item < 0) return;
+    const int64_t gi = item * kPer + wave / SPLIT;
+    const int part = wave % SPLIT;
+    const bool live = gi < a.groups;
+    const int32_t b0 = live ? a.group[gi] : 0;
+    const int32_t br = live ? a.row[b0] : 0;
+    const int count = live ? min(a.ptr[br + 1] - b0, kGroup) : 0;
+    int32_t c0[kGroup];
+    float4_t acc[kGroup];
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+        acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+        c0[i] = 16 * a.col[min(b0 + i, b0 + max(count, 1) - 1)];
+    }
+    if (live) {
+        // load j of a stage: rows 8 (j % 2) .. + 7 of unit j / 2 (dz, then the
+        // blocks' rows of x); lane l lands at chunk l % 8 of row l / 8 and brings
+        // chunk (l % 8) ^ (l / 8), so that an operand's rows are in different banks
+        const uint32_t ld = (uint32_t)a.N * (uint32_t)sizeof(T);
+        const int chunk = (lane & 7) ^ (lane >> 3);
+        uint32_t off[kLoads];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int32_t r = (j < 2 ? 16 * br : c0[j / 2 - 1 < 0 ? 0 : j / 2 - 1]) + 8 * (j % 2) + (lane >> 3);
+            const bool in = j < 2 ? r < a.M : j / 2 <= count && r < a.K;
+            off[j] = in ? (uint32_t)r * ld + (uint32_t)chunk * 16u : kNone;
+        }
+        const i32x4_t bd = dma_buffer(a.dz, a.dz_bytes), bx = dma_buffer(a.x, a.x_bytes);
+        const uint32_t lds0 = lds_address(smem[wave]);
+        const int32_t steps = (int32_t)((a.N + kTokens - 1) / kTokens);
+        const int32_t lo = steps * part / SPLIT, hi = steps * (part + 1) / SPLIT;
+        auto issue = [&](int32_t st) {
+            const uint32_t to = lds0 + (uint32_t)(st & 1) * kStage;
+            const bool in = st * kTokens + V * chunk < a.N;
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j)
+                dma_to_lds(to + (uint32_t)j * 1024u, in ? off[j] + (uint32_t)st * 128u : kNone, j < 2 ? bd : bx);
+        };
+        if (lo < hi) issue(lo);
+        for (int32_t st = lo; st < hi; ++st) {
+            // the last reads of the stage that is loaded next are over
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (st + 1 < hi) {
+                issue(st + 1);
+                dma_wait<kLoads>();
             } else {
-                acc = mfma16<T>(u32x4_t{a[0], a[1], a[2], a[3]}, u32x4_t{d[0], d[1], d[2], d[3]}, acc);
+                dma_wait<0>();
+            }
+            const unsigned char* S = smem[wave][st & 1] + li * 128;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int piece = ((4 * h + g) ^ (li & 7)) * 16;
+                const u32x4_t d = *reinterpret_cast<const u32x4_t*>(S + piece);
+#pragma unroll
+                for (int i = 0; i < kGroup; ++i) {
+                    const u32x4_t xo = *reinterpret_cast<const u32x4_t*>(S + (1 + i) * 2048 + piece);
+                    if constexpr (is_f32<T>) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) acc[i] = mfma32(xo[q], d[q], acc[i]);
+                    } else {
+                        acc[i] = mfma16<T>(xo, d, acc[i]);
+                    }
+                }
             }
         }
     }
     if constexpr (SPLIT > 1) {
-        __shared__ float4_t red[kPer][SPLIT][64];
-        red[wave / SPLIT][part][lane] = acc;
+        static_assert(SPLIT == kGroup && kGroup * 4 * 64 * 16 <= sizeof(smem));
+        float4_t(*red)[kGroup][64] = reinterpret_cast<float4_t(*)[kGroup][64]>(&smem[0][0][0]);
         __syncthreads();
-        if (part > 0) return;
-        for (int p = 1; p < SPLIT; ++p) acc += red[wave / SPLIT][p][lane];
-    }
-    if (b >= nnzb) return;
-    // lane: row li of the block, columns 4 g .. + 3
-    Pack<T, 4> o;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) o.v[q] = (T)(r0 + li < M && c0 + 4 * g + q < K ? acc[q] : 0.f);
-    *reinterpret_cast<Pack<T, 4>*>(dvals + b * 256 + li * 16 + 4 * g) = o;
+        for (int i = 0; i < kGroup; ++i) red[wave][i][lane] = acc[i];
+        __syncthreads();
+        // each wave finishes a block
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i)
+            if (i == part) {
+                acc[i] = red[0][i][lane];
+                for (int p = 1; p < SPLIT; ++p) acc[i] += red[p][i][lane];
+            }
+    }
+    // lane: row li of the block, columns 4 g .. + 3
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+        if (i >= count || (SPLIT > 1 && i != part)) continue;
+        Pack<T, 4> o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o.v[q] = (T)(16 * br + li < a.M && c0[i] + 4 * g + q < a.K ? acc[i][q] : 0.f);
+        *reinterpret_cast<Pack<T, 4>*>(a.dvals + (int64_t)(b0 + i) * 256 + li * 16 + 4 * g) = o;
+    }
+}
+
+template <typename T>
+bool sampled_wave(const SampledArgs<T>& f, int l, hipStream_t s)
+{
+    const BlockIndex& w = *f.weight[l];
+    const int64_t db = narrow_bytes(w.M, f.N, sizeof(T)), xb = narrow_bytes(w.K, f.N, sizeof(T));
+    if (db < 0 || xb < 0 || f.N * sizeof(T) % 16 != 0 || f.N == 0) return false;
+    const SampledWave<T> a{w.group, w.ptr, w.row, w.col, f.dz[l], f.x, f.dvals[l], w.groups, (int32_t)w.M,
+                           (int32_t)w.K, f.N, (uint32_t)db, (uint32_t)xb};
+    const bool split = w.groups < 2048 && f.N * sizeof(T) >= 1024;
+    const int64_t grid = kXcds * xcd_chunk((w.groups + (split ? 0 : 3)) / (split ? 1 : 4));
+    if (split)
+        hipLaunchKernelGGL((ff_sampled_wave_kernel<T, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((ff_sampled_wave_kernel<T, 1>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    XSPMM_LAUNCH_CHECK();
+    return true;
 }
 
 // ---------------------------------------------------------------------------
-// 16-bit tiles: a workgroup takes 128 rows of dz and 128 rows of x, 64 tokens at
+// Tiles: a workgroup takes 128 rows of dz and 128 rows of x, 128 bytes of each at
 // a time through LDS, and multiplies where the tile holds a block.  A wave owns
 // 4 x 4 of its positions, with an accumulator for each.
 //
@@ -114,9 +322,9 @@ constexpr int kWR = 2, kWC = 2, kB = 4;   // a grid of 2 x 2 waves with 4 x 4 po
 constexpr int kEdge = kWR * kB;           // blocks along either edge of a tile
 constexpr int kSide = 16 * kEdge;         // its rows of dz, and of x
 constexpr int kThreads = 64 * kWR * kWC;
-constexpr int kTokens = 64;               // per step: a row's piece is 8 chunks of 16 bytes, a line of memory
-constexpr int kPieces = kTokens / 8;
-constexpr int kStage = 2 * kSide * 2 * kTokens;
+constexpr int kLine = 128;                // bytes of a row per step, a line of memory
+constexpr int kPieces = kLine / 16;
+constexpr int kStage = 2 * kSide * kLine;
 constexpr int kLoads = 2 * kSide * kPieces / kThreads;  // chunks a thread moves per step
 constexpr int kBand = 8;
 static_assert(kWR == kWC && kEdge * kEdge <= kThreads && kB * kB <= 32);
@@ -124,6 +332,8 @@ static_assert(kWR == kWC && kEdge * kEdge <= kThreads && kB * kB <= 32);
 template <typename T, bool DMA>
 __global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const SampledTile<T> a)
 {
+    constexpr int V = 16 / sizeof(T);                // tokens of a chunk
+    constexpr int kTokens = kLine / (int)sizeof(T);  // of a step
     __shared__ __align__(16) unsigned char smem[2 * kStage];
     __shared__ int32_t place[kEdge * kEdge];
     const int t = threadIdx.x, lane = t & 63;
@@ -164,7 +374,8 @@ __global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const Sampled
     // different banks.
     auto swizzle = [](int row) { return row % 8; };
     uint32_t base[kLoads];
-    const uint32_t ld = (uint32_t)a.N * 2u;
+    constexpr uint32_t kSize = sizeof(T);
+    const uint32_t ld = (uint32_t)a.N * kSize;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
         const int row = t / kPieces + j * (kThreads / kPieces);
@@ -178,12 +389,12 @@ __global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const Sampled
     const i32x4_t dma_dz = dma_buffer(s.dz, a.dz_bytes), dma_x = dma_buffer(a.x, a.x_bytes);
     u32x4_t held[DMA ? 1 : kLoads];
     auto issue = [&](int32_t st) {
-        const int32_t n = st * kTokens + 8 * chunk;
+        const int32_t n = st * kTokens + V * chunk;
         if constexpr (DMA) {
             const uint32_t to = lds0 + (uint32_t)(st % 2) * kStage + (uint32_t)wave * 1024u;
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
-                const uint32_t off = n < a.N && base[j] != kNone ? base[j] + (uint32_t)n * 2u : kNone;
+                const uint32_t off = n < a.N && base[j] != kNone ? base[j] + (uint32_t)n * kSize : kNone;
                 dma_to_lds(to + (uint32_t)j * (kThreads * 16u), off, j < kSide * kPieces / kThreads ? dma_dz : dma_x);
             }
         } else {
@@ -191,15 +402,20 @@ __global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const Sampled
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
                 const auto& b = j < kSide * kPieces / kThreads ? bd : bx;
-                if (st + 1 < steps || n + 8 <= a.N) {
-                    const auto v = buffer_load<T, 8>(b, base[j] != kNone ? base[j] + (uint32_t)n * 2u : kNone);
+                if (st + 1 < steps || n + V <= a.N) {
+                    const auto v = buffer_load<T, V>(b, base[j] != kNone ? base[j] + (uint32_t)n * kSize : kNone);
                     held[j] = u32x4_t{v.d[0], v.d[1], v.d[2], v.d[3]};
                 } else {  // the row ends within the chunk
                     held[j] = u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (n + i < a.N && base[j] != kNone)
-                            held[j][i / 2] |= buffer_load<T, 1>(b, base[j] + (uint32_t)(n + i) * 2u).d[0] << (16 * (i % 2));
+                    for (int i = 0; i < V; ++i)
+                        if (n + i < a.N && base[j] != kNone) {
+                            const uint32_t q = buffer_load<T, 1>(b, base[j] + (uint32_t)(n + i) * kSize).d[0];
+                            if constexpr (is_f32<T>)
+                                held[j][i] = q;
+                            else
+                                held[j][i / 2] |= q << (16 * (i % 2));
+                        }
                 }
             }
         }
@@ -213,20 +429,27 @@ __global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const Sampled
 
     auto compute = [&](int32_t st) {
 #pragma unroll
-        for (int h = 0; h < kTokens / 32; ++h) {
+        for (int h = 0; h < kPieces / 4; ++h) {
             const unsigned char* S =
-                smem + (st % 2) * kStage + li * (2 * kTokens) + (((4 * h + g) ^ swizzle(li)) * 16);
+                smem + (st % 2) * kStage + li * kLine + (((4 * h + g) ^ swizzle(li)) * 16);
             u32x4_t xo[kB];
 #pragma unroll
             for (int c = 0; c < kB; ++c)
-                xo[c] = *reinterpret_cast<const u32x4_t*>(S + (kSide + 16 * (wc * kB + c)) * (2 * kTokens));
+                xo[c] = *reinterpret_cast<const u32x4_t*>(S + (kSide + 16 * (wc * kB + c)) * kLine);
 #pragma unroll
             for (int r = 0; r < kB; ++r) {
                 if (!((mask >> (r * kB)) & ((1u << kB) - 1u))) continue;
-                const u32x4_t d = *reinterpret_cast<const u32x4_t*>(S + 16 * (wr * kB + r) * (2 * kTokens));
+                const u32x4_t d = *reinterpret_cast<const u32x4_t*>(S + 16 * (wr * kB + r) * kLine);
 #pragma unroll
                 for (int c = 0; c < kB; ++c)
-                    if (mask & (1u << (r * kB + c))) acc[r][c] = mfma16<T>(xo[c], d, acc[r][c]);
+                    if (mask & (1u << (r * kB + c))) {
+                        if constexpr (is_f32<T>) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) acc[r][c] = mfma32(xo[c][q], d[q], acc[r][c]);
+                        } else {
+                            acc[r][c] = mfma16<T>(xo[c], d, acc[r][c]);
+                        }
+                    }
             }
         }
     };
@@ -281,30 +504,36 @@ void launch_sampled_tile(SampledTile<T>& a, bool aligned, hipStream_t s)
 template <typename T>
 bool sampled_tiles(const SampledArgs<T>& f, int weights, hipStream_t s)
 {
-    if constexpr (is_f32<T>) {
-        return false;
-    } else {
-        const BlockIndex& w = *f.weight[0];
-        SampledTile<T> a{};
-        a.x = f.x;
-        a.M = (int32_t)w.M;
-        a.K = (int32_t)w.K;
-        a.Mb = (int32_t)w.Mb;
-        a.Kb = (int32_t)w.Kb;
-        a.N = f.N;
-        const int64_t db = narrow_bytes(w.M, f.N, 2), xb = narrow_bytes(w.K, f.N, 2);
-        if (db < 0 || xb < 0 || f.N == 0) return false;
-        a.dz_bytes = (uint32_t)db;
-        a.x_bytes = (uint32_t)xb;
-        for (int l = 0; l < weights; ++l) {
-            if (!f.dvals[l]) continue;
-            if (!f.weight[l]->map) return false;
-            a.side[a.sides++] = {f.weight[l]->map, f.dz[l], f.dvals[l]};
-        }
-        if (a.sides == 0) return true;
-        launch_sampled_tile<T>(a, f.N % 8 == 0, s);
-        return true;
+    const BlockIndex& w = *f.weight[0];
+    SampledTile<T> a{};
+    a.x = f.x;
+    a.M = (int32_t)w.M;
+    a.K = (int32_t)w.K;
+    a.Mb = (int32_t)w.Mb;
+    a.Kb = (int32_t)w.Kb;
+    a.N = f.N;
+    const int64_t db = narrow_bytes(w.M, f.N, sizeof(T)), xb = narrow_bytes(w.K, f.N, sizeof(T));
+    if (db < 0 || xb < 0 || f.N == 0) return false;
+    a.dz_bytes = (uint32_t)db;
+    a.x_bytes = (uint32_t)xb;
+    int64_t blocks = 0;
+    for (int l = 0; l < weights; ++l) {
+        if (!f.dvals[l]) continue;
+        if (!f.weight[l]->map) return false;
+        blocks += f.weight[l]->nnzb;
+        a.side[a.sides++] = {f.weight[l]->map, f.dz[l], f.dvals[l]};
     }
+    if (a.sides == 0) return true;
+    // The share of stored blocks from which a tile's rows are cheaper than the rows
+    // of each four blocks (14336 x 4096 fp16, 2048 tokens: 10 % stored 102 us by
+    // fours, 199 by tiles, 25 % 243 and 228; 4096 x 4096 fp32, 512 tokens: 50 % 102
+    // and 114, all 188 and 149), or, off 16 bytes, than those read operand by
+    // operand (fp16, 5 %: 140 us and 180, 10 % 245 and 199).
+    const bool aligned = f.N * sizeof(T) % 16 == 0;
+    const int64_t share = aligned ? (is_f32<T> ? 155 : 56) : (is_f32<T> ? 46 : 18);  // of 256
+    if (blocks * 256 < share * a.sides * w.Mb * w.Kb) return false;
+    launch_sampled_tile<T>(a, aligned, s);
+    return true;
 }
 
 }  // namespace ff
@@ -315,12 +544,13 @@ void sampled_product(const SampledArgs<T>& f, int weights, hipStream_t s)
     if (ff::sampled_tiles<T>(f, weights, s)) return;
     for (int l = 0; l < weights; ++l) {
         const BlockIndex& w = *f.weight[l];
-        if (!f.dvals[l] || w.nnzb == 0) continue;
-        if (w.nnzb < 4096 && f.N >= 512)
-            hipLaunchKernelGGL((ff::ff_sampled_kernel<T, 4>), dim3((unsigned)w.nnzb), dim3(256), 0, s, w.row, w.col,
+        if (!f.dvals[l] || w.nnzb == 0 || ff::sampled_wave<T>(f, l, s)) continue;
+        const int64_t groups = (w.nnzb + ff::kGroup - 1) / ff::kGroup;
+        if (groups < 2048 && f.N >= 256)
+            hipLaunchKernelGGL((ff::ff_sampled_kernel<T, 4>), dim3((unsigned)groups), dim3(256), 0, s, w.row, w.col,
                                f.dz[l], f.x, f.dvals[l], w.nnzb, (int32_t)w.M, (int32_t)w.K, f.N);
         else
-            hipLaunchKernelGGL((ff::ff_sampled_kernel<T, 1>), dim3((unsigned)((w.nnzb + 3) / 4)), dim3(256), 0, s,
+            hipLaunchKernelGGL((ff::ff_sampled_kernel<T, 1>), dim3((unsigned)((groups + 3) / 4)), dim3(256), 0, s,
                                w.row, w.col, f.dz[l], f.x, f.dvals[l], w.nnzb, (int32_t)w.M, (int32_t)w.K, f.N);
         XSPMM_LAUNCH_CHECK();
     }

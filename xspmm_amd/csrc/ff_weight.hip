@@ -98,6 +98,24 @@ __global__ __launch_bounds__(256) void ff_transpose_kernel(const int32_t* __rest
     if (!FILL && lane == 0) counts[j] = at;
 }
 
+__global__ __launch_bounds__(256) void ff_group_count_kernel(const int32_t* __restrict__ ptr, int64_t Mb,
+                                                             int32_t* __restrict__ counts)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    // pointers that do not ascend count for nothing: the host reports them
+    if (i < Mb) counts[i] = max(ptr[i + 1] - ptr[i] + kGroupBlocks - 1, 0) / kGroupBlocks;
+}
+
+__global__ __launch_bounds__(256) void ff_group_kernel(const int32_t* __restrict__ ptr, const int32_t* __restrict__ gptr,
+                                                       const int* __restrict__ bad, int64_t Mb,
+                                                       int32_t* __restrict__ group)
+{
+    const int64_t br = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    if (*bad || br >= Mb) return;
+    const int32_t g0 = gptr[br], g1 = gptr[br + 1], b0 = ptr[br];
+    for (int32_t g = g0 + (int32_t)(threadIdx.x & 63); g < g1; g += 64) group[g] = b0 + (g - g0) * kGroupBlocks;
+}
+
 // exclusive prefix sum of n counts in place, n + 1 results; one workgroup
 __global__ __launch_bounds__(kScanThreads) void ff_scan_kernel(int32_t* __restrict__ v, int64_t n)
 {
@@ -146,6 +164,8 @@ void build_block_index(BlockIndex& out, int64_t M, int64_t K, int64_t Mb, int64_
     const size_t o_col = c.take((size_t)nnzb * 4), o_row = c.take((size_t)nnzb * 4);
     const size_t o_trow = c.take((size_t)nnzb * 4), o_tblk = c.take((size_t)nnzb * 4);
     const size_t o_bad = c.take(4);
+    const size_t o_gptr = c.take((size_t)(Mb + 1) * 4);
+    const size_t o_group = c.take((size_t)(nnzb / kGroupBlocks + (Mb < nnzb ? Mb : nnzb)) * 4);
     const bool map = wants_map(Mb, Kb, nnzb);
     const size_t o_map = c.take(map ? (size_t)(Mb * Kb) * 4 : 0);
     XSPMM_HIP_CHECK(hipMalloc(&out.memory, c.end));
@@ -157,6 +177,8 @@ void build_block_index(BlockIndex& out, int64_t M, int64_t K, int64_t Mb, int64_
     out.trow = reinterpret_cast<int32_t*>(p + o_trow);
     out.tblk = reinterpret_cast<int32_t*>(p + o_tblk);
     if (map) out.map = reinterpret_cast<int32_t*>(p + o_map);
+    out.group = reinterpret_cast<int32_t*>(p + o_group);
+    int32_t* gptr = reinterpret_cast<int32_t*>(p + o_gptr);
     int* bad = reinterpret_cast<int*>(p + o_bad);
 
     auto groups = [](int64_t n, int64_t per) { return dim3((unsigned)((n + per - 1) / per)); };
@@ -174,10 +196,18 @@ void build_block_index(BlockIndex& out, int64_t M, int64_t K, int64_t Mb, int64_
     if (Kb > 0 && nnzb > 0)
         hipLaunchKernelGGL((ff_transpose_kernel<true>), groups(Kb, 4), dim3(256), 0, s, out.ptr, out.col, Mb, Kb, bad,
                            nullptr, out.tptr, out.trow, out.tblk);
+    if (Mb > 0)
+        hipLaunchKernelGGL(ff_group_count_kernel, groups(Mb, 256), dim3(256), 0, s, out.ptr, Mb, gptr);
+    hipLaunchKernelGGL(ff_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, gptr, Mb);
+    if (Mb > 0 && nnzb > 0)
+        hipLaunchKernelGGL(ff_group_kernel, groups(Mb, 4), dim3(256), 0, s, out.ptr, gptr, bad, Mb, out.group);
     XSPMM_LAUNCH_CHECK();
     int found = 0;
+    int32_t made = 0;
     XSPMM_HIP_CHECK(hipMemcpyAsync(&found, bad, 4, hipMemcpyDeviceToHost, s));
+    XSPMM_HIP_CHECK(hipMemcpyAsync(&made, gptr + Mb, 4, hipMemcpyDeviceToHost, s));
     XSPMM_HIP_CHECK(hipStreamSynchronize(s));
+    out.groups = made;
     require(!(found & kBadPtr), "xSpMM: a weight's row pointers must ascend from 0 to the number of blocks.");
     require(!(found & kBadCol), "xSpMM: a weight's block columns must lie in the grid and ascend within a row.");
 }
