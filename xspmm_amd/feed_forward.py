@@ -18,6 +18,7 @@ gradients.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -63,25 +64,30 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-class _Here:
-    """The device of a call's operands as the current one."""
-
-    def __init__(self, device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return _raw_stream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+_current = torch.cuda.current_device
+_Tensor = torch.Tensor
 
 
-def _check(t, name, shape, dtype, device, aligned=True):
-    if type(t) is not torch.Tensor and not isinstance(t, torch.Tensor):
+def _call(index, f, *args):
+    """f(*args, stream) on torch's current stream of device `index`."""
+    if _current() == index:
+        rc = f(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, _raw_stream(index))
+    if rc:
+        X._check(rc)
+
+
+def _check(t, name, shape, dtype, device, mask=15):
+    """The address of an operand that the kernels can take as given (None: no
+    elements); raises otherwise.  mask: low bits that the address may not have."""
+    if (t.__class__ is _Tensor and t.dtype is dtype and t.shape == shape and t.device == device
+            and t.is_contiguous()):
+        at = t.data_ptr()
+        if not at & mask:
+            return at or None
+    if not isinstance(t, _Tensor):
         raise TypeError(f"{name} must be a torch tensor")
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
@@ -91,10 +97,9 @@ def _check(t, name, shape, dtype, device, aligned=True):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    at = t.data_ptr()
-    if aligned and at % 16:
+    if t.data_ptr() & mask:
         raise ValueError(f"{name} must start on a 16-byte boundary")
-    return at or None
+    return t.data_ptr() or None
 
 
 def _activation(name):
@@ -125,21 +130,22 @@ class SparseWeight:
         if device.type != "cuda":
             raise ValueError("a weight's arrays are on the GPU")
         X.icode(rp.dtype)
-        _check(rp, "row_ptr", (int(A.num_block_rows) + 1,), rp.dtype, device, aligned=False)
-        _check(ci, "col_ind", (int(ci.numel()),), rp.dtype, device, aligned=False)
+        _check(rp, "row_ptr", (int(A.num_block_rows) + 1,), rp.dtype, device, mask=0)
+        _check(ci, "col_ind", (int(ci.numel()),), rp.dtype, device, mask=0)
         self.device = device
         self.shape = (int(A.num_rows), int(A.num_cols))
         self.num_blocks = int(ci.numel())
         self.dtype = A.values.dtype
         self.code = _TYPES[self.dtype]
         self.matrix = A
+        self._flat = (self.num_blocks * 256,)
         _check(A.values, "values", (self.num_blocks * 256,), self.dtype, device)
         h = C.c_void_p()
         self._L = _load()
-        with _Here(device) as stream:
+        with torch.cuda.device(device):
             X._check(self._L.xspmm_weight_create(X.icode(rp.dtype), *self.shape, int(A.num_block_rows),
                                                  int(A.num_block_cols), self.num_blocks, X._ptr(rp), X._ptr(ci),
-                                                 stream, C.byref(h)))
+                                                 _raw_stream(device.index), C.byref(h)))
         self._h = h
 
     @property
@@ -154,7 +160,7 @@ class SparseWeight:
     def _values(self):
         if self._h is None:
             raise RuntimeError("SparseWeight is closed")
-        return _check(self.matrix.values, "values", (self.num_blocks * 256,), self.dtype, self.device)
+        return _check(self.matrix.values, "values", self._flat, self.dtype, self.device)
 
     def close(self):
         if self._h is not None:
@@ -169,15 +175,15 @@ class SparseWeight:
 
 
 def _tokens(x, name="x"):
-    if not isinstance(x, torch.Tensor):
+    if not isinstance(x, _Tensor):
         raise TypeError(f"{name} must be a torch tensor")
     if x.dim() != 2:
         raise ValueError(f"{name} must be features x tokens, got {x.dim()} dimensions")
     return x.shape[1]
 
 
-def _optional(t, name, shape, dtype, device, aligned=True):
-    return None if t is None else _check(t, name, shape, dtype, device, aligned)
+def _at(t):
+    return None if t is None else t.data_ptr() or None
 
 
 def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, out=None):
@@ -187,16 +193,12 @@ def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, o
     (M, K), N, dt, dev = W.shape, _tokens(x), W.dtype, W.device
     vals = W._values()
     xp = _check(x, "x", (K, N), dt, dev)
-    bp = _optional(bias, "bias", (M,), dt, dev, aligned=False)
-    rp = _optional(residual, "residual", (M, N), dt, dev)
-    y = torch.empty((M, N), dtype=dt, device=dev) if out is None else out
-    yp = _check(y, "out", (M, N), dt, dev)
-    z = torch.empty((M, N), dtype=dt, device=dev) if keep else None
-    with _Here(dev) as stream:
-        rc = W._L.xspmm_linear(W._h, W.code, act, vals, xp, bp, rp, yp, z.data_ptr() or None if keep else None, N,
-                               stream)
-    if rc:
-        X._check(rc)
+    bp = None if bias is None else _check(bias, "bias", (M,), dt, dev, 0)
+    rp = None if residual is None else _check(residual, "residual", (M, N), dt, dev)
+    y = x.new_empty((M, N)) if out is None else out
+    yp = (y.data_ptr() or None) if out is None else _check(out, "out", (M, N), dt, dev)
+    z = x.new_empty((M, N)) if keep else None
+    _call(dev.index, W._L.xspmm_linear, W._h, W.code, act, vals, xp, bp, rp, yp, _at(z), N)
     return (y, z) if keep else y
 
 
@@ -211,29 +213,21 @@ def sparse_linear_backward(W, x, kept, dy, activation=None, bias=False, need=(Tr
     xp = _check(x, "x", (K, N), dt, dev)
     zp = _check(kept, "kept", (M, N), dt, dev) if act else None
     gp = _check(dy, "dy", (M, N), dt, dev)
-    dx = torch.empty((K, N), dtype=dt, device=dev) if need[0] else None
-    dv = torch.empty(W.num_blocks * 256, dtype=dt, device=dev) if need[1] else None
-    db = torch.empty(M, dtype=dt, device=dev) if bias else None
+    dx = x.new_empty((K, N)) if need[0] else None
+    dv = x.new_empty(W._flat) if need[1] else None
+    db = x.new_empty((M,)) if bias else None
     n = C.c_int64(0)
-    L = W._L
-    with _Here(dev) as stream:
-        rc = L.xspmm_linear_backward_scratch(W._h, W.code, act, N, C.byref(n))
-        if rc:
-            X._check(rc)
-        ws = _scratch(n.value, dev)
-        rc = L.xspmm_linear_backward(W._h, W.code, act, vals, xp, zp, gp, _at(dx), _at(dv), _at(db), N, _at(ws),
-                                     n.value, stream)
+    rc = W._L.xspmm_linear_backward_scratch(W._h, W.code, act, N, C.byref(n))
     if rc:
         X._check(rc)
+    ws = _scratch(n.value, dev)
+    _call(dev.index, W._L.xspmm_linear_backward, W._h, W.code, act, vals, xp, zp, gp, _at(dx), _at(dv), _at(db), N,
+          _at(ws), n.value)
     return dx, dv, db
 
 
-def _at(t):
-    return None if t is None else t.data_ptr() or None
-
-
 def _pair(G, U):
-    if G.shape != U.shape or G.dtype != U.dtype or G.device != U.device:
+    if G.shape != U.shape or G.dtype is not U.dtype or G.device != U.device:
         raise ValueError(f"gate ({G.shape}, {G.dtype}, {G.device}) and up ({U.shape}, {U.dtype}, {U.device}) differ")
     return G.shape
 
@@ -246,16 +240,13 @@ def sparse_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", keep=
     (M, K), N, dt, dev = _pair(G, U), _tokens(x), G.dtype, G.device
     gv, uv = G._values(), U._values()
     xp = _check(x, "x", (K, N), dt, dev)
-    gb = _optional(bias_gate, "bias_gate", (M,), dt, dev, aligned=False)
-    ub = _optional(bias_up, "bias_up", (M,), dt, dev, aligned=False)
-    h = torch.empty((M, N), dtype=dt, device=dev) if out is None else out
-    hp = _check(h, "out", (M, N), dt, dev)
-    zg = torch.empty((M, N), dtype=dt, device=dev) if keep else None
-    zu = torch.empty((M, N), dtype=dt, device=dev) if keep else None
-    with _Here(dev) as stream:
-        rc = G._L.xspmm_gated(G._h, U._h, G.code, act, gv, uv, xp, gb, ub, hp, _at(zg), _at(zu), N, stream)
-    if rc:
-        X._check(rc)
+    gb = None if bias_gate is None else _check(bias_gate, "bias_gate", (M,), dt, dev, 0)
+    ub = None if bias_up is None else _check(bias_up, "bias_up", (M,), dt, dev, 0)
+    h = x.new_empty((M, N)) if out is None else out
+    hp = (h.data_ptr() or None) if out is None else _check(out, "out", (M, N), dt, dev)
+    zg = x.new_empty((M, N)) if keep else None
+    zu = x.new_empty((M, N)) if keep else None
+    _call(dev.index, G._L.xspmm_gated, G._h, U._h, G.code, act, gv, uv, xp, gb, ub, hp, _at(zg), _at(zu), N)
     return (h, zg, zu) if keep else h
 
 
@@ -271,61 +262,59 @@ def sparse_gated_backward(G, U, x, kept_gate, kept_up, dh, activation="silu", bi
     zg = _check(kept_gate, "kept_gate", (M, N), dt, dev)
     zu = _check(kept_up, "kept_up", (M, N), dt, dev)
     hp = _check(dh, "dh", (M, N), dt, dev)
-    dx = torch.empty((K, N), dtype=dt, device=dev) if need[0] else None
-    dg = torch.empty(G.num_blocks * 256, dtype=dt, device=dev) if need[1] else None
-    du = torch.empty(U.num_blocks * 256, dtype=dt, device=dev) if need[2] else None
-    bg = torch.empty(M, dtype=dt, device=dev) if bias else None
-    bu = torch.empty(M, dtype=dt, device=dev) if bias else None
+    dx = x.new_empty((K, N)) if need[0] else None
+    dg = x.new_empty(G._flat) if need[1] else None
+    du = x.new_empty(U._flat) if need[2] else None
+    bg = x.new_empty((M,)) if bias else None
+    bu = x.new_empty((M,)) if bias else None
     n = C.c_int64(0)
-    L = G._L
-    with _Here(dev) as stream:
-        rc = L.xspmm_gated_backward_scratch(G._h, G.code, N, C.byref(n))
-        if rc:
-            X._check(rc)
-        ws = _scratch(n.value, dev)
-        rc = L.xspmm_gated_backward(G._h, U._h, G.code, act, gv, uv, xp, zg, zu, hp, _at(dx), _at(dg), _at(du),
-                                    _at(bg), _at(bu), N, _at(ws), n.value, stream)
+    rc = G._L.xspmm_gated_backward_scratch(G._h, G.code, N, C.byref(n))
     if rc:
         X._check(rc)
+    ws = _scratch(n.value, dev)
+    _call(dev.index, G._L.xspmm_gated_backward, G._h, U._h, G.code, act, gv, uv, xp, zg, zu, hp, _at(dx), _at(dg),
+          _at(du), _at(bg), _at(bu), N, _at(ws), n.value)
     return dx, dg, du, bg, bu
 
 
-def _norm_operands(x, weight, bias):
-    if not isinstance(x, torch.Tensor):
+@functools.lru_cache(maxsize=1024)
+def _norm_scratch(code, K, N, backward):
+    """Bytes of scratch, from the sizes alone."""
+    n = C.c_int64(0)
+    X._check(_load().xspmm_layer_norm_scratch(code, K, N, backward, C.byref(n)))
+    return n.value
+
+
+def _norm_operands(x, weight):
+    if not isinstance(x, _Tensor):
         raise TypeError("x must be a torch tensor")
     if x.dim() != 2:
         raise ValueError(f"x must be features x tokens, got {x.dim()} dimensions")
-    if x.dtype not in _TYPES:
-        raise TypeError(f"unsupported dtype {x.dtype}")
-    if x.device.type != "cuda":
+    dt, dev, (K, N) = x.dtype, x.device, x.shape
+    if dt not in _TYPES:
+        raise TypeError(f"unsupported dtype {dt}")
+    if dev.type != "cuda":
         raise ValueError("x is not on the GPU")
-    K, N = x.shape
     if K == 0:
         raise ValueError("a norm needs at least one feature")
-    dt, dev = x.dtype, x.device
-    return (K, N, dt, dev, _check(x, "x", (K, N), dt, dev), _optional(weight, "weight", (K,), dt, dev, aligned=False),
-            _optional(bias, "bias", (K,), dt, dev, aligned=False))
+    return K, N, dt, dev, _check(x, "x", (K, N), dt, dev), (
+        None if weight is None else _check(weight, "weight", (K,), dt, dev, 0))
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, keep=False, out=None):
     """Layer norm over the features (rows) of every token (column) of x; with
     keep also the tokens' mean and 1 / sqrt(variance + eps) in fp32, which
     ``layer_norm_backward`` takes."""
-    K, N, dt, dev, xp, wp, bp = _norm_operands(x, weight, bias)
-    L = _load()
-    y = torch.empty((K, N), dtype=dt, device=dev) if out is None else out
-    yp = _check(y, "out", (K, N), dt, dev)
+    K, N, dt, dev, xp, wp = _norm_operands(x, weight)
+    bp = None if bias is None else _check(bias, "bias", (K,), dt, dev, 0)
+    y = x.new_empty((K, N)) if out is None else out
+    yp = (y.data_ptr() or None) if out is None else _check(out, "out", (K, N), dt, dev)
     mean = torch.empty(N, dtype=torch.float32, device=dev) if keep else None
     rstd = torch.empty(N, dtype=torch.float32, device=dev) if keep else None
-    n = C.c_int64(0)
-    with _Here(dev) as stream:
-        rc = L.xspmm_layer_norm_scratch(_TYPES[dt], K, N, 0, C.byref(n))
-        if rc:
-            X._check(rc)
-        ws = _scratch(n.value, dev)
-        rc = L.xspmm_layer_norm(_TYPES[dt], K, N, xp, wp, bp, eps, yp, _at(mean), _at(rstd), _at(ws), n.value, stream)
-    if rc:
-        X._check(rc)
+    code = _TYPES[dt]
+    n = _norm_scratch(code, K, N, 0)
+    ws = _scratch(n, dev)
+    _call(dev.index, _load().xspmm_layer_norm, code, K, N, xp, wp, bp, eps, yp, _at(mean), _at(rstd), _at(ws), n)
     return (y, mean, rstd) if keep else y
 
 
@@ -333,22 +322,16 @@ def layer_norm_backward(dy, x, weight, mean, rstd, need=(True, True, True)):
     """(dx, dweight, dbias) of ``layer_norm`` from dy and the statistics it
     kept; weight may be None (ones).  need: which of them are wanted (None
     otherwise)."""
-    K, N, dt, dev, xp, wp, _ = _norm_operands(x, weight, None)
-    L = _load()
+    K, N, dt, dev, xp, wp = _norm_operands(x, weight)
     gp = _check(dy, "dy", (K, N), dt, dev)
-    mp = _check(mean, "mean", (N,), torch.float32, dev, aligned=False)
-    sp = _check(rstd, "rstd", (N,), torch.float32, dev, aligned=False)
-    dx = torch.empty((K, N), dtype=dt, device=dev) if need[0] else None
-    dw = torch.empty(K, dtype=dt, device=dev) if need[1] else None
-    db = torch.empty(K, dtype=dt, device=dev) if need[2] else None
-    n = C.c_int64(0)
-    with _Here(dev) as stream:
-        rc = L.xspmm_layer_norm_scratch(_TYPES[dt], K, N, 1, C.byref(n))
-        if rc:
-            X._check(rc)
-        ws = _scratch(n.value, dev)
-        rc = L.xspmm_layer_norm_backward(_TYPES[dt], K, N, gp, xp, wp, mp, sp, _at(dx), _at(dw), _at(db), _at(ws),
-                                         n.value, stream)
-    if rc:
-        X._check(rc)
+    mp = _check(mean, "mean", (N,), torch.float32, dev, 3)
+    sp = _check(rstd, "rstd", (N,), torch.float32, dev, 3)
+    dx = x.new_empty((K, N)) if need[0] else None
+    dw = x.new_empty((K,)) if need[1] else None
+    db = x.new_empty((K,)) if need[2] else None
+    code = _TYPES[dt]
+    n = _norm_scratch(code, K, N, 1)
+    ws = _scratch(n, dev)
+    _call(dev.index, _load().xspmm_layer_norm_backward, code, K, N, gp, xp, wp, mp, sp, _at(dx), _at(dw), _at(db),
+          _at(ws), n)
     return dx, dw, db
