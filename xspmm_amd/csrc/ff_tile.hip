@@ -50,25 +50,22 @@ struct TileArgs {
     int act;
 };
 
-constexpr int kDeep = 2;  // blocks of a slot per step
+constexpr int kSlots = 8;          // block-rows of a workgroup, half of them a wave's
+constexpr int WS = kSlots / 2, WC = 2;
+constexpr int kWide = 64 * WC;     // its tokens, 64 of them a wave's
+constexpr int kTileThreads = 128 * WC;
+constexpr int kDeep = 4;           // blocks of a slot per step
+constexpr int kPairs = kDeep / 2;
+constexpr int kXRow = 2 * kWide;
+constexpr int kABytes = kSlots * kDeep * 512;
+constexpr int kTileStage = kABytes + 16 * kDeep * kXRow;
+constexpr int kWindow = 256;       // block-columns whose positions are in LDS at a time
+constexpr int kPlaceRow = kWindow + kDeep;
 constexpr int kTileBand = 8;
-
-// A workgroup of 2 x WC waves; a wave owns WS slots x 64 tokens.
-template <int WS, int WC>
-struct Tile {
-    static constexpr int kThreads = 128 * WC;
-    static constexpr int kSlots = 2 * WS;
-    static constexpr int kWide = 64 * WC;         // tokens
-    static constexpr int kXRow = 2 * kWide;
-    static constexpr int kABytes = kSlots * kDeep * 512;
-    static constexpr int kStage = kABytes + 16 * kDeep * kXRow;
-    static constexpr int kStages = WC == 4 ? (WS == 4 ? 6 : 4) : (WS == 4 ? 4 : 3);
-    static constexpr int kWindow = WS == 8 && WC == 2 ? 112 : 256;  // block-columns whose positions are in LDS
-    static constexpr int kOutRow = kWide + 4;     // floats of a row on its way out
-    static_assert(64 * kOutRow * 4 <= kStages * kStage && kWindow % kDeep == 0);
-    // a narrow workgroup shares its CU with another
-    static_assert(kStages * kStage + kSlots * (kWindow + kDeep) * 4 <= (WC == 2 ? 80 : 160) * 1024);
-};
+constexpr int kOutRow = kWide + 4;  // floats of a row on its way out
+constexpr int kTileLds = 2 * kTileStage + kSlots * kPlaceRow * 4;
+// two workgroups share a CU; the sums leave through the same LDS
+static_assert(kTileLds <= 80 * 1024 && 16 * kSlots * kOutRow * 4 <= kTileLds && kWindow % kDeep == 0);
 
 // Chunk c (16 bytes) of row e of the x stage lies at chunk c ^ x_swizzle(e): the
 // rows that one transposed read touches are in different banks.
@@ -84,16 +81,13 @@ __device__ __forceinline__ u32x2_t read_transposed(const unsigned char* p)
                               __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)const_cast<unsigned char*>(p)));
 }
 
-template <typename T, int WS, int WC, bool TR, bool GATED, bool DMA>
-__global__ __launch_bounds__(128 * WC, 2) void ff_tile_kernel(const TileArgs<T> a)
+template <typename T, bool TR, bool GATED, bool DMA>
+__global__ __launch_bounds__(kTileThreads, 2) void ff_tile_kernel(const TileArgs<T> a)
 {
-    using G = Tile<WS, WC>;
-    constexpr int kTileThreads = G::kThreads, kSlots = G::kSlots, kWide = G::kWide, kXRow = G::kXRow;
-    constexpr int kABytes = G::kABytes, kTileStage = G::kStage, kTileStages = G::kStages;
-    constexpr int kWindow = G::kWindow, kOutRow = G::kOutRow;
     constexpr int kOutRows = GATED ? kSlots / 2 : kSlots;  // block-rows of the result
-    __shared__ __align__(16) unsigned char smem[kTileStages * kTileStage];
-    __shared__ uint32_t place[kSlots][kWindow + kDeep];  // byte offsets of the blocks, or kNone
+    __shared__ __align__(16) unsigned char smem[kTileLds];
+    // byte offsets of the blocks, or kNone
+    uint32_t(*const place)[kPlaceRow] = reinterpret_cast<uint32_t(*)[kPlaceRow]>(smem + 2 * kTileStage);
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wr = wave / WC, wc = wave % WC;
@@ -121,9 +115,8 @@ __global__ __launch_bounds__(128 * WC, 2) void ff_tile_kernel(const TileArgs<T> 
 
     const uint32_t lds0 = lds_address(smem);
     const uint32_t ld = (uint32_t)a.N * 2u;
-    constexpr int kAhead = DMA ? kTileStages - 1 : 1;  // steps whose loads are under way
     constexpr int kAPer = kSlots / (2 * WC);                  // a wave's loads of A per step
-    constexpr int kPerStep = kAPer + 2;
+    constexpr int kXPer = kDeep;                       // and of x
 
     // Wave w moves the blocks of kAPer slots from kAPer w on and kRowsPer rows of x
     // from kRowsPer w on, a KB per load.  This lane's bytes: of a block (16 at p = lane % 32), and of x from
@@ -131,15 +124,15 @@ __global__ __launch_bounds__(128 * WC, 2) void ff_tile_kernel(const TileArgs<T> 
     const int p = lane & 31;
     const uint32_t a_lane = (uint32_t)((p >> 1) * 32 + (((p & 1) ^ a_swizzle(p >> 1)) * 16));
     constexpr int kRowsPer = 16 * kDeep / (2 * WC);
-    uint32_t x_lane[2];
+    uint32_t x_lane[kXPer];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int e = kRowsPer * wave + kRowsPer / 2 * u + lane / (8 * WC);
+    for (int u = 0; u < kXPer; ++u) {
+        const int e = kRowsPer * wave + kRowsPer / kXPer * u + lane / (8 * WC);
         const int64_t n = n0 + 8 * (lane % (8 * WC) ^ x_swizzle(e));
         x_lane[u] = n < a.N ? (uint32_t)e * ld + (uint32_t)n * 2u : kNone;
     }
     const uint32_t* const dma_place = &place[kAPer * wave][lane >> 5];
-    const uint32_t* const own_place = &place[WS * wr + lane / 2 % WS][lane & 1];
+    const uint32_t* const own_place = &place[WS * wr + lane / kDeep % WS][lane % kDeep];
 
     // Operands: row 4 g + li / 4 of a block (or of x), 8-byte piece li % 4; of A
     // itself row li, values 4 g .. + 3.
@@ -157,56 +150,53 @@ __global__ __launch_bounds__(128 * WC, 2) void ff_tile_kernel(const TileArgs<T> 
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[s][j] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-    // stored: bit 2 s + d, block d of this wave's slot s
-    auto compute = [&](const unsigned char* S, uint32_t stored) {
-        uint32_t pairs = stored & (stored >> 1), firsts = stored & ~(stored >> 1), seconds = ~stored & (stored >> 1);
-        asm volatile("" : "+s"(pairs), "+s"(firsts), "+s"(seconds));
-        auto a_operand = [&](int s, int d) {
-            const unsigned char* q = S + a_at + (s * kDeep + d) * 512;
-            if constexpr (TR)
-                return read_transposed(q);
-            else
-                return *reinterpret_cast<const u32x2_t*>(q);
-        };
-        u32x2_t x0[4], x1[4];
+    // The operands of a pair of block-columns.  Those of A^T are read with those of
+    // x, of blocks that are not there too (what lies in their places is not used);
+    // those of A, whose reads have bank conflicts, at a block's own instructions.
+    struct Operands {
+        u32x2_t x[kDeep][4], a[kDeep][TR ? WS : 1];
+    };
+    auto a_operand = [&](const unsigned char* S, int s, int d) {
+        const unsigned char* q = S + a_at + (s * kDeep + d) * 512;
+        if constexpr (TR)
+            return read_transposed(q);
+        else
+            return *reinterpret_cast<const u32x2_t*>(q);
+    };
+    auto read = [&](Operands& o, const unsigned char* S, int d) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x0[j] = read_transposed(S + x_at[j]);
-            x1[j] = read_transposed(S + x_at[j] + 16 * kXRow);
-        }
-        // Transposed reads of A have no bank conflicts, so all are made at once, of
-        // blocks that are not there too (dx of 14336 x 4096, every block stored, 2048
-        // tokens: 321 -> 317 us, half stored 267 -> 256); of plain ones, which have,
-        // only those of stored blocks (y: 315 us, all at once 361).
-        u32x2_t a0[TR ? WS : 1], a1[TR ? WS : 1];
+        for (int j = 0; j < 4; ++j) o.x[d][j] = read_transposed(S + x_at[j] + 16 * d * kXRow);
         if constexpr (TR)
 #pragma unroll
-            for (int s = 0; s < WS; ++s) {
-                a0[s] = a_operand(s, 0);
-                a1[s] = a_operand(s, 1);
-            }
-        auto operand0 = [&](int s) { return TR ? a0[TR ? s : 0] : a_operand(s, 0); };
-        auto operand1 = [&](int s) { return TR ? a1[TR ? s : 0] : a_operand(s, 1); };
+            for (int s = 0; s < WS; ++s) o.a[d][s] = a_operand(S, s, d);
+    };
+    // Blocks d and d + 1 of every slot; stored: bit kDeep s + d, block d of this
+    // wave's slot s.  Three conditions of their own, not alternatives: an accumulator
+    // with more than one way to its new value is copied on all of them.
+    auto multiply = [&](const Operands& o, const unsigned char* S, uint32_t stored, int d) {
+        uint32_t pairs = stored & (stored >> 1), firsts = stored & ~(stored >> 1), seconds = ~stored & (stored >> 1);
+        asm volatile("" : "+s"(pairs), "+s"(firsts), "+s"(seconds));
+        auto operand = [&](int s, int e) { return TR ? o.a[e][TR ? s : 0] : a_operand(S, s, e); };
 #pragma unroll
         for (int s = 0; s < WS; ++s) {
-            // three conditions of their own, not alternatives: an accumulator with
-            // more than one way to its new value is copied on all of them
-            if (pairs & (1u << (2 * s))) {
-                const u32x2_t p = operand0(s), q = operand1(s);
+            const uint32_t bit = 1u << (kDeep * s + d);
+            if (pairs & bit) {
+                const u32x2_t p = operand(s, d), q = operand(s, d + 1);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[s][j] = mfma16<T>(u32x4_t{p.x, p.y, q.x, q.y}, u32x4_t{x0[j].x, x0[j].y, x1[j].x, x1[j].y},
+                    acc[s][j] = mfma16<T>(u32x4_t{p.x, p.y, q.x, q.y},
+                                          u32x4_t{o.x[d][j].x, o.x[d][j].y, o.x[d + 1][j].x, o.x[d + 1][j].y},
                                           acc[s][j]);
             }
-            if (firsts & (1u << (2 * s))) {
-                const u32x2_t p = operand0(s);
+            if (firsts & bit) {
+                const u32x2_t p = operand(s, d);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[s][j] = mfma16_half<T>(p, x0[j], acc[s][j]);
+                for (int j = 0; j < 4; ++j) acc[s][j] = mfma16_half<T>(p, o.x[d][j], acc[s][j]);
             }
-            if (seconds & (1u << (2 * s))) {
-                const u32x2_t q = operand1(s);
+            if (seconds & bit) {
+                const u32x2_t q = operand(s, d + 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[s][j] = mfma16_half<T>(q, x1[j], acc[s][j]);
+                for (int j = 0; j < 4; ++j) acc[s][j] = mfma16_half<T>(q, o.x[d + 1][j], acc[s][j]);
             }
         }
     };
@@ -230,89 +220,128 @@ __global__ __launch_bounds__(128 * WC, 2) void ff_tile_kernel(const TileArgs<T> 
             }
             __syncthreads();
             const int32_t steps = min(kWindow, a.in_blocks - c0 + kDeep - 1) / kDeep;
-            uint32_t x_off[2] = {x_lane[0] + (uint32_t)c0 * 16u * ld, x_lane[1] + (uint32_t)c0 * 16u * ld};
-            u32x4_t held[DMA ? 1 : 2];
-            uint32_t flags[kAhead];
+            uint32_t x_off[kXPer];
+#pragma unroll
+            for (int u = 0; u < kXPer; ++u) x_off[u] = x_lane[u] + (uint32_t)c0 * 16u * ld;
+            u32x4_t held[DMA ? 1 : kXPer];
+            // what the next step to load needs of the positions, read ahead of it
+            uint32_t next_own, next_dma[kAPer * kPairs];
+            auto look = [&](int32_t st) {
+                next_own = own_place[st * kDeep];
+#pragma unroll
+                for (int u = 0; u < kAPer * kPairs; ++u)
+                    next_dma[u] = dma_place[u / kPairs * (kPlaceRow) + st * kDeep + 2 * (u % kPairs)];
+            };
             // the loads of step st; what is stored of this wave's own slots in it
             auto issue = [&](int32_t st) -> uint32_t {
-                const uint32_t to = lds0 + (uint32_t)(st % kTileStages) * kTileStage;
-                const uint32_t mine = own_place[st * kDeep];
+                const uint32_t to = lds0 + (uint32_t)(st & 1) * kTileStage;
+                const uint32_t f = (uint32_t)__builtin_amdgcn_readfirstlane(
+                    (int)__ballot(lane < kDeep * WS && next_own != kNone));
 #pragma unroll
-                for (int u = 0; u < kAPer; ++u)
-                    dma_to_lds(to + (uint32_t)((kAPer * wave + u) * kDeep) * 512u,
-                               dma_place[u * (kWindow + kDeep) + st * kDeep] + a_lane,
-                               GATED && slot_side(kAPer * wave + u) ? vals1 : vals0);
+                for (int u = 0; u < kAPer * kPairs; ++u) {
+                    const int s = u / kPairs, h = u % kPairs;
+                    dma_to_lds(to + (uint32_t)((kAPer * wave + s) * kDeep + 2 * h) * 512u, next_dma[u] + a_lane,
+                               GATED && slot_side(kAPer * wave + s) ? vals1 : vals0);
+                }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < kXPer; ++u) {
                     if constexpr (DMA) {
-                        dma_to_lds(to + kABytes + (uint32_t)(kRowsPer * wave + kRowsPer / 2 * u) * kXRow, x_off[u], xb);
+                        dma_to_lds(to + kABytes + (uint32_t)(kRowsPer * wave + kRowsPer / kXPer * u) * kXRow, x_off[u],
+                                   xb);
                     } else {
                         const auto v = buffer_load<T, 8>(xr, x_off[u]);
                         held[u] = u32x4_t{v.d[0], v.d[1], v.d[2], v.d[3]};
                     }
                     x_off[u] += 16u * kDeep * ld;
                 }
-                return (uint32_t)__builtin_amdgcn_readfirstlane((int)__ballot(lane < 2 * WS && mine != kNone));
+                look(st + 1 < steps ? st + 1 : steps - 1);
+                return f;
             };
+            // until the loads of step st are in LDS, of every wave, and what was read
+            // from the other stage in registers
+            auto landed = [&](int32_t st) {
+                if constexpr (!DMA)
 #pragma unroll
-            for (int q = 0; q < kAhead; ++q) flags[q] = q < steps ? issue(q) : 0u;
-            // Step st is multiplied while the loads of the steps after it are under
-            // way; those issued after its barrier go where step st - 1 was read
-            // before it.
-            for (int32_t st = 0; st < steps; ++st) {
-                unsigned char* S = smem + (st % kTileStages) * kTileStage;
-                if constexpr (DMA) {
-                    if (st + kAhead <= steps)
-                        dma_wait<(kAhead - 1) * kPerStep>();
-                    else
-                        dma_wait<0>();
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        *reinterpret_cast<u32x4_t*>(S + kABytes + (kRowsPer * wave + kRowsPer / 2 * u) * kXRow + lane * 16) = held[u];
-                    dma_wait<0>();
-                }
+                    for (int u = 0; u < kXPer; ++u)
+                        *reinterpret_cast<u32x4_t*>(smem + (st & 1) * kTileStage + kABytes +
+                                                    (kRowsPer * wave + kRowsPer / kXPer * u) * kXRow + lane * 16) = held[u];
+                dma_wait<0>();
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __syncthreads();
-                const uint32_t stored = flags[0];
+            };
+            look(0);
+            uint32_t coming = issue(0);
+            if constexpr (TR) {
+                // a step is multiplied from registers while the next one's operands are
+                // read and the loads of the one after that are under way
+                uint32_t stored = coming;
+                Operands even, odd;
+                landed(0);
+                coming = 1 < steps ? issue(1) : 0u;
 #pragma unroll
-                for (int q = 0; q + 1 < kAhead; ++q) flags[q] = flags[q + 1];
-                if (st + kAhead < steps) flags[kAhead - 1] = issue(st + kAhead);
-                compute(S, stored);
+                for (int d = 0; d < kDeep; ++d) read(even, smem, d);
+                auto round = [&](int32_t st, const Operands& now, Operands& then) {
+                    const uint32_t mine = stored;
+                    if (st + 1 < steps) {
+                        stored = coming;
+                        landed(st + 1);
+                        coming = st + 2 < steps ? issue(st + 2) : 0u;
+#pragma unroll
+                        for (int d = 0; d < kDeep; ++d) read(then, smem + ((st + 1) & 1) * kTileStage, d);
+                    }
+#pragma unroll
+                    for (int d = 0; d < kDeep; d += 2) multiply(now, smem, mine, d);
+                };
+                for (int32_t st = 0; st < steps; st += 2) {
+                    round(st, even, odd);
+                    if (st + 1 < steps) round(st + 1, odd, even);
+                }
+            } else {
+                for (int32_t st = 0; st < steps; ++st) {
+                    const uint32_t stored = coming;
+                    landed(st);
+                    if (st + 1 < steps) coming = issue(st + 1);
+                    const unsigned char* S = smem + (st & 1) * kTileStage;
+                    Operands o;
+#pragma unroll
+                    for (int d = 0; d < kDeep; d += 2) {
+                        read(o, S, d);
+                        read(o, S, d + 1);
+                        multiply(o, S, stored, d);
+                    }
+                }
             }
         }
     }
 
-    // The sums leave through LDS, two slots of every wave at a time, so that the
-    // rest is done on eight tokens of a row per thread.
+    // The sums leave through LDS, so that the rest is done on eight tokens of a row
+    // per thread.
     float* O = reinterpret_cast<float*>(smem);
+    __syncthreads();
 #pragma unroll
-    for (int p = 0; p < WS / 2; ++p) {
-        __syncthreads();
+    for (int s = 0; s < WS; ++s)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int s = GATED ? p + WS / 2 * i : 2 * p + i;  // gated: a block-row's gate, then its up
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    O[(32 * wr + 16 * i + 4 * g + q) * kOutRow + 64 * wc + 16 * j + li] = acc[s][j][q];
-        }
-        __syncthreads();
-        constexpr int kOut = GATED ? 32 : 64;  // rows of this round
-#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                O[(16 * (WS * wr + s) + 4 * g + q) * kOutRow + 64 * wc + 16 * j + li] = acc[s][j][q];
+    __syncthreads();
+    {
+        constexpr int kOut = 16 * kOutRows;
+#pragma unroll 1
         for (int v = 0; v < kOut * (kWide / 8) / kTileThreads; ++v) {
             const int at = v * kTileThreads + t, r = at / (kWide / 8), c = at % (kWide / 8) * 8;
-            // r: wave row, then (not gated) slot, then row of the block
-            const int from = GATED ? 32 * (r / 16) + r % 16 : r;
-            const int32_t block = br0 + (GATED ? WS / 2 * (r / 16) + p : WS * (r / 32) + 2 * p + r / 16 % 2);
-            const int64_t row = 16 * (int64_t)block + r % 16, n = n0 + c;
+            // the block-row's slot, of a gated product the gate's, with the up
+            // projection's WS / 2 slots on
+            const int from = GATED ? 16 * (r / (8 * WS) * WS) + r % (8 * WS) : r;
+            const int64_t row = 16 * (int64_t)br0 + r, n = n0 + c;
             if (row >= a.rows || n + 8 <= first || n >= a.N) continue;
             const bool whole = n >= first && n + 8 <= a.N;
             float z[2][8];
 #pragma unroll
             for (int l = 0; l < (GATED ? 2 : 1); ++l) {
-                const float4_t lo = *reinterpret_cast<const float4_t*>(O + (from + 16 * l) * kOutRow + c);
-                const float4_t hi = *reinterpret_cast<const float4_t*>(O + (from + 16 * l) * kOutRow + c + 4);
+                const float4_t lo = *reinterpret_cast<const float4_t*>(O + (from + 8 * WS * l) * kOutRow + c);
+                const float4_t hi = *reinterpret_cast<const float4_t*>(O + (from + 8 * WS * l) * kOutRow + c + 4);
                 const float bias = !TR && a.side[l].bias ? (float)a.side[l].bias[row] : 0.f;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -360,37 +389,31 @@ __global__ __launch_bounds__(128 * WC, 2) void ff_tile_kernel(const TileArgs<T> 
     }
 }
 
-template <typename T, int WS, int WC, bool TR, bool GATED>
-void launch_tile_of(const TileArgs<T>& a, hipStream_t s)
-{
-    constexpr int rows = GATED ? WS : 2 * WS, wide = Tile<WS, WC>::kWide;
-    const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + wide - 1) / wide);
-    const int64_t grid = kXcds * xcd_chunk(items);
-    if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many tokens for one launch.");
-    const dim3 block(Tile<WS, WC>::kThreads);
-    if (a.N % 8 == 0)
-        hipLaunchKernelGGL((ff_tile_kernel<T, WS, WC, TR, GATED, true>), dim3((unsigned)grid), block, 0, s, a);
-    else
-        hipLaunchKernelGGL((ff_tile_kernel<T, WS, WC, TR, GATED, false>), dim3((unsigned)grid), block, 0, s, a);
-    XSPMM_LAUNCH_CHECK();
-}
-
 template <typename T, bool TR, bool GATED>
 void launch_tile(const TileArgs<T>& a, hipStream_t s)
 {
-    const char* e = getenv("WS");
-    const int v = e ? atoi(e) : 84;
-    if (v == 84 && a.N >= 256) launch_tile_of<T, 8, 4, TR, GATED>(a, s);
-    else if (v == 44 && a.N >= 256) launch_tile_of<T, 4, 4, TR, GATED>(a, s);
-    else if (v == 82) launch_tile_of<T, 8, 2, TR, GATED>(a, s);
-    else launch_tile_of<T, 4, 2, TR, GATED>(a, s);
+    constexpr int rows = GATED ? kSlots / 2 : kSlots;
+    const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + kWide - 1) / kWide);
+    const int64_t grid = kXcds * xcd_chunk(items);
+    if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many tokens for one launch.");
+    if (a.N % 8 == 0)
+        hipLaunchKernelGGL((ff_tile_kernel<T, TR, GATED, true>), dim3((unsigned)grid), dim3(kTileThreads), 0, s, a);
+    else
+        hipLaunchKernelGGL((ff_tile_kernel<T, TR, GATED, false>), dim3((unsigned)grid), dim3(kTileThreads), 0, s, a);
+    XSPMM_LAUNCH_CHECK();
 }
 
-bool tiles_pay(int64_t blocks, int64_t grid_blocks, int64_t N)
+// Whether the share of stored blocks is one at which tiles are faster than walking
+// the block-rows one by one (14336 x 4096 fp16, 2048 tokens, us by tiles and by
+// rows: y 25 % 220 and 212, 50 % 257 and 365, all 310 and 640; two weights 25 %
+// 416 and 391, 50 % 486 and 717; dx 25 % 192 and 188, 50 % 218 and 353, all 244 and
+// 670), of a token tile that may be filled in part, and whether they are enough
+// for the chip (a workgroup walks its whole sum).
+bool tiles_pay(int64_t blocks, int64_t grid_blocks, int64_t N, int64_t row_groups)
 {
-    const char* e = getenv("TILE");
-    if (e) return atoi(e);
-    return blocks * 8 >= grid_blocks && N >= 128;
+    const int64_t tiles = (N + kWide - 1) / kWide;
+    if (row_groups * tiles < 256) return false;
+    return (double)blocks * (double)N >= 0.28 * (double)grid_blocks * (double)(tiles * kWide);
 }
 
 }  // namespace ff
@@ -409,7 +432,9 @@ bool feed_forward_tiles(const ForwardArgs<T>& f, int weights, hipStream_t s)
         blocks += wl.nnzb;
     }
     const int64_t xb = narrow_bytes(w.K, f.N, 2);
-    if (xb < 0 || (f.N % 8 != 0 && f.N < 128) || !ff::tiles_pay(blocks, weights * w.Mb * w.Kb, f.N)) return false;
+    if (xb < 0 || (f.N % 8 != 0 && f.N < ff::kWide) ||
+        !ff::tiles_pay(blocks, weights * w.Mb * w.Kb, f.N, w.Mb * weights / ff::kSlots))
+        return false;
     a.residual = f.residual;
     a.y = f.y;
     a.sides = weights;
@@ -442,7 +467,9 @@ bool transposed_tiles(const TransposedArgs<T>& f, int weights, hipStream_t s)
         blocks += wl.nnzb;
     }
     const int64_t xb = narrow_bytes(w.M, f.N, 2);
-    if (xb < 0 || (f.N % 8 != 0 && f.N < 128) || !ff::tiles_pay(blocks, weights * w.Mb * w.Kb, f.N)) return false;
+    if (xb < 0 || (f.N % 8 != 0 && f.N < ff::kWide) ||
+        !ff::tiles_pay(blocks, weights * w.Mb * w.Kb, f.N, w.Kb / ff::kSlots))
+        return false;
     a.y = f.dx;
     a.sides = weights;
     a.rows = (int32_t)w.K;
