@@ -521,3 +521,63 @@ def test_framework_matrix_as_weight():
     want = f64(X.spmm(Bm, B))
     close(X.sparse_linear(W, B), want, 2.0 ** -11 * want.abs() + 200 * EPS32 * 20 + TINY, "y")
     assert math.isfinite(float(want.abs().max()))
+
+
+# ---------------------------------------------------------------------------
+# the layer as a module
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("N", [1, 50, 260])
+def test_feed_forward_module(N):
+    """fp32: outputs and all gradients against the same layer on the unpacked weights in 64 bits.  The bounds are
+    those of a chain of four sums of up to K products, relative to the largest value."""
+    feats, hidden = 96, 200
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    mats = [X.prune_blocks(torch.randn(s, generator=gen, device=DEV) * 0.1, 0.5)
+            for s in ((hidden, feats), (hidden, feats), (feats, hidden))]
+    layer = X.FeedForward(*mats, activation="gelu")
+    x = normal((feats, N), torch.float32, 1).requires_grad_(True)
+    dy = normal((feats, N), torch.float32, 2)
+    with torch.no_grad():
+        served = layer(x)
+    y = layer(x)
+    assert torch.equal(y, served)
+    y.backward(dy)
+
+    def unpack(A, v):
+        rows = torch.repeat_interleave(torch.arange(A.num_block_rows), torch.diff(A.row_ptr.cpu()).long())
+        d = torch.zeros((A.num_block_rows, A.num_block_cols, 16, 16), dtype=torch.float64)
+        d = d.index_put((rows, A.col_ind.cpu().long()), v.view(-1, 16, 16))
+        return d.permute(0, 2, 1, 3).reshape(A.num_block_rows * 16, -1)[:A.num_rows, :A.num_cols]
+
+    vals = [f64(p.detach()).requires_grad_(True) for p in (layer.gate, layer.up, layer.down)]
+    w64, b64 = (f64(p.detach()).requires_grad_(True) for p in (layer.norm_weight, layer.norm_bias))
+    x64 = f64(x.detach()).requires_grad_(True)
+    G, U, D = (unpack(A, v) for A, v in zip(mats, vals))
+    n = norm64(x64, w64, b64, 1e-5)[0]
+    y64 = x64 + D @ (torch.nn.functional.gelu(G @ n) * (U @ n))
+    y64.backward(f64(dy))
+    for got, want in ((y.detach(), y64.detach()), (x.grad, x64.grad), (layer.gate.grad, vals[0].grad),
+                      (layer.up.grad, vals[1].grad), (layer.down.grad, vals[2].grad),
+                      (layer.norm_weight.grad, w64.grad), (layer.norm_bias.grad, b64.grad)):
+        close(got, want, 4 * (hidden + N) * EPS32 * float(want.abs().max()), "module")
+
+
+def test_feed_forward_demo():
+    from xspmm_amd import feed_forward_demo
+
+    out = feed_forward_demo.run(features=128, hidden=320, tokens=256, density=0.4, steps=40, dtype="f16")
+    assert out["error_after"] < 0.7 * out["error_before"], out
+    assert out["served_vs_batch"] < 4 * 2.0 ** -11, out
+
+
+def test_prune_blocks_keeps_the_largest():
+    w = normal((50, 70), torch.float32, 1)
+    A = X.prune_blocks(w, 0.3)
+    assert A.num_blocks == round(0.3 * 4 * 5) and int(A.row_ptr[-1]) == A.num_blocks
+    norms = torch.stack([w[16 * i:16 * i + 16, 16 * j:16 * j + 16].square().sum() for i in range(4) for j in range(5)])
+    rows = torch.repeat_interleave(torch.arange(4), torch.diff(A.row_ptr.cpu()).long())
+    kept = rows * 5 + A.col_ind.cpu()
+    assert set(kept.tolist()) == set(torch.topk(norms, A.num_blocks).indices.tolist())
+    with pytest.raises(ValueError):
+        X.FeedForward(A, A, A)

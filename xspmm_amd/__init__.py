@@ -633,7 +633,7 @@ class SpMMPlan:
 # The feed-forward layer's operators need torch, which the module loads on the
 # first use of one.
 _FEED_FORWARD = ("SparseWeight", "sparse_linear", "sparse_linear_backward", "sparse_gated", "sparse_gated_backward",
-                 "layer_norm", "layer_norm_backward")
+                 "layer_norm", "layer_norm_backward", "FeedForward", "prune_blocks")
 
 
 def __getattr__(name):

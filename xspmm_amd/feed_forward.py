@@ -335,3 +335,104 @@ def layer_norm_backward(dy, x, weight, mean, rstd, need=(True, True, True)):
     _call(dev.index, _load().xspmm_layer_norm_backward, code, K, N, gp, xp, wp, mp, sp, _at(dx), _at(dw), _at(db),
           _at(ws), n)
     return dx, dw, db
+
+
+# ---------------------------------------------------------------------------
+# as a module
+# ---------------------------------------------------------------------------
+
+def prune_blocks(dense, density):
+    """The 16x16 blocks of a dense M x K weight with the largest norms, a share
+    `density` of them (at least one), as a BCSRMatrix on the weight's device."""
+    M, K = dense.shape
+    Mb, Kb = -(-M // 16), -(-K // 16)
+    padded = dense.new_zeros((Mb * 16, Kb * 16))
+    padded[:M, :K] = dense
+    blocks = padded.view(Mb, 16, Kb, 16).permute(0, 2, 1, 3).reshape(Mb * Kb, 256)
+    norms = blocks.float().square().sum(1)
+    keep = torch.topk(norms, max(1, round(density * Mb * Kb))).indices.sort().values
+    row_ptr = torch.zeros(Mb + 1, dtype=torch.int32, device=dense.device)
+    row_ptr[1:] = torch.cumsum(torch.bincount(keep // Kb, minlength=Mb), 0)
+    return X.BCSRMatrix(Mb, Kb, 16, 16, M, K, row_ptr, (keep % Kb).int(), blocks[keep].reshape(-1).contiguous())
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm(x, weight, bias, eps, keep=True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        return (*layer_norm_backward(dy.contiguous(), x, weight, mean, rstd, need=ctx.needs_input_grad[:3]), None)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, W, values, x, bias, activation, residual):
+        W.values = values.detach()
+        y, z = sparse_linear(W, x, bias, activation, residual, keep=True)
+        ctx.W, ctx.activation, ctx.bias = W, activation, bias is not None
+        ctx.save_for_backward(values, x, z)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        values, x, z = ctx.saved_tensors
+        ctx.W.values = values.detach()
+        dy = dy.contiguous()
+        need = ctx.needs_input_grad
+        dx, dv, db = sparse_linear_backward(ctx.W, x, z, dy, ctx.activation, ctx.bias and need[3], (need[2], need[1]))
+        return None, dv, dx, db, None, dy if need[5] else None
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, G, U, gate, up, x, activation):
+        G.values, U.values = gate.detach(), up.detach()
+        h, zg, zu = sparse_gated(G, U, x, activation=activation, keep=True)
+        ctx.G, ctx.U, ctx.activation = G, U, activation
+        ctx.save_for_backward(gate, up, x, zg, zu)
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        gate, up, x, zg, zu = ctx.saved_tensors
+        ctx.G.values, ctx.U.values = gate.detach(), up.detach()
+        need = ctx.needs_input_grad
+        dx, dg, du, _, _ = sparse_gated_backward(ctx.G, ctx.U, x, zg, zu, dh.contiguous(), ctx.activation,
+                                                 need=(need[4], need[2], need[3]))
+        return None, None, dg, du, dx, None
+
+
+class FeedForward(torch.nn.Module):
+    """x + D (act(G n) * (U n)), n = layer_norm(x): a model's feed-forward layer
+    on three BCSR matrices (G and U hidden x features, D features x hidden), with
+    their block values and the norm's weight and bias as parameters.  Which
+    blocks are stored does not change.  x is features x tokens."""
+
+    def __init__(self, gate, up, down, activation="silu", eps=1e-5):
+        super().__init__()
+        self._weights = [SparseWeight(A) for A in (gate, up, down)]
+        G, U, D = self._weights
+        features = _pair(G, U)[1]
+        if D.shape != (features, G.shape[0]) or D.dtype is not G.dtype or D.device != G.device:
+            raise ValueError(f"down is {D.shape}, {D.dtype}, expected {(features, G.shape[0])}, {G.dtype}")
+        _activation(activation)
+        self.activation, self.eps = activation, eps
+        self.gate, self.up, self.down = (torch.nn.Parameter(W.values.clone()) for W in self._weights)
+        like = dict(dtype=G.dtype, device=G.device)
+        self.norm_weight = torch.nn.Parameter(torch.ones(features, **like))
+        self.norm_bias = torch.nn.Parameter(torch.zeros(features, **like))
+
+    def forward(self, x):
+        G, U, D = self._weights
+        if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
+            n = _Norm.apply(x, self.norm_weight, self.norm_bias, self.eps)
+            h = _Gated.apply(G, U, self.gate, self.up, n, self.activation)
+            return _Linear.apply(D, self.down, h, None, None, x)
+        G.values, U.values, D.values = self.gate.detach(), self.up.detach(), self.down.detach()
+        n = layer_norm(x.detach(), self.norm_weight.detach(), self.norm_bias.detach(), self.eps)
+        return sparse_linear(D, sparse_gated(G, U, n, activation=self.activation), residual=x.detach())
