@@ -244,6 +244,33 @@ def test_product_tiles(kind, M, K, N, density):
     close(dx, want, (2 * M + 2) * EPS32 * S + 2 * u * (Ga.abs().t() @ g) + u * want.abs() * 1.01 + TINY, "gated dx")
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(2100, 300, 2056), (300, 2100, 2051), (2100, 4200, 2056), (4200, 520, 4104),
+                                   (520, 4200, 4099)])
+@pytest.mark.parametrize("density", [0.3, 1.0])
+def test_product_tiles_of_a_full_chip(kind, M, K, N, density):
+    """The same where there are tiles enough for every compute unit, of eight block-rows and of sixteen."""
+    test_product_tiles(kind, M, K, N, density)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(2064, 512, 2056), (4208, 512, 4099)])
+def test_product_tiles_leave_absent_blocks_alone(kind, M, K, N):
+    """Infinities and NaN in rows of x reach the block-rows that store a block there, and no others."""
+    dtype, _ = TYPES[kind]
+    W, A, _ = weight(M, K, 0.4, dtype, 5)
+    x, dy = normal((K, N), dtype, 1), normal((M, N), dtype, 2)
+    x[37], dy[53] = math.nan, math.inf
+    stored = A.reshape(M // 16, 16, K // 16, 16).abs().sum((1, 3)) > 0
+    assert 0 < stored[:, 2].sum() < M // 16 and 0 < stored[3].sum() < K // 16
+    y = X.sparse_linear(W, x)
+    hit = stored[:, 2].repeat_interleave(16)
+    assert y[hit].isnan().all() and y[~hit].isfinite().all()
+    dx = X.sparse_linear_backward(W, x, None, dy, need=(True, False))[0]
+    hit = stored[3].repeat_interleave(16)
+    assert not dx[hit].isfinite().any() and dx[~hit].isfinite().all()
+
+
 def test_wanted_gradients_only():
     W, _, _ = weight(64, 64, 0.5, torch.float16, 1)
     x, z, dy = (normal((64, 20), torch.float16, s) for s in (1, 2, 3))

@@ -1,22 +1,32 @@
 // ff_tile.hip -- the products of ff_product.hip for 16-bit values where blocks
-// are not rare: a workgroup takes eight block-rows and 128 tokens, 64 rows of x
-// at a time.
+// are not rare: a workgroup takes sixteen (or eight) block-rows and 128 tokens, 32
+// (or 64) rows of x at a time.
 //
-//   forward      eight block-rows of A, or (gated) four of the gate's and the same
-//                four of the up projection's
-//   transposed   eight block-columns of A; the sum runs over the block-rows of one
+//   forward      block-rows of A, or (gated) half of them the gate's and the others
+//                the same ones of the up projection's
+//   transposed   block-columns of A; the sum runs over the block-rows of one
 //                weight and then of the other
 //
-// Per step, 64 rows of x (16 KB) and the stored blocks among the 8 x 4 that meet
-// them (512 bytes each; absent ones are neither read nor multiplied) go straight
-// from memory into LDS, two stages in turn.  A wave owns four block-rows x 64
+// Per step, the rows of x (8 or 16 KB) and the stored blocks that meet them (512
+// bytes each; absent ones are neither read nor multiplied) go straight from memory
+// into LDS, two stages in turn.  Of eight waves each owns four (two) block-rows x 64
 // tokens and takes the block-columns in pairs.  A lane's operands of a pair are
 // four values of the one block and four of the other, so that two stored blocks
 // make one v_mfma_f32_16x16x32 and a single one, with the same registers, one
 // v_mfma_f32_16x16x16: nothing of x meets a block that is not there.  Rows of x
-// are read from memory once for eight block-rows, where the kernel that walks
-// single block-rows reads them for every block.  Two workgroups share a CU, so that one
-// multiplies while the other waits for its loads.
+// are read from memory once for all the block-rows, where the kernel that walks
+// single block-rows reads them for every block.
+//
+// What a step costs is less the matrix instructions (14336 x 4096, 2048 tokens: 44 %
+// of the time where all blocks are stored, 30 % at a quarter of them) or the memory
+// (without its loads a step is a fifth shorter) than the way of a wave from the
+// barrier over its reads of LDS to its instructions, and the reads themselves.  Hence
+// two workgroups of eight waves on a CU, four waves a SIMD, that take turns (25 %
+// stored: 175 us; with four waves of four block-rows x 64 tokens each 218), and
+// sixteen block-rows where there are enough of them, so that a row of x is read from
+// LDS for four block-rows and not for two (158 us).  Measured: y 157 us at 25 %
+// stored and 250 at 100 % (960 TFLOP/s), both of a gated product's 300 and 475
+// (1010), dx, by eight, 162 and 269.
 #include "feed_forward_device.hpp"
 
 namespace xspmm {
@@ -50,22 +60,30 @@ struct TileArgs {
     int act;
 };
 
-constexpr int kSlots = 8;          // block-rows of a workgroup, half of them a wave's
-constexpr int WS = kSlots / 2, WC = 2;
-constexpr int kWide = 64 * WC;     // its tokens, 64 of them a wave's
-constexpr int kTileThreads = 128 * WC;
-constexpr int kDeep = 4;           // blocks of a slot per step
-constexpr int kPairs = kDeep / 2;
+constexpr int kWide = 128;     // tokens of a workgroup
+constexpr int WC = 2, TT = 4;  // waves along them, a wave's tiles of 16
+constexpr int kTileWaves = 8;
+constexpr int kTileThreads = 64 * kTileWaves;
 constexpr int kXRow = 2 * kWide;
-constexpr int kABytes = kSlots * kDeep * 512;
-constexpr int kTileStage = kABytes + 16 * kDeep * kXRow;
-constexpr int kWindow = 256;       // block-columns whose positions are in LDS at a time
-constexpr int kPlaceRow = kWindow + kDeep;
+constexpr int kWindow = 256;  // block-columns whose positions are in LDS at a time
 constexpr int kTileBand = 8;
 constexpr int kOutRow = kWide + 4;  // floats of a row on its way out
-constexpr int kTileLds = 2 * kTileStage + kSlots * kPlaceRow * 4;
-// two workgroups share a CU; the sums leave through the same LDS
-static_assert(kTileLds <= 80 * 1024 && 16 * kSlots * kOutRow * 4 <= kTileLds && kWindow % kDeep == 0);
+
+template <int SLOTS>
+struct TileShape {
+    static constexpr int kSlots = SLOTS;                       // block-rows
+    static constexpr int WS = kSlots / (kTileWaves / WC);      // a wave's
+    static constexpr int kDeep = 32 / kSlots;                  // blocks of a slot per step
+    static constexpr int kPairs = kDeep / 2;
+    static constexpr int kABytes = kSlots * kDeep * 512;
+    static constexpr int kStage = kABytes + 16 * kDeep * kXRow;
+    static constexpr int kPlaceRow = kWindow + kDeep;
+    static constexpr int kPasses = kSlots / 8;                 // of the sums through the same LDS
+    static constexpr int kUsed = 2 * kStage + kSlots * kPlaceRow * 4, kOut = 16 * 8 * kOutRow * 4;
+    static constexpr int kLds = kUsed > kOut ? kUsed : kOut;
+    // two workgroups share a CU
+    static_assert(kLds <= 80 * 1024 && kWindow % kDeep == 0);
+};
 
 // Chunk c (16 bytes) of row e of the x stage lies at chunk c ^ x_swizzle(e): the
 // rows that one transposed read touches are in different banks.
@@ -81,11 +99,14 @@ __device__ __forceinline__ u32x2_t read_transposed(const unsigned char* p)
                               __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)const_cast<unsigned char*>(p)));
 }
 
-template <typename T, bool TR, bool GATED, bool DMA>
-__global__ __launch_bounds__(kTileThreads, 2) void ff_tile_kernel(const TileArgs<T> a)
+template <typename T, int SLOTS, bool TR, bool GATED, bool DMA>
+__global__ __launch_bounds__(kTileThreads, 4) void ff_tile_kernel(const TileArgs<T> a)
 {
+    using Shape = TileShape<SLOTS>;
+    constexpr int kSlots = Shape::kSlots, WS = Shape::WS, kDeep = Shape::kDeep, kPairs = Shape::kPairs, kABytes = Shape::kABytes;
+    constexpr int kTileStage = Shape::kStage, kPlaceRow = Shape::kPlaceRow, kPasses = Shape::kPasses;
     constexpr int kOutRows = GATED ? kSlots / 2 : kSlots;  // block-rows of the result
-    __shared__ __align__(16) unsigned char smem[kTileLds];
+    __shared__ __align__(16) unsigned char smem[Shape::kLds];
     // byte offsets of the blocks, or kNone
     uint32_t(*const place)[kPlaceRow] = reinterpret_cast<uint32_t(*)[kPlaceRow]>(smem + 2 * kTileStage);
     const int t = threadIdx.x, lane = t & 63;
@@ -115,20 +136,21 @@ __global__ __launch_bounds__(kTileThreads, 2) void ff_tile_kernel(const TileArgs
 
     const uint32_t lds0 = lds_address(smem);
     const uint32_t ld = (uint32_t)a.N * 2u;
-    constexpr int kAPer = kSlots / (2 * WC);                  // a wave's loads of A per step
-    constexpr int kXPer = kDeep;                       // and of x
+    constexpr int kAPer = kSlots / kTileWaves;                      // slots whose blocks a wave loads
+    constexpr int kXPer = 16 * kDeep * kXRow / 1024 / kTileWaves;  // and its loads of x
 
     // Wave w moves the blocks of kAPer slots from kAPer w on and kRowsPer rows of x
-    // from kRowsPer w on, a KB per load.  This lane's bytes: of a block (16 at p = lane % 32), and of x from
-    // the first step on; rows past the last are past the end of x.
+    // from kRowsPer w on, a KB per load.  This lane's bytes: of a block (16 at p =
+    // lane % 32), and of x from the first step on; rows past the last are past the
+    // end of x.
     const int p = lane & 31;
     const uint32_t a_lane = (uint32_t)((p >> 1) * 32 + (((p & 1) ^ a_swizzle(p >> 1)) * 16));
-    constexpr int kRowsPer = 16 * kDeep / (2 * WC);
+    constexpr int kRowsPer = 16 * kDeep / kTileWaves;
     uint32_t x_lane[kXPer];
 #pragma unroll
     for (int u = 0; u < kXPer; ++u) {
-        const int e = kRowsPer * wave + kRowsPer / kXPer * u + lane / (8 * WC);
-        const int64_t n = n0 + 8 * (lane % (8 * WC) ^ x_swizzle(e));
+        const int e = kRowsPer * wave + kRowsPer / kXPer * u + lane / (kWide / 8);
+        const int64_t n = n0 + 8 * (lane % (kWide / 8) ^ x_swizzle(e));
         x_lane[u] = n < a.N ? (uint32_t)e * ld + (uint32_t)n * 2u : kNone;
     }
     const uint32_t* const dma_place = &place[kAPer * wave][lane >> 5];
@@ -137,25 +159,19 @@ __global__ __launch_bounds__(kTileThreads, 2) void ff_tile_kernel(const TileArgs
     // Operands: row 4 g + li / 4 of a block (or of x), 8-byte piece li % 4; of A
     // itself row li, values 4 g .. + 3.
     const int r4 = 4 * g + (li >> 2), piece = (li & 3) >> 1;
-    uint32_t x_at[4];
+    uint32_t x_at[TT];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        x_at[j] = (uint32_t)(kABytes + r4 * kXRow + 8 * (li & 1) + (((2 * (4 * wc + j) + piece) ^ x_swizzle(r4)) * 16));
+    for (int j = 0; j < TT; ++j)
+        x_at[j] = (uint32_t)(kABytes + r4 * kXRow + 8 * (li & 1) + (((2 * (TT * wc + j) + piece) ^ x_swizzle(r4)) * 16));
     const uint32_t a_at = (uint32_t)(WS * wr * kDeep * 512 + (TR ? r4 * 32 + ((piece ^ a_swizzle(r4)) * 16) + 8 * (li & 1)
                                                                 : li * 32 + (((g >> 1) ^ a_swizzle(li)) * 16) + 8 * (g & 1)));
 
-    float4_t acc[WS][4];
+    float4_t acc[WS][TT];
 #pragma unroll
     for (int s = 0; s < WS; ++s)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[s][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < TT; ++j) acc[s][j] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-    // The operands of a pair of block-columns.  Those of A^T are read with those of
-    // x, of blocks that are not there too (what lies in their places is not used);
-    // those of A, whose reads have bank conflicts, at a block's own instructions.
-    struct Operands {
-        u32x2_t x[kDeep][4], a[kDeep][TR ? WS : 1];
-    };
     auto a_operand = [&](const unsigned char* S, int s, int d) {
         const unsigned char* q = S + a_at + (s * kDeep + d) * 512;
         if constexpr (TR)
@@ -163,42 +179,42 @@ __global__ __launch_bounds__(kTileThreads, 2) void ff_tile_kernel(const TileArgs
         else
             return *reinterpret_cast<const u32x2_t*>(q);
     };
-    auto read = [&](Operands& o, const unsigned char* S, int d) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o.x[d][j] = read_transposed(S + x_at[j] + 16 * d * kXRow);
-        if constexpr (TR)
-#pragma unroll
-            for (int s = 0; s < WS; ++s) o.a[d][s] = a_operand(S, s, d);
-    };
     // Blocks d and d + 1 of every slot; stored: bit kDeep s + d, block d of this
     // wave's slot s.  Three conditions of their own, not alternatives: an accumulator
     // with more than one way to its new value is copied on all of them.
-    auto multiply = [&](const Operands& o, const unsigned char* S, uint32_t stored, int d) {
+    auto multiply = [&](const unsigned char* S, uint32_t stored, int d) {
+        u32x2_t x[2][TT];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < TT; ++j) x[e][j] = read_transposed(S + x_at[j] + 16 * (d + e) * kXRow);
+        // ahead of the waves that are still on their way from the barrier: the matrix
+        // units are not to wait for these (5 % of the time)
+        __builtin_amdgcn_s_setprio(1);
         uint32_t pairs = stored & (stored >> 1), firsts = stored & ~(stored >> 1), seconds = ~stored & (stored >> 1);
         asm volatile("" : "+s"(pairs), "+s"(firsts), "+s"(seconds));
-        auto operand = [&](int s, int e) { return TR ? o.a[e][TR ? s : 0] : a_operand(S, s, e); };
 #pragma unroll
         for (int s = 0; s < WS; ++s) {
             const uint32_t bit = 1u << (kDeep * s + d);
             if (pairs & bit) {
-                const u32x2_t p = operand(s, d), q = operand(s, d + 1);
+                const u32x2_t p = a_operand(S, s, d), q = a_operand(S, s, d + 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < TT; ++j)
                     acc[s][j] = mfma16<T>(u32x4_t{p.x, p.y, q.x, q.y},
-                                          u32x4_t{o.x[d][j].x, o.x[d][j].y, o.x[d + 1][j].x, o.x[d + 1][j].y},
-                                          acc[s][j]);
+                                          u32x4_t{x[0][j].x, x[0][j].y, x[1][j].x, x[1][j].y}, acc[s][j]);
             }
             if (firsts & bit) {
-                const u32x2_t p = operand(s, d);
+                const u32x2_t p = a_operand(S, s, d);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[s][j] = mfma16_half<T>(p, o.x[d][j], acc[s][j]);
+                for (int j = 0; j < TT; ++j) acc[s][j] = mfma16_half<T>(p, x[0][j], acc[s][j]);
             }
             if (seconds & bit) {
-                const u32x2_t q = operand(s, d + 1);
+                const u32x2_t q = a_operand(S, s, d + 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[s][j] = mfma16_half<T>(q, o.x[d + 1][j], acc[s][j]);
+                for (int j = 0; j < TT; ++j) acc[s][j] = mfma16_half<T>(q, x[1][j], acc[s][j]);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     };
 
     // Windows of the sum, with the positions of their blocks in LDS.
@@ -240,8 +256,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void ff_tile_kernel(const TileArgs
 #pragma unroll
                 for (int u = 0; u < kAPer * kPairs; ++u) {
                     const int s = u / kPairs, h = u % kPairs;
-                    dma_to_lds(to + (uint32_t)((kAPer * wave + s) * kDeep + 2 * h) * 512u, next_dma[u] + a_lane,
-                               GATED && slot_side(kAPer * wave + s) ? vals1 : vals0);
+                    if (__ballot(next_dma[u] != kNone))
+                        dma_to_lds(to + (uint32_t)((kAPer * wave + s) * kDeep + 2 * h) * 512u, next_dma[u] + a_lane,
+                                   GATED && slot_side(kAPer * wave + s) ? vals1 : vals0);
                 }
 #pragma unroll
                 for (int u = 0; u < kXPer; ++u) {
@@ -271,70 +288,42 @@ __global__ __launch_bounds__(kTileThreads, 2) void ff_tile_kernel(const TileArgs
             };
             look(0);
             uint32_t coming = issue(0);
-            if constexpr (TR) {
-                // a step is multiplied from registers while the next one's operands are
-                // read and the loads of the one after that are under way
-                uint32_t stored = coming;
-                Operands even, odd;
-                landed(0);
-                coming = 1 < steps ? issue(1) : 0u;
+            for (int32_t st = 0; st < steps; ++st) {
+                const uint32_t stored = coming;
+                landed(st);
+                if (st + 1 < steps) coming = issue(st + 1);
 #pragma unroll
-                for (int d = 0; d < kDeep; ++d) read(even, smem, d);
-                auto round = [&](int32_t st, const Operands& now, Operands& then) {
-                    const uint32_t mine = stored;
-                    if (st + 1 < steps) {
-                        stored = coming;
-                        landed(st + 1);
-                        coming = st + 2 < steps ? issue(st + 2) : 0u;
-#pragma unroll
-                        for (int d = 0; d < kDeep; ++d) read(then, smem + ((st + 1) & 1) * kTileStage, d);
-                    }
-#pragma unroll
-                    for (int d = 0; d < kDeep; d += 2) multiply(now, smem, mine, d);
-                };
-                for (int32_t st = 0; st < steps; st += 2) {
-                    round(st, even, odd);
-                    if (st + 1 < steps) round(st + 1, odd, even);
-                }
-            } else {
-                for (int32_t st = 0; st < steps; ++st) {
-                    const uint32_t stored = coming;
-                    landed(st);
-                    if (st + 1 < steps) coming = issue(st + 1);
-                    const unsigned char* S = smem + (st & 1) * kTileStage;
-                    Operands o;
-#pragma unroll
-                    for (int d = 0; d < kDeep; d += 2) {
-                        read(o, S, d);
-                        read(o, S, d + 1);
-                        multiply(o, S, stored, d);
-                    }
-                }
+                for (int d = 0; d < kDeep; d += 2) multiply(smem + (st & 1) * kTileStage, stored, d);
             }
         }
     }
 
-    // The sums leave through LDS, so that the rest is done on eight tokens of a row
-    // per thread.
+    // The sums leave through LDS, eight block-rows of a product at a time, so that the
+    // rest is done on eight tokens of a row per thread.
     float* O = reinterpret_cast<float*>(smem);
-    __syncthreads();
+    constexpr int kPassWaves = kTileWaves / WC / kPasses;  // rows of waves of a pass
+#pragma unroll 1
+    for (int pass = 0; pass < kPasses; ++pass) {
+        __syncthreads();
+        if (wr / kPassWaves == pass)
 #pragma unroll
-    for (int s = 0; s < WS; ++s)
+            for (int s = 0; s < WS; ++s)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < TT; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                O[(16 * (WS * wr + s) + 4 * g + q) * kOutRow + 64 * wc + 16 * j + li] = acc[s][j][q];
-    __syncthreads();
-    {
-        constexpr int kOut = 16 * kOutRows;
+                    for (int q = 0; q < 4; ++q)
+                        O[(16 * (WS * (wr % kPassWaves) + s) + 4 * g + q) * kOutRow + 16 * (TT * wc + j) + li] =
+                            acc[s][j][q];
+        __syncthreads();
+        constexpr int kOut = 16 * kOutRows / kPasses;
+        static_assert(kOut * (kWide / 8) % kTileThreads == 0);
 #pragma unroll 1
         for (int v = 0; v < kOut * (kWide / 8) / kTileThreads; ++v) {
             const int at = v * kTileThreads + t, r = at / (kWide / 8), c = at % (kWide / 8) * 8;
             // the block-row's slot, of a gated product the gate's, with the up
             // projection's WS / 2 slots on
             const int from = GATED ? 16 * (r / (8 * WS) * WS) + r % (8 * WS) : r;
-            const int64_t row = 16 * (int64_t)br0 + r, n = n0 + c;
+            const int64_t row = 16 * (int64_t)br0 + kOut * pass + r, n = n0 + c;
             if (row >= a.rows || n + 8 <= first || n >= a.N) continue;
             const bool whole = n >= first && n + 8 <= a.N;
             float z[2][8];
@@ -389,31 +378,53 @@ __global__ __launch_bounds__(kTileThreads, 2) void ff_tile_kernel(const TileArgs
     }
 }
 
-template <typename T, bool TR, bool GATED>
-void launch_tile(const TileArgs<T>& a, hipStream_t s)
+template <typename T, int SLOTS, bool TR, bool GATED>
+void launch_shape(const TileArgs<T>& a, hipStream_t s)
 {
-    constexpr int rows = GATED ? kSlots / 2 : kSlots;
+    constexpr int rows = GATED ? SLOTS / 2 : SLOTS;
     const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + kWide - 1) / kWide);
     const int64_t grid = kXcds * xcd_chunk(items);
     if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many tokens for one launch.");
     if (a.N % 8 == 0)
-        hipLaunchKernelGGL((ff_tile_kernel<T, TR, GATED, true>), dim3((unsigned)grid), dim3(kTileThreads), 0, s, a);
+        hipLaunchKernelGGL((ff_tile_kernel<T, SLOTS, TR, GATED, true>), dim3((unsigned)grid), dim3(kTileThreads), 0, s,
+                           a);
     else
-        hipLaunchKernelGGL((ff_tile_kernel<T, TR, GATED, false>), dim3((unsigned)grid), dim3(kTileThreads), 0, s, a);
+        hipLaunchKernelGGL((ff_tile_kernel<T, SLOTS, TR, GATED, false>), dim3((unsigned)grid), dim3(kTileThreads), 0, s,
+                           a);
     XSPMM_LAUNCH_CHECK();
 }
 
-// Whether the share of stored blocks is one at which tiles are faster than walking
-// the block-rows one by one (14336 x 4096 fp16, 2048 tokens, us by tiles and by
-// rows: y 25 % 220 and 212, 50 % 257 and 365, all 310 and 640; two weights 25 %
-// 416 and 391, 50 % 486 and 717; dx 25 % 192 and 188, 50 % 218 and 353, all 244 and
-// 670), of a token tile that may be filled in part, and whether they are enough
-// for the chip (a workgroup walks its whole sum).
-bool tiles_pay(int64_t blocks, int64_t grid_blocks, int64_t N, int64_t row_groups)
+// Block-rows of a workgroup; 0 where walking the block-rows one by one is faster.
+//
+// The time of tiles goes by the rounds of two workgroups a CU, a last one of one a
+// CU taking four fifths as long; that of the walk by what is stored.  Sixteen
+// block-rows where there is more than one such workgroup a CU (16-bit, 4096 x 4096
+// gated, 25 % stored, us by sixteen and by eight: 2048 tokens 87 and 103, 1024 tokens,
+// one workgroup a CU, 75 and 55).  The shares from which tiles of a full round pay are
+// from 18 % and 25 % stored, us by tiles and by rows: by sixteen, 14336 x 4096, 2048
+// tokens, 148 and 164, 157 and 211, by eight, 4096 x 14336, 154 and 137, 160 and 185;
+// all stored 256 and 650, 266 and 655.
+double rounds(int64_t workgroups)
+{
+    const int64_t whole = workgroups / 512, rest = workgroups % 512;
+    return (double)whole + (rest == 0 ? 0.0 : rest <= 256 ? 0.8 : 1.0);
+}
+int tile_slots(int64_t blocks, int64_t grid_blocks, int64_t N, int64_t slots)
 {
     const int64_t tiles = (N + kWide - 1) / kWide;
-    if (row_groups * tiles < 256) return false;
-    return (double)blocks * (double)N >= 0.28 * (double)grid_blocks * (double)(tiles * kWide);
+    const int shape = (slots + 15) / 16 * tiles > 256 ? 16 : 8;
+    const int64_t n = (slots + shape - 1) / shape * tiles;
+    const double filled = (double)blocks * (double)N / ((double)grid_blocks * (double)(tiles * kWide));
+    return filled * (double)n >= (shape == 16 ? 0.155 : 0.2) * 512.0 * rounds(n) ? shape : 0;
+}
+
+template <typename T, bool TR, bool GATED>
+void launch_tile(const TileArgs<T>& a, int slots, hipStream_t s)
+{
+    if (slots == 16)
+        launch_shape<T, 16, TR, GATED>(a, s);
+    else
+        launch_shape<T, 8, TR, GATED>(a, s);
 }
 
 }  // namespace ff
@@ -432,9 +443,8 @@ bool feed_forward_tiles(const ForwardArgs<T>& f, int weights, hipStream_t s)
         blocks += wl.nnzb;
     }
     const int64_t xb = narrow_bytes(w.K, f.N, 2);
-    if (xb < 0 || (f.N % 8 != 0 && f.N < ff::kWide) ||
-        !ff::tiles_pay(blocks, weights * w.Mb * w.Kb, f.N, w.Mb * weights / ff::kSlots))
-        return false;
+    const int slots = ff::tile_slots(blocks, weights * w.Mb * w.Kb, f.N, w.Mb * weights);
+    if (xb < 0 || (f.N % 8 != 0 && f.N < ff::kWide) || slots == 0) return false;
     a.residual = f.residual;
     a.y = f.y;
     a.sides = weights;
@@ -447,9 +457,9 @@ bool feed_forward_tiles(const ForwardArgs<T>& f, int weights, hipStream_t s)
     a.x_bytes = (uint32_t)xb;
     a.act = f.act;
     if (weights == 2)
-        ff::launch_tile<T, false, true>(a, s);
+        ff::launch_tile<T, false, true>(a, slots, s);
     else
-        ff::launch_tile<T, false, false>(a, s);
+        ff::launch_tile<T, false, false>(a, slots, s);
     return true;
 }
 
@@ -467,9 +477,8 @@ bool transposed_tiles(const TransposedArgs<T>& f, int weights, hipStream_t s)
         blocks += wl.nnzb;
     }
     const int64_t xb = narrow_bytes(w.M, f.N, 2);
-    if (xb < 0 || (f.N % 8 != 0 && f.N < ff::kWide) ||
-        !ff::tiles_pay(blocks, weights * w.Mb * w.Kb, f.N, w.Kb / ff::kSlots))
-        return false;
+    const int slots = ff::tile_slots(blocks, weights * w.Mb * w.Kb, f.N, w.Kb);
+    if (xb < 0 || (f.N % 8 != 0 && f.N < ff::kWide) || slots == 0) return false;
     a.y = f.dx;
     a.sides = weights;
     a.rows = (int32_t)w.K;
@@ -479,7 +488,7 @@ bool transposed_tiles(const TransposedArgs<T>& f, int weights, hipStream_t s)
     a.in_rows = (int32_t)w.M;
     a.N = f.N;
     a.x_bytes = (uint32_t)xb;
-    ff::launch_tile<T, true, false>(a, s);
+    ff::launch_tile<T, true, false>(a, slots, s);
     return true;
 }
 
