@@ -210,6 +210,14 @@ def test_weight_gradient_tiles(kind, M, K, N, density):
     assert not dv.cpu()[~where[2].reshape(-1)].any()
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,K,N", [(4090, 2040, 136), (2040, 4090, 8), (4090, 2040, 75)])
+@pytest.mark.parametrize("density", [0.3, 0.7])
+def test_weight_gradient_tiles_of_a_full_chip(kind, M, K, N, density):
+    """The same where there are tiles enough for every compute unit."""
+    test_weight_gradient_tiles(kind, M, K, N, density)
+
+
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("M,K,N", [(300, 290, 136), (290, 300, 131), (64, 2100, 128), (2100, 64, 264), (1100, 1300, 200),
                                    (700, 90, 257)])

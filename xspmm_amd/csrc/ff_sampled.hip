@@ -292,8 +292,12 @@ bool sampled_wave(const SampledArgs<T>& f, int l, hipStream_t s)
 
 // ---------------------------------------------------------------------------
 // Tiles: a workgroup takes 128 rows of dz and 128 rows of x, 128 bytes of each at
-// a time through LDS, and multiplies where the tile holds a block.  A wave owns
-// 4 x 4 of its positions, with an accumulator for each.
+// a time through LDS, and multiplies where the tile holds a block.  Each of eight
+// waves owns 2 x 4 of its positions, with an accumulator for each; two workgroups
+// share a CU.  (With four waves of 4 x 4, which read a third less from LDS but are
+// two a SIMD, 14336 x 4096 fp16 of 2048 tokens took 222 us at 25 % stored and 270 at
+// 100 %; so it is 174 and 245, 980 TFLOP/s.  The loads alone, 3.8 GB at 24 TB/s from
+// L2, take 157.)
 //
 // Every row of the tile is read once for all its blocks, where the kernel above
 // reads both rows anew for each block; what is not stored costs its share of the
@@ -318,8 +322,9 @@ struct SampledTile {
     int32_t sides;
 };
 
-constexpr int kWR = 2, kWC = 2, kB = 4;   // a grid of 2 x 2 waves with 4 x 4 positions each
-constexpr int kEdge = kWR * kB;           // blocks along either edge of a tile
+constexpr int kWR = 4, kWC = 2;           // a grid of waves,
+constexpr int kBR = 2, kBC = 4;           // the positions of each
+constexpr int kEdge = kWR * kBR;          // blocks along either edge of a tile
 constexpr int kSide = 16 * kEdge;         // its rows of dz, and of x
 constexpr int kThreads = 64 * kWR * kWC;
 constexpr int kLine = 128;                // bytes of a row per step, a line of memory
@@ -327,10 +332,10 @@ constexpr int kPieces = kLine / 16;
 constexpr int kStage = 2 * kSide * kLine;
 constexpr int kLoads = 2 * kSide * kPieces / kThreads;  // chunks a thread moves per step
 constexpr int kBand = 8;
-static_assert(kWR == kWC && kEdge * kEdge <= kThreads && kB * kB <= 32);
+static_assert(kWR * kBR == kWC * kBC && kEdge * kEdge <= kThreads && kBR * kBC <= 32);
 
 template <typename T, bool DMA>
-__global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const SampledTile<T> a)
+__global__ __launch_bounds__(kThreads, kThreads / 128) void ff_sampled_tile_kernel(const SampledTile<T> a)
 {
     constexpr int V = 16 / sizeof(T);                // tokens of a chunk
     constexpr int kTokens = kLine / (int)sizeof(T);  // of a step
@@ -360,10 +365,10 @@ __global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const Sampled
         place[t] = r < a.Mb && c < a.Kb ? s.map[(int64_t)r * a.Kb + c] : -1;
     }
     __syncthreads();
-    uint32_t mask;  // bit r kB + c: this wave's block (r, c) is stored
+    uint32_t mask;  // bit r kBC + c: this wave's block (r, c) is stored
     {
-        const int r = lane / kB, c = lane % kB;
-        const bool there = lane < kB * kB && place[(wr * kB + r) * kEdge + wc * kB + c] >= 0;
+        const int r = lane / kBC, c = lane % kBC;
+        const bool there = lane < kBR * kBC && place[(wr * kBR + r) * kEdge + wc * kBC + c] >= 0;
         mask = (uint32_t)__ballot(there);
     }
     if (!__syncthreads_or(mask != 0)) return;
@@ -421,28 +426,28 @@ __global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const Sampled
         }
     };
 
-    float4_t acc[kB][kB];
+    float4_t acc[kBR][kBC];
 #pragma unroll
-    for (int r = 0; r < kB; ++r)
+    for (int r = 0; r < kBR; ++r)
 #pragma unroll
-        for (int c = 0; c < kB; ++c) acc[r][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < kBC; ++c) acc[r][c] = float4_t{0.f, 0.f, 0.f, 0.f};
 
     auto compute = [&](int32_t st) {
 #pragma unroll
         for (int h = 0; h < kPieces / 4; ++h) {
             const unsigned char* S =
                 smem + (st % 2) * kStage + li * kLine + (((4 * h + g) ^ swizzle(li)) * 16);
-            u32x4_t xo[kB];
+            u32x4_t xo[kBC];
 #pragma unroll
-            for (int c = 0; c < kB; ++c)
-                xo[c] = *reinterpret_cast<const u32x4_t*>(S + (kSide + 16 * (wc * kB + c)) * kLine);
+            for (int c = 0; c < kBC; ++c)
+                xo[c] = *reinterpret_cast<const u32x4_t*>(S + (kSide + 16 * (wc * kBC + c)) * kLine);
 #pragma unroll
-            for (int r = 0; r < kB; ++r) {
-                if (!((mask >> (r * kB)) & ((1u << kB) - 1u))) continue;
-                const u32x4_t d = *reinterpret_cast<const u32x4_t*>(S + 16 * (wr * kB + r) * kLine);
+            for (int r = 0; r < kBR; ++r) {
+                if (!((mask >> (r * kBC)) & ((1u << kBC) - 1u))) continue;
+                const u32x4_t d = *reinterpret_cast<const u32x4_t*>(S + 16 * (wr * kBR + r) * kLine);
 #pragma unroll
-                for (int c = 0; c < kB; ++c)
-                    if (mask & (1u << (r * kB + c))) {
+                for (int c = 0; c < kBC; ++c)
+                    if (mask & (1u << (r * kBC + c))) {
                         if constexpr (is_f32<T>) {
 #pragma unroll
                             for (int q = 0; q < 4; ++q) acc[r][c] = mfma32(xo[c][q], d[q], acc[r][c]);
@@ -472,12 +477,12 @@ __global__ __launch_bounds__(kThreads) void ff_sampled_tile_kernel(const Sampled
 
     // lane: row li of a block, columns 4 g .. + 3
 #pragma unroll
-    for (int r = 0; r < kB; ++r)
+    for (int r = 0; r < kBR; ++r)
 #pragma unroll
-        for (int c = 0; c < kB; ++c) {
-            if (!(mask & (1u << (r * kB + c)))) continue;
-            const int32_t b = place[(wr * kB + r) * kEdge + wc * kB + c];
-            const int32_t row = 16 * (br0 + wr * kB + r) + li, col = 16 * (bc0 + wc * kB + c) + 4 * g;
+        for (int c = 0; c < kBC; ++c) {
+            if (!(mask & (1u << (r * kBC + c)))) continue;
+            const int32_t b = place[(wr * kBR + r) * kEdge + wc * kBC + c];
+            const int32_t row = 16 * (br0 + wr * kBR + r) + li, col = 16 * (bc0 + wc * kBC + c) + 4 * g;
             Pack<T, 4> o;
 #pragma unroll
             for (int q = 0; q < 4; ++q) o.v[q] = (T)(row < a.M && col + q < a.K ? acc[r][c][q] : 0.f);
@@ -525,13 +530,22 @@ bool sampled_tiles(const SampledArgs<T>& f, int weights, hipStream_t s)
     }
     if (a.sides == 0) return true;
     // The share of stored blocks from which a tile's rows are cheaper than the rows
-    // of each four blocks (14336 x 4096 fp16, 2048 tokens: 10 % stored 102 us by
-    // fours, 199 by tiles, 25 % 243 and 228; 4096 x 4096 fp32, 512 tokens: 50 % 102
-    // and 114, all 188 and 149), or, off 16 bytes, than those read operand by
-    // operand (fp16, 5 %: 140 us and 180, 10 % 245 and 199).
+    // of each four blocks (14336 x 4096 fp16, 2048 tokens, us by tiles and by fours:
+    // 15 % stored 169 and 148, 20 % 173 and 194; 4096 x 4096 fp32, 512 tokens: 45 % 95
+    // and 86, 60 % 113 and 108, 80 % 128 and 139), or, off 16 bytes, than those read
+    // operand by operand (fp16, 2047 tokens, 3 %: 324 and 366; fp32, 511 tokens, 10 %
+    // 62 and 58, 15 % 68 and 72).
+    // Tiles take rounds of two workgroups a CU, and a round of one a CU seven tenths
+    // of that; blocks by fours fill the chip sooner (1024 x 1024, 2048 tokens, all
+    // stored: fp16 25 us by tiles and 19, fp32 143 and 48).  Not so operand by operand
+    // in 16 bits (2047 tokens, 40 % stored 44 us by tiles and 109).
     const bool aligned = f.N * sizeof(T) % 16 == 0;
-    const int64_t share = aligned ? (is_f32<T> ? 155 : 56) : (is_f32<T> ? 46 : 18);  // of 256
-    if (blocks * 256 < share * a.sides * w.Mb * w.Kb) return false;
+    const double share = (aligned ? (is_f32<T> ? 160 : 46) : (is_f32<T> ? 32 : 7)) / 256.0;
+    const int64_t tiles = (int64_t)((a.Mb + kEdge - 1) / kEdge) * ((a.Kb + kEdge - 1) / kEdge) * a.sides;
+    const int64_t rest = tiles % 512;
+    const double rounds = (double)(tiles / 512) + (rest == 0 ? 0.0 : rest <= 256 ? 0.7 : 1.0);
+    const double fill = aligned || is_f32<T> ? (double)tiles / (512.0 * rounds) : 1.0;
+    if ((double)blocks * fill < share * (double)(a.sides * w.Mb * w.Kb)) return false;
     launch_sampled_tile<T>(a, aligned, s);
     return true;
 }
