@@ -11,6 +11,13 @@
 // (n, m, M2): n = na + nb, d = mb - ma, m = ma + d nb / n,
 // M2 = M2a + M2b + d^2 na nb / n, which loses nothing where a feature is far
 // off the others.  All sums are fp32, in a fixed order.
+//
+// Both passes are bound by memory: x (backward: x and dy) is read twice, as no
+// workgroup can hold a column tile wide enough for whole lines of memory, the second
+// time from the cache that sits before HBM where it fits.  Forward, fp16 4096 x
+// 2048: 7.2 + 9.2 us, 2.3 and 3.6 TB/s, of which launch and first latency are about 5
+// (columns held in registers, 16 tokens a workgroup: 20).  Backward, bf16 4096 x
+// 8001: 30 + 31 us, 4.4 and 6.3 TB/s.
 #include "feed_forward_device.hpp"
 
 namespace xspmm {
@@ -27,7 +34,7 @@ struct NormShape {
     int64_t len;      // rows per slice
 };
 
-constexpr int kForwardWaves = 8, kBackwardWaves = 4;
+constexpr int kForwardWaves = 8, kBackwardWaves = 8;
 
 // count (the same for all V columns), means, sums of squared deviations
 template <int V>
@@ -460,52 +467,48 @@ __device__ __forceinline__ float2 sum_strided(const float2* p, int64_t n, int64_
     return {a, b};
 }
 
-// workgroups [0, ceil(N / 64)): a column's means; the rest: a row's sums
+// dweight and dbias of row k
 template <typename T>
-__global__ __launch_bounds__(64) void ln_backward_join_kernel(const float2* __restrict__ colpart,
-                                                               const float2* __restrict__ rowpart,
-                                                               float2* __restrict__ means, T* __restrict__ dw,
-                                                               T* __restrict__ db, int64_t K, int64_t N, NormShape h)
+__device__ __forceinline__ void join_row(const float2* __restrict__ rowpart, T* __restrict__ dw, T* __restrict__ db,
+                                         int64_t k, int64_t K, int64_t tiles)
 {
-    const int64_t cols = (N + 63) / 64;
-    if (blockIdx.x < cols) {
-        const int64_t n = (int64_t)blockIdx.x * 64 + threadIdx.x;
-        if (n >= N) return;
-        const float2 p = sum_strided(colpart + n, h.slices, N);
-        means[n] = float2{p.x / (float)K, p.y / (float)K};
-    } else {
-        const int64_t k = ((int64_t)blockIdx.x - cols) * 64 + threadIdx.x;
-        if (k >= K) return;
-        const float2 p = sum_strided(rowpart + k, h.tiles, K);
-        if (dw) dw[k] = (T)p.x;
-        if (db) db[k] = (T)p.y;
-    }
+    const float2 p = sum_strided(rowpart + k, tiles, K);
+    if (dw) dw[k] = (T)p.x;
+    if (db) db[k] = (T)p.y;
 }
 
+// where dx is not wanted
+template <typename T>
+__global__ __launch_bounds__(64) void ln_backward_rows_kernel(const float2* __restrict__ rowpart, T* __restrict__ dw,
+                                                               T* __restrict__ db, int64_t K, int64_t tiles)
+{
+    const int64_t k = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    if (k < K) join_row(rowpart, dw, db, k, K, tiles);
+}
+
+// As in the forward pass, every workgroup joins the slices' sums of its columns
+// itself, and those of its share of the rows (in a launch of its own between the two,
+// fp16 16384 x 100 took 33 us and bf16 4096 x 2048 30; so it is 17 and 25).
 template <typename T, int V>
 __global__ __launch_bounds__(64 * kBackwardWaves) void ln_backward_apply_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ w, const float* __restrict__ mean,
-    const float* __restrict__ rstd, const float2* __restrict__ means, T* __restrict__ dx, int64_t K, int64_t N,
-    NormShape h)
+    const float* __restrict__ rstd, const float2* __restrict__ colpart, const float2* __restrict__ rowpart,
+    T* __restrict__ dx, T* __restrict__ dw, T* __restrict__ db, int64_t K, int64_t N, NormShape h)
 {
+    constexpr int kThreads = 64 * kBackwardWaves;
+    __shared__ float2 red[kThreads];
+    __shared__ float2 means[64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t tile = blockIdx.x / h.slices, slice = blockIdx.x % h.slices;
     const int64_t at = min((tile * h.np + lane % h.np) * V, N - V);
     const int64_t k1 = min(K, (slice + 1) * h.len);
     const int per = 64 / h.np;
-    const auto m = load_tokens<float, V>(mean + at), r = load_tokens<float, V>(rstd + at);
-    float c1[V], c2[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float2 p = means[at + i];
-        c1[i] = p.x;
-        c2[i] = p.y;
-    }
     constexpr int U = 4;
     const int64_t step = kBackwardWaves * per;
-    for (int64_t k = slice * h.len + wave * per + lane / h.np; k < k1; k += U * step) {
-        Pack<T, V> g[U], v[U];
-        T wt[U];
+    int64_t k = slice * h.len + wave * per + lane / h.np;
+    Pack<T, V> g[U], v[U];
+    T wt[U];
+    auto load = [&] {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t q = min(k + u * step, k1 - 1);
@@ -513,6 +516,41 @@ __global__ __launch_bounds__(64 * kBackwardWaves) void ln_backward_apply_kernel(
             v[u] = load_tokens<T, V>(x + q * N + at);
             if (w) wt[u] = w[q];
         }
+    };
+    if (k < k1) load();  // under way while the sums are joined
+    const auto m = load_tokens<float, V>(mean + at), r = load_tokens<float, V>(rstd + at);
+    const int cols = h.np * V, shares = max(kThreads / cols, 1);
+    const int64_t base = max(min(tile * cols, N - cols), (int64_t)0);  // the last tile moves back
+    for (int c0 = 0; c0 < cols; c0 += kThreads) {
+        const int c = c0 + threadIdx.x % cols, share = threadIdx.x / cols;
+        const int64_t col = base + c;
+        float2 sum = {0.f, 0.f};
+        if (share < shares && col < N && share < h.slices)
+            sum = sum_strided(colpart + share * N + col, (h.slices - share + shares - 1) / shares, shares * N);
+        red[threadIdx.x] = sum;
+        __syncthreads();
+        if (share == 0) {
+            for (int q = 1; q < shares; ++q) {
+                const float2 o = red[q * cols + c];
+                sum.x += o.x;
+                sum.y += o.y;
+            }
+            means[c] = float2{sum.x / (float)K, sum.y / (float)K};
+        }
+        __syncthreads();
+    }
+    {
+        const int64_t rows = (K + gridDim.x - 1) / gridDim.x, end = min(K, (blockIdx.x + 1) * rows);
+        for (int64_t q = blockIdx.x * rows + threadIdx.x; q < end; q += kThreads) join_row(rowpart, dw, db, q, K, h.tiles);
+    }
+    float c1[V], c2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float2 q = means[at - base + i];
+        c1[i] = q.x;
+        c2[i] = q.y;
+    }
+    while (k < k1) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (k + u * step >= k1) break;
@@ -523,6 +561,8 @@ __global__ __launch_bounds__(64 * kBackwardWaves) void ln_backward_apply_kernel(
                 o[i] = ((float)g[u].v[i] * wk - c1[i] - ((float)v[u].v[i] - m.v[i]) * r.v[i] * c2[i]) * r.v[i];
             store_tokens<T, V>(dx + (k + u * step) * N + at, o);
         }
+        k += U * step;
+        if (k < k1) load();
     }
 }
 
@@ -576,7 +616,6 @@ int64_t layer_norm_scratch(int64_t K, int64_t N, int64_t size, int backward)
         const NormShape h = backward_shape(K, N, size);
         c.take((size_t)(h.slices * N) * 8);
         c.take((size_t)(h.tiles * K) * 8);
-        c.take((size_t)N * 8);
     } else {
         if (small_norm(K, N)) return 0;
         const NormShape h = forward_shape(K, N, size);
@@ -625,17 +664,17 @@ void layer_norm_backward(const T* dy, const T* x, const T* weight, const float* 
     Carve c;
     float2* colpart = reinterpret_cast<float2*>(p + c.take((size_t)(h.slices * N) * 8));
     float2* rowpart = reinterpret_cast<float2*>(p + c.take((size_t)(h.tiles * K) * 8));
-    float2* means = reinterpret_cast<float2*>(p + c.take((size_t)N * 8));
     auto go = [&](auto v) {
         constexpr int V = decltype(v)::value;
         if (N > 0)
             hipLaunchKernelGGL((ln_backward_sums_kernel<T, V>), norm_grid(h), dim3(64 * kBackwardWaves), 0, s, dy, x,
                                weight, mean, rstd, colpart, rowpart, K, N, h);
-        hipLaunchKernelGGL((ln_backward_join_kernel<T>), dim3((unsigned)((N + 63) / 64 + (K + 63) / 64)),
-                           dim3(64), 0, s, colpart, rowpart, means, dweight, dbias, K, N, h);
         if (N > 0 && dx)
             hipLaunchKernelGGL((ln_backward_apply_kernel<T, V>), norm_grid(h), dim3(64 * kBackwardWaves), 0, s, dy, x,
-                               weight, mean, rstd, means, dx, K, N, h);
+                               weight, mean, rstd, colpart, rowpart, dx, dweight, dbias, K, N, h);
+        else if (dweight || dbias)
+            hipLaunchKernelGGL((ln_backward_rows_kernel<T>), dim3((unsigned)((K + 63) / 64)), dim3(64), 0, s, rowpart,
+                               dweight, dbias, K, h.tiles);
     };
     constexpr int most = 16 / sizeof(T);
     if (h.v == most)
