@@ -591,7 +591,15 @@ NormShape norm_shape(int64_t K, int64_t N, int v, int np, int waves, int64_t gro
     return h;
 }
 
-NormShape forward_shape(int64_t K, int64_t N, int64_t size) { return N < 64 ? norm_shape(K, N, 1, 64, kForwardWaves, 256) : norm_shape(K, N, (int)(16 / size), 16, kForwardWaves, 256); }
+// Lanes along the tokens: as many as leave 16 tiles, from 8 to 32 (us with 8, 16 and
+// 32: fp16 16384 x 100 14, 16, 16; 4096 x 2048 -, 17, 20; bf16 4096 x 8001, whose rows
+// start anywhere in a line, 63, 59, 37).
+NormShape forward_shape(int64_t K, int64_t N, int64_t size)
+{
+    if (N < 64) return norm_shape(K, N, 1, 64, kForwardWaves, 256);
+    const int v = (int)(16 / size), np = pow2_at_least(N / (16 * v), 32);
+    return norm_shape(K, N, v, np < 8 ? 8 : np, kForwardWaves, 256);
+}
 NormShape backward_shape(int64_t K, int64_t N, int64_t size)
 {
     return norm_shape(K, N, N < 256 ? 1 : (int)(16 / size), 64, kBackwardWaves, 512);
