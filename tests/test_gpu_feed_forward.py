@@ -405,6 +405,38 @@ def test_other_stream_and_repeats():
     assert torch.equal(y, y2) and all(torch.equal(a, b) for a, b in zip(grads, g2))
 
 
+def test_a_graph_of_the_layer():
+    """Captured forward and backward passes, replayed on new inputs with other work between the replays."""
+    G, U, D = (weight(M, K, 0.3, torch.bfloat16, i)[0] for i, (M, K) in enumerate([(400, 300), (400, 300), (300, 400)]))
+    x, dy = normal((300, 70), torch.bfloat16, 1), normal((300, 70), torch.bfloat16, 2)
+    w, b = normal((300,), torch.bfloat16, 3), normal((300,), torch.bfloat16, 4)
+
+    def passes():
+        n, mean, rstd = X.layer_norm(x, w, b, keep=True)
+        h, zg, zu = X.sparse_gated(G, U, n, activation="silu", keep=True)
+        y = X.sparse_linear(D, h, residual=x)
+        dh, dd, _ = X.sparse_linear_backward(D, h, None, dy)
+        dn, dg, du, _, _ = X.sparse_gated_backward(G, U, n, zg, zu, dh, activation="silu")
+        return (y, dd, dg, du) + tuple(X.layer_norm_backward(dn, x, w, mean, rstd))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        passes()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = passes()
+    for seed in range(5, 9):
+        x.copy_(normal((300, 70), torch.bfloat16, seed))
+        dy.copy_(normal((300, 70), torch.bfloat16, seed + 10))
+        want = [t.clone() for t in passes()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------------------------------
 # layer norm
 # ---------------------------------------------------------------------------
@@ -461,6 +493,21 @@ def test_layer_norm_backward(kind, K, N):
               + 8 * EPS32 * (f64(dy).abs() * (f64(x).abs() + f64(mean).abs()) * f64(rstd)).sum(1)
               + u * (f64(dy) * h).sum(1).abs() + TINY, "dweight")
         close(db, f64(dy).sum(1), (N + 16) * EPS32 * f64(dy).abs().sum(1) + u * f64(dy).sum(1).abs() + TINY, "dbias")
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("K,N", [(300, 3001), (1100, 2050), (130, 8001)])
+def test_layer_norm_wide(kind, K, N):
+    """Tiles of every width, and the parameters' gradients without dx."""
+    test_layer_norm(kind, K, N)
+    test_layer_norm_backward(kind, K, N)
+    x, w, dy = (normal(s, TYPES[kind][0], i) for i, s in enumerate([(K, N), (K,), (K, N)]))
+    _, mean, rstd = X.layer_norm(x, w, keep=True)
+    _, dw, db = X.layer_norm_backward(dy, x, w, mean, rstd)
+    none, dw2, db2 = X.layer_norm_backward(dy, x, w, mean, rstd, need=(False, True, True))
+    assert none is None and torch.equal(dw, dw2) and torch.equal(db, db2)
+    dx, none, db2 = X.layer_norm_backward(dy, x, w, mean, rstd, need=(True, False, True))
+    assert none is None and torch.equal(db, db2)
 
 
 def test_layer_norm_constant_and_not_finite():

@@ -8,8 +8,11 @@ This module is the Python view of that C ABI.  It mirrors the reference's
 operator interface -- ``CSRMatrix``, ``BCSRMatrix``, ``csr_to_bcsr``,
 ``compute_1d_jaccard_clustering``, ``apply_permutation``, Tier-1 ``spmm``,
 the Tier-2 pipeline ``spmm_pipeline`` and ``unpermute_dense_matrix`` -- with
-torch tensors as device buffers.  Every call goes to the HIP library; there
-is no CPU fallback, and importing the library fails loudly when it has not
+torch tensors as device buffers.  Beside it stands the feed-forward layer of a
+language model on block-sparse weights (``feed_forward``): ``SparseWeight``,
+``sparse_linear``, ``sparse_gated``, ``layer_norm``, their gradients and the
+``FeedForward`` module.  Every call goes to the HIP library; there is no CPU
+fallback, and importing the library fails loudly when it has not
 been built.
 """
 from __future__ import annotations

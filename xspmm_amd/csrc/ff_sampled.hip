@@ -13,7 +13,9 @@ namespace ff {
 
 // ---------------------------------------------------------------------------
 // One wave per four consecutive blocks (SPLIT waves share their tokens), operands
-// straight from memory: for few blocks and operands of any size.
+// straight from memory: for few blocks and operands of any size.  A load of 16 rows'
+// 16 bytes costs a lookup per row and lane, 64 of them, which is what bounds it
+// (14336 x 4096 fp16, 2047 tokens, 3 % stored: 366 us).
 // ---------------------------------------------------------------------------
 
 constexpr int kGroup = kGroupBlocks;  // stored blocks of a wave
@@ -153,7 +155,9 @@ __global__ __launch_bounds__(256) void ff_sampled_kernel(const int32_t* __restri
 // wave moves 128 bytes of its rows of dz and x at a time into LDS of its own, in
 // whole lines (the operands themselves are 16 bytes of 16 rows, and memory serves
 // one line at a time), one stage ahead of the one that it multiplies.  It waits
-// for nothing but its own loads.
+// for nothing but its own loads.  Bound by the L2: four blocks read five blocks'
+// rows, 14336 x 4096 fp16, 10 % stored, 2048 tokens 1.9 GB in 102 us, 18 TB/s; fp32
+// 4096 x 4096, 10 %, 512 tokens 29.4 us (57 without LDS), 58 TFLOP/s.
 template <typename T>
 struct SampledWave {
     const int32_t* group;
