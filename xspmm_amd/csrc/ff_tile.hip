@@ -17,16 +17,16 @@
 // are read from memory once for all the block-rows, where the kernel that walks
 // single block-rows reads them for every block.
 //
-// What a step costs is less the matrix instructions (14336 x 4096, 2048 tokens: 44 %
-// of the time where all blocks are stored, 30 % at a quarter of them) or the memory
-// (without its loads a step is a fifth shorter) than the way of a wave from the
-// barrier over its reads of LDS to its instructions, and the reads themselves.  Hence
-// two workgroups of eight waves on a CU, four waves a SIMD, that take turns (25 %
-// stored: 175 us; with four waves of four block-rows x 64 tokens each 218), and
-// sixteen block-rows where there are enough of them, so that a row of x is read from
-// LDS for four block-rows and not for two (158 us).  Measured: y 157 us at 25 %
-// stored and 250 at 100 % (960 TFLOP/s), both of a gated product's 300 and 475
-// (1010), dx, by eight, 162 and 269.
+// What bounds it, at 14336 x 4096 and 2048 tokens: the bare steps, with the reads of x
+// from LDS and the barriers but neither loads nor matrix instructions, take 73 us (62
+// of them the reads, 128 bytes a clock and CU), the loads with them 129, the
+// instructions (50 us of the matrix units' time at 25 % stored, 110 at 100 %) 140,
+// all 160.  Hence two workgroups of eight waves on a CU, four waves a SIMD, that take
+// turns (25 % stored: 175 us; with four waves of four block-rows x 64 tokens each
+// 218), and sixteen block-rows where there are enough of them, so that a row of x is
+// read from LDS for four block-rows and not for two (158 us).  Measured: y 157 to 165
+// us at 25 % stored and 250 at 100 % (960 TFLOP/s), both of a gated product's 300 and
+// 475 (1010), dx, by eight, 162 and 269.
 #include "feed_forward_device.hpp"
 
 namespace xspmm {
