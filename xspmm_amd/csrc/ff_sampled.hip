@@ -20,6 +20,26 @@ namespace ff {
 
 constexpr int kGroup = kGroupBlocks;  // stored blocks of a wave
 
+// A weight's blocks by fours; the two weights of a gated layer are the grid's rows.
+template <typename T>
+struct SampledFours {
+    const int32_t* group;
+    const int32_t* ptr;
+    const int32_t* row;
+    const int32_t* col;
+    const T* dz;
+    T* dvals;
+    int64_t nnzb, groups;
+};
+template <typename T>
+struct SampledArray {
+    SampledFours<T> side[2];
+    const T* x;
+    int32_t M, K;
+    int64_t N;
+    uint32_t dz_bytes, x_bytes;
+};
+
 // One step's operands: V tokens of a row per lane
 template <typename T, int ROWS>
 struct SampledStep {
@@ -27,11 +47,16 @@ struct SampledStep {
 };
 
 template <typename T, int SPLIT>
-__global__ __launch_bounds__(256) void ff_sampled_kernel(const int32_t* __restrict__ row, const int32_t* __restrict__ col,
-                                                         const T* __restrict__ dz, const T* __restrict__ x,
-                                                         T* __restrict__ dvals, int64_t nnzb, int32_t M, int32_t K,
-                                                         int64_t N)
+__global__ __launch_bounds__(256) void ff_sampled_kernel(const SampledArray<T> a)
 {
+    const SampledFours<T>& s = a.side[blockIdx.y];
+    const int32_t* const __restrict__ row = s.row;
+    const int32_t* const __restrict__ col = s.col;
+    const T* const __restrict__ dz = s.dz;
+    const T* const __restrict__ x = a.x;
+    T* const __restrict__ dvals = s.dvals;
+    const int64_t nnzb = s.nnzb, N = a.N;
+    const int32_t M = a.M, K = a.K;
     constexpr int V = 16 / sizeof(T);  // tokens a lane takes per step
     constexpr int kStep = 4 * V;
     constexpr int kPer = 4 / SPLIT;
@@ -40,6 +65,7 @@ __global__ __launch_bounds__(256) void ff_sampled_kernel(const int32_t* __restri
     const int li = lane & 15, g = lane >> 4;
     const int64_t b0 = ((int64_t)blockIdx.x * kPer + wave / SPLIT) * kGroup;
     const int part = wave % SPLIT;
+    if ((int64_t)blockIdx.x * kPer * kGroup >= nnzb) return;  // the other weight has more
     float4_t acc[kGroup];
     int32_t r0[kGroup], c0[kGroup];
 #pragma unroll
@@ -158,24 +184,10 @@ __global__ __launch_bounds__(256) void ff_sampled_kernel(const int32_t* __restri
 // for nothing but its own loads.  Bound by the L2: four blocks read five blocks'
 // rows, 14336 x 4096 fp16, 10 % stored, 2048 tokens 1.9 GB in 102 us, 18 TB/s; fp32
 // 4096 x 4096, 10 %, 512 tokens 29.4 us (57 without LDS), 58 TFLOP/s.
-template <typename T>
-struct SampledWave {
-    const int32_t* group;
-    const int32_t* ptr;
-    const int32_t* row;
-    const int32_t* col;
-    const T* dz;
-    const T* x;
-    T* dvals;
-    int64_t groups;
-    int32_t M, K;
-    int64_t N;
-    uint32_t dz_bytes, x_bytes;
-};
-
 template <typename T, int SPLIT>
-__global__ __launch_bounds__(256, 2) void ff_sampled_wave_kernel(const SampledWave<T> a)
+__global__ __launch_bounds__(256, 2) void ff_sampled_wave_kernel(const SampledArray<T> a)
 {
+    const SampledFours<T>& s = a.side[blockIdx.y];
     constexpr int V = 16 / sizeof(T), kTokens = 128 / (int)sizeof(T);
     constexpr int kUnits = 1 + kGroup, kStage = kUnits * 16 * 128, kLoads = 2 * kUnits;
     constexpr int kPer = 4 / SPLIT;
@@ -183,20 +195,21 @@ __global__ __launch_bounds__(256, 2) void ff_sampled_wave_kernel(const SampledWa
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g = lane >> 4;
-    const int64_t item = xcd_item(blockIdx.x, (a.groups + kPer - 1) / kPer);
-    if (item < 0) return;
+    const int64_t items = (s.groups + kPer - 1) / kPer;
+    const int64_t item = xcd_item(blockIdx.x, items);
+    if (item < 0 || blockIdx.x / kXcds >= xcd_chunk(items)) return;  // the other weight has more
     const int64_t gi = item * kPer + wave / SPLIT;
     const int part = wave % SPLIT;
-    const bool live = gi < a.groups;
-    const int32_t b0 = live ? a.group[gi] : 0;
-    const int32_t br = live ? a.row[b0] : 0;
-    const int count = live ? min(a.ptr[br + 1] - b0, kGroup) : 0;
+    const bool live = gi < s.groups;
+    const int32_t b0 = live ? s.group[gi] : 0;
+    const int32_t br = live ? s.row[b0] : 0;
+    const int count = live ? min(s.ptr[br + 1] - b0, kGroup) : 0;
     int32_t c0[kGroup];
     float4_t acc[kGroup];
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
         acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
-        c0[i] = 16 * a.col[min(b0 + i, b0 + max(count, 1) - 1)];
+        c0[i] = 16 * s.col[min(b0 + i, b0 + max(count, 1) - 1)];
     }
     if (live) {
         // load j of a stage: rows 8 (j % 2) .. + 7 of unit j / 2 (dz, then the
@@ -211,7 +224,7 @@ __global__ __launch_bounds__(256, 2) void ff_sampled_wave_kernel(const SampledWa
             const bool in = j < 2 ? r < a.M : j / 2 <= count && r < a.K;
             off[j] = in ? (uint32_t)r * ld + (uint32_t)chunk * 16u : kNone;
         }
-        const i32x4_t bd = dma_buffer(a.dz, a.dz_bytes), bx = dma_buffer(a.x, a.x_bytes);
+        const i32x4_t bd = dma_buffer(s.dz, a.dz_bytes), bx = dma_buffer(a.x, a.x_bytes);
         const uint32_t lds0 = lds_address(smem[wave]);
         const int32_t steps = (int32_t)((a.N + kTokens - 1) / kTokens);
         const int32_t lo = steps * part / SPLIT, hi = steps * (part + 1) / SPLIT;
@@ -272,26 +285,50 @@ __global__ __launch_bounds__(256, 2) void ff_sampled_wave_kernel(const SampledWa
         Pack<T, 4> o;
 #pragma unroll
         for (int q = 0; q < 4; ++q) o.v[q] = (T)(16 * br + li < a.M && c0[i] + 4 * g + q < a.K ? acc[i][q] : 0.f);
-        *reinterpret_cast<Pack<T, 4>*>(a.dvals + (int64_t)(b0 + i) * 256 + li * 16 + 4 * g) = o;
+        *reinterpret_cast<Pack<T, 4>*>(s.dvals + (int64_t)(b0 + i) * 256 + li * 16 + 4 * g) = o;
     }
 }
 
 template <typename T>
-bool sampled_wave(const SampledArgs<T>& f, int l, hipStream_t s)
+void sampled_fours(const SampledArgs<T>& f, int weights, hipStream_t s)
 {
-    const BlockIndex& w = *f.weight[l];
+    const BlockIndex& w = *f.weight[0];
     const int64_t db = narrow_bytes(w.M, f.N, sizeof(T)), xb = narrow_bytes(w.K, f.N, sizeof(T));
-    if (db < 0 || xb < 0 || f.N * sizeof(T) % 16 != 0 || f.N == 0) return false;
-    const SampledWave<T> a{w.group, w.ptr, w.row, w.col, f.dz[l], f.x, f.dvals[l], w.groups, (int32_t)w.M,
-                           (int32_t)w.K, f.N, (uint32_t)db, (uint32_t)xb};
-    const bool split = w.groups < 2048 && f.N * sizeof(T) >= 1024;
-    const int64_t grid = kXcds * xcd_chunk((w.groups + (split ? 0 : 3)) / (split ? 1 : 4));
-    if (split)
-        hipLaunchKernelGGL((ff_sampled_wave_kernel<T, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL((ff_sampled_wave_kernel<T, 1>), dim3((unsigned)grid), dim3(256), 0, s, a);
-    XSPMM_LAUNCH_CHECK();
-    return true;
+    SampledArray<T> a{};
+    a.x = f.x;
+    a.M = (int32_t)w.M;
+    a.K = (int32_t)w.K;
+    a.N = f.N;
+    a.dz_bytes = (uint32_t)db;
+    a.x_bytes = (uint32_t)xb;
+    unsigned sides = 0;
+    int64_t groups = 0, fours = 0, most_groups = 0, most_fours = 0;
+    for (int l = 0; l < weights; ++l) {
+        const BlockIndex& wl = *f.weight[l];
+        if (!f.dvals[l] || wl.nnzb == 0) continue;
+        a.side[sides++] = {wl.group, wl.ptr, wl.row, wl.col, f.dz[l], f.dvals[l], wl.nnzb, wl.groups};
+        const int64_t n = (wl.nnzb + kGroup - 1) / kGroup;
+        groups += wl.groups;
+        fours += n;
+        most_groups = wl.groups > most_groups ? wl.groups : most_groups;
+        most_fours = n > most_fours ? n : most_fours;
+    }
+    if (sides == 0) return;
+    auto go = [&](auto kernel, int64_t grid) {
+        if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many blocks for one launch.");
+        hipLaunchKernelGGL(kernel, dim3((unsigned)grid, sides), dim3(256), 0, s, a);
+        XSPMM_LAUNCH_CHECK();
+    };
+    if (db >= 0 && xb >= 0 && f.N * sizeof(T) % 16 == 0 && f.N != 0) {
+        if (groups < 2048 && f.N * sizeof(T) >= 1024)
+            go(ff_sampled_wave_kernel<T, 4>, kXcds * xcd_chunk(most_groups));
+        else
+            go(ff_sampled_wave_kernel<T, 1>, kXcds * xcd_chunk((most_groups + 3) / 4));
+    } else if (fours < 2048 && f.N >= 256) {
+        go(ff_sampled_kernel<T, 4>, most_fours);
+    } else {
+        go(ff_sampled_kernel<T, 1>, (most_fours + 3) / 4);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -559,19 +596,7 @@ bool sampled_tiles(const SampledArgs<T>& f, int weights, hipStream_t s)
 template <typename T>
 void sampled_product(const SampledArgs<T>& f, int weights, hipStream_t s)
 {
-    if (ff::sampled_tiles<T>(f, weights, s)) return;
-    for (int l = 0; l < weights; ++l) {
-        const BlockIndex& w = *f.weight[l];
-        if (!f.dvals[l] || w.nnzb == 0 || ff::sampled_wave<T>(f, l, s)) continue;
-        const int64_t groups = (w.nnzb + ff::kGroup - 1) / ff::kGroup;
-        if (groups < 2048 && f.N >= 256)
-            hipLaunchKernelGGL((ff::ff_sampled_kernel<T, 4>), dim3((unsigned)groups), dim3(256), 0, s, w.row, w.col,
-                               f.dz[l], f.x, f.dvals[l], w.nnzb, (int32_t)w.M, (int32_t)w.K, f.N);
-        else
-            hipLaunchKernelGGL((ff::ff_sampled_kernel<T, 1>), dim3((unsigned)((groups + 3) / 4)), dim3(256), 0, s,
-                               w.row, w.col, f.dz[l], f.x, f.dvals[l], w.nnzb, (int32_t)w.M, (int32_t)w.K, f.N);
-        XSPMM_LAUNCH_CHECK();
-    }
+    if (!ff::sampled_tiles<T>(f, weights, s)) ff::sampled_fours<T>(f, weights, s);
 }
 
 template void sampled_product<float>(const SampledArgs<float>&, int, hipStream_t);
