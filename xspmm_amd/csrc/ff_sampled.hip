@@ -571,17 +571,25 @@ bool sampled_tiles(const SampledArgs<T>& f, int weights, hipStream_t s)
     }
     if (a.sides == 0) return true;
     // The share of stored blocks from which a tile's rows are cheaper than the rows
-    // of each four blocks (14336 x 4096 fp16, 2048 tokens, us by tiles and by fours:
-    // 15 % stored 169 and 148, 20 % 173 and 194; 4096 x 4096 fp32, 512 tokens: 45 % 95
-    // and 86, 60 % 113 and 108, 80 % 128 and 139), or, off 16 bytes, than those read
-    // operand by operand (fp16, 2047 tokens, 3 %: 324 and 366; fp32, 511 tokens, 10 %
-    // 62 and 58, 15 % 68 and 72).
+    // of each four blocks (14336 x 4096 fp16, us by tiles and by fours: 2048 tokens,
+    // 15 % stored 169 and 148, 20 % 173 and 194; 256 tokens, 10 % 36 and 15, 30 % 41
+    // and 39; 4096 x 4096 fp32, 512 tokens: 45 % 95 and 86, 60 % 113 and 108, 80 % 128
+    // and 139), or, off 16 bytes, than those read operand by operand, which costs more
+    // the more tokens there are (fp16, 2047 tokens, 3 %: 324 and 366; 131, 10 % 54 and
+    // 50; 37, 30 % 48 and 46; 1, 30 % 39 and 25; fp32 4096 x 4096, 511 tokens, 10 % 62
+    // and 58, 15 % 68 and 72; 75, 30 % 26 and 26; 37, 100 % 34 and 38).
     // Tiles take rounds of two workgroups a CU, and a round of one a CU seven tenths
     // of that; blocks by fours fill the chip sooner (1024 x 1024, 2048 tokens, all
     // stored: fp16 25 us by tiles and 19, fp32 143 and 48).  Not so operand by operand
     // in 16 bits (2047 tokens, 40 % stored 44 us by tiles and 109).
     const bool aligned = f.N * sizeof(T) % 16 == 0;
-    const double share = (aligned ? (is_f32<T> ? 160 : 46) : (is_f32<T> ? 32 : 7)) / 256.0;
+    double share;
+    if (aligned)
+        share = is_f32<T> ? 0.62 : f.N < 512 ? 0.27 : 0.18;
+    else if constexpr (is_f32<T>)
+        share = 20.0 / (double)f.N + 0.09;
+    else
+        share = f.N < 28 ? 0.45 : 12.0 / (double)f.N + 0.028;
     const int64_t tiles = (int64_t)((a.Mb + kEdge - 1) / kEdge) * ((a.Kb + kEdge - 1) / kEdge) * a.sides;
     const int64_t rest = tiles % 512;
     const double rounds = (double)(tiles / 512) + (rest == 0 ? 0.0 : rest <= 256 ? 0.7 : 1.0);
