@@ -34,37 +34,38 @@ __global__ __launch_bounds__(256) void ff_act_backward_kernel(const T* __restric
     if (row >= M) return;
     const int64_t at = row * N;
     float sum = 0.f, sum_up = 0.f;
-    auto one = [&](float zv, float uv, float g, float& o, float& ou) {
+    auto one = [&](float zv, float uv, float g, bool own, float& o, float& ou) {
         float value = zv;
         const float slope = act_slope<ACT>(zv, &value);
         o = GATED ? g * uv * slope : g * slope;
         ou = GATED ? g * value : 0.f;
-        sum += o;
-        sum_up += ou;
+        sum += own ? o : 0.f;
+        sum_up += own ? ou : 0.f;
     };
-    for (int64_t n = V * lane; n < N; n += 64 * V) {
-        if (n + V <= N) {
-            const auto g = *reinterpret_cast<const Pack<T, V>*>(dy + at + n);
+    if (N >= V) {
+        for (int64_t n = V * lane; n < N; n += 64 * V) {
+            // the last pack moves back into the row: what it does again gives the
+            // same, and counts once
+            const int64_t m = n + V <= N ? n : N - V;
+            const auto g = *reinterpret_cast<const Pack<T, V>*>(dy + at + m);
             Pack<T, V> zz, uu, o, ou;
-            if (kReads) zz = *reinterpret_cast<const Pack<T, V>*>(z + at + n);
-            if (GATED) uu = *reinterpret_cast<const Pack<T, V>*>(up + at + n);
+            if (kReads) zz = *reinterpret_cast<const Pack<T, V>*>(z + at + m);
+            if (GATED) uu = *reinterpret_cast<const Pack<T, V>*>(up + at + m);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float a, b;
-                one(kReads ? (float)zz.v[i] : 0.f, GATED ? (float)uu.v[i] : 0.f, (float)g.v[i], a, b);
+                one(kReads ? (float)zz.v[i] : 0.f, GATED ? (float)uu.v[i] : 0.f, (float)g.v[i], m + i >= n, a, b);
                 o.v[i] = (T)a;
                 ou.v[i] = (T)b;
             }
-            if (dz) *reinterpret_cast<Pack<T, V>*>(dz + at + n) = o;
-            if (GATED) *reinterpret_cast<Pack<T, V>*>(dup + at + n) = ou;
-        } else {
-            for (int64_t m = n; m < N; ++m) {
-                float a, b;
-                one(kReads ? (float)z[at + m] : 0.f, GATED ? (float)up[at + m] : 0.f, (float)dy[at + m], a, b);
-                if (dz) dz[at + m] = (T)a;
-                if (GATED) dup[at + m] = (T)b;
-            }
+            if (dz) *reinterpret_cast<Pack<T, V>*>(dz + at + m) = o;
+            if (GATED) *reinterpret_cast<Pack<T, V>*>(dup + at + m) = ou;
         }
+    } else if (lane < N) {
+        float a, b;
+        one(kReads ? (float)z[at + lane] : 0.f, GATED ? (float)up[at + lane] : 0.f, (float)dy[at + lane], true, a, b);
+        if (dz) dz[at + lane] = (T)a;
+        if (GATED) dup[at + lane] = (T)b;
     }
     if (dbias) {
         sum = wave_sum(sum);
