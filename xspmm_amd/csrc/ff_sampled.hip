@@ -570,6 +570,7 @@ bool sampled_tiles(const SampledArgs<T>& f, int weights, hipStream_t s)
         a.side[a.sides++] = {f.weight[l]->map, f.dz[l], f.dvals[l]};
     }
     if (a.sides == 0) return true;
+    if (blocks == 0) return false;
     // The share of stored blocks from which a tile's rows are cheaper than the rows
     // of each four blocks (14336 x 4096 fp16, us by tiles and by fours: 2048 tokens,
     // 15 % stored 169 and 148, 20 % 173 and 194; 256 tokens, 10 % 36 and 15, 30 % 41

@@ -520,13 +520,14 @@ __global__ __launch_bounds__(64 * kBackwardWaves) void ln_backward_apply_kernel(
     };
     if (k < k1) load();  // under way while the sums are joined
     const auto m = load_tokens<float, V>(mean + at), r = load_tokens<float, V>(rstd + at);
-    const int cols = h.np * V, shares = max(kThreads / cols, 1);
+    static_assert(64 * V <= kThreads);
+    const int cols = h.np * V, shares = kThreads / cols;
     const int64_t base = max(min(tile * cols, N - cols), (int64_t)0);  // the last tile moves back
-    for (int c0 = 0; c0 < cols; c0 += kThreads) {
-        const int c = c0 + threadIdx.x % cols, share = threadIdx.x / cols;
+    {
+        const int c = threadIdx.x % cols, share = threadIdx.x / cols;
         const int64_t col = base + c;
         float2 sum = {0.f, 0.f};
-        if (share < shares && col < N && share < h.slices)
+        if (col < N && share < h.slices)
             sum = sum_strided(colpart + share * N + col, (h.slices - share + shares - 1) / shares, shares * N);
         red[threadIdx.x] = sum;
         __syncthreads();
