@@ -211,6 +211,29 @@ def test_weight_gradient_tiles(kind, M, K, N, density):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,K,N", [(100, 90, 601), (300, 290, 1031), (20, 10, 77), (90, 100, 64), (70, 200, 33), (33, 50, 1)])
+@pytest.mark.parametrize("density", [0.3, 0.9])
+def test_weight_gradient_of_few_blocks(kind, M, K, N, density):
+    """Blocks by fours, of rows on 16-byte boundaries and off them, shorter than a line and long."""
+    test_weight_gradient_tiles(kind, M, K, N, density)
+
+
+def test_weight_gradient_leaves_other_rows_alone():
+    """What is not finite in the rows after a block's, which share its last line, does not reach it."""
+    M, K = 64, 64
+    for N in (65, 71, 127, 600, 601):
+        W, A, where = weight(M, K, 0.5, torch.float16, N)
+        x, dy = normal((K, N), torch.float16, 1), normal((M, N), torch.float16, 2)
+        whole = X.sparse_linear_backward(W, x, None, dy, need=(False, True))[1].reshape(-1, 16, 16)
+        x[16:32], dy[32:48] = math.nan, math.inf
+        part = X.sparse_linear_backward(W, x, None, dy, need=(False, True))[1].reshape(-1, 16, 16)
+        rows, cols, _ = where
+        clean = ((rows != 2) & (cols != 1)).to(DEV)
+        assert 0 < clean.sum() < len(rows) and torch.equal(part[clean], whole[clean])
+        assert not part[~clean].isfinite().any()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("M,K,N", [(4090, 2040, 136), (2040, 4090, 8), (4090, 2040, 75)])
 @pytest.mark.parametrize("density", [0.3, 0.7])
 def test_weight_gradient_tiles_of_a_full_chip(kind, M, K, N, density):

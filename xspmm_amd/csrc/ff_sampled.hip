@@ -13,9 +13,9 @@ namespace ff {
 
 // ---------------------------------------------------------------------------
 // One wave per four consecutive blocks (SPLIT waves share their tokens), operands
-// straight from memory: for few blocks and operands of any size.  A load of 16 rows'
+// straight from memory: for short rows and operands of any size.  A load of 16 rows'
 // 16 bytes costs a lookup per row and lane, 64 of them, which is what bounds it
-// (14336 x 4096 fp16, 2047 tokens, 3 % stored: 366 us).
+// (14336 x 4096 fp16, one token, 30 % stored: 25 us; 2047 tokens, 3 %: 366).
 // ---------------------------------------------------------------------------
 
 constexpr int kGroup = kGroupBlocks;  // stored blocks of a wave
@@ -177,21 +177,47 @@ __global__ __launch_bounds__(256) void ff_sampled_kernel(const SampledArray<T> a
     }
 }
 
-// The same for blocks of one block-row, where rows are on 16-byte boundaries: a
-// wave moves 128 bytes of its rows of dz and x at a time into LDS of its own, in
-// whole lines (the operands themselves are 16 bytes of 16 rows, and memory serves
-// one line at a time), one stage ahead of the one that it multiplies.  It waits
-// for nothing but its own loads.  Bound by the L2: four blocks read five blocks'
-// rows, 14336 x 4096 fp16, 10 % stored, 2048 tokens 1.9 GB in 102 us, 18 TB/s; fp32
-// 4096 x 4096, 10 %, 512 tokens 29.4 us (57 without LDS), 58 TFLOP/s.
-template <typename T, int SPLIT>
+// V tokens of a row from n on, at offset `off` of its array; whole: the row goes on
+// past them.  Where the row ends within them they come one by one: what follows is
+// another row's, and a load past the array's end gives whole dwords of zeros.
+template <typename T>
+__device__ __forceinline__ u32x4_t row_chunk(__amdgpu_buffer_rsrc_t b, uint32_t off, int32_t n, int64_t N, bool whole)
+{
+    constexpr int V = 16 / sizeof(T);
+    if (whole || n + V <= N) {
+        const auto v = buffer_load<T, V>(b, off);
+        return u32x4_t{v.d[0], v.d[1], v.d[2], v.d[3]};
+    }
+    u32x4_t o = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (n + i < N && off != kNone) {
+            const uint32_t q = buffer_load<T, 1>(b, off + (uint32_t)i * (uint32_t)sizeof(T)).d[0];
+            if constexpr (is_f32<T>)
+                o[i] = q;
+            else
+                o[i / 2] |= q << (16 * (i % 2));
+        }
+    return o;
+}
+
+// The same for blocks of one block-row: a wave moves 128 bytes of its rows of dz and
+// x at a time into LDS of its own, in whole lines (the operands themselves are 16
+// bytes of 16 rows, and memory serves one line at a time), while it multiplies the
+// 128 bytes before.  It waits for nothing but its own loads.  DMA: rows on 16-byte
+// boundaries go straight into LDS; others pass through registers and touch two lines
+// for each.  Bound by the L2: four blocks read five blocks' rows, 14336 x 4096 fp16,
+// 10 % stored, 2048 tokens 1.9 GB in 102 us, 18 TB/s, 2047 tokens 196 us (883 operand
+// by operand); fp32 4096 x 4096, 10 %, 512 tokens 29.4 us (57 without LDS), 58 TFLOP/s.
+template <typename T, int SPLIT, bool DMA>
 __global__ __launch_bounds__(256, 2) void ff_sampled_wave_kernel(const SampledArray<T> a)
 {
     const SampledFours<T>& s = a.side[blockIdx.y];
     constexpr int V = 16 / sizeof(T), kTokens = 128 / (int)sizeof(T);
     constexpr int kUnits = 1 + kGroup, kStage = kUnits * 16 * 128, kLoads = 2 * kUnits;
     constexpr int kPer = 4 / SPLIT;
-    __shared__ __align__(16) unsigned char smem[4][2][kStage];
+    constexpr int kStages = DMA ? 2 : 1;
+    __shared__ __align__(16) unsigned char smem[4][kStages][kStage];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g = lane >> 4;
@@ -228,24 +254,40 @@ __global__ __launch_bounds__(256, 2) void ff_sampled_wave_kernel(const SampledAr
         const uint32_t lds0 = lds_address(smem[wave]);
         const int32_t steps = (int32_t)((a.N + kTokens - 1) / kTokens);
         const int32_t lo = steps * part / SPLIT, hi = steps * (part + 1) / SPLIT;
+        u32x4_t held[DMA ? 1 : kLoads];
         auto issue = [&](int32_t st) {
-            const uint32_t to = lds0 + (uint32_t)(st & 1) * kStage;
-            const bool in = st * kTokens + V * chunk < a.N;
+            const int32_t n = st * kTokens + V * chunk;
+            if constexpr (DMA) {
+                const uint32_t to = lds0 + (uint32_t)(st & 1) * kStage;
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j)
-                dma_to_lds(to + (uint32_t)j * 1024u, in ? off[j] + (uint32_t)st * 128u : kNone, j < 2 ? bd : bx);
+                for (int j = 0; j < kLoads; ++j)
+                    dma_to_lds(to + (uint32_t)j * 1024u, n < a.N ? off[j] + (uint32_t)st * 128u : kNone, j < 2 ? bd : bx);
+            } else {
+                const auto rd = make_buffer(s.dz, a.dz_bytes), rx = make_buffer(a.x, a.x_bytes);
+#pragma unroll
+                for (int j = 0; j < kLoads; ++j)
+                    held[j] = row_chunk<T>(j < 2 ? rd : rx, off[j] != kNone ? off[j] + (uint32_t)st * 128u : kNone, n, a.N,
+                                           st + 1 < steps);
+            }
         };
         if (lo < hi) issue(lo);
         for (int32_t st = lo; st < hi; ++st) {
-            // the last reads of the stage that is loaded next are over
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (st + 1 < hi) {
-                issue(st + 1);
-                dma_wait<kLoads>();
+            if constexpr (DMA) {
+                // the last reads of the stage that is loaded next are over
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (st + 1 < hi) {
+                    issue(st + 1);
+                    dma_wait<kLoads>();
+                } else {
+                    dma_wait<0>();
+                }
             } else {
-                dma_wait<0>();
+#pragma unroll
+                for (int j = 0; j < kLoads; ++j)
+                    *reinterpret_cast<u32x4_t*>(smem[wave][0] + j * 1024 + lane * 16) = held[j];
+                if (st + 1 < hi) issue(st + 1);
             }
-            const unsigned char* S = smem[wave][st & 1] + li * 128;
+            const unsigned char* S = smem[wave][DMA ? st & 1 : 0] + li * 128;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int piece = ((4 * h + g) ^ (li & 7)) * 16;
@@ -319,11 +361,16 @@ void sampled_fours(const SampledArgs<T>& f, int weights, hipStream_t s)
         hipLaunchKernelGGL(kernel, dim3((unsigned)grid, sides), dim3(256), 0, s, a);
         XSPMM_LAUNCH_CHECK();
     };
-    if (db >= 0 && xb >= 0 && f.N * sizeof(T) % 16 == 0 && f.N != 0) {
-        if (groups < 2048 && f.N * sizeof(T) >= 1024)
-            go(ff_sampled_wave_kernel<T, 4>, kXcds * xcd_chunk(most_groups));
+    // rows of at least a line, through LDS (off 16 bytes, 14336 x 4096 fp16, 30 %
+    // stored: 75 tokens 56 us and 86 operand by operand, 37 tokens 49 and 46)
+    const bool aligned = f.N * sizeof(T) % 16 == 0;
+    if (db >= 0 && xb >= 0 && f.N != 0 && (aligned || f.N * sizeof(T) >= 128)) {
+        const bool split = groups < 2048 && f.N * sizeof(T) >= 1024;
+        const int64_t grid = kXcds * xcd_chunk(split ? most_groups : (most_groups + 3) / 4);
+        if (aligned)
+            split ? go(ff_sampled_wave_kernel<T, 4, true>, grid) : go(ff_sampled_wave_kernel<T, 1, true>, grid);
         else
-            go(ff_sampled_wave_kernel<T, 1>, kXcds * xcd_chunk((most_groups + 3) / 4));
+            split ? go(ff_sampled_wave_kernel<T, 4, false>, grid) : go(ff_sampled_wave_kernel<T, 1, false>, grid);
     } else if (fours < 2048 && f.N >= 256) {
         go(ff_sampled_kernel<T, 4>, most_fours);
     } else {
@@ -446,24 +493,9 @@ __global__ __launch_bounds__(kThreads, kThreads / 128) void ff_sampled_tile_kern
         } else {
             const auto bd = make_buffer(s.dz, a.dz_bytes), bx = make_buffer(a.x, a.x_bytes);
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j) {
-                const auto& b = j < kSide * kPieces / kThreads ? bd : bx;
-                if (st + 1 < steps || n + V <= a.N) {
-                    const auto v = buffer_load<T, V>(b, base[j] != kNone ? base[j] + (uint32_t)n * kSize : kNone);
-                    held[j] = u32x4_t{v.d[0], v.d[1], v.d[2], v.d[3]};
-                } else {  // the row ends within the chunk
-                    held[j] = u32x4_t{0u, 0u, 0u, 0u};
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (n + i < a.N && base[j] != kNone) {
-                            const uint32_t q = buffer_load<T, 1>(b, base[j] + (uint32_t)(n + i) * kSize).d[0];
-                            if constexpr (is_f32<T>)
-                                held[j][i] = q;
-                            else
-                                held[j][i / 2] |= q << (16 * (i % 2));
-                        }
-                }
-            }
+            for (int j = 0; j < kLoads; ++j)
+                held[j] = row_chunk<T>(j < kSide * kPieces / kThreads ? bd : bx,
+                                       base[j] != kNone ? base[j] + (uint32_t)n * kSize : kNone, n, a.N, st + 1 < steps);
         }
     };
 
@@ -572,29 +604,28 @@ bool sampled_tiles(const SampledArgs<T>& f, int weights, hipStream_t s)
     if (a.sides == 0) return true;
     if (blocks == 0) return false;
     // The share of stored blocks from which a tile's rows are cheaper than the rows
-    // of each four blocks (14336 x 4096 fp16, us by tiles and by fours: 2048 tokens,
-    // 15 % stored 169 and 148, 20 % 173 and 194; 256 tokens, 10 % 36 and 15, 30 % 41
-    // and 39; 4096 x 4096 fp32, 512 tokens: 45 % 95 and 86, 60 % 113 and 108, 80 % 128
-    // and 139), or, off 16 bytes, than those read operand by operand, which costs more
-    // the more tokens there are (fp16, 2047 tokens, 3 %: 324 and 366; 131, 10 % 54 and
-    // 50; 37, 30 % 48 and 46; 1, 30 % 39 and 25; fp32 4096 x 4096, 511 tokens, 10 % 62
-    // and 58, 15 % 68 and 72; 75, 30 % 26 and 26; 37, 100 % 34 and 38).
+    // of each four blocks.  On 16 bytes (14336 x 4096 fp16, us by tiles and by fours:
+    // 2048 tokens, 15 % stored 169 and 148, 20 % 173 and 194; 256 tokens, 10 % 36 and
+    // 15, 30 % 41 and 39; 4096 x 4096 fp32, 512 tokens: 45 % 95 and 86, 60 % 113 and
+    // 108, 80 % 128 and 139) and off (fp16, 2047 tokens, 15 % 360 and 289, 20 % 354 and
+    // 386; 301, 10 % 86 and 41, 30 % 88 and 102; 37, operand by operand, 30 % 48 and
+    // 46; 1, 30 % 39 and 25, 100 % 45 and 69; fp32, 511 tokens, 30 % 84 and 76, 45 % 100
+    // and 115; 1, 100 % 25 and 21).
     // Tiles take rounds of two workgroups a CU, and a round of one a CU seven tenths
     // of that; blocks by fours fill the chip sooner (1024 x 1024, 2048 tokens, all
-    // stored: fp16 25 us by tiles and 19, fp32 143 and 48).  Not so operand by operand
-    // in 16 bits (2047 tokens, 40 % stored 44 us by tiles and 109).
+    // stored: fp16 25 us by tiles and 19, fp32 143 and 48).
     const bool aligned = f.N * sizeof(T) % 16 == 0;
     double share;
     if (aligned)
         share = is_f32<T> ? 0.62 : f.N < 512 ? 0.27 : 0.18;
     else if constexpr (is_f32<T>)
-        share = 20.0 / (double)f.N + 0.09;
+        share = f.N < 32 ? 2.0 : 0.4;
     else
-        share = f.N < 28 ? 0.45 : 12.0 / (double)f.N + 0.028;
+        share = f.N < 28 ? 0.45 : f.N < 64 ? 0.35 : 0.2;
     const int64_t tiles = (int64_t)((a.Mb + kEdge - 1) / kEdge) * ((a.Kb + kEdge - 1) / kEdge) * a.sides;
     const int64_t rest = tiles % 512;
     const double rounds = (double)(tiles / 512) + (rest == 0 ? 0.0 : rest <= 256 ? 0.7 : 1.0);
-    const double fill = aligned || is_f32<T> ? (double)tiles / (512.0 * rounds) : 1.0;
+    const double fill = (double)tiles / (512.0 * rounds);
     if ((double)blocks * fill < share * (double)(a.sides * w.Mb * w.Kb)) return false;
     launch_sampled_tile<T>(a, aligned, s);
     return true;
