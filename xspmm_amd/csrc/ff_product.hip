@@ -25,7 +25,8 @@
 // 25 % 210 us, 18 TB/s (there the tiles of ff_tile.hip take over).  With few blocks a
 // wave the chain of loads (row pointer, block-column, x) shows: 8192 x 8192, 5 %,
 // 256 tokens 13.0 us, of which 4.8 are launch, pointers, the sums of four waves and
-// the results.  fp32, 4096 x 4096, 10 %, 512 tokens, dx: 26 us, 66 TFLOP/s.
+// the results.  fp32, 4096 x 4096, 512 tokens, dx: 10 %
+// stored 26 us, 66 TFLOP/s, all 165 us, 104.
 #include "feed_forward_device.hpp"
 
 namespace xspmm {
@@ -197,9 +198,9 @@ struct Walk {
     {
         if constexpr (is_f32<T>) {
 #pragma unroll
-            for (int c = 0; c < VEC; ++c)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[c] = mfma32(st.a[i], st.b[i].d[c], acc[c]);
+                for (int c = 0; c < VEC; ++c) acc[c] = mfma32(st.a[i], st.b[i].d[c], acc[c]);
         } else {
             const u32x4_t a = {st.a[0], st.a[1], st.a[2], st.a[3]};
             if constexpr (ONE) {
@@ -233,7 +234,12 @@ struct Walk {
             for (int p = 0; p < kAhead; ++p) {
                 const int32_t next = b + (p + kAhead - 1) * kPer;
                 load(s[(p + kAhead - 1) % kAhead], next < last ? next : last, end);
+                // 32-bit products are bound by the matrix units as much as by loads, and
+                // a wave with its operands goes first (4096 x 4096 fp32 gated, 30 %
+                // stored, 512 tokens 124 -> 109 us; in 16 bits dx loses a tenth)
+                if constexpr (is_f32<T>) __builtin_amdgcn_s_setprio(1);
                 multiply(acc, s[p]);
+                if constexpr (is_f32<T>) __builtin_amdgcn_s_setprio(0);
                 if (b + (p + 1) * kPer >= end) return;
             }
         }
