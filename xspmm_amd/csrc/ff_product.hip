@@ -25,8 +25,8 @@
 // 25 % 210 us, 18 TB/s (there the tiles of ff_tile.hip take over).  With few blocks a
 // wave the chain of loads (row pointer, block-column, x) shows: 8192 x 8192, 5 %,
 // 256 tokens 13.0 us, of which 4.8 are launch, pointers, the sums of four waves and
-// the results.  fp32, 4096 x 4096, 512 tokens, dx: 10 %
-// stored 26 us, 66 TFLOP/s, all 165 us, 104.
+// the results.  fp32, 4096 x 4096, 512 tokens, dx: 10 % stored 26 us, 66 TFLOP/s, all
+// 165 us, 104.
 #include "feed_forward_device.hpp"
 
 namespace xspmm {
