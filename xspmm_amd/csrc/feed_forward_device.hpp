@@ -99,7 +99,8 @@ __device__ __forceinline__ uint32_t lds_address(const void* p)
 
 // A load straight into LDS: lane l's 16 bytes at byte `off` of the buffer land at
 // LDS address lds + 16 l (zeros past its end).  The compiler does not see it:
-// dma_wait() before the barrier that lets the others read.
+// dma_wait() before the barrier that lets the others read, and the wait state that
+// the load wants after a scalar write of M0.
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i32x4_t dma_buffer(const void* base, uint32_t bytes)
 {
@@ -108,7 +109,7 @@ __device__ __forceinline__ i32x4_t dma_buffer(const void* base, uint32_t bytes)
 }
 __device__ __forceinline__ void dma_to_lds(uint32_t lds, uint32_t off, i32x4_t buffer)
 {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(lds), "v"(off), "s"(buffer)
                  : "memory", "m0");

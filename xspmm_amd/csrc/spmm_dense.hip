@@ -108,10 +108,11 @@ __device__ __forceinline__ uint32_t lds_address(const void* p)
 // One direct-to-LDS load: lane l's 16 bytes at byte `off` of the buffer land
 // at LDS address lds + 16 l (buffer_load_dwordx4 ... lds, address base in M0).
 // Issued as inline assembly so that the compiler adds no wait of its own: the
-// callers wait with explicit s_waitcnt vmcnt.
+// callers wait with explicit s_waitcnt vmcnt.  So the wait state that the load
+// wants after a scalar write of M0 is written out too.
 __device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t off, i32x4_t rsrc)
 {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(lds), "v"(off), "s"(rsrc)
                  : "memory", "m0");
