@@ -1,0 +1,144 @@
+"""The feed-forward module and the operators' gradients through autograd: weights
+that share a matrix, second derivatives, gradients as other layers hand them over,
+what is kept for the backward pass, copies.
+
+Bounds as in the operators' own tests: chains of fp32 sums, relative to the
+largest value."""
+from __future__ import annotations
+
+import copy
+import io
+import threading
+
+import pytest
+import torch
+
+import xspmm_amd as X
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+EPS32 = 2.0 ** -24
+
+
+def normal(shape, seed, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(DEV, dtype)
+
+
+def pruned(M, K, seed, dtype=torch.float32, density=0.5):
+    return X.prune_blocks(normal((M, K), seed, dtype) * 0.1, density)
+
+
+def unpack(A, v):
+    """The M x K matrix of block values v, differentiable."""
+    rows = torch.repeat_interleave(torch.arange(A.num_block_rows), torch.diff(A.row_ptr.cpu()).long())
+    d = torch.zeros((A.num_block_rows, A.num_block_cols, 16, 16), dtype=torch.float64)
+    d = d.index_put((rows, A.col_ind.cpu().long()), v.view(-1, 16, 16))
+    return d.permute(0, 2, 1, 3).reshape(A.num_block_rows * 16, -1)[:A.num_rows, :A.num_cols]
+
+
+def f64(t):
+    return t.detach().double().cpu()
+
+
+def near(got, want, bound, what):
+    got = f64(got)
+    off = float((got - want).abs().max())
+    assert got.shape == want.shape and off <= bound * float(want.abs().max()), (what, off)
+
+
+def layer64(mats, layer, x):
+    """The layer on the unpacked weights, and everything that has a gradient."""
+    leaves = [f64(p).requires_grad_(True) for p in (layer.gate, layer.up, layer.down, layer.norm_weight,
+                                                    layer.norm_bias, x)]
+    G, U, D = (unpack(A, v) for A, v in zip(mats, leaves))
+    w, b, xx = leaves[3:]
+    m = xx.mean(0)
+    n = (xx - m) / torch.sqrt((xx - m).square().mean(0) + 1e-5) * w[:, None] + b[:, None]
+    return xx + D @ (torch.nn.functional.silu(G @ n) * (U @ n)), leaves
+
+
+# ---------------------------------------------------------------------------
+# one matrix, several weights
+# ---------------------------------------------------------------------------
+
+def check_shared(mats):
+    feats, N = mats[0].num_cols, 40
+    before = [A.values.clone() for A in mats]
+    at = [A.values.data_ptr() for A in mats]
+    layer = X.FeedForward(*mats)
+    with torch.no_grad():  # as after an update
+        for i, p in enumerate((layer.gate, layer.up, layer.down)):
+            p.add_(0.1 * normal(p.shape, 10 + i))
+    x = normal((feats, N), 3).requires_grad_(True)
+    dy = normal((feats, N), 4)
+    with torch.no_grad():
+        served = layer(x)
+    y = layer(x)
+    y.backward(dy)
+    y64, leaves = layer64(mats, layer, x)
+    y64.backward(f64(dy))
+    assert torch.equal(y.detach(), served)
+    bound = 4 * (mats[0].num_rows + N) * EPS32
+    near(y, y64.detach(), bound, "y")
+    for name, p, want in zip(("gate", "up", "down", "weight", "bias", "x"),
+                             (layer.gate, layer.up, layer.down, layer.norm_weight, layer.norm_bias, x), leaves):
+        near(p.grad, want.grad, bound, name)
+    for A, v, a in zip(mats, before, at):  # the matrices are the caller's
+        assert A.values.data_ptr() == a and torch.equal(A.values, v)
+
+
+def test_gate_and_up_of_one_matrix():
+    A = pruned(200, 96, 1)
+    check_shared((A, A, pruned(96, 200, 2)))
+
+
+def test_three_weights_of_one_square_matrix():
+    A = pruned(96, 96, 1)
+    check_shared((A, A, A))
+
+
+def test_operators_of_one_matrix():
+    A = pruned(64, 48, 1)
+    G, U = X.SparseWeight(A), X.SparseWeight(A)
+    x = normal((48, 10), 2)
+    first = A.values
+    U.values = A.values * 2
+    assert A.values is first and G.values is first
+    assert torch.equal(X.sparse_linear(U, x), 2 * X.sparse_linear(G, x))
+    # until set, they are the matrix's, read at every call
+    y = X.sparse_linear(G, x)
+    A.values = A.values * 4
+    assert torch.equal(X.sparse_linear(G, x), 4 * y) and torch.equal(X.sparse_linear(U, x), 2 * y)
+    # and a call can bring its own
+    assert torch.equal(X.sparse_linear(G, x, values=first), y)
+    h = X.sparse_gated(G, U, x, values=(first, first))
+    assert torch.equal(h, X.sparse_gated(X.SparseWeight(A), G, x, values=(first, first)))
+    for bad in (first[:-256], first.half(), first.cpu()):
+        with pytest.raises((TypeError, ValueError)):
+            X.sparse_linear(G, x, values=bad)
+
+
+def test_layers_of_one_matrix_in_threads():
+    A, D = pruned(200, 96, 1), pruned(96, 200, 2)
+    x = normal((96, 33), 3)
+    layers = [X.FeedForward(A, A, D) for _ in range(2)]
+    with torch.no_grad():
+        for i, layer in enumerate(layers):
+            layer.gate.mul_(1 + i)
+        alone = [layer(x) for layer in layers]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(layer, want):
+        with torch.no_grad():
+            for _ in range(50):
+                if not torch.equal(layer(x), want):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=work, args=p) for p in zip(layers, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

@@ -115,12 +115,14 @@ def _scratch(n, device):
 
 class SparseWeight:
     """Where the 16x16 blocks of a BCSR matrix stand, laid out once for products
-    with the matrix and with its transpose.  The block values stay the matrix's
-    own (``values``, num_blocks * 256 of them) and may change between calls; the
-    positions are read once, here, and synchronize torch's current stream."""
+    with the matrix and with its transpose.  The positions are read once, here,
+    and synchronize torch's current stream.  The block values (``values``,
+    num_blocks * 256 of them) may change between calls: they are the matrix's,
+    read at every call, until others are set here, which leaves the matrix as it
+    is; and a call can bring its own (``values=``)."""
 
     def __init__(self, A):
-        self._h = None
+        self._h = self._own = None
         if A.r_block != 16 or A.c_block != 16:
             raise ValueError("a weight has 16x16 blocks")
         if A.values.dtype not in _TYPES:
@@ -150,17 +152,22 @@ class SparseWeight:
 
     @property
     def values(self):
-        return self.matrix.values
+        return self.matrix.values if self._own is None else self._own
 
     @values.setter
     def values(self, v):
         _check(v, "values", (self.num_blocks * 256,), self.dtype, self.device)
-        self.matrix.values = v
+        self._own = v
 
-    def _values(self):
+    def _values(self, v=None):
+        """The address of the block values of a call: v, or the weight's."""
         if self._h is None:
             raise RuntimeError("SparseWeight is closed")
-        return _check(self.matrix.values, "values", self._flat, self.dtype, self.device)
+        if v is None:
+            v = self._own
+            if v is None:
+                v = self.matrix.values
+        return _check(v, "values", self._flat, self.dtype, self.device)
 
     def close(self):
         if self._h is not None:
@@ -186,12 +193,13 @@ def _at(t):
     return None if t is None else t.data_ptr() or None
 
 
-def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, out=None):
+def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, out=None, values=None):
     """act(W x + bias) + residual, M x N; with keep also W x + bias, which
-    ``sparse_linear_backward`` takes where there is an activation."""
+    ``sparse_linear_backward`` takes where there is an activation.  values: block
+    values in the place of W's."""
     act = _activation(activation)
     (M, K), N, dt, dev = W.shape, _tokens(x), W.dtype, W.device
-    vals = W._values()
+    vals = W._values(values)
     xp = _check(x, "x", (K, N), dt, dev)
     bp = None if bias is None else _check(bias, "bias", (M,), dt, dev, 0)
     rp = None if residual is None else _check(residual, "residual", (M, N), dt, dev)
@@ -202,14 +210,15 @@ def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, o
     return (y, z) if keep else y
 
 
-def sparse_linear_backward(W, x, kept, dy, activation=None, bias=False, need=(True, True)):
+def sparse_linear_backward(W, x, kept, dy, activation=None, bias=False, need=(True, True), values=None):
     """(dx, dvalues, dbias) from dy = the gradient of ``sparse_linear``'s result
     and `kept` = W x + bias (not read, and may be None, without an activation).
     bias: whether the layer has one (dbias is None otherwise); need: whether dx
-    and dvalues are wanted (None otherwise).  The residual's gradient is dy."""
+    and dvalues are wanted (None otherwise); values as in the forward pass.  The
+    residual's gradient is dy."""
     act = _activation(activation)
     (M, K), N, dt, dev = W.shape, _tokens(dy, "dy"), W.dtype, W.device
-    vals = W._values()
+    vals = W._values(values)
     xp = _check(x, "x", (K, N), dt, dev)
     zp = _check(kept, "kept", (M, N), dt, dev) if act else None
     gp = _check(dy, "dy", (M, N), dt, dev)
@@ -232,13 +241,14 @@ def _pair(G, U):
     return G.shape
 
 
-def sparse_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", keep=False, out=None):
+def sparse_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", keep=False, out=None,
+                 values=(None, None)):
     """act(G x + bias_gate) * (U x + bias_up), M x N; with keep also the two
     sums, which ``sparse_gated_backward`` takes.  G and U have blocks of their
-    own."""
+    own.  values: block values in the place of G's and U's (None: theirs)."""
     act = _activation(activation)
     (M, K), N, dt, dev = _pair(G, U), _tokens(x), G.dtype, G.device
-    gv, uv = G._values(), U._values()
+    gv, uv = G._values(values[0]), U._values(values[1])
     xp = _check(x, "x", (K, N), dt, dev)
     gb = None if bias_gate is None else _check(bias_gate, "bias_gate", (M,), dt, dev, 0)
     ub = None if bias_up is None else _check(bias_up, "bias_up", (M,), dt, dev, 0)
@@ -250,14 +260,15 @@ def sparse_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", keep=
     return (h, zg, zu) if keep else h
 
 
-def sparse_gated_backward(G, U, x, kept_gate, kept_up, dh, activation="silu", bias=False, need=(True, True, True)):
+def sparse_gated_backward(G, U, x, kept_gate, kept_up, dh, activation="silu", bias=False, need=(True, True, True),
+                          values=(None, None)):
     """(dx, dvalues of G, dvalues of U, dbias_gate, dbias_up) from dh = the
     gradient of ``sparse_gated``'s result and the two sums it kept.  bias:
     whether the biases' gradients are wanted; need: whether the first three are
-    (None otherwise)."""
+    (None otherwise); values as in the forward pass."""
     act = _activation(activation)
     (M, K), N, dt, dev = _pair(G, U), _tokens(dh, "dh"), G.dtype, G.device
-    gv, uv = G._values(), U._values()
+    gv, uv = G._values(values[0]), U._values(values[1])
     xp = _check(x, "x", (K, N), dt, dev)
     zg = _check(kept_gate, "kept_gate", (M, N), dt, dev)
     zu = _check(kept_up, "kept_up", (M, N), dt, dev)
@@ -372,8 +383,7 @@ class _Norm(torch.autograd.Function):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, W, values, x, bias, activation, residual):
-        W.values = values.detach()
-        y, z = sparse_linear(W, x, bias, activation, residual, keep=True)
+        y, z = sparse_linear(W, x, bias, activation, residual, keep=True, values=values)
         ctx.W, ctx.activation, ctx.bias = W, activation, bias is not None
         ctx.save_for_backward(values, x, z)
         return y
@@ -381,18 +391,17 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         values, x, z = ctx.saved_tensors
-        ctx.W.values = values.detach()
         dy = dy.contiguous()
         need = ctx.needs_input_grad
-        dx, dv, db = sparse_linear_backward(ctx.W, x, z, dy, ctx.activation, ctx.bias and need[3], (need[2], need[1]))
+        dx, dv, db = sparse_linear_backward(ctx.W, x, z, dy, ctx.activation, ctx.bias and need[3], (need[2], need[1]),
+                                            values=values)
         return None, dv, dx, db, None, dy if need[5] else None
 
 
 class _Gated(torch.autograd.Function):
     @staticmethod
     def forward(ctx, G, U, gate, up, x, activation):
-        G.values, U.values = gate.detach(), up.detach()
-        h, zg, zu = sparse_gated(G, U, x, activation=activation, keep=True)
+        h, zg, zu = sparse_gated(G, U, x, activation=activation, keep=True, values=(gate, up))
         ctx.G, ctx.U, ctx.activation = G, U, activation
         ctx.save_for_backward(gate, up, x, zg, zu)
         return h
@@ -400,18 +409,18 @@ class _Gated(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dh):
         gate, up, x, zg, zu = ctx.saved_tensors
-        ctx.G.values, ctx.U.values = gate.detach(), up.detach()
         need = ctx.needs_input_grad
         dx, dg, du, _, _ = sparse_gated_backward(ctx.G, ctx.U, x, zg, zu, dh.contiguous(), ctx.activation,
-                                                 need=(need[4], need[2], need[3]))
+                                                 need=(need[4], need[2], need[3]), values=(gate, up))
         return None, None, dg, du, dx, None
 
 
 class FeedForward(torch.nn.Module):
     """x + D (act(G n) * (U n)), n = layer_norm(x): a model's feed-forward layer
     on three BCSR matrices (G and U hidden x features, D features x hidden), with
-    their block values and the norm's weight and bias as parameters.  Which
-    blocks are stored does not change.  x is features x tokens."""
+    their block values and the norm's weight and bias as parameters.  The matrices
+    are read, not kept up to date; weights may share one.  Which blocks are stored
+    does not change.  x is features x tokens."""
 
     def __init__(self, gate, up, down, activation="silu", eps=1e-5):
         super().__init__()
@@ -433,6 +442,7 @@ class FeedForward(torch.nn.Module):
             n = _Norm.apply(x, self.norm_weight, self.norm_bias, self.eps)
             h = _Gated.apply(G, U, self.gate, self.up, n, self.activation)
             return _Linear.apply(D, self.down, h, None, None, x)
-        G.values, U.values, D.values = self.gate.detach(), self.up.detach(), self.down.detach()
+        gate, up, down = self.gate.detach(), self.up.detach(), self.down.detach()
         n = layer_norm(x.detach(), self.norm_weight.detach(), self.norm_bias.detach(), self.eps)
-        return sparse_linear(D, sparse_gated(G, U, n, activation=self.activation), residual=x.detach())
+        h = sparse_gated(G, U, n, activation=self.activation, values=(gate, up))
+        return sparse_linear(D, h, residual=x.detach(), values=down)
