@@ -142,3 +142,33 @@ def test_layers_of_one_matrix_in_threads():
     for t in threads:
         t.join()
     assert not wrong
+
+
+# ---------------------------------------------------------------------------
+# second derivatives
+# ---------------------------------------------------------------------------
+
+def second_order(f, inputs, through):
+    """Asks for the gradient of a first gradient."""
+    y = f()
+    first = torch.autograd.grad(y.square().sum() if through == "square" else y.sum(), inputs[0], create_graph=True)[0]
+    penalty = first.square().sum() + sum(t.sum() for t in inputs)
+    if through == "backward":
+        penalty.backward()
+    else:
+        torch.autograd.grad(penalty, inputs)
+
+
+@pytest.mark.parametrize("through", ["square", "sum", "backward"])
+def test_second_derivatives_are_refused(through):
+    """A gradient penalty would get a wrong value: what the kernels compute has no graph of its own."""
+    A, D = pruned(64, 48, 1), pruned(48, 64, 2)
+    layer = X.FeedForward(A, A, D)
+    x = normal((48, 20), 3).requires_grad_(True)
+    for inputs in ([x], [layer.gate, x], [layer.down, x], [layer.norm_weight, x]):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            second_order(lambda: layer(x), inputs, through)
+    # first derivatives with a graph kept are as without
+    want = torch.autograd.grad(layer(x).sum(), [x, layer.gate])
+    got = torch.autograd.grad(layer(x).sum(), [x, layer.gate], create_graph=True)
+    assert all(torch.equal(a.detach(), b) for a, b in zip(got, want))

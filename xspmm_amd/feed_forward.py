@@ -367,6 +367,39 @@ def prune_blocks(dense, density):
     return X.BCSRMatrix(Mb, Kb, 16, 16, M, K, row_ptr, (keep % Kb).int(), blocks[keep].reshape(-1).contiguous())
 
 
+class _NoSecond(torch.autograd.Function):
+    """Gradients as they are, with a derivative that is refused: `n` of them, then
+    all that they depend on, so that every way back to it comes through here."""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the feed-forward operators have no second derivatives")
+
+
+def _first_order(backward):
+    """A backward pass whose results come from kernels and so have no graph.  Where
+    one is asked for (create_graph), their derivative raises instead of being taken
+    for zero."""
+    @functools.wraps(backward)
+    def first_order(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            found = backward(ctx, *grads)
+        given = [t for t in found if t is not None]
+        on = [t for t in (*grads, *ctx.saved_tensors) if t is not None and t.requires_grad]
+        if not on:
+            return found
+        marked = iter(_NoSecond.apply(len(given), *given, *on))
+        return tuple(None if t is None else next(marked) for t in found)
+
+    return first_order
+
+
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -375,6 +408,7 @@ class _Norm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         return (*layer_norm_backward(dy.contiguous(), x, weight, mean, rstd, need=ctx.needs_input_grad[:3]), None)
@@ -385,12 +419,13 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, W, values, x, bias, activation, residual):
         y, z = sparse_linear(W, x, bias, activation, residual, keep=True, values=values)
         ctx.W, ctx.activation, ctx.bias = W, activation, bias is not None
-        ctx.save_for_backward(values, x, z)
+        ctx.save_for_backward(values, x, z, bias)
         return y
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):
-        values, x, z = ctx.saved_tensors
+        values, x, z, _ = ctx.saved_tensors
         dy = dy.contiguous()
         need = ctx.needs_input_grad
         dx, dv, db = sparse_linear_backward(ctx.W, x, z, dy, ctx.activation, ctx.bias and need[3], (need[2], need[1]),
@@ -407,6 +442,7 @@ class _Gated(torch.autograd.Function):
         return h
 
     @staticmethod
+    @_first_order
     def backward(ctx, dh):
         gate, up, x, zg, zu = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -420,7 +456,8 @@ class FeedForward(torch.nn.Module):
     on three BCSR matrices (G and U hidden x features, D features x hidden), with
     their block values and the norm's weight and bias as parameters.  The matrices
     are read, not kept up to date; weights may share one.  Which blocks are stored
-    does not change.  x is features x tokens."""
+    does not change.  x is features x tokens.  There are no second derivatives:
+    asking for one raises."""
 
     def __init__(self, gate, up, down, activation="silu", eps=1e-5):
         super().__init__()
