@@ -172,3 +172,27 @@ def test_second_derivatives_are_refused(through):
     want = torch.autograd.grad(layer(x).sum(), [x, layer.gate])
     got = torch.autograd.grad(layer(x).sum(), [x, layer.gate], create_graph=True)
     assert all(torch.equal(a.detach(), b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------
+# gradients as other layers hand them over
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_gradients_off_sixteen_bytes(dtype):
+    """The backward pass of torch.cat hands over a contiguous view that starts anywhere."""
+    A, D = pruned(64, 48, 1, dtype), pruned(48, 64, 2, dtype)
+    layer = X.FeedForward(A, A, D)
+    head = normal((3, 5), 4, dtype)
+    dy = normal((51, 5), 5, dtype)
+    grads = []
+    for joined in (True, False):
+        layer.zero_grad()
+        x = normal((48, 5), 3, dtype).requires_grad_(True)
+        y = layer(x)
+        if joined:
+            torch.cat([head, y]).backward(dy)
+        else:
+            y.backward(dy[3:].clone())
+        grads.append([x.grad] + [p.grad for p in layer.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))

@@ -380,6 +380,13 @@ class _NoSecond(torch.autograd.Function):
         raise RuntimeError("the feed-forward operators have no second derivatives")
 
 
+def _incoming(g):
+    """An incoming gradient as the kernels take it: other layers may hand over any
+    strides, and contiguous views that start anywhere."""
+    g = g.contiguous()
+    return g.clone() if g.data_ptr() & 15 else g
+
+
 def _first_order(backward):
     """A backward pass whose results come from kernels and so have no graph.  Where
     one is asked for (create_graph), their derivative raises instead of being taken
@@ -411,7 +418,7 @@ class _Norm(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
-        return (*layer_norm_backward(dy.contiguous(), x, weight, mean, rstd, need=ctx.needs_input_grad[:3]), None)
+        return (*layer_norm_backward(_incoming(dy), x, weight, mean, rstd, need=ctx.needs_input_grad[:3]), None)
 
 
 class _Linear(torch.autograd.Function):
@@ -426,7 +433,7 @@ class _Linear(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy):
         values, x, z, _ = ctx.saved_tensors
-        dy = dy.contiguous()
+        dy = _incoming(dy)
         need = ctx.needs_input_grad
         dx, dv, db = sparse_linear_backward(ctx.W, x, z, dy, ctx.activation, ctx.bias and need[3], (need[2], need[1]),
                                             values=values)
@@ -446,7 +453,7 @@ class _Gated(torch.autograd.Function):
     def backward(ctx, dh):
         gate, up, x, zg, zu = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dg, du, _, _ = sparse_gated_backward(ctx.G, ctx.U, x, zg, zu, dh.contiguous(), ctx.activation,
+        dx, dg, du, _, _ = sparse_gated_backward(ctx.G, ctx.U, x, zg, zu, _incoming(dh), ctx.activation,
                                                  need=(need[4], need[2], need[3]), values=(gate, up))
         return None, None, dg, du, dx, None
 
