@@ -196,3 +196,17 @@ def test_gradients_off_sixteen_bytes(dtype):
             y.backward(dy[3:].clone())
         grads.append([x.grad] + [p.grad for p in layer.parameters()])
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_nothing_is_kept_that_no_pass_reads():
+    """The down projection has no activation, so its sum is neither written nor saved."""
+    A, D = pruned(64, 48, 1), pruned(512, 64, 2)
+    W = X.SparseWeight(D)
+    h = normal((64, 1024), 3).requires_grad_(True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = X.feed_forward._Linear.apply(W, W.values, h, None, None, None)
+    assert torch.cuda.memory_allocated() - before <= 512 * 1024 * 4 + (64 << 10)
+    y.sum().backward()
+    want = torch.autograd.grad((unpack(D, f64(D.values)) @ (h64 := f64(h).requires_grad_(True))).sum(), h64)[0]
+    near(h.grad, want, 600 * EPS32, "dx")

@@ -424,7 +424,10 @@ class _Norm(torch.autograd.Function):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, W, values, x, bias, activation, residual):
-        y, z = sparse_linear(W, x, bias, activation, residual, keep=True, values=values)
+        # without an activation the backward pass does not read W x + bias
+        keep = _activation(activation) != 0
+        y = sparse_linear(W, x, bias, activation, residual, keep=keep, values=values)
+        y, z = y if keep else (y, None)
         ctx.W, ctx.activation, ctx.bias = W, activation, bias is not None
         ctx.save_for_backward(values, x, z, bias)
         return y
