@@ -210,3 +210,84 @@ def test_nothing_is_kept_that_no_pass_reads():
     y.sum().backward()
     want = torch.autograd.grad((unpack(D, f64(D.values)) @ (h64 := f64(h).requires_grad_(True))).sum(), h64)[0]
     near(h.grad, want, 600 * EPS32, "dx")
+
+
+# ---------------------------------------------------------------------------
+# the operators themselves through autograd
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("activation", [None, "gelu"])
+def test_linear_through_autograd(activation):
+    A = pruned(64, 48, 1)
+    W = X.SparseWeight(A)
+    W.values = A.values.clone().requires_grad_(True)
+    x, b, r = (normal(s, i).requires_grad_(True) for i, s in enumerate([(48, 20), (64,), (64, 20)]))
+    dy = normal((64, 20), 5)
+    y, kept = X.sparse_linear(W, x, bias=b, activation=activation, residual=r, keep=True)
+    with torch.no_grad():
+        y2, kept2 = X.sparse_linear(W, x, bias=b, activation=activation, residual=r, keep=True)
+    assert torch.equal(y, y2) and torch.equal(kept, kept2) and y.requires_grad and not kept.requires_grad
+    got = torch.autograd.grad(y, [W.values, x, b, r], dy)
+    leaves = [f64(t).requires_grad_(True) for t in (W.values, x, b, r)]
+    z = unpack(A, leaves[0]) @ leaves[1] + leaves[2][:, None]
+    y64 = (torch.nn.functional.gelu(z) if activation else z) + leaves[3]
+    for name, g, w in zip(("values", "x", "bias", "residual"), got, torch.autograd.grad(y64, leaves, f64(dy))):
+        near(g, w, 400 * EPS32, name)
+    # one at a time
+    for i, t in enumerate((x, b, r)):
+        args = [t if j == i else u.detach() for j, u in enumerate((x, b, r))]
+        y = X.sparse_linear(W, args[0], bias=args[1], activation=activation, residual=args[2], values=W.values.detach())
+        assert torch.equal(torch.autograd.grad(y, t, dy)[0], got[1 + i])
+
+
+def test_gated_through_autograd():
+    A, B = pruned(64, 48, 1), pruned(64, 48, 2)
+    G, U = X.SparseWeight(A), X.SparseWeight(B)
+    gv, uv = (m.values.clone().requires_grad_(True) for m in (A, B))
+    x, bg, bu = (normal(s, i).requires_grad_(True) for i, s in enumerate([(48, 20), (64,), (64,)]))
+    dh = normal((64, 20), 5)
+    h = X.sparse_gated(G, U, x, bg, bu, values=(gv, uv))
+    got = torch.autograd.grad(h, [gv, uv, x, bg, bu], dh)
+    leaves = [f64(t).requires_grad_(True) for t in (gv, uv, x, bg, bu)]
+    zg = unpack(A, leaves[0]) @ leaves[2] + leaves[3][:, None]
+    zu = unpack(B, leaves[1]) @ leaves[2] + leaves[4][:, None]
+    h64 = torch.nn.functional.silu(zg) * zu
+    near(h, h64.detach(), 200 * EPS32, "h")
+    for name, g, w in zip(("gate", "up", "x", "bias gate", "bias up"), got, torch.autograd.grad(h64, leaves, f64(dh))):
+        near(g, w, 400 * EPS32, name)
+    h, zg, zu = X.sparse_gated(G, U, x, bg, bu, keep=True)
+    assert h.requires_grad and not zg.requires_grad and not zu.requires_grad
+    h = X.sparse_gated(G, U, x.detach(), None, bu)
+    assert torch.equal(torch.autograd.grad(h, bu, dh)[0], torch.autograd.grad(
+        X.sparse_gated(G, U, x, None, bu), bu, dh)[0])
+
+
+def test_norm_through_autograd():
+    x, w, b = (normal(s, i).requires_grad_(True) for i, s in enumerate([(96, 20), (96,), (96,)]))
+    dy = normal((96, 20), 5)
+    y, mean, rstd = X.layer_norm(x, w, b, keep=True)
+    assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
+    got = torch.autograd.grad(y, [x, w, b], dy)
+    want = X.layer_norm_backward(dy, x.detach(), w.detach(), mean, rstd)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    y = X.layer_norm(x.detach(), None, b)
+    assert torch.equal(torch.autograd.grad(y, b, dy)[0], got[2])
+
+
+def test_no_graph_where_none_is_wanted():
+    A = pruned(64, 48, 1)
+    W = X.SparseWeight(A)
+    x = normal((48, 20), 1)
+    assert not X.sparse_linear(W, x).requires_grad and not X.layer_norm(x).requires_grad
+    x.requires_grad_(True)
+    with torch.no_grad():
+        assert not X.sparse_linear(W, x).requires_grad
+        assert not X.sparse_gated(W, W, x).requires_grad
+        assert not X.layer_norm(x).requires_grad
+    out = torch.empty((64, 20), device=DEV)
+    for call in (lambda: X.sparse_linear(W, x, out=out), lambda: X.sparse_gated(W, W, x, out=out),
+                 lambda: X.layer_norm(x, out=torch.empty_like(x))):
+        with pytest.raises(RuntimeError, match="out"):
+            call()
+        with torch.no_grad():
+            call()

@@ -12,8 +12,9 @@ take besides the framework's two.  Sums are fp32, rounded once.
   *_backward               their gradients
 
 The operators run on torch's current stream and allocate their results and
-scratch with torch.  ``FeedForward`` puts them together as a module with
-gradients.
+scratch with torch.  Where an operand has a gradient, the first three go through
+autograd, to the same kernels; what they keep, and the results of the backward
+operators, have none.  ``FeedForward`` puts them together as a module.
 """
 from __future__ import annotations
 
@@ -65,7 +66,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 _current = torch.cuda.current_device
+_grad_enabled = torch.is_grad_enabled
 _Tensor = torch.Tensor
+_PLAIN = (_Tensor, torch.nn.Parameter)
 
 
 def _call(index, f, *args):
@@ -82,7 +85,7 @@ def _call(index, f, *args):
 def _check(t, name, shape, dtype, device, mask=15):
     """The address of an operand that the kernels can take as given (None: no
     elements); raises otherwise.  mask: low bits that the address may not have."""
-    if (t.__class__ is _Tensor and t.dtype is dtype and t.shape == shape and t.device == device
+    if (t.__class__ in _PLAIN and t.dtype is dtype and t.shape == shape and t.device == device
             and t.is_contiguous()):
         at = t.data_ptr()
         if not at & mask:
@@ -107,6 +110,11 @@ def _activation(name):
         return ACTIVATIONS[name]
     except (KeyError, TypeError):
         raise ValueError(f"unknown activation {name!r}: one of {', '.join(k for k in ACTIVATIONS if k)}") from None
+
+
+def _no_out(out):
+    if out is not None:
+        raise RuntimeError("out= has no gradient: call it under torch.no_grad(), or without out")
 
 
 def _scratch(n, device):
@@ -160,14 +168,14 @@ class SparseWeight:
         self._own = v
 
     def _values(self, v=None):
-        """The address of the block values of a call: v, or the weight's."""
+        """The block values of a call, v or the weight's, and their address."""
         if self._h is None:
             raise RuntimeError("SparseWeight is closed")
         if v is None:
             v = self._own
             if v is None:
                 v = self.matrix.values
-        return _check(v, "values", self._flat, self.dtype, self.device)
+        return v, _check(v, "values", self._flat, self.dtype, self.device)
 
     def close(self):
         if self._h is not None:
@@ -184,9 +192,10 @@ class SparseWeight:
 def _tokens(x, name="x"):
     if not isinstance(x, _Tensor):
         raise TypeError(f"{name} must be a torch tensor")
-    if x.dim() != 2:
-        raise ValueError(f"{name} must be features x tokens, got {x.dim()} dimensions")
-    return x.shape[1]
+    shape = x.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} must be features x tokens, got {len(shape)} dimensions")
+    return shape[1]
 
 
 def _at(t):
@@ -199,15 +208,22 @@ def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, o
     values in the place of W's."""
     act = _activation(activation)
     (M, K), N, dt, dev = W.shape, _tokens(x), W.dtype, W.device
-    vals = W._values(values)
+    v, vals = W._values(values)
     xp = _check(x, "x", (K, N), dt, dev)
     bp = None if bias is None else _check(bias, "bias", (M,), dt, dev, 0)
     rp = None if residual is None else _check(residual, "residual", (M, N), dt, dev)
+    if (x.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad)) and _grad_enabled():
+        _no_out(out)
+        return _Linear.apply(W, v, x, bias, activation, residual, keep)
     y = x.new_empty((M, N)) if out is None else out
     yp = (y.data_ptr() or None) if out is None else _check(out, "out", (M, N), dt, dev)
-    z = x.new_empty((M, N)) if keep else None
+    if not keep:
+        _call(dev.index, W._L.xspmm_linear, W._h, W.code, act, vals, xp, bp, rp, yp, None, N)
+        return y
+    z = x.new_empty((M, N))
     _call(dev.index, W._L.xspmm_linear, W._h, W.code, act, vals, xp, bp, rp, yp, _at(z), N)
-    return (y, z) if keep else y
+    return y, z
 
 
 def sparse_linear_backward(W, x, kept, dy, activation=None, bias=False, need=(True, True), values=None):
@@ -218,7 +234,7 @@ def sparse_linear_backward(W, x, kept, dy, activation=None, bias=False, need=(Tr
     residual's gradient is dy."""
     act = _activation(activation)
     (M, K), N, dt, dev = W.shape, _tokens(dy, "dy"), W.dtype, W.device
-    vals = W._values(values)
+    _, vals = W._values(values)
     xp = _check(x, "x", (K, N), dt, dev)
     zp = _check(kept, "kept", (M, N), dt, dev) if act else None
     gp = _check(dy, "dy", (M, N), dt, dev)
@@ -248,16 +264,22 @@ def sparse_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", keep=
     own.  values: block values in the place of G's and U's (None: theirs)."""
     act = _activation(activation)
     (M, K), N, dt, dev = _pair(G, U), _tokens(x), G.dtype, G.device
-    gv, uv = G._values(values[0]), U._values(values[1])
+    (g, gv), (u, uv) = G._values(values[0]), U._values(values[1])
     xp = _check(x, "x", (K, N), dt, dev)
     gb = None if bias_gate is None else _check(bias_gate, "bias_gate", (M,), dt, dev, 0)
     ub = None if bias_up is None else _check(bias_up, "bias_up", (M,), dt, dev, 0)
+    if (x.requires_grad or g.requires_grad or u.requires_grad or (bias_gate is not None and bias_gate.requires_grad)
+            or (bias_up is not None and bias_up.requires_grad)) and _grad_enabled():
+        _no_out(out)
+        return _Gated.apply(G, U, g, u, x, bias_gate, bias_up, activation, keep)
     h = x.new_empty((M, N)) if out is None else out
     hp = (h.data_ptr() or None) if out is None else _check(out, "out", (M, N), dt, dev)
-    zg = x.new_empty((M, N)) if keep else None
-    zu = x.new_empty((M, N)) if keep else None
+    if not keep:
+        _call(dev.index, G._L.xspmm_gated, G._h, U._h, G.code, act, gv, uv, xp, gb, ub, hp, None, None, N)
+        return h
+    zg, zu = x.new_empty((M, N)), x.new_empty((M, N))
     _call(dev.index, G._L.xspmm_gated, G._h, U._h, G.code, act, gv, uv, xp, gb, ub, hp, _at(zg), _at(zu), N)
-    return (h, zg, zu) if keep else h
+    return h, zg, zu
 
 
 def sparse_gated_backward(G, U, x, kept_gate, kept_up, dh, activation="silu", bias=False, need=(True, True, True),
@@ -268,7 +290,7 @@ def sparse_gated_backward(G, U, x, kept_gate, kept_up, dh, activation="silu", bi
     (None otherwise); values as in the forward pass."""
     act = _activation(activation)
     (M, K), N, dt, dev = _pair(G, U), _tokens(dh, "dh"), G.dtype, G.device
-    gv, uv = G._values(values[0]), U._values(values[1])
+    (_, gv), (_, uv) = G._values(values[0]), U._values(values[1])
     xp = _check(x, "x", (K, N), dt, dev)
     zg = _check(kept_gate, "kept_gate", (M, N), dt, dev)
     zu = _check(kept_up, "kept_up", (M, N), dt, dev)
@@ -318,6 +340,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, keep=False, out=None):
     ``layer_norm_backward`` takes."""
     K, N, dt, dev, xp, wp = _norm_operands(x, weight)
     bp = None if bias is None else _check(bias, "bias", (K,), dt, dev, 0)
+    if (x.requires_grad or (weight is not None and weight.requires_grad)
+            or (bias is not None and bias.requires_grad)) and _grad_enabled():
+        _no_out(out)
+        return _Norm.apply(x, weight, bias, eps, keep)
     y = x.new_empty((K, N)) if out is None else out
     yp = (y.data_ptr() or None) if out is None else _check(out, "out", (K, N), dt, dev)
     mean = torch.empty(N, dtype=torch.float32, device=dev) if keep else None
@@ -407,58 +433,65 @@ def _first_order(backward):
     return first_order
 
 
+def _result(ctx, y, *kept):
+    """Results of a forward pass, of which the kept ones have no gradient."""
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(*kept)
+    return (y, *kept)
+
+
 class _Norm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
+    def forward(ctx, x, weight, bias, eps, keep=False):
         y, mean, rstd = layer_norm(x, weight, bias, eps, keep=True)
         ctx.save_for_backward(x, weight, mean, rstd)
-        return y
+        return _result(ctx, y, mean, rstd) if keep else y
 
     @staticmethod
     @_first_order
-    def backward(ctx, dy):
+    def backward(ctx, dy, *_):
         x, weight, mean, rstd = ctx.saved_tensors
-        return (*layer_norm_backward(_incoming(dy), x, weight, mean, rstd, need=ctx.needs_input_grad[:3]), None)
+        return (*layer_norm_backward(_incoming(dy), x, weight, mean, rstd, need=ctx.needs_input_grad[:3]), None, None)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, W, values, x, bias, activation, residual):
+    def forward(ctx, W, values, x, bias, activation, residual, keep=False):
         # without an activation the backward pass does not read W x + bias
-        keep = _activation(activation) != 0
-        y = sparse_linear(W, x, bias, activation, residual, keep=keep, values=values)
-        y, z = y if keep else (y, None)
+        wanted = keep or _activation(activation) != 0
+        y = sparse_linear(W, x, bias, activation, residual, keep=wanted, values=values)
+        y, z = y if wanted else (y, None)
         ctx.W, ctx.activation, ctx.bias = W, activation, bias is not None
-        ctx.save_for_backward(values, x, z, bias)
-        return y
+        ctx.save_for_backward(values, x, z if _activation(activation) else None, bias)
+        return _result(ctx, y, z) if keep else y
 
     @staticmethod
     @_first_order
-    def backward(ctx, dy):
-        values, x, z, _ = ctx.saved_tensors
+    def backward(ctx, dy, *_):
+        values, x, z, _bias = ctx.saved_tensors
         dy = _incoming(dy)
         need = ctx.needs_input_grad
         dx, dv, db = sparse_linear_backward(ctx.W, x, z, dy, ctx.activation, ctx.bias and need[3], (need[2], need[1]),
                                             values=values)
-        return None, dv, dx, db, None, dy if need[5] else None
+        return None, dv, dx, db, None, dy if need[5] else None, None
 
 
 class _Gated(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, G, U, gate, up, x, activation):
-        h, zg, zu = sparse_gated(G, U, x, activation=activation, keep=True, values=(gate, up))
+    def forward(ctx, G, U, gate, up, x, bias_gate, bias_up, activation, keep=False):
+        h, zg, zu = sparse_gated(G, U, x, bias_gate, bias_up, activation, keep=True, values=(gate, up))
         ctx.G, ctx.U, ctx.activation = G, U, activation
-        ctx.save_for_backward(gate, up, x, zg, zu)
-        return h
+        ctx.save_for_backward(gate, up, x, zg, zu, bias_gate, bias_up)
+        return _result(ctx, h, zg, zu) if keep else h
 
     @staticmethod
     @_first_order
-    def backward(ctx, dh):
-        gate, up, x, zg, zu = ctx.saved_tensors
+    def backward(ctx, dh, *_):
+        gate, up, x, zg, zu, _bg, _bu = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dg, du, _, _ = sparse_gated_backward(ctx.G, ctx.U, x, zg, zu, _incoming(dh), ctx.activation,
-                                                 need=(need[4], need[2], need[3]), values=(gate, up))
-        return None, None, dg, du, dx, None
+        dx, dg, du, bg, bu = sparse_gated_backward(ctx.G, ctx.U, x, zg, zu, _incoming(dh), ctx.activation,
+                                                   need[5] or need[6], (need[4], need[2], need[3]), (gate, up))
+        return None, None, dg, du, dx, bg if need[5] else None, bu if need[6] else None, None, None
 
 
 class FeedForward(torch.nn.Module):
@@ -485,11 +518,6 @@ class FeedForward(torch.nn.Module):
 
     def forward(self, x):
         G, U, D = self._weights
-        if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
-            n = _Norm.apply(x, self.norm_weight, self.norm_bias, self.eps)
-            h = _Gated.apply(G, U, self.gate, self.up, n, self.activation)
-            return _Linear.apply(D, self.down, h, None, None, x)
-        gate, up, down = self.gate.detach(), self.up.detach(), self.down.detach()
-        n = layer_norm(x.detach(), self.norm_weight.detach(), self.norm_bias.detach(), self.eps)
-        h = sparse_gated(G, U, n, activation=self.activation, values=(gate, up))
-        return sparse_linear(D, h, residual=x.detach(), values=down)
+        n = layer_norm(x, self.norm_weight, self.norm_bias, self.eps)
+        h = sparse_gated(G, U, n, activation=self.activation, values=(self.gate, self.up))
+        return sparse_linear(D, h, residual=x, values=self.down)
