@@ -291,3 +291,39 @@ def test_no_graph_where_none_is_wanted():
             call()
         with torch.no_grad():
             call()
+
+
+# ---------------------------------------------------------------------------
+# copies
+# ---------------------------------------------------------------------------
+
+def test_copies_have_handles_of_their_own():
+    A = pruned(64, 48, 1)
+    W = X.SparseWeight(A)
+    W.values = A.values * 2
+    x = normal((48, 20), 1)
+    y = X.sparse_linear(W, x)
+    shallow, deep = copy.copy(W), copy.deepcopy(W)
+    assert shallow.matrix is A and deep.matrix is not A
+    W.close()
+    for V in (shallow, deep):
+        assert torch.equal(X.sparse_linear(V, x), y)
+    assert deep.values.data_ptr() != shallow.values.data_ptr()
+    shallow.close()
+    assert torch.equal(X.sparse_linear(deep, x), y)
+
+
+def test_copy_of_a_layer():
+    A, D = pruned(64, 48, 1), pruned(48, 64, 2)
+    layer = X.FeedForward(A, A, D)
+    x = normal((48, 20), 1)
+    with torch.no_grad():
+        want = layer(x)
+        other = copy.deepcopy(layer)
+        layer.gate.zero_()
+        assert torch.equal(other(x), want) and torch.equal(layer(x), x)
+        buffer = io.BytesIO()
+        torch.save(other, buffer)
+        buffer.seek(0)
+        again = torch.load(buffer, weights_only=False)  # what this test wrote itself
+        assert torch.equal(again(x), want)

@@ -188,6 +188,10 @@ class SparseWeight:
         except Exception:
             pass
 
+    def __reduce__(self):
+        # copies lay their matrix out again: two that held one handle would free it twice
+        return SparseWeight, (self.matrix,), {"_own": self._own}
+
 
 def _tokens(x, name="x"):
     if not isinstance(x, _Tensor):
