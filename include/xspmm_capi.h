@@ -400,8 +400,9 @@ int xspmm_mtx_free(xspmm_mtx_t m);
  * of one value type (XSPMM_F32, XSPMM_F16 or XSPMM_BF16); sums are fp32 and are
  * rounded once, when they are stored.  Block values, activations and gradients
  * start on a 16-byte boundary (biases and per-feature arrays need not).  The
- * results may not overlap the operands.  N = 0 is allowed: sums over no tokens
- * are zero.  Asynchronous on `stream`; nothing is allocated.
+ * results may not overlap the operands (xspmm_linear's y may be its residual).
+ * N = 0 is allowed: sums over no tokens are zero.  Asynchronous on `stream`;
+ * nothing is allocated.
  */
 #define XSPMM_ACT_NONE 0
 #define XSPMM_ACT_RELU 1

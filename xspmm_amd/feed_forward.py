@@ -117,6 +117,16 @@ def _no_out(out):
         raise RuntimeError("out= has no gradient: call it under torch.no_grad(), or without out")
 
 
+def _apart(out, **operands):
+    """Raises where a result shares memory with an operand: workgroups read the
+    operands after others have written."""
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    for name, t in operands.items():
+        if t is not None and t.data_ptr() < hi and lo < t.data_ptr() + t.numel() * t.element_size():
+            raise ValueError(f"out overlaps {name}")
+
+
 def _scratch(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
@@ -209,7 +219,8 @@ def _at(t):
 def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, out=None, values=None):
     """act(W x + bias) + residual, M x N; with keep also W x + bias, which
     ``sparse_linear_backward`` takes where there is an activation.  values: block
-    values in the place of W's."""
+    values in the place of W's.  out: memory for the result, apart from every
+    operand, or the residual itself."""
     act = _activation(activation)
     (M, K), N, dt, dev = W.shape, _tokens(x), W.dtype, W.device
     v, vals = W._values(values)
@@ -220,8 +231,12 @@ def sparse_linear(W, x, bias=None, activation=None, residual=None, keep=False, o
             or (residual is not None and residual.requires_grad)) and _grad_enabled():
         _no_out(out)
         return _Linear.apply(W, v, x, bias, activation, residual, keep)
-    y = x.new_empty((M, N)) if out is None else out
-    yp = (y.data_ptr() or None) if out is None else _check(out, "out", (M, N), dt, dev)
+    if out is None:
+        y = x.new_empty((M, N))
+        yp = y.data_ptr() or None
+    else:
+        y, yp = out, _check(out, "out", (M, N), dt, dev)
+        _apart(out, x=x, values=v, bias=bias, residual=None if yp == rp else residual)
     if not keep:
         _call(dev.index, W._L.xspmm_linear, W._h, W.code, act, vals, xp, bp, rp, yp, None, N)
         return y
@@ -265,7 +280,8 @@ def sparse_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", keep=
                  values=(None, None)):
     """act(G x + bias_gate) * (U x + bias_up), M x N; with keep also the two
     sums, which ``sparse_gated_backward`` takes.  G and U have blocks of their
-    own.  values: block values in the place of G's and U's (None: theirs)."""
+    own.  values: block values in the place of G's and U's (None: theirs).  out:
+    memory for the result, apart from every operand."""
     act = _activation(activation)
     (M, K), N, dt, dev = _pair(G, U), _tokens(x), G.dtype, G.device
     (g, gv), (u, uv) = G._values(values[0]), U._values(values[1])
@@ -276,8 +292,12 @@ def sparse_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", keep=
             or (bias_up is not None and bias_up.requires_grad)) and _grad_enabled():
         _no_out(out)
         return _Gated.apply(G, U, g, u, x, bias_gate, bias_up, activation, keep)
-    h = x.new_empty((M, N)) if out is None else out
-    hp = (h.data_ptr() or None) if out is None else _check(out, "out", (M, N), dt, dev)
+    if out is None:
+        h = x.new_empty((M, N))
+        hp = h.data_ptr() or None
+    else:
+        h, hp = out, _check(out, "out", (M, N), dt, dev)
+        _apart(out, x=x, gate_values=g, up_values=u, bias_gate=bias_gate, bias_up=bias_up)
     if not keep:
         _call(dev.index, G._L.xspmm_gated, G._h, U._h, G.code, act, gv, uv, xp, gb, ub, hp, None, None, N)
         return h
@@ -341,15 +361,19 @@ def _norm_operands(x, weight):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, keep=False, out=None):
     """Layer norm over the features (rows) of every token (column) of x; with
     keep also the tokens' mean and 1 / sqrt(variance + eps) in fp32, which
-    ``layer_norm_backward`` takes."""
+    ``layer_norm_backward`` takes.  out: memory for the result, apart from x."""
     K, N, dt, dev, xp, wp = _norm_operands(x, weight)
     bp = None if bias is None else _check(bias, "bias", (K,), dt, dev, 0)
     if (x.requires_grad or (weight is not None and weight.requires_grad)
             or (bias is not None and bias.requires_grad)) and _grad_enabled():
         _no_out(out)
         return _Norm.apply(x, weight, bias, eps, keep)
-    y = x.new_empty((K, N)) if out is None else out
-    yp = (y.data_ptr() or None) if out is None else _check(out, "out", (K, N), dt, dev)
+    if out is None:
+        y = x.new_empty((K, N))
+        yp = y.data_ptr() or None
+    else:
+        y, yp = out, _check(out, "out", (K, N), dt, dev)
+        _apart(out, x=x, weight=weight, bias=bias)
     mean = torch.empty(N, dtype=torch.float32, device=dev) if keep else None
     rstd = torch.empty(N, dtype=torch.float32, device=dev) if keep else None
     code = _TYPES[dt]
