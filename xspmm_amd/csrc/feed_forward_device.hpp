@@ -154,23 +154,60 @@ __device__ __forceinline__ float4_t mfma32(uint32_t a, uint32_t b, float4_t c)
 }
 
 // ---------------------------------------------------------------------------
-// activations, in fp32.  Every form takes its sigmoid or error function from
-// values that neither overflow nor cancel: infinite sums give the limits.
+// activations, in fp32.  Sums are taken to where an activation and its slope have
+// reached their limits, so that infinite ones give these, too (a NaN stays).
 // ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float at_least(float z, float low) { return z < low ? low : z; }
+__device__ __forceinline__ float within(float z, float most) { return z < -most ? -most : z > most ? most : z; }
 
 __device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
 
+// The normal distribution's density (times sqrt(2 pi)) and integral P(z), which is
+// (1 + erf(z / sqrt 2)) / 2 but keeps its digits where it vanishes: 1 + erf cancels, at
+// z = -5 to a hundredth of the value.  P(-|z|) = exp(-z^2 / 2) t Q(t), t = 1 / (1 + 0.35
+// |z|); Q has degree 8, with the smallest largest relative error (half of 2^-24) on
+// |z| <= 16.5.  All in all (6 + 0.6 z^2) 2^-24 of P, most of it exp's argument.  One exp
+// and no branch: an erfc costs a product of 14336 x 4096 and 2048 tokens 14 us of 277.
+__device__ __forceinline__ float normal_density(float z) { return expf(-0.5f * z * z); }
+__device__ __forceinline__ float normal_integral(float z, float density)
+{
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, fabsf(z), 1.f));
+    float q = -0.0291653033f;
+    q = fmaf(q, t, 0.144067645f);
+    q = fmaf(q, t, -0.255916327f);
+    q = fmaf(q, t, 0.159409836f);
+    q = fmaf(q, t, -0.0232758019f);
+    q = fmaf(q, t, 0.105580017f);
+    q = fmaf(q, t, 0.119814134f);
+    q = fmaf(q, t, 0.139864534f);
+    q = fmaf(q, t, 0.139621243f);
+    q *= t * density;
+    return z < 0.f ? q : 1.f - q;
+}
+
 constexpr float kGeluA = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;
+// where the sigmoid, and the two gelus' share of z, are 0 and 1 in fp32
+constexpr float kSiluEnd = 128.f, kGeluEnd = 16.f;
 
 template <int ACT>
 __device__ __forceinline__ float act_value(float z)
 {
-    if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;  // a NaN stays
-    if constexpr (ACT == kActSilu) return z / (1.f + expf(-z));
-    if constexpr (ACT == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if constexpr (ACT == kActRelu) return at_least(z, 0.f);
+    if constexpr (ACT == kActSilu) {
+        const float c = at_least(z, -kSiluEnd);
+        return c / (1.f + expf(-c));
+    }
+    if constexpr (ACT == kActGelu) {
+        const float c = at_least(z, -kGeluEnd);
+        return c * normal_integral(c, normal_density(c));
+    }
     // 0.5 (1 + tanh u) = sigmoid(2u)
-    if constexpr (ACT == kActGeluTanh) return z / (1.f + expf(-kGeluA * (z + kGeluB * z * z * z)));
+    if constexpr (ACT == kActGeluTanh) {
+        const float c = at_least(z, -kGeluEnd);
+        return c / (1.f + expf(-kGeluA * (c + kGeluB * c * c * c)));
+    }
     return z;
 }
 
@@ -179,26 +216,23 @@ template <int ACT>
 __device__ __forceinline__ float act_slope(float z, float* value)
 {
     if constexpr (ACT == kActRelu) {
-        *value = z < 0.f ? 0.f : z;
+        *value = at_least(z, 0.f);
         return z > 0.f ? 1.f : z == z ? 0.f : z;
     }
     if constexpr (ACT == kActSilu) {
-        const float p = sigmoid(z);
-        *value = z * p;
-        return p * (1.f + z * (1.f - p));
+        const float c = within(z, kSiluEnd), p = sigmoid(c);
+        *value = at_least(z, -kSiluEnd) * p;
+        return p * (1.f + c * (1.f - p));
     }
     if constexpr (ACT == kActGelu) {
-        const float p = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-        *value = z * p;
-        return p + 0.3989422804014327f * z * expf(-0.5f * z * z);
+        const float c = within(z, kGeluEnd), e = normal_density(c), p = normal_integral(c, e);
+        *value = at_least(z, -kGeluEnd) * p;
+        return p + 0.3989422804014327f * c * e;
     }
     if constexpr (ACT == kActGeluTanh) {
-        // beyond |z| = 16 the sigmoid is 0 or 1 in fp32 and the slope with it;
-        // the clamp keeps z^3 finite there
-        const float c = fminf(fmaxf(z, -16.f), 16.f);
-        const float p = sigmoid(kGeluA * (c + kGeluB * c * c * c));
-        *value = z * p;
-        return z == z ? p + c * p * (1.f - p) * kGeluA * (1.f + 3.f * kGeluB * c * c) : z;
+        const float c = within(z, kGeluEnd), p = sigmoid(kGeluA * (c + kGeluB * c * c * c));
+        *value = at_least(z, -kGeluEnd) * p;
+        return p + c * p * (1.f - p) * kGeluA * (1.f + 3.f * kGeluB * c * c);
     }
     *value = z;
     return 1.f;
