@@ -92,3 +92,22 @@ def test_activations_keep_their_digits_where_they_vanish():
         off = (got.double().cpu() - want).abs()
         bound = (64 + 8 * u.abs()) * EPS32 * want.abs()
         assert (off <= bound)[within].all(), float((off / want.abs())[within].max())
+
+
+@pytest.mark.parametrize("K,N", [(1000, 100), (130, 1000), (4000, 20)])
+def test_norm_of_large_means(K, N):
+    """A mean whose square is past fp32's range, deviations whose squares are not."""
+    j = torch.randint(0, 8, (K, N), generator=torch.Generator().manual_seed(1)).double()
+    x64 = 2.0 ** 65 * (1 + j * 2.0 ** -12)
+    x = x64.float().to(DEV)
+    assert torch.equal(x.double().cpu(), x64)
+    y, mean, rstd = X.layer_norm(x, keep=True)
+    m = x64.mean(0)
+    r = 1 / torch.sqrt((x64 - m).square().mean(0) + 1e-5)
+    assert ((mean.double().cpu() - m).abs() <= 64 * EPS32 * m).all()
+    want = (x64 - m) * r
+    off = (y.double().cpu() - want).abs()
+    assert (off <= 128 * EPS32 * (want.abs() + 2 * m * r)).all(), float(off.max())
+    # of one sign throughout, and of a feature far off
+    x[5] = -2.0 ** 66
+    assert X.layer_norm(x).isfinite().all()

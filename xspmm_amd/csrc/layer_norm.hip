@@ -42,6 +42,7 @@ struct Moments {
     float n, m[V], s[V];
 };
 
+// d * weight first: where a part is empty that is zero, and d * d may be past fp32's range.
 template <int V>
 __device__ __forceinline__ void join(Moments<V>& a, const Moments<V>& b)
 {
@@ -52,7 +53,7 @@ __device__ __forceinline__ void join(Moments<V>& a, const Moments<V>& b)
     for (int i = 0; i < V; ++i) {
         const float d = b.m[i] - a.m[i];
         a.m[i] += d * share;
-        a.s[i] += b.s[i] + d * d * weight;
+        a.s[i] += b.s[i] + d * (d * weight);
     }
 }
 
