@@ -401,8 +401,10 @@ int xspmm_mtx_free(xspmm_mtx_t m);
  * rounded once, when they are stored.  Block values, activations and gradients
  * start on a 16-byte boundary (biases and per-feature arrays need not).  The
  * results may not overlap the operands (xspmm_linear's y may be its residual).
- * N = 0 is allowed: sums over no tokens are zero.  Asynchronous on `stream`;
- * nothing is allocated.
+ * N = 0 is allowed: sums over no tokens are zero.  N is at most 2^30, and results
+ * that take more than one launch's 2^32 threads fail with XSPMM_ERR_INVALID
+ * (products of operands over 2 GiB, from 2^36 elements on at 64 rows or more).
+ * Asynchronous on `stream`; nothing is allocated.
  */
 #define XSPMM_ACT_NONE 0
 #define XSPMM_ACT_RELU 1
@@ -415,8 +417,8 @@ int xspmm_mtx_free(xspmm_mtx_t m);
  * arrays (16x16 blocks, block columns strictly ascending within a row, as
  * csr_to_bcsr makes them) and the same blocks by block-column.  The arrays are
  * not referenced afterwards; the values are passed to every call, so they may
- * change between calls.  Arrays that are no such matrix fail with
- * XSPMM_ERR_INVALID.  Synchronizes `stream`.
+ * change between calls.  Arrays that are no such matrix, and more than 2^30 - 64
+ * rows or columns, fail with XSPMM_ERR_INVALID.  Synchronizes `stream`.
  */
 typedef struct xspmm_weight_s* xspmm_weight_t;
 int xspmm_weight_create(int itype, int64_t M, int64_t K, int64_t Mb, int64_t Kb, int64_t nnzb, const void* brp,

@@ -95,6 +95,14 @@ struct SampledArgs {
 template <typename T>
 void sampled_product(const SampledArgs<T>& a, int weights, hipStream_t s);
 
+// A launch holds less than 2^32 threads along its first dimension.
+inline dim3 launch_grid(int64_t groups, int threads, unsigned sides = 1)
+{
+    if (groups > 0xffffffffLL / threads)
+        throw std::invalid_argument("xSpMM: too many tokens or blocks for one launch.");
+    return dim3((unsigned)groups, sides);
+}
+
 // Bytes of `rows` rows of N elements where those of whole blocks of rows stay
 // below 2^31, else -1.
 inline int64_t narrow_bytes(int64_t rows, int64_t N, int64_t size)

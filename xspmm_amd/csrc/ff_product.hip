@@ -384,10 +384,8 @@ void launch(const ProductArgs<T>& a, hipStream_t s)
     constexpr int rows = SPLIT > kWaves ? 1 : kWaves / SPLIT, threads = 64 * (SPLIT > kWaves ? SPLIT : kWaves);
     constexpr int tile = ONE ? 1 : 16 * VEC;
     const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + tile - 1) / tile);
-    const int64_t grid = kXcds * xcd_chunk(items);
-    if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many tokens for one launch.");
-    hipLaunchKernelGGL((ff_product_kernel<T, VEC, NACC, TR, SPLIT, WIDE, ONE>), dim3((unsigned)grid), dim3(threads), 0,
-                       s, a);
+    hipLaunchKernelGGL((ff_product_kernel<T, VEC, NACC, TR, SPLIT, WIDE, ONE>),
+                       launch_grid(kXcds * xcd_chunk(items), threads), dim3(threads), 0, s, a);
     XSPMM_LAUNCH_CHECK();
 }
 

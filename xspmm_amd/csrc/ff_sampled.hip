@@ -357,8 +357,7 @@ void sampled_fours(const SampledArgs<T>& f, int weights, hipStream_t s)
     }
     if (sides == 0) return;
     auto go = [&](auto kernel, int64_t grid) {
-        if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many blocks for one launch.");
-        hipLaunchKernelGGL(kernel, dim3((unsigned)grid, sides), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(kernel, launch_grid(grid, 256, sides), dim3(256), 0, s, a);
         XSPMM_LAUNCH_CHECK();
     };
     // rows of at least a line, through LDS (off 16 bytes, 14336 x 4096 fp16, 30 %
@@ -567,14 +566,11 @@ template <typename T>
 void launch_sampled_tile(SampledTile<T>& a, bool aligned, hipStream_t s)
 {
     a.items = (int64_t)((a.Mb + kEdge - 1) / kEdge) * ((a.Kb + kEdge - 1) / kEdge);
-    const int64_t grid = kXcds * xcd_chunk(a.items * a.sides);
-    if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many blocks for one launch.");
+    const dim3 grid = launch_grid(kXcds * xcd_chunk(a.items * a.sides), kThreads);
     if (aligned)
-        hipLaunchKernelGGL((ff_sampled_tile_kernel<T, true>), dim3((unsigned)grid),
-                           dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((ff_sampled_tile_kernel<T, true>), grid, dim3(kThreads), 0, s, a);
     else
-        hipLaunchKernelGGL((ff_sampled_tile_kernel<T, false>), dim3((unsigned)grid),
-                           dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((ff_sampled_tile_kernel<T, false>), grid, dim3(kThreads), 0, s, a);
     XSPMM_LAUNCH_CHECK();
 }
 

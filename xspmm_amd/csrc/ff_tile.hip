@@ -383,14 +383,11 @@ void launch_shape(const TileArgs<T>& a, hipStream_t s)
 {
     constexpr int rows = GATED ? SLOTS / 2 : SLOTS;
     const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + kWide - 1) / kWide);
-    const int64_t grid = kXcds * xcd_chunk(items);
-    if (grid > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many tokens for one launch.");
+    const dim3 grid = launch_grid(kXcds * xcd_chunk(items), kTileThreads);
     if (a.N % 8 == 0)
-        hipLaunchKernelGGL((ff_tile_kernel<T, SLOTS, TR, GATED, true>), dim3((unsigned)grid), dim3(kTileThreads), 0, s,
-                           a);
+        hipLaunchKernelGGL((ff_tile_kernel<T, SLOTS, TR, GATED, true>), grid, dim3(kTileThreads), 0, s, a);
     else
-        hipLaunchKernelGGL((ff_tile_kernel<T, SLOTS, TR, GATED, false>), dim3((unsigned)grid), dim3(kTileThreads), 0, s,
-                           a);
+        hipLaunchKernelGGL((ff_tile_kernel<T, SLOTS, TR, GATED, false>), grid, dim3(kTileThreads), 0, s, a);
     XSPMM_LAUNCH_CHECK();
 }
 

@@ -150,7 +150,8 @@ void build_block_index(BlockIndex& out, int64_t M, int64_t K, int64_t Mb, int64_
         if (!ok) throw std::invalid_argument(what);
     };
     require(M >= 0 && K >= 0 && nnzb >= 0, "xSpMM: weight dimensions must be non-negative.");
-    require(M < 0x7ffffff0LL && K < 0x7ffffff0LL, "xSpMM: a weight has at most 2^31 - 17 rows and columns.");
+    // a wave per block-row, and per block-column, of one launch
+    require(M <= (1LL << 30) - 64 && K <= (1LL << 30) - 64, "xSpMM: a weight has at most 2^30 - 64 rows and columns.");
     require(Mb == (M + 15) / 16 && Kb == (K + 15) / 16, "xSpMM: a weight's block grid must cover it with 16x16 blocks.");
     require(nnzb < 0x7fffffffLL, "xSpMM: a weight has at most 2^31 - 2 blocks.");
     require(brp != nullptr && (nnzb == 0 || bci != nullptr), "xSpMM: null weight array.");

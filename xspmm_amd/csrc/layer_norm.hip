@@ -679,12 +679,8 @@ NormShape backward_shape(int64_t K, int64_t N, int64_t size)
 }
 bool small_norm(int64_t K, int64_t N) { return K * N <= 65536 || N <= 16; }
 
-dim3 norm_grid(const NormShape& h)
-{
-    const int64_t g = h.tiles * h.slices;
-    if (g > 0x7fffffffLL) throw std::invalid_argument("xSpMM: too many tokens for one launch.");
-    return dim3((unsigned)g);
-}
+static_assert(kForwardWaves == kBackwardWaves);
+dim3 norm_grid(const NormShape& h) { return launch_grid(h.tiles * h.slices, 64 * kForwardWaves); }
 
 }  // namespace ff
 
