@@ -89,7 +89,7 @@ def test_activations_around_two_gib(kind, M, K, N):
 
 
 # block values past 2 GiB
-@pytest.mark.parametrize("kind,blocks", [("f16", 2050), ("f32", 1450)])
+@pytest.mark.parametrize("kind,blocks", [("f16", 2050), ("bf16", 2050), ("f32", 1450)])
 @pytest.mark.parametrize("N", [1, 33, 65])
 def test_block_values_past_two_gib(kind, blocks, N):
     print(kind, blocks, N, flush=True)

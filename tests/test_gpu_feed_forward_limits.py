@@ -111,3 +111,19 @@ def test_norm_of_large_means(K, N):
     # of one sign throughout, and of a feature far off
     x[5] = -2.0 ** 66
     assert X.layer_norm(x).isfinite().all()
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("N", [1, 40])
+def test_weights_of_no_rows_and_of_no_columns(kind, N):
+    dtype = KINDS[kind]
+    tall, wide = no_blocks(40, 0, dtype), no_blocks(0, 40, dtype)
+    none, x = torch.empty((0, N), dtype=dtype, device=DEV), torch.ones((40, N), dtype=dtype, device=DEV)
+    b = torch.arange(40, device=DEV).to(dtype)
+    assert torch.equal(X.sparse_linear(tall, none, bias=b), b[:, None].expand(40, N))
+    assert X.sparse_linear(wide, x).shape == (0, N) and X.sparse_gated(wide, wide, x).shape == (0, N)
+    dx, dv, db = X.sparse_linear_backward(tall, none, x, x, activation="relu", bias=True)
+    assert dx.shape == (0, N) and dv.numel() == 0 and (db == N).all()
+    dx, dv, db = X.sparse_linear_backward(wide, x, none, none, activation="relu", bias=True)
+    assert dx.shape == (40, N) and not dx.any() and db.numel() == 0
+    assert not X.sparse_gated_backward(wide, wide, x, none, none, none)[0].any()
