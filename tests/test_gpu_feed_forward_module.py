@@ -327,3 +327,22 @@ def test_copy_of_a_layer():
         buffer.seek(0)
         again = torch.load(buffer, weights_only=False)  # what this test wrote itself
         assert torch.equal(again(x), want)
+
+
+def test_a_layer_holds_its_values_once():
+    """The caller's matrices are not kept alive by the layers made from them."""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    A, D = pruned(1024, 512, 1), pruned(512, 1024, 2)
+    layer = X.FeedForward(A, A, D)
+    x = normal((512, 16), 3)
+    with torch.no_grad():
+        want = layer(x)
+    size = sum(p.numel() * 4 for p in layer.parameters())
+    del A, D
+    held = torch.cuda.memory_allocated() - before
+    assert size <= held <= 1.1 * size + 2 * x.numel() * 4 + (256 << 10)
+    with torch.no_grad():
+        assert torch.equal(layer(x), want)
+        layer.up.zero_()
+        assert torch.equal(layer(x), x)

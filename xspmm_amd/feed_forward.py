@@ -19,6 +19,7 @@ operators, have none.  ``FeedForward`` puts them together as a module.
 from __future__ import annotations
 
 import ctypes as C
+import dataclasses
 import functools
 
 import torch
@@ -532,14 +533,16 @@ class FeedForward(torch.nn.Module):
 
     def __init__(self, gate, up, down, activation="silu", eps=1e-5):
         super().__init__()
-        self._weights = [SparseWeight(A) for A in (gate, up, down)]
+        # matrices of its own, whose values the parameters share
+        self._weights = [SparseWeight(dataclasses.replace(A, values=A.values.detach().clone()))
+                         for A in (gate, up, down)]
         G, U, D = self._weights
         features = _pair(G, U)[1]
         if D.shape != (features, G.shape[0]) or D.dtype is not G.dtype or D.device != G.device:
             raise ValueError(f"down is {D.shape}, {D.dtype}, expected {(features, G.shape[0])}, {G.dtype}")
         _activation(activation)
         self.activation, self.eps = activation, eps
-        self.gate, self.up, self.down = (torch.nn.Parameter(W.values.clone()) for W in self._weights)
+        self.gate, self.up, self.down = (torch.nn.Parameter(W.values) for W in self._weights)
         like = dict(dtype=G.dtype, device=G.device)
         self.norm_weight = torch.nn.Parameter(torch.ones(features, **like))
         self.norm_bias = torch.nn.Parameter(torch.zeros(features, **like))
