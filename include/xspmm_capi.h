@@ -435,7 +435,7 @@ int xspmm_linear(xspmm_weight_t weight, int vtype, int act, const void* vals, co
 
 /*
  * Its backward pass from dy: dz = dy act'(keep), rounded to the value type
- * before the products; dx = A^T dz (K x N), dvals = the stored blocks of
+ * before the products (XSPMM_F16: infinite past 65504, zero below 6e-8); dx = A^T dz (K x N), dvals = the stored blocks of
  * dz x^T (zero past the edges of A), dbias = sums of dz over the tokens.  Each
  * result may be NULL.  The residual's gradient is dy itself.  keep is not read
  * with XSPMM_ACT_NONE.  scratch (256-byte aligned) holds dz: as many bytes as

@@ -112,13 +112,12 @@ T* result(void* p, bool needed, const char* what)
     return const_cast<T*>(operand<T>(p, needed, what));
 }
 
-void require_layer(const BlockIndex& w, int act, int64_t N)
+void require_layer(int act, int64_t N)
 {
     require(act >= XSPMM_ACT_NONE && act <= XSPMM_ACT_GELU_TANH, "unknown activation code");
     require(N >= 0, "xSpMM: negative N.");
-    // products of element counts stay below 2^62
+    // a weight has less than 2^30 rows: two fp32 arrays of a pass stay below 2^63 bytes
     require(N <= (int64_t(1) << 30), "xSpMM: at most 2^30 tokens.");
-    (void)w;
 }
 
 // 256-byte aligned bytes of one M x N array of a backward pass
@@ -552,7 +551,7 @@ int xspmm_linear(xspmm_weight_t weight, int vtype, int act, const void* vals, co
     return guarded([&] {
         require(weight != nullptr, "xspmm_linear: null weight.");
         const BlockIndex& w = weight->index;
-        require_layer(w, act, N);
+        require_layer(act, N);
         with_layer_type(vtype, [&](auto tv) {
             using T = typename decltype(tv)::type;
             const bool any = w.M > 0 && N > 0;
@@ -579,7 +578,7 @@ int xspmm_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act, cons
         require(gate != nullptr && up != nullptr, "xspmm_gated: null weight.");
         const BlockIndex &g = gate->index, &u = up->index;
         require(g.M == u.M && g.K == u.K, "xspmm_gated: gate and up differ in shape.");
-        require_layer(g, act, N);
+        require_layer(act, N);
         with_layer_type(vtype, [&](auto tv) {
             using T = typename decltype(tv)::type;
             const bool any = g.M > 0 && N > 0;
@@ -605,7 +604,7 @@ int xspmm_linear_backward_scratch(xspmm_weight_t weight, int vtype, int act, int
 {
     return guarded([&] {
         require(weight != nullptr && bytes != nullptr, "xspmm_linear_backward_scratch: null argument.");
-        require_layer(weight->index, act, N);
+        require_layer(act, N);
         with_layer_type(vtype, [](auto) {});
         *bytes = act == XSPMM_ACT_NONE ? 0 : layer_array(vtype, weight->index.M, N);
     });
@@ -618,7 +617,7 @@ int xspmm_linear_backward(xspmm_weight_t weight, int vtype, int act, const void*
     return guarded([&] {
         require(weight != nullptr, "xspmm_linear_backward: null weight.");
         const BlockIndex& w = weight->index;
-        require_layer(w, act, N);
+        require_layer(act, N);
         with_layer_type(vtype, [&](auto tv) {
             using T = typename decltype(tv)::type;
             const bool any = w.M > 0 && N > 0, act_too = act != XSPMM_ACT_NONE;
@@ -660,7 +659,7 @@ int xspmm_gated_backward_scratch(xspmm_weight_t gate, int vtype, int64_t N, int6
 {
     return guarded([&] {
         require(gate != nullptr && bytes != nullptr, "xspmm_gated_backward_scratch: null argument.");
-        require_layer(gate->index, XSPMM_ACT_NONE, N);
+        require_layer(XSPMM_ACT_NONE, N);
         with_layer_type(vtype, [](auto) {});
         *bytes = 2 * layer_array(vtype, gate->index.M, N);
     });
@@ -675,7 +674,7 @@ int xspmm_gated_backward(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int 
         require(gate != nullptr && up != nullptr, "xspmm_gated_backward: null weight.");
         const BlockIndex &wg = gate->index, &wu = up->index;
         require(wg.M == wu.M && wg.K == wu.K, "xspmm_gated_backward: gate and up differ in shape.");
-        require_layer(wg, act, N);
+        require_layer(act, N);
         with_layer_type(vtype, [&](auto tv) {
             using T = typename decltype(tv)::type;
             const bool any = wg.M > 0 && N > 0;

@@ -4,7 +4,11 @@ Activations are features x tokens, contiguous, as the B and C of ``spmm``; a
 weight is a ``BCSRMatrix`` of 16x16 blocks (``csr_to_bcsr``) whose block
 positions a ``SparseWeight`` lays out once.  Every array of a call has the
 weight's value type: float16, float32, or bfloat16, which the operators here
-take besides the framework's two.  Sums are fp32, rounded once.
+take besides the framework's two.  Sums are fp32, rounded once.  The products of
+the backward pass take the sums' gradient (dy act', gated dy up act' and dy act)
+rounded to the value type, as their matrix instructions have 16-bit operands: in 16
+bits that adds as much error again as the results' own rounding, and fp16's range
+holds for it (past 65504 it is infinite, below 6e-8 zero).
 
   sparse_linear            y = act(A x + bias) + residual
   sparse_gated             h = act(G x + bias_gate) * (U x + bias_up)
@@ -251,7 +255,8 @@ def sparse_linear_backward(W, x, kept, dy, activation=None, bias=False, need=(Tr
     and `kept` = W x + bias (not read, and may be None, without an activation).
     bias: whether the layer has one (dbias is None otherwise); need: whether dx
     and dvalues are wanted (None otherwise); values as in the forward pass.  The
-    residual's gradient is dy."""
+    residual's gradient is dy.  dx and dvalues are products of dy act'(kept) rounded
+    to the value type, dbias is its sum before that."""
     act = _activation(activation)
     (M, K), N, dt, dev = W.shape, _tokens(dy, "dy"), W.dtype, W.device
     _, vals = W._values(values)
@@ -312,7 +317,9 @@ def sparse_gated_backward(G, U, x, kept_gate, kept_up, dh, activation="silu", bi
     """(dx, dvalues of G, dvalues of U, dbias_gate, dbias_up) from dh = the
     gradient of ``sparse_gated``'s result and the two sums it kept.  bias:
     whether the biases' gradients are wanted; need: whether the first three are
-    (None otherwise); values as in the forward pass."""
+    (None otherwise); values as in the forward pass.  As in
+    ``sparse_linear_backward``, the products take dh up act'(gate) and dh act(gate)
+    rounded to the value type, the biases' gradients do not."""
     act = _activation(activation)
     (M, K), N, dt, dev = _pair(G, U), _tokens(dh, "dh"), G.dtype, G.device
     (_, gv), (_, uv) = G._values(values[0]), U._values(values[1])
@@ -528,8 +535,8 @@ class FeedForward(torch.nn.Module):
     on three BCSR matrices (G and U hidden x features, D features x hidden), with
     their block values and the norm's weight and bias as parameters.  The matrices
     are read, not kept up to date; weights may share one.  Which blocks are stored
-    does not change.  x is features x tokens.  There are no second derivatives:
-    asking for one raises."""
+    does not change, and is not in the state dict.  x is features x tokens.  There
+    are no second derivatives: asking for one raises."""
 
     def __init__(self, gate, up, down, activation="silu", eps=1e-5):
         super().__init__()
