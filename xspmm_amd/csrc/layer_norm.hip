@@ -677,6 +677,10 @@ NormShape backward_shape(int64_t K, int64_t N, int64_t size)
     const int v = (int)(16 / size), np = pow2_at_least(N / (16 * v), 64);
     return norm_shape(K, N, v, np < 16 ? 16 : np, kBackwardWaves, 256);
 }
+// One launch where a workgroup holds its columns, and up to 16 tokens.  us of a
+// captured call in one launch and in slices, fp16: 4096 features of 1 token 6.6 and 38,
+// of 4 10.9 and 17; but of 8 19 and 13, 16384 features of 4 36 and 17, of 16 71 and 12
+// (rows beyond kHeld are read three times, one load at a time).
 bool small_norm(int64_t K, int64_t N) { return K * N <= 65536 || N <= 16; }
 
 static_assert(kForwardWaves == kBackwardWaves);

@@ -70,7 +70,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-_current = torch.cuda.current_device
+# without the check of an initialized GPU, which what has an operand there needs none of
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _grad_enabled = torch.is_grad_enabled
 _Tensor = torch.Tensor
 _PLAIN = (_Tensor, torch.nn.Parameter)
