@@ -24,9 +24,10 @@
 // all 160.  Hence two workgroups of eight waves on a CU, four waves a SIMD, that take
 // turns (25 % stored: 175 us; with four waves of four block-rows x 64 tokens each
 // 218), and sixteen block-rows where there are enough of them, so that a row of x is
-// read from LDS for four block-rows and not for two (158 us).  Measured: y 157 to 165
-// us at 25 % stored and 250 at 100 % (960 TFLOP/s), both of a gated product's 300 and
-// 475 (1010), dx, by eight, 162 and 269.
+// read from LDS for four block-rows and not for two (158 us).  Measured: y 155 to 165
+// us at 25 % stored and 240 to 254 at 100 % (960 TFLOP/s), both of a gated product's
+// 283 to 300 and 461 to 482 (1010), dx, by eight, 154 to 162 and 253 to 269.  silu and
+// the gelus add 10 to 14, after a workgroup's last step; bias and relu nothing.
 #include "feed_forward_device.hpp"
 
 namespace xspmm {
