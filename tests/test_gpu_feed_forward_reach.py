@@ -8,7 +8,10 @@ they share with the operators' other tests).
 from __future__ import annotations
 
 import pytest
+import torch
 
+import xspmm_amd as X
+from test_gpu_feed_forward import TYPES, normal, weight
 from test_gpu_feed_forward import test_product_tiles as product_forms
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +59,18 @@ def test_hundred_and_twenty_eight_tokens_a_wave(kind, M, K, N, density):
 def test_tiles_of_sixteen_and_eight(kind, M, K, N, density):
     """Sixteen slots and eight, gated and not, rows on 16-byte boundaries and off them."""
     product_forms(kind, M, K, N, density)
+
+
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("N", [1, 200, 2056, 2051])
+def test_gradients_repeat(kind, N):
+    """Bit for bit, with other work in between: sums have one order, and no pass keeps anything for the next."""
+    dtype, M, K = TYPES[kind][0], 2100, 1040
+    G, U = weight(M, K, 0.3, dtype, 1)[0], weight(M, K, 0.6, dtype, 2)[0]
+    x, zg, zu, dh = (normal(s, dtype, i) for i, s in enumerate([(K, N), (M, N), (M, N), (M, N)]))
+    first = X.sparse_gated_backward(G, U, x, zg, zu, dh, bias=True)
+    for i in range(3):
+        X.sparse_gated_backward(U, G, x * 2, zu, zg, dh, bias=True)
+        torch.full((1 << 22,), float("nan"), device=x.device)  # what scratch may hold
+        again = X.sparse_gated_backward(G, U, x, zg, zu, dh, bias=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))

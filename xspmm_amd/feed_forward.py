@@ -370,7 +370,8 @@ def _norm_operands(x, weight):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, keep=False, out=None):
     """Layer norm over the features (rows) of every token (column) of x; with
     keep also the tokens' mean and 1 / sqrt(variance + eps) in fp32, which
-    ``layer_norm_backward`` takes.  out: memory for the result, apart from x."""
+    ``layer_norm_backward`` takes.  out: memory for the result, apart from
+    every operand."""
     K, N, dt, dev, xp, wp = _norm_operands(x, weight)
     bp = None if bias is None else _check(bias, "bias", (K,), dt, dev, 0)
     if (x.requires_grad or (weight is not None and weight.requires_grad)
