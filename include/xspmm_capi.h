@@ -487,6 +487,49 @@ int xspmm_layer_norm_backward(int vtype, int64_t K, int64_t N, const void* dy, c
                               const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
                               void* scratch, int64_t scratch_bytes, void* stream);
 
+/*
+ * The layer's products in 8-bit integers, for serving.  A weight's rows and the
+ * tokens (columns of x) are rounded to whole numbers q = round(127 v / m), half to
+ * even, and a scale m / 127 in fp32 each, m the largest magnitude of the row's
+ * stored values or of the token's features.  Sums are exact 32-bit integers, so a
+ * weight has at most 133136 columns (more fail with XSPMM_ERR_INVALID).  A row or
+ * token that holds an infinity or a NaN has the scale NaN and gives NaN.
+ *
+ * A weight's whole numbers stand as its block values do (256 of a block);
+ * tokens' are ceil(K / 16) x N x 16 bytes, 16 consecutive features of a token side by
+ * side, zeros past the last.  Both start on a 16-byte boundary, scales anywhere.
+ * vtype is the type of the block values, x, the biases, the residual and y.
+ */
+
+/* q (256 of every block, zeros past the matrix) and scale (M) of a weight's block values. */
+int xspmm_int8_weight(xspmm_weight_t weight, int vtype, const void* vals, int8_t* q, float* scale, void* stream);
+
+/*
+ * q (ceil(K / 16) x N x 16) and scale (N) of x (K x N).  scratch (256-byte aligned)
+ * has as many bytes as xspmm_quantize_tokens_scratch says.
+ */
+int xspmm_quantize_tokens_scratch(int64_t K, int64_t N, int64_t* bytes);
+int xspmm_quantize_tokens(int vtype, int64_t K, int64_t N, const void* x, int8_t* q, float* scale, void* scratch,
+                          int64_t scratch_bytes, void* stream);
+
+/*
+ * y = act(A x + bias) + residual in 8 bits.  Either x is NULL, and xq and x_scale
+ * are the tokens as xspmm_quantize_tokens makes them, or x (K x N) is quantized
+ * within the call and xq and x_scale are not read: scratch (256-byte aligned) then
+ * has as many bytes as xspmm_int8_scratch says.  bias and residual may be NULL; y may
+ * be the residual.
+ */
+int xspmm_int8_scratch(int64_t K, int64_t N, int64_t* bytes);
+int xspmm_int8_linear(xspmm_weight_t weight, int vtype, int act, const int8_t* q, const float* scale, const void* x,
+                      const int8_t* xq, const float* x_scale, const void* bias, const void* residual, void* y, int64_t N,
+                      void* scratch, int64_t scratch_bytes, void* stream);
+
+/* h = act(G x + gate_bias) * (U x + up_bias) in 8 bits, likewise. */
+int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act, const int8_t* gate_q,
+                     const float* gate_scale, const int8_t* up_q, const float* up_scale, const void* x,
+                     const int8_t* xq, const float* x_scale, const void* gate_bias, const void* up_bias, void* h,
+                     int64_t N, void* scratch, int64_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

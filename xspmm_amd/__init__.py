@@ -633,16 +633,21 @@ class SpMMPlan:
 
 
 
-# The feed-forward layer's operators need torch, which the module loads on the
+# The feed-forward layer's operators need torch, which their modules load on the
 # first use of one.
-_FEED_FORWARD = ("SparseWeight", "sparse_linear", "sparse_linear_backward", "sparse_gated", "sparse_gated_backward",
-                 "layer_norm", "layer_norm_backward", "FeedForward", "prune_blocks")
+_LAYER = {
+    "feed_forward": ("SparseWeight", "sparse_linear", "sparse_linear_backward", "sparse_gated", "sparse_gated_backward",
+                     "layer_norm", "layer_norm_backward", "FeedForward", "prune_blocks"),
+    "int8": ("Int8Weight", "Int8Tokens", "quantize_tokens", "int8_linear", "int8_gated", "Int8FeedForward"),
+}
 
 
 def __getattr__(name):
-    if name in _FEED_FORWARD:
-        from . import feed_forward
-        for n in _FEED_FORWARD:
-            globals()[n] = getattr(feed_forward, n)
-        return globals()[name]
+    for module, names in _LAYER.items():
+        if name in names:
+            import importlib
+            m = importlib.import_module("." + module, __name__)
+            for n in names:
+                globals()[n] = getattr(m, n)
+            return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -10,6 +10,7 @@
 #include <utility>
 
 #include "feed_forward.hpp"
+#include "int8.hpp"
 #include "internal.hpp"
 #include "xspmm_capi.h"
 
@@ -131,6 +132,48 @@ void require_scratch(const void* p, int64_t have, int64_t need)
 {
     require(have >= need && (need == 0 || p != nullptr), "xSpMM: the scratch is smaller than its query says.");
     require(reinterpret_cast<uintptr_t>(p) % 256 == 0 || need == 0, "xSpMM: scratch must start on a 256-byte boundary.");
+}
+
+// Sizes of tokens in 8 bits, and the bytes that quantizing them within a product
+// takes: whole numbers, scales, and the maxima of slices.
+void require_tokens(int64_t K, int64_t N)
+{
+    require(K >= 0 && N >= 0 && K <= (int64_t(1) << 30) - 64 && N <= (int64_t(1) << 30), "xSpMM: bad size of tokens.");
+}
+struct TokenMemory {
+    size_t q, scale, part, end;
+};
+TokenMemory token_memory(int64_t K, int64_t N)
+{
+    Carve c;
+    TokenMemory m{};
+    m.q = c.take((size_t)((K + 15) / 16 * 16) * (size_t)N);
+    m.scale = c.take((size_t)N * 4);
+    m.part = c.take((size_t)quantize_tokens_scratch(K, N));
+    m.end = c.end;
+    return m;
+}
+
+// The tokens of a product: as they come, or quantized into its scratch.
+template <typename T>
+void int8_tokens(Int8Args<T>& a, const BlockIndex& w, bool any, const void* x, const int8_t* xq, const float* x_scale,
+                 void* scratch, int64_t scratch_bytes, hipStream_t s)
+{
+    require(w.K <= kInt8MostFeatures, "xSpMM: a weight in 8 bits has at most 133136 columns.");
+    if (!any) return;
+    if (x == nullptr) {
+        a.x = operand<int8_t>(xq, w.K > 0, "xq");
+        a.x_scale = x_scale;
+        require(x_scale != nullptr, "xSpMM: x_scale is null.");
+        return;
+    }
+    const TokenMemory m = token_memory(w.K, a.N);
+    require_scratch(scratch, scratch_bytes, (int64_t)m.end);
+    char* p = static_cast<char*>(scratch);
+    quantize_tokens<T>(operand<T>(x, false, "x"), reinterpret_cast<int8_t*>(p + m.q),
+                       reinterpret_cast<float*>(p + m.scale), w.K, a.N, p + m.part, s);
+    a.x = reinterpret_cast<int8_t*>(p + m.q);
+    a.x_scale = reinterpret_cast<float*>(p + m.scale);
 }
 
 }  // namespace
@@ -770,6 +813,114 @@ int xspmm_layer_norm_backward(int vtype, int64_t K, int64_t N, const void* dy, c
             layer_norm_backward<T>(operand<T>(dy, any, "dy"), operand<T>(x, any, "x"), static_cast<const T*>(weight),
                                    mean, rstd, result<T>(dx, false, "dx"), static_cast<T*>(dweight),
                                    static_cast<T*>(dbias), K, N, scratch, as_stream(stream));
+        });
+    });
+}
+
+int xspmm_int8_weight(xspmm_weight_t weight, int vtype, const void* vals, int8_t* q, float* scale, void* stream)
+{
+    return guarded([&] {
+        require(weight != nullptr, "xspmm_int8_weight: null weight.");
+        const BlockIndex& w = weight->index;
+        require(w.K <= kInt8MostFeatures, "xSpMM: a weight in 8 bits has at most 133136 columns.");
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            require(w.M == 0 || scale != nullptr, "xspmm_int8_weight: scale is null.");
+            int8_weight<T>(w, operand<T>(vals, w.nnzb > 0, "vals"), result<int8_t>(q, w.nnzb > 0, "q"), scale,
+                           as_stream(stream));
+        });
+    });
+}
+
+int xspmm_quantize_tokens_scratch(int64_t K, int64_t N, int64_t* bytes)
+{
+    return guarded([&] {
+        require(bytes != nullptr, "xspmm_quantize_tokens_scratch: bytes is null.");
+        require_tokens(K, N);
+        *bytes = quantize_tokens_scratch(K, N);
+    });
+}
+
+int xspmm_quantize_tokens(int vtype, int64_t K, int64_t N, const void* x, int8_t* q, float* scale, void* scratch,
+                          int64_t scratch_bytes, void* stream)
+{
+    return guarded([&] {
+        require_tokens(K, N);
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = K > 0 && N > 0;
+            require(N == 0 || scale != nullptr, "xspmm_quantize_tokens: scale is null.");
+            require_scratch(scratch, scratch_bytes, quantize_tokens_scratch(K, N));
+            quantize_tokens<T>(operand<T>(x, any, "x"), result<int8_t>(q, any, "q"), scale, K, N, scratch,
+                               as_stream(stream));
+        });
+    });
+}
+
+int xspmm_int8_scratch(int64_t K, int64_t N, int64_t* bytes)
+{
+    return guarded([&] {
+        require(bytes != nullptr, "xspmm_int8_scratch: bytes is null.");
+        require_tokens(K, N);
+        *bytes = (int64_t)token_memory(K, N).end;
+    });
+}
+
+int xspmm_int8_linear(xspmm_weight_t weight, int vtype, int act, const int8_t* q, const float* scale, const void* x,
+                      const int8_t* xq, const float* x_scale, const void* bias, const void* residual, void* y, int64_t N,
+                      void* scratch, int64_t scratch_bytes, void* stream)
+{
+    return guarded([&] {
+        require(weight != nullptr, "xspmm_int8_linear: null weight.");
+        const BlockIndex& w = weight->index;
+        require_layer(act, N);
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = w.M > 0 && N > 0;
+            require(!any || scale != nullptr, "xspmm_int8_linear: scale is null.");
+            Int8Args<T> a{};
+            a.weight[0] = &w;
+            a.vals[0] = operand<int8_t>(q, any && w.nnzb > 0, "q");
+            a.scale[0] = scale;
+            a.bias[0] = static_cast<const T*>(bias);
+            a.residual = operand<T>(residual, false, "residual");
+            a.y = result<T>(y, any, "y");
+            a.N = N;
+            a.act = act;
+            int8_tokens<T>(a, w, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
+            if (any) int8_product<T>(a, 1, as_stream(stream));
+        });
+    });
+}
+
+int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act, const int8_t* gate_q,
+                     const float* gate_scale, const int8_t* up_q, const float* up_scale, const void* x,
+                     const int8_t* xq, const float* x_scale, const void* gate_bias, const void* up_bias, void* h,
+                     int64_t N, void* scratch, int64_t scratch_bytes, void* stream)
+{
+    return guarded([&] {
+        require(gate != nullptr && up != nullptr, "xspmm_int8_gated: null weight.");
+        const BlockIndex &g = gate->index, &u = up->index;
+        require(g.M == u.M && g.K == u.K, "xspmm_int8_gated: gate and up differ in shape.");
+        require_layer(act, N);
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = g.M > 0 && N > 0;
+            require(!any || (gate_scale != nullptr && up_scale != nullptr), "xspmm_int8_gated: a scale is null.");
+            Int8Args<T> a{};
+            a.weight[0] = &g;
+            a.weight[1] = &u;
+            a.vals[0] = operand<int8_t>(gate_q, any && g.nnzb > 0, "gate_q");
+            a.vals[1] = operand<int8_t>(up_q, any && u.nnzb > 0, "up_q");
+            a.scale[0] = gate_scale;
+            a.scale[1] = up_scale;
+            a.bias[0] = static_cast<const T*>(gate_bias);
+            a.bias[1] = static_cast<const T*>(up_bias);
+            a.y = result<T>(h, any, "h");
+            a.N = N;
+            a.act = act;
+            int8_tokens<T>(a, g, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
+            if (any) int8_product<T>(a, 2, as_stream(stream));
         });
     });
 }
