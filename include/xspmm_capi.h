@@ -530,6 +530,22 @@ int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act,
                      const int8_t* xq, const float* x_scale, const void* gate_bias, const void* up_bias, void* h,
                      int64_t N, void* scratch, int64_t scratch_bytes, void* stream);
 
+/*
+ * An update of a weight's stored blocks (zeros elsewhere), orthogonalised:
+ * X = U / (|U| + eps), |U| the root of the sum of squares, then `steps` times
+ * X <- a X + (b S + c S S) X with S = X X^T (of U^T where U has fewer columns than
+ * rows); out receives X at the stored blocks, zero past the edges of the weight.
+ * 16-bit updates take products of fp16 operands: |b S + c S S| must stay below 16 (with
+ * the usual 3.4445, -4.775, 2.0315 it is below 3).  An update that holds an infinity or
+ * a NaN gives NaN.  steps >= 1, eps >= 0, finite coefficients, weights of at most 2^20
+ * rows and columns.  out may be the update.  scratch (256-byte aligned) has as many
+ * bytes as xspmm_orthogonalize_scratch says: several dense matrices of the weight's
+ * size.  Asynchronous on `stream`; nothing is allocated.
+ */
+int xspmm_orthogonalize_scratch(xspmm_weight_t weight, int vtype, int64_t* bytes);
+int xspmm_orthogonalize(xspmm_weight_t weight, int vtype, const void* update, void* out, int steps, float a, float b,
+                        float c, float eps, void* scratch, int64_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

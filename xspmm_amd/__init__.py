@@ -639,6 +639,7 @@ _LAYER = {
     "feed_forward": ("SparseWeight", "sparse_linear", "sparse_linear_backward", "sparse_gated", "sparse_gated_backward",
                      "layer_norm", "layer_norm_backward", "FeedForward", "prune_blocks"),
     "int8": ("Int8Weight", "Int8Tokens", "quantize_tokens", "int8_linear", "int8_gated", "Int8FeedForward"),
+    "orthogonal": ("orthogonalize", "OrthogonalMomentum"),
 }
 
 

@@ -4,6 +4,7 @@
 // XSPMM_ERR_HIP, any other failure -> XSPMM_ERR_UNSUPPORTED).
 #include <hip/hip_fp16.h>
 
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <string>
@@ -11,6 +12,7 @@
 
 #include "feed_forward.hpp"
 #include "int8.hpp"
+#include "orthogonal.hpp"
 #include "internal.hpp"
 #include "xspmm_capi.h"
 
@@ -921,6 +923,38 @@ int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act,
             a.act = act;
             int8_tokens<T>(a, g, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
             if (any) int8_product<T>(a, 2, as_stream(stream));
+        });
+    });
+}
+
+int xspmm_orthogonalize_scratch(xspmm_weight_t weight, int vtype, int64_t* bytes)
+{
+    return guarded([&] {
+        require(weight != nullptr && bytes != nullptr, "xspmm_orthogonalize_scratch: null argument.");
+        const BlockIndex& w = weight->index;
+        require(w.M <= kOrthogonalMostSide && w.K <= kOrthogonalMostSide,
+                "xSpMM: an orthogonalised update has at most 2^20 rows and columns.");
+        with_layer_type(vtype, [&](auto tv) { *bytes = orthogonal_scratch(w, sizeof(typename decltype(tv)::type)); });
+    });
+}
+
+int xspmm_orthogonalize(xspmm_weight_t weight, int vtype, const void* update, void* out, int steps, float a, float b,
+                        float c, float eps, void* scratch, int64_t scratch_bytes, void* stream)
+{
+    return guarded([&] {
+        require(weight != nullptr, "xspmm_orthogonalize: null weight.");
+        const BlockIndex& w = weight->index;
+        require(w.M <= kOrthogonalMostSide && w.K <= kOrthogonalMostSide,
+                "xSpMM: an orthogonalised update has at most 2^20 rows and columns.");
+        require(steps >= 1, "xSpMM: an update is orthogonalised in one step at least.");
+        require(eps >= 0.f && std::isfinite(eps), "xSpMM: eps is finite and not negative.");
+        require(std::isfinite(a) && std::isfinite(b) && std::isfinite(c), "xSpMM: coefficients must be finite.");
+        with_layer_type(vtype, [&](auto tv) {
+            using T = typename decltype(tv)::type;
+            const bool any = w.nnzb > 0;
+            require_scratch(scratch, scratch_bytes, orthogonal_scratch(w, sizeof(T)));
+            orthogonalize<T>(w, operand<T>(update, any, "update"), result<T>(out, any, "out"), {a, b, c, eps, steps},
+                             scratch, as_stream(stream));
         });
     });
 }
