@@ -169,6 +169,10 @@ void int8_tokens(Int8Args<T>& a, const BlockIndex& w, bool any, const void* x, c
         require(x_scale != nullptr, "xSpMM: x_scale is null.");
         return;
     }
+    if (int8_rounds_itself(w.K, a.N)) {
+        a.raw = operand<T>(x, false, "x");
+        return;
+    }
     const TokenMemory m = token_memory(w.K, a.N);
     require_scratch(scratch, scratch_bytes, (int64_t)m.end);
     char* p = static_cast<char*>(scratch);
@@ -864,7 +868,7 @@ int xspmm_int8_scratch(int64_t K, int64_t N, int64_t* bytes)
     return guarded([&] {
         require(bytes != nullptr, "xspmm_int8_scratch: bytes is null.");
         require_tokens(K, N);
-        *bytes = (int64_t)token_memory(K, N).end;
+        *bytes = int8_rounds_itself(K, N) ? 0 : (int64_t)token_memory(K, N).end;
     });
 }
 

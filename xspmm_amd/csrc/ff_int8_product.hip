@@ -8,50 +8,11 @@
 // columns are: four stored blocks of a block-row make one instruction, and absent
 // ones of the last four are zeros in A.  Sums are whole numbers and exact in any
 // order; a result is float(sum) * row's scale * token's scale, then as in fp32.
-#include "feed_forward_device.hpp"
-#include "int8.hpp"
+#include "int8_device.hpp"
 
 namespace xspmm {
 namespace detail {
 namespace ff {
-
-typedef int int4_t __attribute__((ext_vector_type(4)));
-
-struct Int8Side {
-    const int32_t* ptr;
-    const int32_t* col;
-    const int8_t* vals;
-    const float* scale;
-    const void* bias;
-};
-
-template <typename T>
-struct Int8Product {
-    Int8Side side[2];
-    const int8_t* x;
-    const float* x_scale;
-    const T* residual;
-    T* y;
-    int32_t rows, block_rows;
-    int64_t N;
-    int act;
-};
-
-template <typename T, int NACC>
-__device__ __forceinline__ float int8_finish(const Int8Product<T>& a, const int (&sum)[NACC], int64_t row, int64_t n,
-                                             float x_scale)
-{
-    float z[NACC];
-#pragma unroll
-    for (int l = 0; l < NACC; ++l) {
-        z[l] = (float)sum[l] * a.side[l].scale[row] * x_scale;
-        if (a.side[l].bias) z[l] += (float)static_cast<const T*>(a.side[l].bias)[row];
-    }
-    with_act(a.act, [&](auto act) { z[0] = act_value<decltype(act)::value>(z[0]); });
-    if constexpr (NACC == 2) z[0] *= z[1];
-    if (a.residual) z[0] += (float)a.residual[row * a.N + n];
-    return z[0];
-}
 
 // A wave's share of a block-row times VT tiles of 16 tokens.  Tokens past the last
 // read the last one's features, and so do absent blocks (of zeros) the first's.
@@ -102,9 +63,7 @@ __global__ __launch_bounds__(64 * (SPLIT > 4 ? SPLIT : 4)) void ff_int8_walk_ker
                 load(st, q);
 #pragma unroll
                 for (int j = 0; j < VT; ++j)
-                    acc[l][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4_t, st.a),
-                                                                      __builtin_bit_cast(int4_t, st.x[j]), acc[l][j],
-                                                                      0, 0, 0);
+                    acc[l][j] = mfma8(st.a, st.x[j], acc[l][j]);
             }
         }
     }
@@ -150,6 +109,161 @@ __global__ __launch_bounds__(64 * (SPLIT > 4 ? SPLIT : 4)) void ff_int8_walk_ker
     }
 }
 
+// Few tokens and few features: a workgroup rounds its (up to 16) tokens itself, into LDS,
+// with its first blocks on their way meanwhile, and then walks ROWS block-rows, 16 /
+// ROWS waves to each.
+constexpr int kFewTokens = 16, kFewThreads = 1024;
+constexpr int kFewBlocks = 2048;  // blocks of 16 features of a token, in all
+
+// KEPT: such blocks of a thread
+template <typename T, int NACC, int ROWS, int KEPT, bool ONE>
+__global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_kernel(const Int8Product<T> a)
+{
+    constexpr int SPLIT = 16 / ROWS, kAhead = KEPT == 1 && NACC == 2 ? 2 : 4;
+    __shared__ __align__(16) u32x4_t xs[KEPT * kFewThreads];
+    __shared__ int red[ROWS][SPLIT][NACC][4][64];
+    __shared__ uint32_t most[16];
+    __shared__ float scales[kFewTokens];
+    const int t = threadIdx.x, lane = t & 63, li = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int64_t tile = blockIdx.x % ((a.N + kFewTokens - 1) / kFewTokens);
+    const int32_t br = (int32_t)(blockIdx.x / ((a.N + kFewTokens - 1) / kFewTokens)) * ROWS + wave / SPLIT;
+    const int part = wave % SPLIT;
+    const int64_t n0 = tile * kFewTokens;
+    const int nt = ONE ? 1 : (int)min((int64_t)kFewTokens, a.N - n0);
+    const int blocks = a.in_blocks * nt;
+
+    float v[KEPT][16][1];
+#pragma unroll
+    for (int u = 0; u < KEPT; ++u) {
+        const int e = t + kFewThreads * u;
+        if (e < blocks) {
+            if constexpr (ONE) {
+                const int32_t k = 16 * e;
+                if (k + 16 <= a.in_rows) {
+                    const Pack<T, 16> p = *reinterpret_cast<const Pack<T, 16>*>(a.raw + k);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[u][i][0] = (float)p.v[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[u][i][0] = k + i < a.in_rows ? (float)a.raw[k + i] : 0.f;
+                }
+            } else {
+                load_features<T, 1>(a.raw, a.in_rows, a.N, e / nt, n0 + e % nt, v[u]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[u][i][0] = 0.f;
+        }
+    }
+
+    // this wave's share of its block-row, of either weight
+    int32_t lo[NACC], hi[NACC];
+    u32x4_t first[NACC][kAhead];
+    int32_t column[NACC][kAhead];
+    auto load = [&](int l, int32_t q, u32x4_t& w, int32_t& c) {
+        const int32_t mine = q + g < hi[l] ? q + g : lo[l];
+        w = *reinterpret_cast<const u32x4_t*>(a.side[l].vals + (int64_t)mine * 256 + li * 16);
+        if (q + g >= hi[l]) w = u32x4_t{0u, 0u, 0u, 0u};
+        c = a.side[l].col[mine];
+    };
+#pragma unroll
+    for (int l = 0; l < NACC; ++l) {
+        lo[l] = hi[l] = 0;
+        if (br < a.block_rows) {
+            const int32_t b = a.side[l].ptr[br], e = a.side[l].ptr[br + 1], steps = (e - b + 3) / 4;
+            lo[l] = b + 4 * (int32_t)((int64_t)steps * part / SPLIT);
+            hi[l] = min(b + 4 * (int32_t)((int64_t)steps * (part + 1) / SPLIT), e);
+        }
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p)
+            if (lo[l] + 4 * p < hi[l]) load(l, lo[l] + 4 * p, first[l][p], column[l][p]);
+    }
+
+    // the tokens' scales
+    if constexpr (ONE) {
+        uint32_t m[1] = {0u};
+#pragma unroll
+        for (int u = 0; u < KEPT; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m[0] = max(m[0], magnitude(v[u][i][0]));
+        join<kFewThreads, 1, 1>(m, most);
+        const Rounding round(m[0]);
+        if (t == 0) scales[0] = round.scale;
+#pragma unroll
+        for (int u = 0; u < KEPT; ++u)
+            if (t + kFewThreads * u < blocks) {
+                float w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = v[u][i][0];
+                xs[t + kFewThreads * u] = round_features(w, round);
+            }
+    } else {
+        if (t < kFewTokens) most[t] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < KEPT; ++u)
+            if (t + kFewThreads * u < blocks) {
+                uint32_t m = 0u;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[u][i][0]));
+                atomicMax(&most[(t + kFewThreads * u) % nt], m);
+            }
+        __syncthreads();
+        if (t < nt) scales[t] = Rounding(most[t]).scale;
+#pragma unroll
+        for (int u = 0; u < KEPT; ++u)
+            if (t + kFewThreads * u < blocks) {
+                float w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = v[u][i][0];
+                xs[t + kFewThreads * u] = round_features(w, Rounding(most[(t + kFewThreads * u) % nt]));
+            }
+    }
+    __syncthreads();
+
+    int4_t acc[NACC];
+    const int n = min(li, nt - 1);
+#pragma unroll
+    for (int l = 0; l < NACC; ++l) {
+        acc[l] = int4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p)
+            if (lo[l] + 4 * p < hi[l]) acc[l] = mfma8(first[l][p], xs[column[l][p] * nt + n], acc[l]);
+        for (int32_t q = lo[l] + 4 * kAhead; q < hi[l]; q += 4) {
+            u32x4_t w;
+            int32_t c;
+            load(l, q, w, c);
+            acc[l] = mfma8(w, xs[c * nt + n], acc[l]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) red[wave / SPLIT][part][l][q][lane] = acc[l][q];
+    }
+    __syncthreads();
+    const int64_t row = 16 * (int64_t)br + 4 * g + part;
+    if (part >= 4 || row >= a.rows || li >= nt) return;
+    int sum[NACC];
+#pragma unroll
+    for (int l = 0; l < NACC; ++l) {
+        sum[l] = 0;
+#pragma unroll
+        for (int p = 0; p < SPLIT; ++p) sum[l] += red[wave / SPLIT][p][l][part][lane];
+    }
+    a.y[row * a.N + n0 + li] = (T)int8_finish<T, NACC>(a, sum, row, n0 + li, scales[li]);
+}
+
+template <typename T, int NACC, int ROWS, int KEPT>
+void launch_few(const Int8Product<T>& a, hipStream_t s)
+{
+    const int64_t items = (int64_t)((a.block_rows + ROWS - 1) / ROWS) * ((a.N + kFewTokens - 1) / kFewTokens);
+    const dim3 grid = launch_grid(items, kFewThreads), threads(kFewThreads);
+    if (a.N == 1)
+        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, KEPT, true>), grid, threads, 0, s, a);
+    else
+        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, KEPT, false>), grid, threads, 0, s, a);
+    XSPMM_LAUNCH_CHECK();
+}
+
 template <typename T, int VT, int NACC, int SPLIT>
 void launch_walk(const Int8Product<T>& a, hipStream_t s)
 {
@@ -163,6 +277,23 @@ void launch_walk(const Int8Product<T>& a, hipStream_t s)
 template <typename T, int NACC>
 void launch_int8(const Int8Product<T>& a, int64_t blocks, hipStream_t s)
 {
+    if (a.raw) {
+        // Sixteen waves to a block-row while there are no more than two workgroups a CU
+        // (16 waves each), half and a quarter of them beyond (us of one and two rows a
+        // workgroup: fp16 4096 x 14336, 25 % stored, one token 6.7 and 7.8; bf16 gate and
+        // up of 14336 x 4096 13.0 and 10.1, of four rows 10.3).
+        const int64_t nt = a.N < kFewTokens ? a.N : kFewTokens;
+        const int64_t groups = a.block_rows * ((a.N + kFewTokens - 1) / kFewTokens);
+        if (a.in_blocks * nt > 1024)
+            launch_few<T, NACC, 1, 2>(a, s);
+        else if (groups <= 512)
+            launch_few<T, NACC, 1, 1>(a, s);
+        else if (groups <= 1024)
+            launch_few<T, NACC, 2, 1>(a, s);
+        else
+            launch_few<T, NACC, 4, 1>(a, s);
+        return;
+    }
     auto waves = [&](int v) { return (int64_t)a.block_rows * ((a.N + 16 * v - 1) / (16 * v)); };
     int vt = 4;
     while (vt > 1 && (16 * vt >= 2 * a.N || waves(vt) < 256)) vt /= 2;
@@ -181,6 +312,12 @@ void launch_int8(const Int8Product<T>& a, int64_t blocks, hipStream_t s)
 
 }  // namespace ff
 
+bool int8_rounds_itself(int64_t K, int64_t N)
+{
+    const int64_t Kb = (K + 15) / 16, nt = N < ff::kFewTokens ? N : ff::kFewTokens;
+    return N <= 64 && Kb * nt <= ff::kFewBlocks;
+}
+
 template <typename T>
 void int8_product(const Int8Args<T>& f, int weights, hipStream_t s)
 {
@@ -190,10 +327,15 @@ void int8_product(const Int8Args<T>& f, int weights, hipStream_t s)
     int64_t blocks = 0;
     for (int l = 0; l < weights; ++l) {
         const BlockIndex& wl = *f.weight[l];
-        a.side[l] = {wl.ptr, wl.col, f.vals[l], f.scale[l], f.bias[l]};
+        a.side[l] = {wl.ptr, wl.col, wl.map, f.vals[l], f.scale[l], f.bias[l]};
+        const int64_t vb = narrow_bytes(wl.nnzb, 256, 1);
+        a.vals_bytes[l] = vb < 0 ? 0u : (uint32_t)vb;
         blocks += wl.nnzb;
     }
+    a.raw = f.raw;
     a.x = f.x;
+    a.in_rows = (int32_t)w.K;
+    a.in_blocks = (int32_t)w.Kb;
     a.x_scale = f.x_scale;
     a.residual = f.residual;
     a.y = f.y;
@@ -201,6 +343,7 @@ void int8_product(const Int8Args<T>& f, int weights, hipStream_t s)
     a.block_rows = (int32_t)w.Mb;
     a.N = f.N;
     a.act = f.act;
+    if (!a.raw && int8_tiles<T>(a, weights, blocks, s)) return;
     if (weights == 2)
         ff::launch_int8<T, 2>(a, blocks, s);
     else

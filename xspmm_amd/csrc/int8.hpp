@@ -30,6 +30,7 @@ struct Int8Args {
     const int8_t* vals[2];
     const float* scale[2];  // of the rows
     const T* bias[2];
+    const T* raw;  // activations that the product rounds itself, or null
     const int8_t* x;
     const float* x_scale;
     const T* residual;
@@ -37,6 +38,8 @@ struct Int8Args {
     int64_t N;
     int act;
 };
+// Whether a product of N tokens rounds them itself, without memory for the result.
+bool int8_rounds_itself(int64_t K, int64_t N);
 template <typename T>
 void int8_product(const Int8Args<T>& a, int weights, hipStream_t s);
 
