@@ -31,17 +31,34 @@ struct Halves {
     _Float16* lo;  // null where products take the upper half alone and nothing else reads it
 };
 
-constexpr int kDeepK = 64;  // of a product's step
+// X, S and b S + c S S lie as blocks of 16 x 32 halves, 1 KB each, that follow each other
+// along the rows: one load into LDS, of an operand's rows or of a step's columns, is one
+// block, and so is one store of a result.  (From rows of whole matrices a step takes 64
+// bytes each, half a line, and gets half of L2's rate: 538 us instead of NN for a X + Y X
+// at 4096 x 14336.)
+constexpr int kBlock = 512;
+__device__ __forceinline__ int64_t block_place(int64_t r, int64_t c, int64_t ld)
+{
+    return (r / 16 * (ld / 32) + c / 32) * kBlock;
+}
 
-template <int TILE>
+constexpr int kDeepK = 32;  // of a product's step
+
+// A workgroup of four waves takes TI rows and 128 columns, a wave half of either.  Two
+// workgroups share a CU and are not in step: while one multiplies, the other reads its
+// operands, or reads and writes X at a tile's end (512 KB of a tile of 256 x 256, which
+// with one workgroup of eight waves a CU took 157 of 545 us at 4096 x 14336).
+constexpr int kTileJ = 128;
+constexpr int kProductWaves = 4, kProductThreads = 64 * kProductWaves;
+template <int TI>
 struct Shape {
-    static constexpr int kWaves = TILE == 256 ? 8 : 4;
-    static constexpr int kThreads = 64 * kWaves;
-    static constexpr int kWaveI = TILE / 2, kWaveJ = TILE / (kWaves / 2);  // a wave's rows and columns
+    static constexpr int kWaveI = TI / 2, kWaveJ = kTileJ / 2;  // a wave's rows and columns
     static constexpr int FI = kWaveI / 16, FJ = kWaveJ / 16;
-    static constexpr int kSide = TILE * kDeepK * 2;  // bytes of one operand's stage
-    static constexpr int kStage = 2 * kSide;
-    static constexpr int kLds = 2 * kStage;
+    static constexpr int kSideI = TI * kDeepK * 2, kSideJ = kTileJ * kDeepK * 2;  // bytes of an operand's step
+    static constexpr int kStage = kSideI + kSideJ;
+    static constexpr int kStages = TI == 256 ? 3 : 4;  // steps in LDS
+    static constexpr int kLds = kStages * kStage;
+    static_assert(kLds <= 80 * 1024);
 };
 
 // What becomes of a product's sums.
@@ -102,94 +119,134 @@ __device__ __forceinline__ void halves(float v, _Float16& hi, _Float16& lo)
     lo = (_Float16)(v - (float)hi);
 }
 
-// Element i, j .. + 3 of a product's sums (i0, j0: of its 16 x 16 tile).
-template <typename T, int PURPOSE>
-__device__ __forceinline__ void finish_four(const Finish<T>& f, const float4_t v, int64_t i, int64_t j, int64_t i0,
-                                            int64_t j0, bool mirror)
+// N values as halves, side by side.
+template <int N>
+__device__ __forceinline__ void store_halves(const Halves& to, int64_t at, const float (&v)[N])
 {
-    typedef Pack<_Float16, 4> P;
-    const int64_t at = i * f.ld + j;
-    if constexpr (PURPOSE == kGram || PURPOSE == kSquare) {
-        P hi, lo;
-        float w[4];
+    Pack<_Float16, N> hi, lo;
+#pragma unroll
+    for (int q = 0; q < N; ++q) halves(v[q], hi.v[q], lo.v[q]);
+    *reinterpret_cast<Pack<_Float16, N>*>(to.hi + at) = hi;
+    if (to.lo) *reinterpret_cast<Pack<_Float16, N>*>(to.lo + at) = lo;
+}
+
+// Two tiles of 16 x 16 side by side, of which a lane has row li and columns 4 g .. + 3
+// each: lanes of even g take the first one's columns 4 g .. + 7 (with the next lanes'),
+// those of odd g the second one's, 16 + 4 (g - 1) .. + 7.
+__device__ __forceinline__ void pair_up(const float4_t a, const float4_t b, float (&v)[8])
+{
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[q]), __float_as_uint(b[q]), false, false);
+        v[q] = __uint_as_float(r[0]);
+        v[4 + q] = __uint_as_float(r[1]);
+    }
+}
+// which of the four eights of 32 columns that is
+__device__ __forceinline__ int paired_chunk(int g) { return 2 * (g & 1) + (g >> 1); }
+
+// A product's sums of 32 x 32 elements at (i, j), two pairs of tiles: S, or b S + c S S, and
+// its mirror image.  turn: 2 (4 with lower halves) KB of LDS of this wave's.
+template <typename T, int PURPOSE>
+__device__ __forceinline__ void finish_symmetric(const Finish<T>& f, float (&v)[2][8], int64_t i, int64_t j, int li,
+                                                 int g, bool mirror, _Float16* turn)
+{
+    typedef Pack<_Float16, 8> P;
+    const int chunk = paired_chunk(g), lane = 16 * g + li;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int64_t at = block_place(i + 16 * u, j, f.ld) + li * 32 + 8 * chunk;
         if constexpr (PURPOSE == kGram) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) w[q] = v[q] * (1.f / kHeld);
+            for (int q = 0; q < 8; ++q) v[u][q] *= 1.f / kHeld;
         } else {
             const P sh = *reinterpret_cast<const P*>(f.s.hi + at);
             P sl{};
             if (f.s.lo) sl = *reinterpret_cast<const P*>(f.s.lo + at);
+            const int64_t row = i + 16 * u + li, column = j + 8 * chunk;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                w[q] = f.b * ((float)sh.v[q] + (float)sl.v[q]) + f.c * (v[q] * (1.f / kHeld));
-                if (i == j + q) {
-                    f.diagonal[i] = w[q] * (1.f / kHeld);
-                    w[q] = 0.f;
+            for (int q = 0; q < 8; ++q) {
+                v[u][q] = f.b * ((float)sh.v[q] + (float)sl.v[q]) + f.c * (v[u][q] * (1.f / kHeld));
+                if (row == column + q) {
+                    f.diagonal[row] = v[u][q] * (1.f / kHeld);
+                    v[u][q] = 0.f;
                 }
             }
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) halves(w[q], hi.v[q], lo.v[q]);
-        *reinterpret_cast<P*>(f.out.hi + at) = hi;
-        if (f.out.lo) *reinterpret_cast<P*>(f.out.lo + at) = lo;
-        if (mirror) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                f.out.hi[(j + q) * f.ld + i] = hi.v[q];
-                if (f.out.lo) f.out.lo[(j + q) * f.ld + i] = lo.v[q];
-            }
-        }
+        store_halves<8>(f.out, at, v[u]);
     }
-    if constexpr (PURPOSE == kApply || PURPOSE == kLast) {
-        const P xh = *reinterpret_cast<const P*>(f.x.hi + at), xl = *reinterpret_cast<const P*>(f.x.lo + at);
-        const float d = f.a + f.diagonal[i];
-        float w[4];
+    if (!mirror) return;
+    // through LDS: column by column, 64 bytes of 32 rows each
 #pragma unroll
-        for (int q = 0; q < 4; ++q) w[q] = fmaf(d, (float)xh.v[q] + (float)xl.v[q], v[q] * (1.f / kHeld));
-        if constexpr (PURPOSE == kApply) {
-            P hi, lo;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) halves(w[q], hi.v[q], lo.v[q]);
-            *reinterpret_cast<P*>(f.out.hi + at) = hi;
-            *reinterpret_cast<P*>(f.out.lo + at) = lo;
-        } else {
-            const int64_t r = f.transposed ? j : i, c = f.transposed ? i : j;
-            const int32_t b = block_at(f, (int32_t)((f.transposed ? j0 : i0) / 16), (int32_t)((f.transposed ? i0 : j0) / 16));
-            if (b < 0) return;
-            T* o = f.blocks + (int64_t)b * 256 + (r % 16) * 16 + c % 16;
-            if (f.transposed) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    o[16 * q] = r + q < f.M && c < f.K ? (T)(w[q] * (1.f / kHeld)) : (T)0.f;
-            } else {
-                Pack<T, 4> k;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) k.v[q] = r < f.M && c + q < f.K ? (T)(w[q] * (1.f / kHeld)) : (T)0.f;
-                *reinterpret_cast<Pack<T, 4>*>(o) = k;
-            }
+        for (int q = 0; q < 8; ++q) {
+            _Float16 hi, lo;
+            halves(v[u][q], hi, lo);
+            const int at = (8 * chunk + q) * 32 + 16 * u + li;
+            turn[at] = hi;
+            if (f.out.lo) turn[1024 + at] = lo;
         }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int64_t at = block_place(j + 16 * u, i, f.ld) + lane * 8;
+        *reinterpret_cast<P*>(f.out.hi + at) = *reinterpret_cast<const P*>(turn + u * 512 + lane * 8);
+        if (f.out.lo) *reinterpret_cast<P*>(f.out.lo + at) = *reinterpret_cast<const P*>(turn + 1024 + u * 512 + lane * 8);
     }
+    __builtin_amdgcn_wave_barrier();
 }
 
-// tile t of the lower triangle: row i, column j <= i
-__device__ __forceinline__ void triangle(int64_t t, int32_t& i, int32_t& j)
+// a X + Y X of 16 x 32 elements at (i, j): X, or (kLast) what of it is stored.
+template <typename T, int PURPOSE>
+__device__ __forceinline__ void finish_product(const Finish<T>& f, float (&v)[8], int64_t i, int64_t j, int li, int g)
 {
-    int32_t r = (int32_t)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((int64_t)r * (r + 1) / 2 > t) --r;
-    while ((int64_t)(r + 1) * (r + 2) / 2 <= t) ++r;
-    i = r;
-    j = (int32_t)(t - (int64_t)r * (r + 1) / 2);
+    typedef Pack<_Float16, 8> P;
+    const int chunk = paired_chunk(g);
+    const int64_t at = block_place(i, j, f.ld) + li * 32 + 8 * chunk;
+    const P xh = *reinterpret_cast<const P*>(f.x.hi + at), xl = *reinterpret_cast<const P*>(f.x.lo + at);
+    const float d = f.a + f.diagonal[i + li];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = fmaf(d, (float)xh.v[q] + (float)xl.v[q], v[q] * (1.f / kHeld));
+    if constexpr (PURPOSE == kApply) {
+        store_halves<8>(f.out, at, v);
+    } else {
+        const int64_t column = j + 8 * chunk;
+        const int64_t r = f.transposed ? column : i + li, c = f.transposed ? i + li : column;
+        const int32_t b = block_at(f, (int32_t)(r / 16), (int32_t)(c / 16));
+        if (b < 0) return;
+        T* o = f.blocks + (int64_t)b * 256 + r % 16 * 16 + c % 16;
+        if (f.transposed) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) o[16 * q] = r + q < f.M && c < f.K ? (T)(v[q] * (1.f / kHeld)) : (T)0.f;
+        } else {
+            Pack<T, 8> k;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) k.v[q] = r < f.M && c + q < f.K ? (T)(v[q] * (1.f / kHeld)) : (T)0.f;
+            *reinterpret_cast<Pack<T, 8>*>(o) = k;
+        }
+    }
 }
 
+// Tiles of TI x 128, of a symmetric result those that have an element on or below the
+// diagonal: TI / 128 * (i + 1) of them in row i.
 __host__ __device__ __forceinline__ int64_t product_tiles(const Product& a)
 {
-    return a.lower ? (int64_t)a.tiles_i * (a.tiles_i + 1) / 2 : (int64_t)a.tiles_i * a.tiles_j;
+    return a.lower ? (int64_t)a.tiles_i * (a.tiles_i + 1) / 2 * (a.tiles_j / a.tiles_i)
+                   : (int64_t)a.tiles_i * a.tiles_j;
 }
 
+template <int TI>
 __device__ __forceinline__ void tile_place(const Product& a, int64_t t, int32_t& ti, int32_t& tj)
 {
     if (a.lower) {
-        triangle(t, ti, tj);
+        constexpr int per = TI / kTileJ;
+        const int64_t pair = t / per;
+        int32_t r = (int32_t)((sqrtf(8.f * (float)pair + 1.f) - 1.f) * 0.5f);
+        while ((int64_t)r * (r + 1) / 2 > pair) --r;
+        while ((int64_t)(r + 1) * (r + 2) / 2 <= pair) ++r;
+        ti = r;
+        tj = (int32_t)(t - (int64_t)r * (r + 1) / 2 * per);
     } else {
         // bands of 8 rows of tiles, column by column
         const int64_t band = t / (8 * (int64_t)a.tiles_j) * 8;
@@ -197,6 +254,8 @@ __device__ __forceinline__ void tile_place(const Product& a, int64_t t, int32_t&
         ti = (int32_t)(band + in % h);
         tj = (int32_t)(in / h);
     }
+    ti = __builtin_amdgcn_readfirstlane(ti);
+    tj = __builtin_amdgcn_readfirstlane(tj);
 }
 
 typedef __attribute__((address_space(3))) short4_t lds_short4_t;
@@ -206,56 +265,70 @@ __device__ __forceinline__ u32x2_t read_across(const unsigned char* p)
                               __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)const_cast<unsigned char*>(p)));
 }
 
-// Rows of 128 bytes, chunk c (16 bytes) of row r at c ^ (r & 7); rows of TILE values,
-// chunk c of row k at c ^ 2 (k & 7): what one read touches is in different banks.
-template <typename T, int TILE, bool ACROSS, int PASSES, int PURPOSE>
-__global__ __launch_bounds__(Shape<TILE>::kThreads, 2) void ff_orthogonal_product_kernel(const Product a, const Finish<T> f)
+// Chunk c (16 bytes) of row r of a block lies in LDS at c ^ row_swizzle(r), of one that is
+// read across its rows at c ^ across_swizzle(r), so that what is read at once is in
+// different banks.  A read of 16 bytes a lane takes sixteen lanes at once, lanes 0-3, 12-15,
+// 20-27 first and 4-11, 16-19, 28-31 next: eight rows of one g and the other eight of the
+// next; a transposed read of 8 bytes takes 32.
+__device__ __forceinline__ int row_swizzle(int r)
 {
-    using S = Shape<TILE>;
-    constexpr int FI = S::FI, FJ = S::FJ;
+    const int x = (r >> 2) & 3;  // 0, 2, 3, 1
+    return ((x ^ (x >> 1)) & 1) << 1 | x >> 1;
+}
+__device__ __forceinline__ int across_swizzle(int r) { return (r >> 3) << 1; }
+
+template <typename T, int TI, bool ACROSS, int PASSES, int PURPOSE>
+__global__ __launch_bounds__(kProductThreads, 2) void ff_orthogonal_product_kernel(const Product a, const Finish<T> f)
+{
+    using S = Shape<TI>;
+    constexpr int FI = S::FI, FJ = S::FJ, kStages = S::kStages;
     __shared__ __align__(16) unsigned char smem[S::kLds];
     const int t = threadIdx.x, lane = t & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wi = wave & 1, wj = wave >> 1;
     const int64_t tiles = product_tiles(a), item = xcd_item(blockIdx.x, tiles * a.splits);
     if (item < 0) return;
-    const int64_t tile = item / a.splits;
-    const int32_t split = (int32_t)(item % a.splits);
+    const int32_t split = __builtin_amdgcn_readfirstlane((int32_t)(item % a.splits));
     int32_t ti, tj;
-    tile_place(a, tile, ti, tj);
-    const int64_t i0 = (int64_t)ti * TILE, j0 = (int64_t)tj * TILE;
+    tile_place<TI>(a, item / a.splits, ti, tj);
+    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * kTileJ;
     const int32_t from = (int32_t)((int64_t)a.steps * split / a.splits);
     const int32_t count = (int32_t)((int64_t)a.steps * (split + 1) / a.splits) - from;
     const uint32_t lds0 = lds_address(smem);
 
-    // this lane's bytes of what the wave loads, a KB at a time
-    constexpr int kPer = S::kSide / 1024 / S::kWaves;
-    uint32_t p_lane[kPer], q_lane[kPer];
+    // This lane's bytes of the blocks that the wave loads.
+    constexpr int kPerI = S::kSideI / 1024 / kProductWaves, kPerJ = S::kSideJ / 1024 / kProductWaves;
+    const int row = lane >> 2;
+    const uint32_t across_p = (uint32_t)(a.p_ld / 32) * 1024u, across_q = (uint32_t)(a.q_ld / 32) * 1024u;
+    const uint32_t in_row = (uint32_t)(row * 64 + (((lane & 3) ^ row_swizzle(row)) * 16));
+    const uint32_t in_across = (uint32_t)(row * 64 + (((lane & 3) ^ across_swizzle(row)) * 16));
+    uint32_t p_lane[kPerI], q_lane[kPerJ];
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-        const int r = 8 * (wave * kPer + u) + (lane >> 3);
-        p_lane[u] = (uint32_t)(r * a.p_ld * 2) + 16u * (uint32_t)((lane & 7) ^ (r & 7));
-        if constexpr (ACROSS) {
-            constexpr int kChunks = TILE / 8;
-            const int at = (wave * kPer + u) * 64 + lane, k = at / kChunks, c = at % kChunks;
-            q_lane[u] = (uint32_t)(k * a.q_ld * 2) + 16u * (uint32_t)(c ^ (2 * (k & 7)));
-        } else {
-            q_lane[u] = (uint32_t)(r * a.q_ld * 2) + 16u * (uint32_t)((lane & 7) ^ (r & 7));
-        }
+    for (int u = 0; u < kPerI; ++u) p_lane[u] = (uint32_t)(wave * kPerI + u) * across_p + in_row;
+#pragma unroll
+    for (int u = 0; u < kPerJ; ++u) {
+        const int b = wave * kPerJ + u;
+        q_lane[u] = ACROSS ? (uint32_t)(b / (kTileJ / 32)) * across_q + (uint32_t)(b % (kTileJ / 32)) * 1024u + in_across
+                           : (uint32_t)b * across_q + in_row;
     }
-    const uint32_t p_bytes = (uint32_t)(TILE * a.p_ld * 2);
-    const uint32_t q_bytes = (uint32_t)((ACROSS ? kDeepK : TILE) * a.q_ld * 2);
+    const uint32_t p_bytes = (uint32_t)(TI / 16) * across_p;
+    const uint32_t q_bytes = (uint32_t)((ACROSS ? kDeepK : kTileJ) / 16) * across_q;
 
-    auto issue = [&](int pass, int32_t step, int stage) {
-        const _Float16* p = a.p[pass] + i0 * a.p_ld + (int64_t)step * kDeepK;
-        const _Float16* q = ACROSS ? a.q[pass] + (int64_t)step * kDeepK * a.q_ld + j0
-                                   : a.q[pass] + j0 * a.q_ld + (int64_t)step * kDeepK;
+    // the loads of step n of all passes', one after the other, into stage `stage`
+    const int32_t all = PASSES * count;
+    constexpr int kLoads = kPerI + kPerJ;
+    auto issue = [&](int32_t n, int stage) {
+        const int pass = PASSES == 1 ? 0 : n / count;
+        const int32_t step = from + (PASSES == 1 ? n : n % count);
+        const int64_t k = (int64_t)step * kDeepK;
+        const _Float16* p = a.p[pass] + block_place(i0, k, a.p_ld);
+        const _Float16* q = a.q[pass] + (ACROSS ? block_place(k, j0, a.q_ld) : block_place(j0, k, a.q_ld));
         const i32x4_t pb = dma_buffer(p, p_bytes), qb = dma_buffer(q, q_bytes);
         const uint32_t to = lds0 + (uint32_t)(stage * S::kStage);
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) dma_to_lds(to + (uint32_t)(wave * kPer + u) * 1024u, p_lane[u], pb);
+        for (int u = 0; u < kPerI; ++u) dma_to_lds(to + (uint32_t)(wave * kPerI + u) * 1024u, p_lane[u], pb);
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) dma_to_lds(to + S::kSide + (uint32_t)(wave * kPer + u) * 1024u, q_lane[u], qb);
+        for (int u = 0; u < kPerJ; ++u) dma_to_lds(to + S::kSideI + (uint32_t)(wave * kPerJ + u) * 1024u, q_lane[u], qb);
     };
 
     float4_t acc[FI][FJ];
@@ -265,85 +338,116 @@ __global__ __launch_bounds__(Shape<TILE>::kThreads, 2) void ff_orthogonal_produc
         for (int j = 0; j < FJ; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
 
     auto multiply = [&](int stage) {
+        u32x4_t x[FI], y[FJ];
         const unsigned char* P = smem + stage * S::kStage;
-        const unsigned char* Q = P + S::kSide;
+        const unsigned char* Q = P + S::kSideI;
 #pragma unroll
-        for (int h = 0; h < kDeepK / 32; ++h) {
-            u32x4_t x[FI], y[FJ];
-#pragma unroll
-            for (int j = 0; j < FJ; ++j) {
-                if constexpr (ACROSS) {
-                    const int k = 32 * h + 8 * g + (li >> 2), c = 2 * (wj * FJ + j) + ((li & 3) >> 1);
-                    const u32x2_t lo = read_across(Q + k * (TILE * 2) + ((c ^ (2 * (k & 7))) * 16) + 8 * (li & 1));
-                    const u32x2_t hi =
-                        read_across(Q + (k + 4) * (TILE * 2) + ((c ^ (2 * ((k + 4) & 7))) * 16) + 8 * (li & 1));
-                    y[j] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
-                } else {
-                    const int r = wj * S::kWaveJ + 16 * j + li;
-                    y[j] = *reinterpret_cast<const u32x4_t*>(Q + r * 128 + (((4 * h + g) ^ (r & 7)) * 16));
-                }
+        for (int j = 0; j < FJ; ++j) {
+            if constexpr (ACROSS) {
+                // rows 8 g .. + 7 of the step, 8 bytes (four columns) a lane
+                const int r = 8 * (g & 1) + (li >> 2), c = (2 * (j & 1) + ((li & 3) >> 1)) ^ across_swizzle(r);
+                const unsigned char* q = Q + ((g >> 1) * (kTileJ / 32) + 2 * wj + j / 2) * 1024 + r * 64 + c * 16 + 8 * (li & 1);
+                const u32x2_t lo = read_across(q), hi = read_across(q + 4 * 64);
+                y[j] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+            } else {
+                const int r = wj * S::kWaveJ + 16 * j + li;
+                y[j] = *reinterpret_cast<const u32x4_t*>(Q + r * 64 + ((g ^ row_swizzle(li)) * 16));
             }
-#pragma unroll
-            for (int i = 0; i < FI; ++i) {
-                const int r = wi * S::kWaveI + 16 * i + li;
-                x[i] = *reinterpret_cast<const u32x4_t*>(P + r * 128 + (((4 * h + g) ^ (r & 7)) * 16));
-            }
-#pragma unroll
-            for (int i = 0; i < FI; ++i)
-#pragma unroll
-                for (int j = 0; j < FJ; ++j) acc[i][j] = mfma16<_Float16>(y[j], x[i], acc[i][j]);
         }
-    };
-
-    // the steps of all passes one after the other
-    const int32_t all = PASSES * count;
-    if (all > 0) issue(0, from, 0);
-    for (int32_t st = 0; st < all; ++st) {
-        dma_wait<0>();
-        __syncthreads();
-        if (st + 1 < all) {
-            const int32_t n = st + 1;
-            issue(PASSES == 1 ? 0 : n / count, from + (PASSES == 1 ? n : n % count), n & 1);
+#pragma unroll
+        for (int i = 0; i < FI; ++i) {
+            const int r = wi * S::kWaveI + 16 * i + li;
+            x[i] = *reinterpret_cast<const u32x4_t*>(P + r * 64 + ((g ^ row_swizzle(li)) * 16));
         }
-        multiply(st & 1);
-    }
-
-    if constexpr (PURPOSE == kPart) {
-        float* part = a.part + item * (int64_t)(TILE * TILE);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < FI; ++i)
 #pragma unroll
-            for (int j = 0; j < FJ; ++j)
-                *reinterpret_cast<float4_t*>(part + (wi * S::kWaveI + 16 * i + li) * TILE + wj * S::kWaveJ + 16 * j + 4 * g) =
-                    acc[i][j];
+            for (int j = 0; j < FJ; ++j) acc[i][j] = mfma16<_Float16>(y[j], x[i], acc[i][j]);
+        __builtin_amdgcn_s_setprio(0);
+    };
+
+    // kStages - 1 steps are under way at most, the latest kStages - 2 of them past the wait
+#pragma unroll
+    for (int n = 0; n < kStages - 1; ++n)
+        if (n < all) issue(n, n);
+    for (int32_t n = 0, stage = 0; n < all; ++n) {
+        if (n + kStages - 2 < all)
+            dma_wait<(kStages - 2) * kLoads>();
+        else
+            dma_wait<0>();
+        // all have read what stood where the next loads go
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        const int before = stage == 0 ? kStages - 1 : stage - 1;
+        if (n + kStages - 1 < all) issue(n + kStages - 1, before);
+        multiply(stage);
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+    }
+
+    // a lane has columns 4 g .. + 3 of row li of every tile of 16 x 16
+    static_assert(FJ == 4 && FI % 2 == 0);
+    const int64_t iw = i0 + wi * S::kWaveI, jw = j0 + wj * S::kWaveJ;
+    if constexpr (PURPOSE == kPart) {
+        float4_t* part = reinterpret_cast<float4_t*>(a.part) + (item * (TI * kTileJ / 256) + wave * (FI * FJ)) * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) part[(i * FJ + j) * 64] = acc[i][j];
+    } else if constexpr (PURPOSE == kGram || PURPOSE == kSquare) {
+        __syncthreads();
+        _Float16* turn = reinterpret_cast<_Float16*>(smem) + wave * 2048;
+#pragma unroll
+        for (int i = 0; i < FI; i += 2)
+#pragma unroll
+            for (int j = 0; j < FJ; j += 2) {
+                float v[2][8];
+                pair_up(acc[i][j], acc[i][j + 1], v[0]);
+                pair_up(acc[i + 1][j], acc[i + 1][j + 1], v[1]);
+                finish_symmetric<T, PURPOSE>(f, v, iw + 16 * i, jw + 16 * j, li, g, j0 + kTileJ <= i0, turn);
+            }
     } else {
 #pragma unroll
         for (int i = 0; i < FI; ++i)
 #pragma unroll
-            for (int j = 0; j < FJ; ++j) {
-                const int64_t it = i0 + wi * S::kWaveI + 16 * i, jt = j0 + wj * S::kWaveJ + 16 * j;
-                finish_four<T, PURPOSE>(f, acc[i][j], it + li, jt + 4 * g, it, jt, a.lower && ti != tj);
+            for (int j = 0; j < FJ; j += 2) {
+                float v[8];
+                pair_up(acc[i][j], acc[i][j + 1], v);
+                finish_product<T, PURPOSE>(f, v, iw + 16 * i, jw + 16 * j, li, g);
             }
     }
 }
 
-// The shares of a tile's sums, in their order.
-template <typename T, int TILE, int PURPOSE>
+// The shares of a tile's sums, in their order; a wave to 32 x 32 of them.
+template <typename T, int TI, int PURPOSE>
 __global__ __launch_bounds__(256) void ff_orthogonal_join_kernel(const Product a, const Finish<T> f)
 {
-    constexpr int kPieces = TILE * TILE / 1024;  // of a tile: 256 threads, four values each
+    using S = Shape<TI>;
+    constexpr int FI = S::FI, FJ = S::FJ, kPieces = TI * kTileJ / 4096;  // workgroups of a tile
+    __shared__ __align__(16) _Float16 turn[4][2048];
+    const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t tile = blockIdx.x / kPieces;
-    const int piece = (int)(blockIdx.x % kPieces);
+    // the product's wave, and its tiles (i, j) to (i + 1, j + 1)
+    const int piece = (int)(blockIdx.x % kPieces) * 4 + wave, of = piece / (FI * FJ / 4);
+    const int i = piece % (FI * FJ / 4) / (FJ / 2) * 2, j = piece % (FJ / 2) * 2;
     int32_t ti, tj;
-    tile_place(a, tile, ti, tj);
-    // pieces are 16 x 64: four rows of 16 x 16 tiles' lanes as the sums have them
-    const int t = threadIdx.x, lane = t & 63, li = lane & 15, g = lane >> 4;
-    const int i = piece / (TILE / 64) * 16 + li, j = piece % (TILE / 64) * 64 + (t >> 6) * 16 + 4 * g;
-    const float* part = a.part + tile * a.splits * (int64_t)(TILE * TILE) + i * TILE + j;
-    float4_t v = *reinterpret_cast<const float4_t*>(part);
-    for (int32_t s = 1; s < a.splits; ++s) v += *reinterpret_cast<const float4_t*>(part + s * (int64_t)(TILE * TILE));
-    const int64_t it = (int64_t)ti * TILE + i - li, jt = (int64_t)tj * TILE + j - 4 * g;
-    finish_four<T, PURPOSE>(f, v, it + li, jt + 4 * g, it, jt, a.lower && ti != tj);
+    tile_place<TI>(a, tile, ti, tj);
+    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * kTileJ;
+    const float4_t* part =
+        reinterpret_cast<const float4_t*>(a.part) + (tile * a.splits * (TI * kTileJ / 256) + of * (FI * FJ)) * 64 + lane;
+    float4_t v[2][2] = {};
+    for (int32_t s = 0; s < a.splits; ++s)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+                v[u][w] += part[(s * (int64_t)(TI * kTileJ / 256) + (i + u) * FJ + j + w) * 64];
+    float e[2][8];
+    pair_up(v[0][0], v[0][1], e[0]);
+    pair_up(v[1][0], v[1][1], e[1]);
+    finish_symmetric<T, PURPOSE>(f, e, i0 + (of & 1) * S::kWaveI + 16 * i, j0 + (of >> 1) * S::kWaveJ + 16 * j, li, g,
+                                 j0 + kTileJ <= i0, turn[wave]);
 }
 
 // Sums of squares of the stored values inside the weight, a share of the blocks each.
@@ -389,9 +493,9 @@ __global__ __launch_bounds__(256) void ff_orthogonal_start_kernel(const Finish<T
     const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) + eps;
     // an update of zeros stays one
     const double by = norm == 0.0 ? 0.0 : (double)kHeld / norm;
-    const int64_t per = f.ld / 8;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + t; e < rows * per; e += (int64_t)gridDim.x * 256) {
-        const int64_t i = e / per, j = e % per * 8;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + t; e < rows * f.ld / 8; e += (int64_t)gridDim.x * 256) {
+        const int64_t block = e / 64, per = f.ld / 32;
+        const int64_t i = block / per * 16 + e % 64 / 4, j = block % per * 32 + e % 4 * 8;
         const int64_t r = f.transposed ? j : i, c = f.transposed ? i : j;
         const int32_t b = block_at(f, (int32_t)(r / 16), (int32_t)(c / 16));
         Pack<_Float16, 8> hi{}, lo{};
@@ -404,15 +508,15 @@ __global__ __launch_bounds__(256) void ff_orthogonal_start_kernel(const Finish<T
                 halves(w, hi.v[q], lo.v[q]);
             }
         }
-        *reinterpret_cast<Pack<_Float16, 8>*>(f.out.hi + i * f.ld + j) = hi;
-        *reinterpret_cast<Pack<_Float16, 8>*>(f.out.lo + i * f.ld + j) = lo;
+        *reinterpret_cast<Pack<_Float16, 8>*>(f.out.hi + e * 8) = hi;
+        *reinterpret_cast<Pack<_Float16, 8>*>(f.out.lo + e * 8) = lo;
     }
 }
 
 // Sizes and memory of one orthogonalised update.
 struct OrthogonalPlan {
     bool transposed, split;
-    int tile;
+    int tile;      // rows of one
     int64_t m, k;  // rows and columns of X, to whole tiles
     int gram_splits, square_splits;
     size_t x_hi[2], x_lo[2], s_hi, s_lo, b_hi, b_lo, diagonal, norm, part, end;
@@ -426,14 +530,14 @@ OrthogonalPlan orthogonal_plan(const BlockIndex& w, int64_t size)
     const int64_t rows = p.transposed ? w.K : w.M, columns = p.transposed ? w.M : w.K;
     p.tile = rows <= 1024 ? 128 : 256;
     p.m = (rows + p.tile - 1) / p.tile * p.tile;
-    p.k = (columns + p.tile - 1) / p.tile * p.tile;
-    const int64_t n = p.m / p.tile, tiles = n * (n + 1) / 2;
-    // shares of a sum: rounds of 256 workgroups, a share each
+    p.k = (columns + kTileJ - 1) / kTileJ * kTileJ;
+    const int64_t n = p.m / p.tile, tiles = n * (n + 1) / 2 * (p.tile / kTileJ);
+    // shares of a sum: rounds of 512 workgroups, a share each
     auto splits = [&](int64_t steps) {
         int best = 1;
         double least = 1e30;
-        for (int s = 1; s <= 8 && steps / s >= 4; ++s) {
-            const double time = (double)((tiles * s + 255) / 256) * ((double)steps / s + 2.0) + (s > 1 ? 4.0 + 0.02 * s * tiles : 0.0);
+        for (int s = 1; s <= 8 && steps / s >= 8; ++s) {
+            const double time = (double)((tiles * s + 511) / 512) * ((double)steps / s + 4.0) + (s > 1 ? 8.0 + 0.02 * s * tiles : 0.0);
             if (time < least) {
                 least = time;
                 best = s;
@@ -456,30 +560,30 @@ OrthogonalPlan orthogonal_plan(const BlockIndex& w, int64_t size)
     p.diagonal = c.take((size_t)p.m * 4);
     p.norm = c.take(kNormShares * 8);
     const int most = p.gram_splits > p.square_splits ? p.gram_splits : p.square_splits;
-    p.part = c.take(most > 1 ? (size_t)(tiles * most) * p.tile * p.tile * 4 : 0);
+    p.part = c.take(most > 1 ? (size_t)(tiles * most) * p.tile * kTileJ * 4 : 0);
     p.end = c.end;
     return p;
 }
 
-template <typename T, int TILE, bool ACROSS, int PASSES, int PURPOSE>
+template <typename T, int TI, bool ACROSS, int PASSES, int PURPOSE>
 void launch_orthogonal(const Product& a, const Finish<T>& f, hipStream_t s)
 {
     const int64_t tiles = product_tiles(a);
-    constexpr int threads = Shape<TILE>::kThreads;
+    constexpr int threads = kProductThreads;
     const dim3 grid = launch_grid(kXcds * xcd_chunk(tiles * a.splits), threads);
     if (a.splits > 1) {
         if constexpr (!ACROSS) {
-            hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TILE, ACROSS, PASSES, kPart>), grid, dim3(threads), 0, s, a, f);
-            hipLaunchKernelGGL((ff_orthogonal_join_kernel<T, TILE, PURPOSE>), launch_grid(tiles * (TILE * TILE / 1024), 256),
+            hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TI, ACROSS, PASSES, kPart>), grid, dim3(threads), 0, s, a, f);
+            hipLaunchKernelGGL((ff_orthogonal_join_kernel<T, TI, PURPOSE>), launch_grid(tiles * (TI * kTileJ / 4096), 256),
                                dim3(256), 0, s, a, f);
         }
     } else {
-        hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TILE, ACROSS, PASSES, PURPOSE>), grid, dim3(threads), 0, s, a, f);
+        hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TI, ACROSS, PASSES, PURPOSE>), grid, dim3(threads), 0, s, a, f);
     }
     XSPMM_LAUNCH_CHECK();
 }
 
-template <typename T, int TILE>
+template <typename T, int TI>
 void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const OrthogonalArgs& o, const OrthogonalPlan& p,
                       char* at, hipStream_t s)
 {
@@ -522,32 +626,33 @@ void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const Orthog
         a.part = reinterpret_cast<float*>(at + p.part);
         operands(a, from, from);
         a.p_ld = a.q_ld = p.k;
-        a.tiles_i = a.tiles_j = (int32_t)(p.m / TILE);
+        a.tiles_i = (int32_t)(p.m / TI);
+        a.tiles_j = (int32_t)(p.m / kTileJ);
         a.steps = (int32_t)(p.k / kDeepK);
         a.splits = p.gram_splits;
         a.lower = true;
         f.out = S;
         f.ld = p.m;
-        launch_orthogonal<T, TILE, false, PASSES, kGram>(a, f, s);
+        launch_orthogonal<T, TI, false, PASSES, kGram>(a, f, s);
         operands(a, S, S);
         a.p_ld = a.q_ld = p.m;
         a.steps = (int32_t)(p.m / kDeepK);
         a.splits = p.square_splits;
         f.s = S;
         f.out = B;
-        launch_orthogonal<T, TILE, false, PASSES, kSquare>(a, f, s);
+        launch_orthogonal<T, TI, false, PASSES, kSquare>(a, f, s);
         operands(a, B, from);
         a.q_ld = p.k;
-        a.tiles_j = (int32_t)(p.k / TILE);
+        a.tiles_j = (int32_t)(p.k / kTileJ);
         a.splits = 1;
         a.lower = false;
         f.x = from;
         f.out = to;
         f.ld = p.k;
         if (step + 1 < o.steps)
-            launch_orthogonal<T, TILE, true, PASSES, kApply>(a, f, s);
+            launch_orthogonal<T, TI, true, PASSES, kApply>(a, f, s);
         else
-            launch_orthogonal<T, TILE, true, PASSES, kLast>(a, f, s);
+            launch_orthogonal<T, TI, true, PASSES, kLast>(a, f, s);
     }
 }
 
