@@ -46,19 +46,22 @@ constexpr int kDeepK = 32;  // of a product's step
 
 // A workgroup of four waves takes TI rows and 128 columns, a wave half of either.  Two
 // workgroups share a CU and are not in step: while one multiplies, the other reads its
-// operands, or reads and writes X at a tile's end (512 KB of a tile of 256 x 256, which
-// with one workgroup of eight waves a CU took 157 of 545 us at 4096 x 14336).
+// operands, or reads and writes X at a tile's end (512 KB of 256 x 256 elements, which
+// with one workgroup of eight waves a CU took 157 of 545 us at 4096 x 14336).  Operands
+// in two halves (SPLIT) take twice the LDS, and three products of each step's: one
+// workgroup a CU has as much to multiply as two have without.
 constexpr int kTileJ = 128;
 constexpr int kProductWaves = 4, kProductThreads = 64 * kProductWaves;
-template <int TI>
+template <int TI, bool SPLIT>
 struct Shape {
     static constexpr int kWaveI = TI / 2, kWaveJ = kTileJ / 2;  // a wave's rows and columns
     static constexpr int FI = kWaveI / 16, FJ = kWaveJ / 16;
+    static constexpr int kHalves = SPLIT ? 2 : 1;
     static constexpr int kSideI = TI * kDeepK * 2, kSideJ = kTileJ * kDeepK * 2;  // bytes of an operand's step
-    static constexpr int kStage = kSideI + kSideJ;
+    static constexpr int kStage = kHalves * (kSideI + kSideJ);
     static constexpr int kStages = TI == 256 ? 3 : 4;  // steps in LDS
     static constexpr int kLds = kStages * kStage;
-    static_assert(kLds <= 80 * 1024);
+    static_assert(kLds <= (SPLIT ? 160 : 80) * 1024);
 };
 
 // What becomes of a product's sums.
@@ -71,8 +74,8 @@ enum Purpose {
 };
 
 struct Product {
-    const _Float16* p[3];  // rows i, k along them
-    const _Float16* q[3];  // rows j, k along them; or rows k, j along them
+    Halves p;  // rows i, k along them
+    Halves q;  // rows j, k along them; or rows k, j along them
     int64_t p_ld, q_ld;
     int32_t tiles_i, tiles_j;
     int32_t steps;   // of kDeepK
@@ -277,11 +280,12 @@ __device__ __forceinline__ int row_swizzle(int r)
 }
 __device__ __forceinline__ int across_swizzle(int r) { return (r >> 3) << 1; }
 
-template <typename T, int TI, bool ACROSS, int PASSES, int PURPOSE>
-__global__ __launch_bounds__(kProductThreads, 2) void ff_orthogonal_product_kernel(const Product a, const Finish<T> f)
+template <typename T, int TI, bool ACROSS, int PURPOSE>
+__global__ __launch_bounds__(kProductThreads, is_f32<T> ? 1 : 2) void ff_orthogonal_product_kernel(const Product a, const Finish<T> f)
 {
-    using S = Shape<TI>;
-    constexpr int FI = S::FI, FJ = S::FJ, kStages = S::kStages;
+    constexpr bool SPLIT = is_f32<T>;
+    using S = Shape<TI, SPLIT>;
+    constexpr int FI = S::FI, FJ = S::FJ, kStages = S::kStages, kHalves = S::kHalves;
     __shared__ __align__(16) unsigned char smem[S::kLds];
     const int t = threadIdx.x, lane = t & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -293,7 +297,7 @@ __global__ __launch_bounds__(kProductThreads, 2) void ff_orthogonal_product_kern
     tile_place<TI>(a, item / a.splits, ti, tj);
     const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * kTileJ;
     const int32_t from = (int32_t)((int64_t)a.steps * split / a.splits);
-    const int32_t count = (int32_t)((int64_t)a.steps * (split + 1) / a.splits) - from;
+    const int32_t all = (int32_t)((int64_t)a.steps * (split + 1) / a.splits) - from;
     const uint32_t lds0 = lds_address(smem);
 
     // This lane's bytes of the blocks that the wave loads.
@@ -314,21 +318,22 @@ __global__ __launch_bounds__(kProductThreads, 2) void ff_orthogonal_product_kern
     const uint32_t p_bytes = (uint32_t)(TI / 16) * across_p;
     const uint32_t q_bytes = (uint32_t)((ACROSS ? kDeepK : kTileJ) / 16) * across_q;
 
-    // the loads of step n of all passes', one after the other, into stage `stage`
-    const int32_t all = PASSES * count;
-    constexpr int kLoads = kPerI + kPerJ;
+    // the loads of step n into stage `stage`: of either half p's and q's
+    constexpr int kLoads = kHalves * (kPerI + kPerJ);
     auto issue = [&](int32_t n, int stage) {
-        const int pass = PASSES == 1 ? 0 : n / count;
-        const int32_t step = from + (PASSES == 1 ? n : n % count);
-        const int64_t k = (int64_t)step * kDeepK;
-        const _Float16* p = a.p[pass] + block_place(i0, k, a.p_ld);
-        const _Float16* q = a.q[pass] + (ACROSS ? block_place(k, j0, a.q_ld) : block_place(j0, k, a.q_ld));
-        const i32x4_t pb = dma_buffer(p, p_bytes), qb = dma_buffer(q, q_bytes);
-        const uint32_t to = lds0 + (uint32_t)(stage * S::kStage);
+        const int64_t k = (int64_t)(from + n) * kDeepK;
+        const int64_t at_p = block_place(i0, k, a.p_ld), at_q = ACROSS ? block_place(k, j0, a.q_ld) : block_place(j0, k, a.q_ld);
 #pragma unroll
-        for (int u = 0; u < kPerI; ++u) dma_to_lds(to + (uint32_t)(wave * kPerI + u) * 1024u, p_lane[u], pb);
+        for (int h = 0; h < kHalves; ++h) {
+            const i32x4_t pb = dma_buffer((h ? a.p.lo : a.p.hi) + at_p, p_bytes);
+            const i32x4_t qb = dma_buffer((h ? a.q.lo : a.q.hi) + at_q, q_bytes);
+            const uint32_t to = lds0 + (uint32_t)(stage * S::kStage + h * (S::kSideI + S::kSideJ));
 #pragma unroll
-        for (int u = 0; u < kPerJ; ++u) dma_to_lds(to + S::kSideI + (uint32_t)(wave * kPerJ + u) * 1024u, q_lane[u], qb);
+            for (int u = 0; u < kPerI; ++u) dma_to_lds(to + (uint32_t)(wave * kPerI + u) * 1024u, p_lane[u], pb);
+#pragma unroll
+            for (int u = 0; u < kPerJ; ++u)
+                dma_to_lds(to + S::kSideI + (uint32_t)(wave * kPerJ + u) * 1024u, q_lane[u], qb);
+        }
     };
 
     float4_t acc[FI][FJ];
@@ -337,9 +342,12 @@ __global__ __launch_bounds__(kProductThreads, 2) void ff_orthogonal_product_kern
 #pragma unroll
         for (int j = 0; j < FJ; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-    auto multiply = [&](int stage) {
+    struct Operands {
         u32x4_t x[FI], y[FJ];
-        const unsigned char* P = smem + stage * S::kStage;
+    };
+    auto read = [&](int stage, int h, Operands& o) {
+        auto& [x, y] = o;
+        const unsigned char* P = smem + stage * S::kStage + h * (S::kSideI + S::kSideJ);
         const unsigned char* Q = P + S::kSideI;
 #pragma unroll
         for (int j = 0; j < FJ; ++j) {
@@ -359,15 +367,16 @@ __global__ __launch_bounds__(kProductThreads, 2) void ff_orthogonal_product_kern
             const int r = wi * S::kWaveI + 16 * i + li;
             x[i] = *reinterpret_cast<const u32x4_t*>(P + r * 64 + ((g ^ row_swizzle(li)) * 16));
         }
-        __builtin_amdgcn_s_setprio(1);
+    };
+    auto multiply = [&](const u32x4_t (&x)[FI], const u32x4_t (&y)[FJ]) {
 #pragma unroll
         for (int i = 0; i < FI; ++i)
 #pragma unroll
             for (int j = 0; j < FJ; ++j) acc[i][j] = mfma16<_Float16>(y[j], x[i], acc[i][j]);
-        __builtin_amdgcn_s_setprio(0);
     };
 
-    // kStages - 1 steps are under way at most, the latest kStages - 2 of them past the wait
+    // Step n goes to stage n % kStages; kStages - 1 steps are under way at most, the latest
+    // kStages - 2 of them past the wait for one.
 #pragma unroll
     for (int n = 0; n < kStages - 1; ++n)
         if (n < all) issue(n, n);
@@ -376,12 +385,20 @@ __global__ __launch_bounds__(kProductThreads, 2) void ff_orthogonal_product_kern
             dma_wait<(kStages - 2) * kLoads>();
         else
             dma_wait<0>();
-        // all have read what stood where the next loads go
+        // all have in registers what stood where the next loads go
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __syncthreads();
-        const int before = stage == 0 ? kStages - 1 : stage - 1;
-        if (n + kStages - 1 < all) issue(n + kStages - 1, before);
-        multiply(stage);
+        if (n + kStages - 1 < all) issue(n + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+        Operands hi, lo;
+        read(stage, 0, hi);
+        if constexpr (SPLIT) read(stage, 1, lo);
+        __builtin_amdgcn_s_setprio(1);
+        multiply(hi.x, hi.y);
+        if constexpr (SPLIT) {
+            multiply(hi.x, lo.y);
+            multiply(lo.x, hi.y);
+        }
+        __builtin_amdgcn_s_setprio(0);
         stage = stage == kStages - 1 ? 0 : stage + 1;
     }
 
@@ -422,7 +439,7 @@ __global__ __launch_bounds__(kProductThreads, 2) void ff_orthogonal_product_kern
 template <typename T, int TI, int PURPOSE>
 __global__ __launch_bounds__(256) void ff_orthogonal_join_kernel(const Product a, const Finish<T> f)
 {
-    using S = Shape<TI>;
+    using S = Shape<TI, is_f32<T>>;
     constexpr int FI = S::FI, FJ = S::FJ, kPieces = TI * kTileJ / 4096;  // workgroups of a tile
     __shared__ __align__(16) _Float16 turn[4][2048];
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
@@ -528,16 +545,21 @@ OrthogonalPlan orthogonal_plan(const BlockIndex& w, int64_t size)
     p.transposed = w.M > w.K;
     p.split = size == 4;
     const int64_t rows = p.transposed ? w.K : w.M, columns = p.transposed ? w.M : w.K;
-    p.tile = rows <= 1024 ? 128 : 256;
+    // one tile of 128 x 128 a CU at most, or larger ones that are faster where there are many
+    p.tile = (rows + 127) / 128 * ((columns + 127) / 128) <= 256 ? 128 : 256;
     p.m = (rows + p.tile - 1) / p.tile * p.tile;
     p.k = (columns + kTileJ - 1) / kTileJ * kTileJ;
     const int64_t n = p.m / p.tile, tiles = n * (n + 1) / 2 * (p.tile / kTileJ);
-    // shares of a sum: rounds of 512 workgroups, a share each
+    // Shares of a sum: rounds of workgroups, two a CU (one where operands are split, whose
+    // steps take three times as long), and what a launch and joining cost, in steps' time.
+    const int64_t at_once = p.split ? 256 : 512;
+    const double step = p.split ? 3.0 : 1.0;
     auto splits = [&](int64_t steps) {
         int best = 1;
         double least = 1e30;
         for (int s = 1; s <= 8 && steps / s >= 8; ++s) {
-            const double time = (double)((tiles * s + 511) / 512) * ((double)steps / s + 4.0) + (s > 1 ? 8.0 + 0.02 * s * tiles : 0.0);
+            const double join = s == 1 ? 0.0 : 19.0 + 0.08 * (double)(s * tiles);
+            const double time = (double)((tiles * s + at_once - 1) / at_once) * ((double)steps / s * step + 28.0) + join;
             if (time < least) {
                 least = time;
                 best = s;
@@ -565,7 +587,7 @@ OrthogonalPlan orthogonal_plan(const BlockIndex& w, int64_t size)
     return p;
 }
 
-template <typename T, int TI, bool ACROSS, int PASSES, int PURPOSE>
+template <typename T, int TI, bool ACROSS, int PURPOSE>
 void launch_orthogonal(const Product& a, const Finish<T>& f, hipStream_t s)
 {
     const int64_t tiles = product_tiles(a);
@@ -573,12 +595,12 @@ void launch_orthogonal(const Product& a, const Finish<T>& f, hipStream_t s)
     const dim3 grid = launch_grid(kXcds * xcd_chunk(tiles * a.splits), threads);
     if (a.splits > 1) {
         if constexpr (!ACROSS) {
-            hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TI, ACROSS, PASSES, kPart>), grid, dim3(threads), 0, s, a, f);
+            hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TI, ACROSS, kPart>), grid, dim3(threads), 0, s, a, f);
             hipLaunchKernelGGL((ff_orthogonal_join_kernel<T, TI, PURPOSE>), launch_grid(tiles * (TI * kTileJ / 4096), 256),
                                dim3(256), 0, s, a, f);
         }
     } else {
-        hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TI, ACROSS, PASSES, PURPOSE>), grid, dim3(threads), 0, s, a, f);
+        hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TI, ACROSS, PURPOSE>), grid, dim3(threads), 0, s, a, f);
     }
     XSPMM_LAUNCH_CHECK();
 }
@@ -587,7 +609,6 @@ template <typename T, int TI>
 void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const OrthogonalArgs& o, const OrthogonalPlan& p,
                       char* at, hipStream_t s)
 {
-    constexpr int PASSES = is_f32<T> ? 3 : 1;
     auto half = [&](size_t offset) { return reinterpret_cast<_Float16*>(at + offset); };
     const Halves x[2] = {{half(p.x_hi[0]), half(p.x_lo[0])}, {half(p.x_hi[1]), half(p.x_lo[1])}};
     const Halves S = {half(p.s_hi), p.split ? half(p.s_lo) : nullptr};
@@ -613,18 +634,11 @@ void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const Orthog
     f.ld = p.k;
     hipLaunchKernelGGL((ff_orthogonal_start_kernel<T>), dim3(4096), dim3(256), 0, s, f, update, norm, (double)o.eps, p.m);
     XSPMM_LAUNCH_CHECK();
-    // upper times upper half, upper times lower, lower times upper
-    auto operands = [&](Product& a, const Halves& l, const Halves& r) {
-        a.p[0] = a.p[1] = l.hi;
-        a.q[0] = a.q[2] = r.hi;
-        a.p[2] = l.lo;
-        a.q[1] = r.lo;
-    };
     for (int step = 0; step < o.steps; ++step) {
         const Halves &from = x[step % 2], &to = x[(step + 1) % 2];
         Product a{};
         a.part = reinterpret_cast<float*>(at + p.part);
-        operands(a, from, from);
+        a.p = a.q = from;
         a.p_ld = a.q_ld = p.k;
         a.tiles_i = (int32_t)(p.m / TI);
         a.tiles_j = (int32_t)(p.m / kTileJ);
@@ -633,15 +647,16 @@ void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const Orthog
         a.lower = true;
         f.out = S;
         f.ld = p.m;
-        launch_orthogonal<T, TI, false, PASSES, kGram>(a, f, s);
-        operands(a, S, S);
+        launch_orthogonal<T, TI, false, kGram>(a, f, s);
+        a.p = a.q = S;
         a.p_ld = a.q_ld = p.m;
         a.steps = (int32_t)(p.m / kDeepK);
         a.splits = p.square_splits;
         f.s = S;
         f.out = B;
-        launch_orthogonal<T, TI, false, PASSES, kSquare>(a, f, s);
-        operands(a, B, from);
+        launch_orthogonal<T, TI, false, kSquare>(a, f, s);
+        a.p = B;
+        a.q = from;
         a.q_ld = p.k;
         a.tiles_j = (int32_t)(p.k / kTileJ);
         a.splits = 1;
@@ -650,9 +665,9 @@ void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const Orthog
         f.out = to;
         f.ld = p.k;
         if (step + 1 < o.steps)
-            launch_orthogonal<T, TI, true, PASSES, kApply>(a, f, s);
+            launch_orthogonal<T, TI, true, kApply>(a, f, s);
         else
-            launch_orthogonal<T, TI, true, PASSES, kLast>(a, f, s);
+            launch_orthogonal<T, TI, true, kLast>(a, f, s);
     }
 }
 
