@@ -260,6 +260,14 @@ __device__ __forceinline__ int64_t xcd_item(int64_t w, int64_t total)
     return i < total ? i : -1;
 }
 
+// The same in 32 bits (a launch has less than 2^32 threads): divisions of 64 bits take a
+// wave more than half a microsecond each.
+__device__ __forceinline__ uint32_t xcd_item32(uint32_t w, uint32_t total)
+{
+    const uint32_t i = w % kXcds * ((total + kXcds - 1) / kXcds) + w / kXcds;
+    return i < total ? i : ~0u;
+}
+
 }  // namespace ff
 }  // namespace detail
 }  // namespace xspmm

@@ -28,13 +28,14 @@ __global__ __launch_bounds__(64 * (SPLIT > 4 ? SPLIT : 4)) void ff_int8_walk_ker
     constexpr int kRowsPerGroup = SPLIT > 4 ? 1 : 4 / SPLIT;
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t groups = (a.block_rows + kRowsPerGroup - 1) / kRowsPerGroup;
-    const int64_t tiles = (a.N + 16 * VT - 1) / (16 * VT);
-    const int64_t item = xcd_item(blockIdx.x, groups * tiles);
-    if (item < 0) return;
-    const int32_t br = (int32_t)(item % groups) * kRowsPerGroup + wave / SPLIT;
+    const uint32_t groups = (uint32_t)(a.block_rows + kRowsPerGroup - 1) / kRowsPerGroup;
+    const uint32_t tiles = (uint32_t)((a.N + 16 * VT - 1) / (16 * VT));
+    const uint32_t item = xcd_item32(blockIdx.x, groups * tiles);
+    if (item == ~0u) return;
+    const uint32_t tile = item / groups;
+    const int32_t br = (int32_t)(item - tile * groups) * kRowsPerGroup + wave / SPLIT;
     const int part = wave % SPLIT;
-    const int64_t n0 = item / groups * (16 * VT);
+    const int64_t n0 = (int64_t)tile * (16 * VT);
     int64_t at[VT];  // this lane's bytes of x at block-column 0
 #pragma unroll
     for (int j = 0; j < VT; ++j) at[j] = 16 * min(n0 + 16 * j + li, a.N - 1);
@@ -48,8 +49,7 @@ __global__ __launch_bounds__(64 * (SPLIT > 4 ? SPLIT : 4)) void ff_int8_walk_ker
         for (int l = 0; l < NACC; ++l) {
             const Int8Side& s = a.side[l];
             const int32_t b = s.ptr[br], e = s.ptr[br + 1], steps = (e - b + 3) / 4;
-            const int32_t lo = b + 4 * (int32_t)((int64_t)steps * part / SPLIT);
-            const int32_t hi = min(b + 4 * (int32_t)((int64_t)steps * (part + 1) / SPLIT), e);
+            const int32_t lo = b + 4 * (steps * part / SPLIT), hi = min(b + 4 * (steps * (part + 1) / SPLIT), e);
             auto load = [&](Int8Step<VT>& st, int32_t q) {
                 const int32_t mine = q + g < hi ? q + g : lo;
                 st.a = *reinterpret_cast<const u32x4_t*>(s.vals + (int64_t)mine * 256 + li * 16);
@@ -126,10 +126,10 @@ __global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_ke
     __shared__ float scales[kFewTokens];
     const int t = threadIdx.x, lane = t & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int64_t tile = blockIdx.x % ((a.N + kFewTokens - 1) / kFewTokens);
-    const int32_t br = (int32_t)(blockIdx.x / ((a.N + kFewTokens - 1) / kFewTokens)) * ROWS + wave / SPLIT;
+    const uint32_t tiles = (uint32_t)((a.N + kFewTokens - 1) / kFewTokens), group = blockIdx.x / tiles;
+    const int32_t br = (int32_t)group * ROWS + wave / SPLIT;
     const int part = wave % SPLIT;
-    const int64_t n0 = tile * kFewTokens;
+    const int64_t n0 = (int64_t)(blockIdx.x - group * tiles) * kFewTokens;
     const int nt = ONE ? 1 : (int)min((int64_t)kFewTokens, a.N - n0);
     const int blocks = a.in_blocks * nt;
 
@@ -172,8 +172,8 @@ __global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_ke
         lo[l] = hi[l] = 0;
         if (br < a.block_rows) {
             const int32_t b = a.side[l].ptr[br], e = a.side[l].ptr[br + 1], steps = (e - b + 3) / 4;
-            lo[l] = b + 4 * (int32_t)((int64_t)steps * part / SPLIT);
-            hi[l] = min(b + 4 * (int32_t)((int64_t)steps * (part + 1) / SPLIT), e);
+            lo[l] = b + 4 * (steps * part / SPLIT);
+            hi[l] = min(b + 4 * (steps * (part + 1) / SPLIT), e);
         }
 #pragma unroll
         for (int p = 0; p < kAhead; ++p)

@@ -38,11 +38,12 @@ __global__ __launch_bounds__(kI8Threads, 2) void ff_int8_tile_kernel(const Int8P
     int32_t br0, n0;
     {
         // bands of kI8Band row groups, token tile by token tile
-        const int64_t tiles = (a.N + kI8Wide - 1) / kI8Wide, groups = (a.block_rows + kOutRows - 1) / kOutRows;
-        const int64_t item = xcd_item(blockIdx.x, groups * tiles);
-        if (item < 0) return;
-        const int64_t band = item / (kI8Band * tiles) * kI8Band;
-        const int64_t h = min((int64_t)kI8Band, groups - band), in = item - band * tiles;
+        const uint32_t tiles = (uint32_t)((a.N + kI8Wide - 1) / kI8Wide);
+        const uint32_t groups = (uint32_t)(a.block_rows + kOutRows - 1) / kOutRows;
+        const uint32_t item = xcd_item32(blockIdx.x, groups * tiles);
+        if (item == ~0u) return;
+        const uint32_t band = item / (kI8Band * tiles) * kI8Band;
+        const uint32_t h = min((uint32_t)kI8Band, groups - band), in = item - band * tiles;
         // (uniform, which the compiler does not see behind the divisions)
         br0 = __builtin_amdgcn_readfirstlane((int32_t)(band + in % h) * kOutRows);
         n0 = __builtin_amdgcn_readfirstlane((int32_t)(in / h) * kI8Wide);

@@ -44,20 +44,22 @@ __device__ __forceinline__ int64_t block_place(int64_t r, int64_t c, int64_t ld)
 
 constexpr int kDeepK = 32;  // of a product's step
 
-// A workgroup of four waves takes TI rows and 128 columns, a wave half of either.  Two
+// A workgroup of four waves takes TI rows and 128 columns (of 64 rows, 64), a wave half of
+// either.  Two
 // workgroups share a CU and are not in step: while one multiplies, the other reads its
 // operands, or reads and writes X at a tile's end (512 KB of 256 x 256 elements, which
 // with one workgroup of eight waves a CU took 157 of 545 us at 4096 x 14336).  Operands
 // in two halves (SPLIT) take twice the LDS, and three products of each step's: one
 // workgroup a CU has as much to multiply as two have without.
-constexpr int kTileJ = 128;
+constexpr int tile_columns(int rows) { return rows == 64 ? 64 : 128; }
 constexpr int kProductWaves = 4, kProductThreads = 64 * kProductWaves;
 template <int TI, bool SPLIT>
 struct Shape {
-    static constexpr int kWaveI = TI / 2, kWaveJ = kTileJ / 2;  // a wave's rows and columns
+    static constexpr int TJ = tile_columns(TI);
+    static constexpr int kWaveI = TI / 2, kWaveJ = TJ / 2;  // a wave's rows and columns
     static constexpr int FI = kWaveI / 16, FJ = kWaveJ / 16;
     static constexpr int kHalves = SPLIT ? 2 : 1;
-    static constexpr int kSideI = TI * kDeepK * 2, kSideJ = kTileJ * kDeepK * 2;  // bytes of an operand's step
+    static constexpr int kSideI = TI * kDeepK * 2, kSideJ = TJ * kDeepK * 2;  // bytes of an operand's step
     static constexpr int kStage = kHalves * (kSideI + kSideJ);
     static constexpr int kStages = TI == 256 ? 3 : 4;  // steps in LDS
     static constexpr int kLds = kStages * kStage;
@@ -80,6 +82,7 @@ struct Product {
     int32_t tiles_i, tiles_j;
     int32_t steps;   // of kDeepK
     int32_t splits;  // of the steps
+    uint32_t items;  // tiles times splits
     float* part;
     bool lower;      // tiles on and below the diagonal, and their mirror images
 };
@@ -231,8 +234,8 @@ __device__ __forceinline__ void finish_product(const Finish<T>& f, float (&v)[8]
     }
 }
 
-// Tiles of TI x 128, of a symmetric result those that have an element on or below the
-// diagonal: TI / 128 * (i + 1) of them in row i.
+// Tiles, of a symmetric result those that have an element on or below the diagonal: TI / TJ
+// * (i + 1) of them in row i.
 __host__ __device__ __forceinline__ int64_t product_tiles(const Product& a)
 {
     return a.lower ? (int64_t)a.tiles_i * (a.tiles_i + 1) / 2 * (a.tiles_j / a.tiles_i)
@@ -240,20 +243,20 @@ __host__ __device__ __forceinline__ int64_t product_tiles(const Product& a)
 }
 
 template <int TI>
-__device__ __forceinline__ void tile_place(const Product& a, int64_t t, int32_t& ti, int32_t& tj)
+__device__ __forceinline__ void tile_place(const Product& a, uint32_t t, int32_t& ti, int32_t& tj)
 {
     if (a.lower) {
-        constexpr int per = TI / kTileJ;
-        const int64_t pair = t / per;
-        int32_t r = (int32_t)((sqrtf(8.f * (float)pair + 1.f) - 1.f) * 0.5f);
-        while ((int64_t)r * (r + 1) / 2 > pair) --r;
-        while ((int64_t)(r + 1) * (r + 2) / 2 <= pair) ++r;
-        ti = r;
-        tj = (int32_t)(t - (int64_t)r * (r + 1) / 2 * per);
+        constexpr uint32_t per = TI / tile_columns(TI);
+        const uint32_t pair = t / per;
+        uint32_t r = (uint32_t)((sqrtf(8.f * (float)pair + 1.f) - 1.f) * 0.5f);
+        while ((uint64_t)r * (r + 1) / 2 > pair) --r;
+        while ((uint64_t)(r + 1) * (r + 2) / 2 <= pair) ++r;
+        ti = (int32_t)r;
+        tj = (int32_t)(t - (uint32_t)((uint64_t)r * (r + 1) / 2) * per);
     } else {
         // bands of 8 rows of tiles, column by column
-        const int64_t band = t / (8 * (int64_t)a.tiles_j) * 8;
-        const int64_t h = min((int64_t)8, a.tiles_i - band), in = t - band * a.tiles_j;
+        const uint32_t wide = (uint32_t)a.tiles_j, band = t / (8 * wide) * 8;
+        const uint32_t h = min(8u, (uint32_t)a.tiles_i - band), in = t - band * wide;
         ti = (int32_t)(band + in % h);
         tj = (int32_t)(in / h);
     }
@@ -285,19 +288,20 @@ __global__ __launch_bounds__(kProductThreads, is_f32<T> ? 1 : 2) void ff_orthogo
 {
     constexpr bool SPLIT = is_f32<T>;
     using S = Shape<TI, SPLIT>;
-    constexpr int FI = S::FI, FJ = S::FJ, kStages = S::kStages, kHalves = S::kHalves;
+    constexpr int FI = S::FI, FJ = S::FJ, TJ = S::TJ, kStages = S::kStages, kHalves = S::kHalves;
     __shared__ __align__(16) unsigned char smem[S::kLds];
     const int t = threadIdx.x, lane = t & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wi = wave & 1, wj = wave >> 1;
-    const int64_t tiles = product_tiles(a), item = xcd_item(blockIdx.x, tiles * a.splits);
-    if (item < 0) return;
-    const int32_t split = __builtin_amdgcn_readfirstlane((int32_t)(item % a.splits));
+    const uint32_t item = xcd_item32(blockIdx.x, a.items);
+    if (item == ~0u) return;
+    const uint32_t tile = a.splits == 1 ? item : item / (uint32_t)a.splits;
+    const int32_t split = __builtin_amdgcn_readfirstlane((int32_t)(item - tile * (uint32_t)a.splits));
     int32_t ti, tj;
-    tile_place<TI>(a, item / a.splits, ti, tj);
-    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * kTileJ;
-    const int32_t from = (int32_t)((int64_t)a.steps * split / a.splits);
-    const int32_t all = (int32_t)((int64_t)a.steps * (split + 1) / a.splits) - from;
+    tile_place<TI>(a, tile, ti, tj);
+    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * TJ;
+    // (at most 2^15 steps and 8 shares)
+    const int32_t from = a.steps * split / a.splits, all = a.steps * (split + 1) / a.splits - from;
     const uint32_t lds0 = lds_address(smem);
 
     // This lane's bytes of the blocks that the wave loads.
@@ -312,11 +316,11 @@ __global__ __launch_bounds__(kProductThreads, is_f32<T> ? 1 : 2) void ff_orthogo
 #pragma unroll
     for (int u = 0; u < kPerJ; ++u) {
         const int b = wave * kPerJ + u;
-        q_lane[u] = ACROSS ? (uint32_t)(b / (kTileJ / 32)) * across_q + (uint32_t)(b % (kTileJ / 32)) * 1024u + in_across
+        q_lane[u] = ACROSS ? (uint32_t)(b / (TJ / 32)) * across_q + (uint32_t)(b % (TJ / 32)) * 1024u + in_across
                            : (uint32_t)b * across_q + in_row;
     }
     const uint32_t p_bytes = (uint32_t)(TI / 16) * across_p;
-    const uint32_t q_bytes = (uint32_t)((ACROSS ? kDeepK : kTileJ) / 16) * across_q;
+    const uint32_t q_bytes = (uint32_t)((ACROSS ? kDeepK : TJ) / 16) * across_q;
 
     // the loads of step n into stage `stage`: of either half p's and q's
     constexpr int kLoads = kHalves * (kPerI + kPerJ);
@@ -354,7 +358,7 @@ __global__ __launch_bounds__(kProductThreads, is_f32<T> ? 1 : 2) void ff_orthogo
             if constexpr (ACROSS) {
                 // rows 8 g .. + 7 of the step, 8 bytes (four columns) a lane
                 const int r = 8 * (g & 1) + (li >> 2), c = (2 * (j & 1) + ((li & 3) >> 1)) ^ across_swizzle(r);
-                const unsigned char* q = Q + ((g >> 1) * (kTileJ / 32) + 2 * wj + j / 2) * 1024 + r * 64 + c * 16 + 8 * (li & 1);
+                const unsigned char* q = Q + ((g >> 1) * (TJ / 32) + wj * (FJ / 2) + j / 2) * 1024 + r * 64 + c * 16 + 8 * (li & 1);
                 const u32x2_t lo = read_across(q), hi = read_across(q + 4 * 64);
                 y[j] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
             } else {
@@ -403,10 +407,10 @@ __global__ __launch_bounds__(kProductThreads, is_f32<T> ? 1 : 2) void ff_orthogo
     }
 
     // a lane has columns 4 g .. + 3 of row li of every tile of 16 x 16
-    static_assert(FJ == 4 && FI % 2 == 0);
+    static_assert(FJ % 2 == 0 && FI % 2 == 0);
     const int64_t iw = i0 + wi * S::kWaveI, jw = j0 + wj * S::kWaveJ;
     if constexpr (PURPOSE == kPart) {
-        float4_t* part = reinterpret_cast<float4_t*>(a.part) + (item * (TI * kTileJ / 256) + wave * (FI * FJ)) * 64 + lane;
+        float4_t* part = reinterpret_cast<float4_t*>(a.part) + ((int64_t)item * (TI * TJ / 256) + wave * (FI * FJ)) * 64 + lane;
 #pragma unroll
         for (int i = 0; i < FI; ++i)
 #pragma unroll
@@ -421,7 +425,7 @@ __global__ __launch_bounds__(kProductThreads, is_f32<T> ? 1 : 2) void ff_orthogo
                 float v[2][8];
                 pair_up(acc[i][j], acc[i][j + 1], v[0]);
                 pair_up(acc[i + 1][j], acc[i + 1][j + 1], v[1]);
-                finish_symmetric<T, PURPOSE>(f, v, iw + 16 * i, jw + 16 * j, li, g, j0 + kTileJ <= i0, turn);
+                finish_symmetric<T, PURPOSE>(f, v, iw + 16 * i, jw + 16 * j, li, g, j0 + TJ <= i0, turn);
             }
     } else {
 #pragma unroll
@@ -440,31 +444,31 @@ template <typename T, int TI, int PURPOSE>
 __global__ __launch_bounds__(256) void ff_orthogonal_join_kernel(const Product a, const Finish<T> f)
 {
     using S = Shape<TI, is_f32<T>>;
-    constexpr int FI = S::FI, FJ = S::FJ, kPieces = TI * kTileJ / 4096;  // workgroups of a tile
+    constexpr int FI = S::FI, FJ = S::FJ, TJ = S::TJ, kPieces = TI * TJ / 4096;  // workgroups of a tile
     __shared__ __align__(16) _Float16 turn[4][2048];
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t tile = blockIdx.x / kPieces;
+    const uint32_t tile = blockIdx.x / kPieces;
     // the product's wave, and its tiles (i, j) to (i + 1, j + 1)
     const int piece = (int)(blockIdx.x % kPieces) * 4 + wave, of = piece / (FI * FJ / 4);
     const int i = piece % (FI * FJ / 4) / (FJ / 2) * 2, j = piece % (FJ / 2) * 2;
     int32_t ti, tj;
     tile_place<TI>(a, tile, ti, tj);
-    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * kTileJ;
+    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * TJ;
     const float4_t* part =
-        reinterpret_cast<const float4_t*>(a.part) + (tile * a.splits * (TI * kTileJ / 256) + of * (FI * FJ)) * 64 + lane;
+        reinterpret_cast<const float4_t*>(a.part) + ((int64_t)tile * a.splits * (TI * TJ / 256) + of * (FI * FJ)) * 64 + lane;
     float4_t v[2][2] = {};
     for (int32_t s = 0; s < a.splits; ++s)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int w = 0; w < 2; ++w)
-                v[u][w] += part[(s * (int64_t)(TI * kTileJ / 256) + (i + u) * FJ + j + w) * 64];
+                v[u][w] += part[(s * (int64_t)(TI * TJ / 256) + (i + u) * FJ + j + w) * 64];
     float e[2][8];
     pair_up(v[0][0], v[0][1], e[0]);
     pair_up(v[1][0], v[1][1], e[1]);
     finish_symmetric<T, PURPOSE>(f, e, i0 + (of & 1) * S::kWaveI + 16 * i, j0 + (of >> 1) * S::kWaveJ + 16 * j, li, g,
-                                 j0 + kTileJ <= i0, turn[wave]);
+                                 j0 + TJ <= i0, turn[wave]);
 }
 
 // Sums of squares of the stored values inside the weight, a share of the blocks each.
@@ -510,9 +514,12 @@ __global__ __launch_bounds__(256) void ff_orthogonal_start_kernel(const Finish<T
     const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) + eps;
     // an update of zeros stays one
     const double by = norm == 0.0 ? 0.0 : (double)kHeld / norm;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + t; e < rows * f.ld / 8; e += (int64_t)gridDim.x * 256) {
-        const int64_t block = e / 64, per = f.ld / 32;
-        const int64_t i = block / per * 16 + e % 64 / 4, j = block % per * 32 + e % 4 * 8;
+    // a wave per block (less than 2^31 of them: they have 1 KB each)
+    const int lane = t & 63;
+    const uint32_t per = (uint32_t)(f.ld / 32), blocks = (uint32_t)(rows / 16) * per;
+    for (uint32_t block = blockIdx.x * 4 + (uint32_t)(t >> 6); block < blocks; block += gridDim.x * 4) {
+        const uint32_t br = block / per;
+        const int64_t e = (int64_t)block * 64 + lane, i = (int64_t)br * 16 + lane / 4, j = (int64_t)(block - br * per) * 32 + lane % 4 * 8;
         const int64_t r = f.transposed ? j : i, c = f.transposed ? i : j;
         const int32_t b = block_at(f, (int32_t)(r / 16), (int32_t)(c / 16));
         Pack<_Float16, 8> hi{}, lo{};
@@ -545,11 +552,15 @@ OrthogonalPlan orthogonal_plan(const BlockIndex& w, int64_t size)
     p.transposed = w.M > w.K;
     p.split = size == 4;
     const int64_t rows = p.transposed ? w.K : w.M, columns = p.transposed ? w.M : w.K;
-    // one tile of 128 x 128 a CU at most, or larger ones that are faster where there are many
-    p.tile = (rows + 127) / 128 * ((columns + 127) / 128) <= 256 ? 128 : 256;
+    // The largest tiles of which there are enough: a CU gets no more than 25 GB/s of what
+    // other dies have written, and few workgroups wait for that (1792 x 512: 195 us by 128,
+    // NN by 64), while small tiles read their operands more often.
+    auto count = [&](int64_t side) { return (rows + side - 1) / side * ((columns + side - 1) / side); };
+    p.tile = count(64) <= 256 ? 64 : count(128) <= 256 ? 128 : 256;
+    const int64_t tj = tile_columns(p.tile);
     p.m = (rows + p.tile - 1) / p.tile * p.tile;
-    p.k = (columns + kTileJ - 1) / kTileJ * kTileJ;
-    const int64_t n = p.m / p.tile, tiles = n * (n + 1) / 2 * (p.tile / kTileJ);
+    p.k = (columns + tj - 1) / tj * tj;
+    const int64_t n = p.m / p.tile, tiles = n * (n + 1) / 2 * (p.tile / tj);
     // Shares of a sum: rounds of workgroups, two a CU (one where operands are split, whose
     // steps take three times as long), and what a launch and joining cost, in steps' time.
     const int64_t at_once = p.split ? 256 : 512;
@@ -582,21 +593,22 @@ OrthogonalPlan orthogonal_plan(const BlockIndex& w, int64_t size)
     p.diagonal = c.take((size_t)p.m * 4);
     p.norm = c.take(kNormShares * 8);
     const int most = p.gram_splits > p.square_splits ? p.gram_splits : p.square_splits;
-    p.part = c.take(most > 1 ? (size_t)(tiles * most) * p.tile * kTileJ * 4 : 0);
+    p.part = c.take(most > 1 ? (size_t)(tiles * most * p.tile * tj) * 4 : 0);
     p.end = c.end;
     return p;
 }
 
 template <typename T, int TI, bool ACROSS, int PURPOSE>
-void launch_orthogonal(const Product& a, const Finish<T>& f, hipStream_t s)
+void launch_orthogonal(Product a, const Finish<T>& f, hipStream_t s)
 {
     const int64_t tiles = product_tiles(a);
     constexpr int threads = kProductThreads;
     const dim3 grid = launch_grid(kXcds * xcd_chunk(tiles * a.splits), threads);
+    a.items = (uint32_t)(tiles * a.splits);
     if (a.splits > 1) {
         if constexpr (!ACROSS) {
             hipLaunchKernelGGL((ff_orthogonal_product_kernel<T, TI, ACROSS, kPart>), grid, dim3(threads), 0, s, a, f);
-            hipLaunchKernelGGL((ff_orthogonal_join_kernel<T, TI, PURPOSE>), launch_grid(tiles * (TI * kTileJ / 4096), 256),
+            hipLaunchKernelGGL((ff_orthogonal_join_kernel<T, TI, PURPOSE>), launch_grid(tiles * (TI * tile_columns(TI) / 4096), 256),
                                dim3(256), 0, s, a, f);
         }
     } else {
@@ -641,7 +653,7 @@ void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const Orthog
         a.p = a.q = from;
         a.p_ld = a.q_ld = p.k;
         a.tiles_i = (int32_t)(p.m / TI);
-        a.tiles_j = (int32_t)(p.m / kTileJ);
+        a.tiles_j = (int32_t)(p.m / tile_columns(TI));
         a.steps = (int32_t)(p.k / kDeepK);
         a.splits = p.gram_splits;
         a.lower = true;
@@ -658,7 +670,7 @@ void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const Orthog
         a.p = B;
         a.q = from;
         a.q_ld = p.k;
-        a.tiles_j = (int32_t)(p.k / kTileJ);
+        a.tiles_j = (int32_t)(p.k / tile_columns(TI));
         a.splits = 1;
         a.lower = false;
         f.x = from;
@@ -686,6 +698,8 @@ void orthogonalize(const BlockIndex& w, const T* update, T* out, const Orthogona
     const ff::OrthogonalPlan p = ff::orthogonal_plan(w, sizeof(T));
     if (p.tile == 256)
         ff::orthogonal_steps<T, 256>(w, update, out, o, p, static_cast<char*>(scratch), s);
+    else if (p.tile == 64)
+        ff::orthogonal_steps<T, 64>(w, update, out, o, p, static_cast<char*>(scratch), s);
     else
         ff::orthogonal_steps<T, 128>(w, update, out, o, p, static_cast<char*>(scratch), s);
 }
