@@ -247,9 +247,16 @@ bool int8_tiles(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStr
     const int rows = weights == 2 ? ff::kI8Slots / 2 : ff::kI8Slots;
     const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + ff::kI8Wide - 1) / ff::kI8Wide);
     if (!a.side[0].map || (weights == 2 && !a.side[1].map)) return false;
-    if (a.vals_bytes[0] == 0 || (weights == 2 && a.vals_bytes[1] == 0)) return false;
-    if (a.N > (1 << 21) || a.N < 128 || items < 64) return false;
-    if (blocks * 8 < (int64_t)weights * a.block_rows * a.in_blocks) return false;
+    if (a.vals_bytes[0] == 0 || (weights == 2 && a.vals_bytes[1] == 0) || a.N > (1 << 21)) return false;
+    // us of a step of four block-columns by tiles (rounds of two workgroups a CU, a last one
+    // of one), whose loads take most of it whatever is stored, against the walk's by stored
+    // blocks: 14336 x 4096 and 2048 tokens 95 and 117 us at 25 % stored, 83 and 68 at 10 %,
+    // 4096 x 14336 and 512 tokens 122 and 107 with all stored.
+    const double share = (double)blocks / ((double)weights * a.block_rows * a.in_blocks);
+    const int64_t whole = items / 512, rest = items % 512;
+    const double full = 0.6 + 0.3 * share, last = rest == 0 ? 0.0 : rest <= 256 ? 0.42 + 0.2 * share : full;
+    const double tiles = 4.0 + (double)((a.in_blocks + 3) / 4) * ((double)whole * full + last);
+    if (tiles > 0.9e-6 * (double)blocks * (double)a.N) return false;
     const dim3 grid = launch_grid(ff::kXcds * ff::xcd_chunk(items), ff::kI8Threads);
     if (weights == 2)
         hipLaunchKernelGGL((ff::ff_int8_tile_kernel<T, true>), grid, dim3(ff::kI8Threads), 0, s, a);

@@ -481,6 +481,7 @@ __global__ __launch_bounds__(256) void ff_square_sum_kernel(const T* __restrict_
     __shared__ double red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double sum = 0.0;
+#pragma unroll 4
     for (int64_t b = blockIdx.x * 4 + wave; b < nnzb; b += 4 * kNormShares) {
         const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(u + b * 256 + 4 * lane);
         const int32_t r = 16 * row[b] + lane / 4, c = 16 * col[b] + 4 * (lane & 3);
@@ -553,10 +554,12 @@ OrthogonalPlan orthogonal_plan(const BlockIndex& w, int64_t size)
     p.split = size == 4;
     const int64_t rows = p.transposed ? w.K : w.M, columns = p.transposed ? w.M : w.K;
     // The largest tiles of which there are enough: a CU gets no more than 25 GB/s of what
-    // other dies have written, and few workgroups wait for that (1792 x 512: 195 us by 128,
-    // NN by 64), while small tiles read their operands more often.
+    // other dies have just written, and few workgroups wait for that, while small tiles read
+    // their operands more often.  us by 64 and 128 rows: bf16 512 x 1792 137 and 195, 1000 x
+    // 2500 227 and 275, 2048 x 2048 434 and 452, fp32 1000 x 2500 334 and 362; by 128 and
+    // 256: bf16 1536 x 4096 410 and 440, 2048 x 5632 706 and 661, fp32 1536 x 4096 757 and 726.
     auto count = [&](int64_t side) { return (rows + side - 1) / side * ((columns + side - 1) / side); };
-    p.tile = count(64) <= 256 ? 64 : count(128) <= 256 ? 128 : 256;
+    p.tile = count(64) <= 1024 ? 64 : count(128) <= (p.split ? 256 : 512) ? 128 : 256;
     const int64_t tj = tile_columns(p.tile);
     p.m = (rows + p.tile - 1) / p.tile * p.tile;
     p.k = (columns + tj - 1) / tj * tj;
