@@ -343,7 +343,7 @@ void int8_product(const Int8Args<T>& f, int weights, hipStream_t s)
     a.block_rows = (int32_t)w.Mb;
     a.N = f.N;
     a.act = f.act;
-    if (!a.raw && int8_tiles<T>(a, weights, blocks, s)) return;
+    if (!a.raw && (int8_lists<T>(a, weights, blocks, s) || int8_tiles<T>(a, weights, blocks, s))) return;
     if (weights == 2)
         ff::launch_int8<T, 2>(a, blocks, s);
     else

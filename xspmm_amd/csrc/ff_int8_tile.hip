@@ -172,11 +172,9 @@ __global__ __launch_bounds__(kI8Threads, 2) void ff_int8_tile_kernel(const Int8P
     // eight tokens of a row per thread.  What the rest needs is in registers by then: the
     // scales of a lane's tokens, and of a wave's rows one row (16 s + r) per lane.
     constexpr int kSides = GATED ? 2 : 1, kResults = kI8Rows / kSides;
-    const int c = 8 * li;
-    const int64_t n = n0 + c;
     float xs[8], rs[kSides], bias[kSides];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) xs[q] = a.x_scale[min(n + q, a.N - 1)];
+    for (int q = 0; q < 8; ++q) xs[q] = a.x_scale[min((int64_t)n0 + 8 * li + q, a.N - 1)];
     {
         const int64_t row = min(16 * (int64_t)slot_row(lane / 16 % kResults) + li, (int64_t)a.rows - 1);
 #pragma unroll
@@ -197,44 +195,7 @@ __global__ __launch_bounds__(kI8Threads, 2) void ff_int8_tile_kernel(const Int8P
                 for (int q = 0; q < 4; ++q)
                     O[(l * 16 + 4 * g + q) * kI8OutRow + 16 * j + li] = (float)acc[l * kResults + s][j][q];
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int v = 0; v < 4; ++v) {
-            const int r = 4 * v + g;
-            const int64_t row = 16 * (int64_t)slot_row(s) + r;
-            float z[kSides][8];
-#pragma unroll
-            for (int l = 0; l < kSides; ++l) {
-                const float4_t lo = *reinterpret_cast<const float4_t*>(O + (l * 16 + r) * kI8OutRow + c);
-                const float4_t hi = *reinterpret_cast<const float4_t*>(O + (l * 16 + r) * kI8OutRow + c + 4);
-                const float scale = __shfl(rs[l], 16 * s + r), add = __shfl(bias[l], 16 * s + r);
-#pragma unroll
-                for (int q = 0; q < 8; ++q) z[l][q] = (q < 4 ? lo[q] : hi[q - 4]) * scale * xs[q] + add;
-            }
-            if (row >= a.rows || n >= a.N) continue;
-            with_act(a.act, [&](auto act) {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) z[0][q] = finish_act<T, decltype(act)::value>(z[0][q]);
-            });
-            if constexpr (GATED)
-#pragma unroll
-                for (int q = 0; q < 8; ++q) z[0][q] *= z[1][q];
-            const int64_t at = row * a.N + n;
-            if (n + 8 <= a.N) {
-                if (a.residual) {
-                    const Pack<T, 8> k = *reinterpret_cast<const Pack<T, 8>*>(a.residual + at);
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) z[0][q] += (float)k.v[q];
-                }
-                Pack<T, 8> k;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) k.v[q] = (T)z[0][q];
-                *reinterpret_cast<Pack<T, 8>*>(a.y + at) = k;
-            } else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (n + q < a.N) a.y[at + q] = (T)(z[0][q] + (a.residual ? (float)a.residual[at + q] : 0.f));
-            }
-        }
+        int8_rows<T, kSides, kI8Wide>(a, O, 16 * (int64_t)slot_row(s), n0, xs, rs, bias, 16 * s);
         __builtin_amdgcn_wave_barrier();
     }
 }

@@ -221,7 +221,62 @@ __device__ __forceinline__ float int8_finish(const Int8Product<T>& a, const int 
     return z[0];
 }
 
+// Sixteen rows of a product and WIDE tokens, whose sums a wave has left in O (rows of
+// WIDE + 4 floats, SIDES times 16 of them): eight tokens of a row a thread.  xs: the scales
+// of the thread's tokens; lane `shift` + r has row r's scale and bias.
+template <typename T, int SIDES, int WIDE>
+__device__ __forceinline__ void int8_rows(const Int8Product<T>& a, const float* O, int64_t row0, int64_t n0,
+                                          const float (&xs)[8], const float (&rs)[SIDES], const float (&bias)[SIDES],
+                                          int shift)
+{
+    constexpr int kLanes = WIDE / 8, kAtOnce = 64 / kLanes, kRow = WIDE + 4;
+    const int lane = threadIdx.x & 63, c = lane % kLanes * 8;
+    const int64_t n = n0 + c;
+#pragma unroll 1
+    for (int v = 0; v < 16 / kAtOnce; ++v) {
+        const int r = kAtOnce * v + lane / kLanes;
+        const int64_t row = row0 + r;
+        float z[SIDES][8];
+#pragma unroll
+        for (int l = 0; l < SIDES; ++l) {
+            const float4_t lo = *reinterpret_cast<const float4_t*>(O + (l * 16 + r) * kRow + c);
+            const float4_t hi = *reinterpret_cast<const float4_t*>(O + (l * 16 + r) * kRow + c + 4);
+            const float scale = __shfl(rs[l], shift + r), add = __shfl(bias[l], shift + r);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) z[l][q] = (q < 4 ? lo[q] : hi[q - 4]) * scale * xs[q] + add;
+        }
+        if (row >= a.rows || n >= a.N) continue;
+        with_act(a.act, [&](auto act) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) z[0][q] = finish_act<T, decltype(act)::value>(z[0][q]);
+        });
+        if constexpr (SIDES == 2)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) z[0][q] *= z[1][q];
+        const int64_t at = row * a.N + n;
+        if (n + 8 <= a.N) {
+            if (a.residual) {
+                const Pack<T, 8> k = *reinterpret_cast<const Pack<T, 8>*>(a.residual + at);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) z[0][q] += (float)k.v[q];
+            }
+            Pack<T, 8> k;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) k.v[q] = (T)z[0][q];
+            *reinterpret_cast<Pack<T, 8>*>(a.y + at) = k;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (n + q < a.N) a.y[at + q] = (T)(z[0][q] + (a.residual ? (float)a.residual[at + q] : 0.f));
+        }
+    }
+}
+
 }  // namespace ff
+
+// The product by lists of blocks and x in LDS: false where that does not apply or pay.
+template <typename T>
+bool int8_lists(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s);
 
 // The product by tiles: false where that does not apply or pay.
 template <typename T>
