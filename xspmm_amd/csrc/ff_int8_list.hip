@@ -3,12 +3,18 @@
 // walks what is stored of a block-row in a window, four blocks at a time wherever their
 // columns are, so that all that is loaded and multiplied is stored.
 //
-// A workgroup of four waves takes 32 block-rows (gated: 16 of either weight) and 64
+// A workgroup of eight waves takes 32 block-rows (gated: 16 of either weight) and 64
 // tokens; a window is 32 block-columns (32 KB of x), two in turn, two workgroups a CU.
-// A wave lists its eight block-rows' blocks a window ahead: a lane looks at four entries of
+// A wave lists its four block-rows' blocks a window ahead: a lane looks at two entries of
 // the weight's map, and the lists are what is stored, pushed together.  Of every row the
-// first 4 Q blocks are fetched, four rows ahead, and multiplied without a question (zeros
+// first 4 Q blocks are fetched, two rows ahead, and multiplied without a question (zeros
 // where there are fewer); more than that is rare and fetched when it is met.
+//
+// What bounds it is latency, of a window's x, lists and first blocks one after the other
+// (at 5 % stored a window takes 2 us, its instructions a quarter of that): waves of eight
+// block-rows with twice the registers, two a SIMD, take 163 us for gate and up of 14336 x
+// 4096, 2048 tokens, 25 % stored, bf16; of four, four a SIMD, 147.  One product 76 (by
+// tiles 95, by the walk 117), 10 % stored 56 (83, 68).
 #include "int8_device.hpp"
 
 namespace xspmm {
@@ -17,19 +23,20 @@ namespace ff {
 
 constexpr int kListWide = 64;  // tokens of a workgroup
 constexpr int kListTiles = kListWide / 16;
-constexpr int kListWaves = 4, kListThreads = 64 * kListWaves;
-constexpr int kListRows = 8;     // a wave's block-rows, of both weights
+constexpr int kListWaves = 8, kListThreads = 64 * kListWaves;
+constexpr int kListRows = 4;     // a wave's block-rows, of both weights
 constexpr int kListSlots = kListRows * kListWaves;
 constexpr int kListWindow = 32;  // block-columns
 constexpr int kListStage = kListWindow * kListWide * 16;
-constexpr int kListAhead = 4;    // rows whose blocks are on their way
+constexpr int kListAhead = 2;    // rows whose blocks are on their way
+constexpr int kListLanes = 64 / kListRows, kListColumns = kListWindow / kListLanes;  // of a row's list
 constexpr int kListOut = 2 * 16 * (kListWide + 4) * 4;  // a wave's bytes on their way out
 constexpr int kListLds = 2 * kListStage + 2 * kListSlots * kListWindow * 4;
 constexpr int kListBand = 8;
 static_assert(kListLds <= 80 * 1024 && kListWaves * kListOut <= kListLds);
 
 template <typename T, bool GATED, int Q>
-__global__ __launch_bounds__(kListThreads, 2) void ff_int8_list_kernel(const Int8Product<T> a)
+__global__ __launch_bounds__(kListThreads, 4) void ff_int8_list_kernel(const Int8Product<T> a)
 {
     constexpr int kSides = GATED ? 2 : 1, kResults = kListRows / kSides;
     constexpr int kOutRows = kListSlots / kSides;  // block-rows of the result
@@ -69,27 +76,31 @@ __global__ __launch_bounds__(kListThreads, 2) void ff_int8_list_kernel(const Int
     // Lists of this wave's rows, two windows in turn: 256 times a block's position plus its
     // column in the window, or kNone.
     uint32_t* const lists = reinterpret_cast<uint32_t*>(smem + 2 * kListStage) + wave * (2 * kListRows * kListWindow);
-    const int mine = lane / 8;  // the row that this lane looks at, four columns of it
+    const int mine = lane / kListLanes, at_c = lane % kListLanes * kListColumns;  // what this lane looks at
     const int32_t my_row = br0 + wave * kResults + mine % kResults;
     const int32_t* const my_map =
         a.side[mine / kResults].map + (int64_t)(my_row < a.block_rows ? my_row : 0) * a.in_blocks;
-    auto look = [&](int32_t c0, int32_t (&p)[4]) {
+    auto look = [&](int32_t c0, int32_t (&p)[kListColumns]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int32_t c = c0 + 4 * (lane & 7) + j;
+        for (int j = 0; j < kListColumns; ++j) {
+            const int32_t c = c0 + at_c + j;
             p[j] = my_row < a.block_rows && c < a.in_blocks ? my_map[c] : -1;
         }
     };
     // fours: of every row how many fours of blocks it has, 4 bits each
-    auto list = [&](uint32_t* to, const int32_t (&p)[4]) -> uint32_t {
-        *reinterpret_cast<u32x4_t*>(to + 4 * lane) = u32x4_t{kNone, kNone, kNone, kNone};
-        int at = mine * kListWindow;
-        uint64_t there[4];
+    auto list = [&](uint32_t* to, const int32_t (&p)[kListColumns]) -> uint32_t {
+        constexpr int kEach = kListRows * kListWindow / 64;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kEach; ++j) to[kEach * lane + j] = kNone;
+        constexpr uint32_t kRow = (uint32_t)((1ull << kListLanes) - 1);
+        int at = mine * kListWindow;
+        uint64_t there[kListColumns];
+#pragma unroll
+        for (int j = 0; j < kListColumns; ++j) {
             there[j] = __ballot(p[j] >= 0);
-            const uint32_t row = (uint32_t)(there[j] >> (8 * mine)) & 0xffu;
-            if (p[j] >= 0) to[at + __popc(row & ((1u << (lane & 7)) - 1u))] = (uint32_t)p[j] * 256u + (uint32_t)(4 * (lane & 7) + j);
+            const uint32_t row = (uint32_t)(there[j] >> (kListLanes * mine)) & kRow;
+            if (p[j] >= 0)
+                to[at + __popc(row & ((1u << (lane % kListLanes)) - 1u))] = (uint32_t)p[j] * 256u + (uint32_t)(at_c + j);
             at += __popc(row);
         }
         uint32_t fours = 0;
@@ -97,7 +108,7 @@ __global__ __launch_bounds__(kListThreads, 2) void ff_int8_list_kernel(const Int
         for (int s = 0; s < kListRows; ++s) {
             uint32_t n = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) n += (uint32_t)__popc((uint32_t)(there[j] >> (8 * s)) & 0xffu);
+            for (int j = 0; j < kListColumns; ++j) n += (uint32_t)__popc((uint32_t)(there[j] >> (kListLanes * s)) & kRow);
             fours |= (n + 3) / 4 << (4 * s);
         }
         return (uint32_t)__builtin_amdgcn_readfirstlane((int)fours);
@@ -126,7 +137,7 @@ __global__ __launch_bounds__(kListThreads, 2) void ff_int8_list_kernel(const Int
     constexpr int kList = kListRows * kListWindow;
     u32x4_t w[kListAhead][Q];
     uint32_t e[kListAhead][Q], following[Q];
-    int32_t seen[4];
+    int32_t seen[kListColumns];
     look(0, seen);
     issue(0, 0);
     uint32_t fours = list(lists, seen);
@@ -172,11 +183,12 @@ __global__ __launch_bounds__(kListThreads, 2) void ff_int8_list_kernel(const Int
     }
 
     // the sums leave through LDS, as in the tiles
-    float xs[8], rs[kResults / 4][kSides], bias[kResults / 4][kSides];
+    constexpr int kFour = (kResults + 3) / 4;
+    float xs[8], rs[kFour][kSides], bias[kFour][kSides];
 #pragma unroll
     for (int q = 0; q < 8; ++q) xs[q] = a.x_scale[min((int64_t)n0 + 8 * (lane & 7) + q, a.N - 1)];
 #pragma unroll
-    for (int h = 0; h < kResults / 4; ++h) {
+    for (int h = 0; h < kFour; ++h) {
         const int64_t row = min(16 * (int64_t)slot_row(4 * h + lane / 16) + li, (int64_t)a.rows - 1);
 #pragma unroll
         for (int l = 0; l < kSides; ++l) {
@@ -214,27 +226,41 @@ void launch_list(const Int8Product<T>& a, int weights, int64_t items, hipStream_
 
 }  // namespace ff
 
+// us, measured at 14336 x 4096, 4096 x 14336 and 2048 x 2048 with 64 to 2048 tokens and 5 to
+// 40 % stored (within a tenth): a window's loads, one after the other, and its blocks, in
+// rounds of two workgroups a CU, a last one of one.
 template <typename T>
-bool int8_lists(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s)
+double int8_lists_us(const ff::Int8Product<T>& a, int weights, int64_t blocks)
+{
+    if (!a.side[0].map || (weights == 2 && !a.side[1].map) || a.N > (1 << 21)) return 1e30;
+    if (a.vals_bytes[0] == 0 || (weights == 2 && a.vals_bytes[1] == 0)) return 1e30;
+    const int rows = ff::kListSlots / weights;
+    const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + ff::kListWide - 1) / ff::kListWide);
+    const double share = (double)blocks / ((double)weights * a.block_rows * a.in_blocks);
+    const int64_t rest = items % 512;
+    const double full = 2.7 + 7.5 * share, last = rest == 0 ? 0.0 : rest <= 256 ? 1.75 + 5.5 * share : full;
+    const int64_t windows = (a.in_blocks + ff::kListWindow - 1) / ff::kListWindow;
+    return 6.0 + (double)windows * ((double)(items / 512) * full + last);
+}
+
+template <typename T>
+void int8_lists(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s)
 {
     const int rows = ff::kListSlots / weights;
     const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + ff::kListWide - 1) / ff::kListWide);
-    if (!a.side[0].map || (weights == 2 && !a.side[1].map)) return false;
-    if (a.vals_bytes[0] == 0 || (weights == 2 && a.vals_bytes[1] == 0) || a.N > (1 << 21)) return false;
-    if (a.N < 64) return false;
+    // so that four times Q blocks are more than a row has in most windows
     const double share = (double)blocks / ((double)weights * a.block_rows * a.in_blocks);
     if (share < 0.06)
         ff::launch_list<T, 1>(a, weights, items, s);
     else if (share < 0.15)
         ff::launch_list<T, 2>(a, weights, items, s);
-    else if (share < 0.5)
-        ff::launch_list<T, 3>(a, weights, items, s);
     else
-        return false;
-    return true;
+        ff::launch_list<T, 3>(a, weights, items, s);
 }
 
-#define XSPMM_INT8_LIST(T) template bool int8_lists<T>(const ff::Int8Product<T>&, int, int64_t, hipStream_t);
+#define XSPMM_INT8_LIST(T)                                                       \
+    template double int8_lists_us<T>(const ff::Int8Product<T>&, int, int64_t);     \
+    template void int8_lists<T>(const ff::Int8Product<T>&, int, int64_t, hipStream_t);
 XSPMM_INT8_LIST(float)
 XSPMM_INT8_LIST(_Float16)
 XSPMM_INT8_LIST(__bf16)

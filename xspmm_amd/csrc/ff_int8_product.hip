@@ -343,7 +343,23 @@ void int8_product(const Int8Args<T>& f, int weights, hipStream_t s)
     a.block_rows = (int32_t)w.Mb;
     a.N = f.N;
     a.act = f.act;
-    if (!a.raw && (int8_lists<T>(a, weights, blocks, s) || int8_tiles<T>(a, weights, blocks, s))) return;
+    if (!a.raw) {
+        // The walk by blocks, whose x comes through L1, and results: 14336 x 4096 and 2048
+        // tokens 48 us at 5 % stored, 117 at 25 %, 370 with all.  The others have a chain of
+        // loads for every window of x: they pay where there are tokens enough, lists up to
+        // some 45 % stored (90 us at 40 %, tiles 103), tiles from there on (119; lists
+        // of 4096 x 14336 114 at 40 %, tiles 118).
+        const double walk = 5.0 + 7.4e-7 * (double)blocks * (double)a.N + 7e-7 * (double)weights * (double)w.M * (double)a.N;
+        const double lists = int8_lists_us<T>(a, weights, blocks), tiles = int8_tiles_us<T>(a, weights, blocks);
+        if (lists < walk && lists <= tiles) {
+            int8_lists<T>(a, weights, blocks, s);
+            return;
+        }
+        if (tiles < walk) {
+            int8_tiles<T>(a, weights, s);
+            return;
+        }
+    }
     if (weights == 2)
         ff::launch_int8<T, 2>(a, blocks, s);
     else

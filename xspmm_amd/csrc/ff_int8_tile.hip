@@ -1,13 +1,20 @@
-// ff_int8_tile.hip -- the products of ff_int8_product.hip where blocks are not rare and
-// tokens many: a workgroup of eight waves takes 32 block-rows (gated: 16 of the gate's and
-// the same ones of the up projection's) and 128 tokens.
+// ff_int8_tile.hip -- the products of ff_int8_product.hip where most blocks are stored and
+// tokens many: a workgroup of four waves takes 16 block-rows (gated: eight of the gate's
+// and the same ones of the up projection's) and 128 tokens, two workgroups a CU.
 //
-// The tokens' features go straight from memory into LDS, a window of 32 block-columns
+// The tokens' features go straight from memory into LDS, a window of 16 block-columns
 // at a time, two in turn.  A wave owns four block-rows and walks the window by four
 // block-columns: a row's four blocks (absent ones are zeros and not read) make one
 // v_mfma_i32_16x16x64_i8 with each of the eight tiles of 16 tokens, if any of them is
 // stored.  A value of x is read from LDS once for four block-rows; a block is read
-// from memory by the one wave that needs it, two steps ahead, its position three.
+// from memory by the one wave that needs it, three steps ahead, its position two windows.
+//
+// 14336 x 4096, all stored, 2048 tokens, fp16, bias and gelu: 140 us, 1.7 Pop/s.  The
+// matrix units are busy for 57 us of that at the 2 GHz that the card then runs at; a
+// step's loads, 24 KB a workgroup through the 64 bytes a clock of a CU's L1, take three
+// quarters of the matrix instructions' time beside them, and the gelus and the results 25
+// us, of which the other workgroup hides a part (one workgroup of eight waves: 142 and,
+// with gate and up and 25 % stored, 204 instead of 187).
 #include "int8_device.hpp"
 
 namespace xspmm {
@@ -202,32 +209,37 @@ __global__ __launch_bounds__(kI8Threads, 2) void ff_int8_tile_kernel(const Int8P
 
 }  // namespace ff
 
+// us, as int8_lists_us: a step of four block-columns, whose loads take most of it whatever
+// is stored.
 template <typename T>
-bool int8_tiles(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s)
+double int8_tiles_us(const ff::Int8Product<T>& a, int weights, int64_t blocks)
 {
-    const int rows = weights == 2 ? ff::kI8Slots / 2 : ff::kI8Slots;
+    if (!a.side[0].map || (weights == 2 && !a.side[1].map) || a.N > (1 << 21)) return 1e30;
+    if (a.vals_bytes[0] == 0 || (weights == 2 && a.vals_bytes[1] == 0)) return 1e30;
+    const int rows = ff::kI8Slots / weights;
     const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + ff::kI8Wide - 1) / ff::kI8Wide);
-    if (!a.side[0].map || (weights == 2 && !a.side[1].map)) return false;
-    if (a.vals_bytes[0] == 0 || (weights == 2 && a.vals_bytes[1] == 0) || a.N > (1 << 21)) return false;
-    // us of a step of four block-columns by tiles (rounds of two workgroups a CU, a last one
-    // of one), whose loads take most of it whatever is stored, against the walk's by stored
-    // blocks: 14336 x 4096 and 2048 tokens 95 and 117 us at 25 % stored, 83 and 68 at 10 %,
-    // 4096 x 14336 and 512 tokens 122 and 107 with all stored.
     const double share = (double)blocks / ((double)weights * a.block_rows * a.in_blocks);
-    const int64_t whole = items / 512, rest = items % 512;
+    const int64_t rest = items % 512;
     const double full = 0.6 + 0.3 * share, last = rest == 0 ? 0.0 : rest <= 256 ? 0.42 + 0.2 * share : full;
-    const double tiles = 4.0 + (double)((a.in_blocks + 3) / 4) * ((double)whole * full + last);
-    if (tiles > 0.9e-6 * (double)blocks * (double)a.N) return false;
+    return 8.0 + (double)((a.in_blocks + 3) / 4) * ((double)(items / 512) * full + last);
+}
+
+template <typename T>
+void int8_tiles(const ff::Int8Product<T>& a, int weights, hipStream_t s)
+{
+    const int rows = ff::kI8Slots / weights;
+    const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + ff::kI8Wide - 1) / ff::kI8Wide);
     const dim3 grid = launch_grid(ff::kXcds * ff::xcd_chunk(items), ff::kI8Threads);
     if (weights == 2)
         hipLaunchKernelGGL((ff::ff_int8_tile_kernel<T, true>), grid, dim3(ff::kI8Threads), 0, s, a);
     else
         hipLaunchKernelGGL((ff::ff_int8_tile_kernel<T, false>), grid, dim3(ff::kI8Threads), 0, s, a);
     XSPMM_LAUNCH_CHECK();
-    return true;
 }
 
-#define XSPMM_INT8_TILE(T) template bool int8_tiles<T>(const ff::Int8Product<T>&, int, int64_t, hipStream_t);
+#define XSPMM_INT8_TILE(T)                                                       \
+    template double int8_tiles_us<T>(const ff::Int8Product<T>&, int, int64_t);     \
+    template void int8_tiles<T>(const ff::Int8Product<T>&, int, hipStream_t);
 XSPMM_INT8_TILE(float)
 XSPMM_INT8_TILE(_Float16)
 XSPMM_INT8_TILE(__bf16)

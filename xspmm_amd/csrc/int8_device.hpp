@@ -187,7 +187,7 @@ __device__ __forceinline__ int4_t mfma8(u32x4_t a, u32x4_t b, int4_t c)
 // An activation of a result in 16 bits: exponentials by the hardware's exp2, off by the
 // rounding of its argument (2^-24 of up to 185, 1e-5 of the value), and quotients by its
 // reciprocal: 2^-16 in all where the result's own rounding is 2^-11 at least.  With expf
-// and a division the epilogue of 14336 x 2048 gelus takes NN us longer.
+// and a division the epilogue of 14336 x 2048 gelus takes 10 us longer.
 __device__ __forceinline__ float exp_quick(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 template <typename T, int ACT>
 __device__ __forceinline__ float finish_act(float z)
@@ -274,13 +274,16 @@ __device__ __forceinline__ void int8_rows(const Int8Product<T>& a, const float* 
 
 }  // namespace ff
 
-// The product by lists of blocks and x in LDS: false where that does not apply or pay.
+// The product by lists of blocks, and by tiles, both with x in LDS: the time to expect (us;
+// past any other where it does not apply) and the launch.
 template <typename T>
-bool int8_lists(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s);
-
-// The product by tiles: false where that does not apply or pay.
+double int8_lists_us(const ff::Int8Product<T>& a, int weights, int64_t blocks);
 template <typename T>
-bool int8_tiles(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s);
+void int8_lists(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s);
+template <typename T>
+double int8_tiles_us(const ff::Int8Product<T>& a, int weights, int64_t blocks);
+template <typename T>
+void int8_tiles(const ff::Int8Product<T>& a, int weights, hipStream_t s);
 
 }  // namespace detail
 }  // namespace xspmm
