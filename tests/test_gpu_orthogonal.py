@@ -2,8 +2,8 @@
 
 The bound of a case comes from the arithmetic itself: the same formula in 64 bits with
 the operands of its products rounded as the operator states (fp16, or two fp16 halves
-each for fp32 updates, whose sums are then fp32) is off by some rms; another order of
-the same roundings is off by about as much, and twice that (four times in fp32, where
+each for fp16 and fp32 updates, whose sums are then fp32) is off by some rms; another order of
+the same roundings is off by about as much, and twice that (four times with halves, where
 the sums' order counts) is allowed, beside the result's own rounding.  A single
 element may be off by eight times the rms: a sum of thousands of independent roundings
 is near normal, and 8 deviations are past any number of elements here.  Roundings are
@@ -51,13 +51,13 @@ def rounded(U, kind, steps=5, abc=ABC, eps=1e-7):
     both = lambda t: hi(t) + hi(t - hi(t))
 
     def product(p, q):
-        if kind != "f32":
+        if kind == "bf16":
             return hi(p) @ hi(q)
         ph, qh = hi(p), hi(q)
         pl, ql = hi(p - ph), hi(q - qh)
         return (ph.float() @ qh.float() + ph.float() @ ql.float() + pl.float() @ qh.float()).double()
 
-    held = both if kind == "f32" else hi
+    held = hi if kind == "bf16" else both
     for _ in range(steps):
         x = both(x)
         s = held(product(x, x.t().contiguous()) / 4096)
@@ -76,7 +76,7 @@ def check(got, U, where, kind, **how):
     w, got = at_blocks(want, where), f64(got)
     assert got.shape == w.shape and torch.isfinite(got).all()
     # values below fp16's normal numbers round by up to 2^-25
-    allowed = (4 if kind == "f32" else 2) * rms(near - want) + u * rms(w) + 2.0 ** -25
+    allowed = (2 if kind == "bf16" else 4) * rms(near - want) + u * rms(w) + 2.0 ** -25
     assert rms(got - w) <= allowed, (rms(got - w), allowed, rms(w))
     size = [want.square().mean(d, keepdim=True).sqrt() for d in (0, 1)]
     size = [(t / (t.square().mean().sqrt() + 1e-300)).clamp(min=1) for t in size]

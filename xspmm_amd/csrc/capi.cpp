@@ -938,7 +938,7 @@ int xspmm_orthogonalize_scratch(xspmm_weight_t weight, int vtype, int64_t* bytes
         const BlockIndex& w = weight->index;
         require(w.M <= kOrthogonalMostSide && w.K <= kOrthogonalMostSide,
                 "xSpMM: an orthogonalised update has at most 2^20 rows and columns.");
-        with_layer_type(vtype, [&](auto tv) { *bytes = orthogonal_scratch(w, sizeof(typename decltype(tv)::type)); });
+        with_layer_type(vtype, [&](auto tv) { *bytes = orthogonal_scratch<typename decltype(tv)::type>(w); });
     });
 }
 
@@ -956,7 +956,7 @@ int xspmm_orthogonalize(xspmm_weight_t weight, int vtype, const void* update, vo
         with_layer_type(vtype, [&](auto tv) {
             using T = typename decltype(tv)::type;
             const bool any = w.nnzb > 0;
-            require_scratch(scratch, scratch_bytes, orthogonal_scratch(w, sizeof(T)));
+            require_scratch(scratch, scratch_bytes, orthogonal_scratch<T>(w));
             orthogonalize<T>(w, operand<T>(update, any, "update"), result<T>(out, any, "out"), {a, b, c, eps, steps},
                              scratch, as_stream(stream));
         });

@@ -6,15 +6,16 @@
 // the usual coefficients five steps bring all but the smallest ones near 1.  X has the
 // weight's smaller side as its rows (U^T is X where U has fewer columns).
 //
-// Products are of fp16 operands with fp32 sums.  16-bit updates: X is held as two halves,
-// of which products take the upper one and a X both, so that X loses nothing from step
+// Products are of fp16 operands with fp32 sums.  bf16 updates: X is held as two halves, of
+// which products take the upper one and a X both, so that X loses nothing from step
 // to step.  (A rounding E of X that went through a X would grow with the
 // singular values that grow, 3.4 times a step; through S and the product it does not:
 // what b S + c S S multiplies by E vanishes where the singular values do.)  The
 // diagonal of b S + c S S stays in fp32 and multiplies X itself.  Together 3e-4 to 1e-3
 // of the result's rms, rank 32 to full, where a bf16 result's rounding is 1.7e-3; with
-// X in one half 2e-2 at rank 32.  fp32 updates: every operand in two halves, three
-// products each (the fourth is below 2^-22): 1e-5 and less.
+// X in one half 2e-2 at rank 32.  fp16 and fp32 updates: every operand in two halves, three
+// products each (the fourth is below 2^-22): 1e-5 and less, beside a rounding of 2e-4 in
+// fp16.  (Of fp16 updates the last four of five steps would have to be so.)
 // Halves hold 2^12 times their values: an element of X is between 1 / sqrt(elements),
 // far below fp16's normal numbers in a large matrix, and 1.2.
 #include "feed_forward_device.hpp"
@@ -25,6 +26,10 @@ namespace detail {
 namespace ff {
 
 constexpr float kHeld = 4096.f;  // times what a half stands for
+
+// whether products take both halves
+template <typename T>
+constexpr bool is_split = !__is_same(T, __bf16);
 
 struct Halves {
     _Float16* hi;
@@ -284,9 +289,9 @@ __device__ __forceinline__ int row_swizzle(int r)
 __device__ __forceinline__ int across_swizzle(int r) { return (r >> 3) << 1; }
 
 template <typename T, int TI, bool ACROSS, int PURPOSE>
-__global__ __launch_bounds__(kProductThreads, is_f32<T> ? 1 : 2) void ff_orthogonal_product_kernel(const Product a, const Finish<T> f)
+__global__ __launch_bounds__(kProductThreads, is_split<T> ? 1 : 2) void ff_orthogonal_product_kernel(const Product a, const Finish<T> f)
 {
-    constexpr bool SPLIT = is_f32<T>;
+    constexpr bool SPLIT = is_split<T>;
     using S = Shape<TI, SPLIT>;
     constexpr int FI = S::FI, FJ = S::FJ, TJ = S::TJ, kStages = S::kStages, kHalves = S::kHalves;
     __shared__ __align__(16) unsigned char smem[S::kLds];
@@ -443,7 +448,7 @@ __global__ __launch_bounds__(kProductThreads, is_f32<T> ? 1 : 2) void ff_orthogo
 template <typename T, int TI, int PURPOSE>
 __global__ __launch_bounds__(256) void ff_orthogonal_join_kernel(const Product a, const Finish<T> f)
 {
-    using S = Shape<TI, is_f32<T>>;
+    using S = Shape<TI, is_split<T>>;
     constexpr int FI = S::FI, FJ = S::FJ, TJ = S::TJ, kPieces = TI * TJ / 4096;  // workgroups of a tile
     __shared__ __align__(16) _Float16 turn[4][2048];
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
@@ -547,11 +552,11 @@ struct OrthogonalPlan {
     size_t x_hi[2], x_lo[2], s_hi, s_lo, b_hi, b_lo, diagonal, norm, part, end;
 };
 
-OrthogonalPlan orthogonal_plan(const BlockIndex& w, int64_t size)
+OrthogonalPlan orthogonal_plan(const BlockIndex& w, bool split)
 {
     OrthogonalPlan p{};
     p.transposed = w.M > w.K;
-    p.split = size == 4;
+    p.split = split;
     const int64_t rows = p.transposed ? w.K : w.M, columns = p.transposed ? w.M : w.K;
     // The largest tiles of which there are enough: a CU gets no more than 25 GB/s of what
     // other dies have just written, and few workgroups wait for that, while small tiles read
@@ -688,17 +693,18 @@ void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const Orthog
 
 }  // namespace ff
 
-int64_t orthogonal_scratch(const BlockIndex& w, int64_t size)
+template <typename T>
+int64_t orthogonal_scratch(const BlockIndex& w)
 {
     if (w.nnzb == 0) return 0;
-    return (int64_t)ff::orthogonal_plan(w, size).end;
+    return (int64_t)ff::orthogonal_plan(w, ff::is_split<T>).end;
 }
 
 template <typename T>
 void orthogonalize(const BlockIndex& w, const T* update, T* out, const OrthogonalArgs& o, void* scratch, hipStream_t s)
 {
     if (w.nnzb == 0) return;
-    const ff::OrthogonalPlan p = ff::orthogonal_plan(w, sizeof(T));
+    const ff::OrthogonalPlan p = ff::orthogonal_plan(w, ff::is_split<T>);
     if (p.tile == 256)
         ff::orthogonal_steps<T, 256>(w, update, out, o, p, static_cast<char*>(scratch), s);
     else if (p.tile == 64)
@@ -707,7 +713,8 @@ void orthogonalize(const BlockIndex& w, const T* update, T* out, const Orthogona
         ff::orthogonal_steps<T, 128>(w, update, out, o, p, static_cast<char*>(scratch), s);
 }
 
-#define XSPMM_ORTHOGONAL(T) \
+#define XSPMM_ORTHOGONAL(T)                                     \
+    template int64_t orthogonal_scratch<T>(const BlockIndex&); \
     template void orthogonalize<T>(const BlockIndex&, const T*, T*, const OrthogonalArgs&, void*, hipStream_t);
 XSPMM_ORTHOGONAL(float)
 XSPMM_ORTHOGONAL(_Float16)

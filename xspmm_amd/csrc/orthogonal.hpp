@@ -16,7 +16,8 @@ struct OrthogonalArgs {
 // Sides of a weight whose update may be orthogonalised.
 constexpr int64_t kOrthogonalMostSide = int64_t(1) << 20;
 
-int64_t orthogonal_scratch(const BlockIndex& w, int64_t size);
+template <typename T>
+int64_t orthogonal_scratch(const BlockIndex& w);
 template <typename T>
 void orthogonalize(const BlockIndex& w, const T* update, T* out, const OrthogonalArgs& o, void* scratch, hipStream_t s);
 
