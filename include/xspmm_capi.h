@@ -516,10 +516,10 @@ int xspmm_quantize_tokens(int vtype, int64_t K, int64_t N, const void* x, int8_t
  * y = act(A x + bias) + residual in 8 bits.  Either x is NULL, and xq and x_scale
  * are the tokens as xspmm_quantize_tokens makes them, or x (K x N) is quantized
  * within the call and xq and x_scale are not read: scratch (256-byte aligned) then
- * has as many bytes as xspmm_int8_scratch says.  bias and residual may be NULL; y may
- * be the residual.
+ * has as many bytes as xspmm_int8_scratch says for one weight (xspmm_int8_gated: two) of
+ * M x K.  bias and residual may be NULL; y may be the residual.
  */
-int xspmm_int8_scratch(int64_t K, int64_t N, int64_t* bytes);
+int xspmm_int8_scratch(int weights, int64_t M, int64_t K, int64_t N, int64_t* bytes);
 int xspmm_int8_linear(xspmm_weight_t weight, int vtype, int act, const int8_t* q, const float* scale, const void* x,
                       const int8_t* xq, const float* x_scale, const void* bias, const void* residual, void* y, int64_t N,
                       void* scratch, int64_t scratch_bytes, void* stream);

@@ -19,9 +19,9 @@ def lib():
     return orthogonal._load()
 
 
-def scratch(f, K, N):
+def scratch(f, *sizes):
     n = C.c_int64(-1)
-    assert f(K, N, C.byref(n)) == X.OK
+    assert f(*sizes, C.byref(n)) == X.OK
     return n.value
 
 
@@ -30,20 +30,25 @@ def test_scratch(lib, K, N):
     maxima = scratch(lib.xspmm_quantize_tokens_scratch, K, N)
     # a maximum of every token and slice, a small share of what is read
     assert maxima % 4 == 0 and 0 <= maxima <= 4 * N * (-(-K // 16)) and (maxima == 0 or maxima >= 4 * N)
-    whole = scratch(lib.xspmm_int8_scratch, K, N)
-    # none where the product rounds its tokens itself, else the whole numbers, the scales and the maxima
-    assert whole == 0 if N <= 64 and K * min(N, 16) <= 16 * 1024 else True
-    assert whole == 0 or whole >= -(-K // 16) * 16 * N + 4 * N + maxima
+    for weights, M in ((1, 4096), (2, 14336), (2, 16)):
+        whole = scratch(lib.xspmm_int8_scratch, weights, M, K, N)
+        # none where the product rounds its tokens itself, else the whole numbers, the scales and the maxima
+        if N == 1 and K <= 32768:
+            assert whole == 0
+        assert whole == 0 or whole >= -(-K // 16) * 16 * N + 4 * N + maxima
 
 
 def test_scratch_empty_and_refused(lib):
-    for f in (lib.xspmm_quantize_tokens_scratch, lib.xspmm_int8_scratch):
+    whole = lambda K, N, out: lib.xspmm_int8_scratch(1, 64, K, N, out)
+    for f in (lib.xspmm_quantize_tokens_scratch, whole):
         for K, N in ((0, 5), (5, 0), (0, 0)):
             assert scratch(f, K, N) >= 0
         n = C.c_int64(0)
         for K, N in ((-1, 5), (5, -1), (1 << 31, 5), (5, (1 << 30) + 1)):
             refused(lib, lambda: f(K, N, C.byref(n)))
         refused(lib, lambda: f(5, 5, None))
+    for weights, M in ((0, 5), (3, 5), (1, -1)):
+        refused(lib, lambda: lib.xspmm_int8_scratch(weights, M, 5, 5, C.byref(n)))
 
 
 def test_null_weights(lib):

@@ -158,7 +158,7 @@ TokenMemory token_memory(int64_t K, int64_t N)
 
 // The tokens of a product: as they come, or quantized into its scratch.
 template <typename T>
-void int8_tokens(Int8Args<T>& a, const BlockIndex& w, bool any, const void* x, const int8_t* xq, const float* x_scale,
+void int8_tokens(Int8Args<T>& a, const BlockIndex& w, int weights, bool any, const void* x, const int8_t* xq, const float* x_scale,
                  void* scratch, int64_t scratch_bytes, hipStream_t s)
 {
     require(w.K <= kInt8MostFeatures, "xSpMM: a weight in 8 bits has at most 133136 columns.");
@@ -169,7 +169,7 @@ void int8_tokens(Int8Args<T>& a, const BlockIndex& w, bool any, const void* x, c
         require(x_scale != nullptr, "xSpMM: x_scale is null.");
         return;
     }
-    if (int8_rounds_itself(w.K, a.N)) {
+    if (int8_rounds_itself(weights, w.M, w.K, a.N)) {
         a.raw = operand<T>(x, false, "x");
         return;
     }
@@ -863,12 +863,14 @@ int xspmm_quantize_tokens(int vtype, int64_t K, int64_t N, const void* x, int8_t
     });
 }
 
-int xspmm_int8_scratch(int64_t K, int64_t N, int64_t* bytes)
+int xspmm_int8_scratch(int weights, int64_t M, int64_t K, int64_t N, int64_t* bytes)
 {
     return guarded([&] {
         require(bytes != nullptr, "xspmm_int8_scratch: bytes is null.");
+        require(weights == 1 || weights == 2, "xspmm_int8_scratch: a product has one weight or two.");
+        require(M >= 0, "xSpMM: bad size of a weight.");
         require_tokens(K, N);
-        *bytes = int8_rounds_itself(K, N) ? 0 : (int64_t)token_memory(K, N).end;
+        *bytes = int8_rounds_itself(weights, M, K, N) ? 0 : (int64_t)token_memory(K, N).end;
     });
 }
 
@@ -893,7 +895,7 @@ int xspmm_int8_linear(xspmm_weight_t weight, int vtype, int act, const int8_t* q
             a.y = result<T>(y, any, "y");
             a.N = N;
             a.act = act;
-            int8_tokens<T>(a, w, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
+            int8_tokens<T>(a, w, 1, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
             if (any) int8_product<T>(a, 1, as_stream(stream));
         });
     });
@@ -925,7 +927,7 @@ int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act,
             a.y = result<T>(h, any, "h");
             a.N = N;
             a.act = act;
-            int8_tokens<T>(a, g, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
+            int8_tokens<T>(a, g, 2, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
             if (any) int8_product<T>(a, 2, as_stream(stream));
         });
     });

@@ -113,7 +113,6 @@ __global__ __launch_bounds__(64 * (SPLIT > 4 ? SPLIT : 4)) void ff_int8_walk_ker
 // with its first blocks on their way meanwhile, and then walks ROWS block-rows, 16 /
 // ROWS waves to each.
 constexpr int kFewTokens = 16, kFewThreads = 1024;
-constexpr int kFewBlocks = 2048;  // blocks of 16 features of a token, in all
 
 // KEPT: such blocks of a thread
 template <typename T, int NACC, int ROWS, int KEPT, bool ONE>
@@ -252,15 +251,17 @@ __global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_ke
     a.y[row * a.N + n0 + li] = (T)int8_finish<T, NACC>(a, sum, row, n0 + li, scales[li]);
 }
 
-template <typename T, int NACC, int ROWS, int KEPT>
+template <typename T, int NACC, int ROWS>
 void launch_few(const Int8Product<T>& a, hipStream_t s)
 {
     const int64_t items = (int64_t)((a.block_rows + ROWS - 1) / ROWS) * ((a.N + kFewTokens - 1) / kFewTokens);
     const dim3 grid = launch_grid(items, kFewThreads), threads(kFewThreads);
-    if (a.N == 1)
-        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, KEPT, true>), grid, threads, 0, s, a);
+    if (a.N > 1)
+        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, 1, false>), grid, threads, 0, s, a);
+    else if (a.in_blocks <= kFewThreads)
+        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, 1, true>), grid, threads, 0, s, a);
     else
-        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, KEPT, false>), grid, threads, 0, s, a);
+        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, 2, true>), grid, threads, 0, s, a);
     XSPMM_LAUNCH_CHECK();
 }
 
@@ -282,16 +283,13 @@ void launch_int8(const Int8Product<T>& a, int64_t blocks, hipStream_t s)
         // (16 waves each), half and a quarter of them beyond (us of one and two rows a
         // workgroup: fp16 4096 x 14336, 25 % stored, one token 6.7 and 7.8; bf16 gate and
         // up of 14336 x 4096 13.0 and 10.1, of four rows 10.3).
-        const int64_t nt = a.N < kFewTokens ? a.N : kFewTokens;
         const int64_t groups = a.block_rows * ((a.N + kFewTokens - 1) / kFewTokens);
-        if (a.in_blocks * nt > 1024)
-            launch_few<T, NACC, 1, 2>(a, s);
-        else if (groups <= 512)
-            launch_few<T, NACC, 1, 1>(a, s);
+        if (groups <= 512)
+            launch_few<T, NACC, 1>(a, s);
         else if (groups <= 1024)
-            launch_few<T, NACC, 2, 1>(a, s);
+            launch_few<T, NACC, 2>(a, s);
         else
-            launch_few<T, NACC, 4, 1>(a, s);
+            launch_few<T, NACC, 4>(a, s);
         return;
     }
     auto waves = [&](int v) { return (int64_t)a.block_rows * ((a.N + 16 * v - 1) / (16 * v)); };
@@ -312,10 +310,16 @@ void launch_int8(const Int8Product<T>& a, int64_t blocks, hipStream_t s)
 
 }  // namespace ff
 
-bool int8_rounds_itself(int64_t K, int64_t N)
+// One token, and more where every workgroup's rounding them anew costs less than a launch:
+// us with and without, bf16, 16384 x 1024 30 % stored 16 tokens 10.4 and 11.1, 48 tokens 15.7
+// and 10.9; gate and up of 14336 x 4096 25 % stored one token 10.0 and 12.6, two 16.9 and
+// 13.6; 4096 x 4096 10 % stored four tokens 8.5 and 11.1.
+bool int8_rounds_itself(int weights, int64_t M, int64_t K, int64_t N)
 {
-    const int64_t Kb = (K + 15) / 16, nt = N < ff::kFewTokens ? N : ff::kFewTokens;
-    return N <= 64 && Kb * nt <= ff::kFewBlocks;
+    const int64_t Mb = (M + 15) / 16, Kb = (K + 15) / 16;
+    if (N == 1) return Kb <= 2 * ff::kFewThreads;
+    const int64_t tokens = N < ff::kFewTokens ? N : ff::kFewTokens, tiles = (N + ff::kFewTokens - 1) / ff::kFewTokens;
+    return Kb * tokens <= ff::kFewThreads && weights * Mb * tiles <= 1024;
 }
 
 template <typename T>

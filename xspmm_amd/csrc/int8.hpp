@@ -39,7 +39,7 @@ struct Int8Args {
     int act;
 };
 // Whether a product of N tokens rounds them itself, without memory for the result.
-bool int8_rounds_itself(int64_t K, int64_t N);
+bool int8_rounds_itself(int weights, int64_t M, int64_t K, int64_t N);
 template <typename T>
 void int8_product(const Int8Args<T>& a, int weights, hipStream_t s);
 

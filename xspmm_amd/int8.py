@@ -46,7 +46,7 @@ def _load():
             "xspmm_int8_weight": [p, i32, p, p, p, p],
             "xspmm_quantize_tokens_scratch": [i64, i64, out],
             "xspmm_quantize_tokens": [i32, i64, i64, p, p, p, p, i64, p],
-            "xspmm_int8_scratch": [i64, i64, out],
+            "xspmm_int8_scratch": [i32, i64, i64, i64, out],
             "xspmm_int8_linear": [p, i32, i32, p, p, p, p, p, p, p, p, i64, p, i64, p],
             "xspmm_int8_gated": [p, p, i32, i32, p, p, p, p, p, p, p, p, p, p, i64, p, i64, p],
         }.items():
@@ -57,9 +57,9 @@ def _load():
 
 
 @functools.lru_cache(maxsize=1024)
-def _bytes(query, K, N):
+def _bytes(query, *sizes):
     n = C.c_int64(0)
-    X._check(getattr(_load(), query)(K, N, C.byref(n)))
+    X._check(getattr(_load(), query)(*sizes, C.byref(n)))
     return n.value
 
 
@@ -137,7 +137,7 @@ def quantize_tokens(x):
     return Int8Tokens(q, scale, (K, N))
 
 
-def _tokens(x, K, dtype, device):
+def _tokens(x, weights, M, K, dtype, device):
     """(tokens, the addresses of x, of whole numbers and of scales, scratch, its
     bytes, what must stay alive) of a product's activations."""
     if isinstance(x, Int8Tokens):
@@ -152,7 +152,7 @@ def _tokens(x, K, dtype, device):
     if xp is None and N:  # no features: zeros
         s = torch.zeros(N, dtype=torch.float32, device=device)
         return N, None, None, s.data_ptr(), None, 0, s
-    n = _bytes("xspmm_int8_scratch", K, N)
+    n = _bytes("xspmm_int8_scratch", weights, M, K, N)
     ws = _scratch(n, device)
     return N, xp, None, None, None if ws is None else ws.data_ptr(), n, ws
 
@@ -179,7 +179,7 @@ def int8_linear(W, x, bias=None, activation=None, residual=None, out=None):
     act = _activation(activation)
     (M, K), dt, dev = W.shape, W.dtype, W.device
     vals, scale = W._operands()
-    N, xp, q, s, ws, n, held = _tokens(x, K, dt, dev)
+    N, xp, q, s, ws, n, held = _tokens(x, 1, M, K, dt, dev)
     bp = None if bias is None else _check(bias, "bias", (M,), dt, dev, 0)
     rp = None if residual is None else _check(residual, "residual", (M, N), dt, dev)
     _no_gradients(None if held is x else x, bias, residual)
@@ -197,7 +197,7 @@ def int8_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", out=Non
     act = _activation(activation)
     (M, K), dt, dev = _pair(G, U), G.dtype, G.device
     (gv, gs), (uv, us) = G._operands(), U._operands()
-    N, xp, q, s, ws, n, held = _tokens(x, K, dt, dev)
+    N, xp, q, s, ws, n, held = _tokens(x, 2, M, K, dt, dev)
     gb = None if bias_gate is None else _check(bias_gate, "bias_gate", (M,), dt, dev, 0)
     ub = None if bias_up is None else _check(bias_up, "bias_up", (M,), dt, dev, 0)
     _no_gradients(None if held is x else x, bias_gate, bias_up)
