@@ -116,6 +116,61 @@ def test_shapes(kind, M, K, density):
     check(X.orthogonalize(W, v), U, where, kind)
 
 
+# tiles of 128 rows (bf16) and of 256, whole and in part
+@pytest.mark.parametrize("kind,M,K", [("bf16", 2000, 2200), ("bf16", 2048, 2304), ("bf16", 2900, 3100), ("bf16", 3100, 2830),
+                                      ("f16", 2050, 2300), ("f32", 2050, 2300), ("f32", 2600, 2049)])
+@pytest.mark.parametrize("density", [0.1, 1.0])
+def test_larger_tiles(kind, M, K, density):
+    W, where, v, U = update(M, K, density, kind, M + K)
+    check(X.orthogonalize(W, v), U, where, kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_past_four_gib(kind):
+    """X of 2^32 bytes and more, against the polynomial of S in 64 bits: X = Q X0, Q <- B Q and
+    S <- B S B with B = a + b S + c S S.  bf16 results are off by up to 1e-3 of their rms and
+    their rounding, fp32 ones by 1e-5; twice that is allowed."""
+    M, K, per = 2100, (1 << 20) - 5, 130
+    dtype, u = TYPES[kind]
+    Mb, Kb = -(-M // 16), -(-K // 16)
+    g = torch.Generator().manual_seed(1)
+    cols = torch.stack([torch.randperm(Kb, generator=g)[:per].sort().values for _ in range(Mb)])
+    ptr = torch.arange(Mb + 1, dtype=torch.int32, device=DEV) * per
+    v = torch.randn(Mb * per * 256, generator=g).to(dtype).to(DEV)
+    rows, col = torch.arange(Mb, device=DEV).repeat_interleave(per), cols.reshape(-1).to(DEV)
+    inside = (16 * rows[:, None] + torch.arange(16, device=DEV) < M)[:, :, None] & (
+        16 * col[:, None] + torch.arange(16, device=DEV) < K)[:, None, :]
+    v *= inside.reshape(-1)
+    W = X.SparseWeight(X.BCSRMatrix(Mb, Kb, 16, 16, M, K, ptr, col.int(), v))
+    got = X.orthogonalize(W, v).view(-1, 16, 16)
+    a, b, c = ABC
+    v64 = v.double().view(-1, 16, 16)
+    S = torch.zeros((Mb * 16, Mb * 16), dtype=torch.float64, device=DEV)
+    step, slabs = 4096, []
+    v64 = v64 / (v64.norm() + 1e-7)
+    for c0 in range(0, Kb, step):  # block-columns
+        on = ((col >= c0) & (col < c0 + step)).nonzero().flatten()
+        d = torch.zeros((Mb, step, 16, 16), dtype=torch.float64, device=DEV)
+        d[rows[on], col[on] - c0] = v64[on]
+        d = d.permute(0, 2, 1, 3).reshape(Mb * 16, step * 16)
+        S += d @ d.t()
+        slabs.append((c0, on))
+    Q = torch.eye(Mb * 16, dtype=torch.float64, device=DEV)
+    for _ in range(5):
+        B = b * S + c * (S @ S)
+        B.diagonal().add_(a)
+        Q, S = B @ Q, B @ S @ B
+    error = size = 0.0
+    for c0, on in slabs:
+        d = torch.zeros((Mb, step, 16, 16), dtype=torch.float64, device=DEV)
+        d[rows[on], col[on] - c0] = v64[on]
+        want = (Q @ d.permute(0, 2, 1, 3).reshape(Mb * 16, step * 16)).view(Mb, 16, step, 16).transpose(1, 2)
+        want = want[rows[on], col[on] - c0] * inside[on]
+        error += float((got[on].double() - want).square().sum())
+        size += float(want.square().sum())
+    assert error ** 0.5 <= 2 * ((1e-3 if kind == "bf16" else 1e-5) + u) * size ** 0.5
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("rank", [1, 16, 100])
 def test_low_rank(kind, rank):

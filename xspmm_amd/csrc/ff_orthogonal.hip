@@ -477,17 +477,16 @@ __global__ __launch_bounds__(256) void ff_orthogonal_join_kernel(const Product a
 }
 
 // Sums of squares of the stored values inside the weight, a share of the blocks each.
-constexpr int kNormShares = 512;
+constexpr int kNormShares = 512, kNormWaves = 16;
 template <typename T>
-__global__ __launch_bounds__(256) void ff_square_sum_kernel(const T* __restrict__ u, const int32_t* __restrict__ row,
+__global__ __launch_bounds__(64 * kNormWaves) void ff_square_sum_kernel(const T* __restrict__ u, const int32_t* __restrict__ row,
                                                             const int32_t* __restrict__ col, int64_t nnzb, int32_t M,
                                                             int32_t K, double* __restrict__ part)
 {
-    __shared__ double red[4];
+    __shared__ double red[kNormWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double sum = 0.0;
-#pragma unroll 4
-    for (int64_t b = blockIdx.x * 4 + wave; b < nnzb; b += 4 * kNormShares) {
+    for (int64_t b = blockIdx.x * kNormWaves + wave; b < nnzb; b += kNormWaves * kNormShares) {
         const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(u + b * 256 + 4 * lane);
         const int32_t r = 16 * row[b] + lane / 4, c = 16 * col[b] + 4 * (lane & 3);
 #pragma unroll
@@ -500,7 +499,11 @@ __global__ __launch_bounds__(256) void ff_square_sum_kernel(const T* __restrict_
     for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
     if (lane == 0) red[wave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    if (threadIdx.x == 0) {
+        double all = red[0];
+        for (int w = 1; w < kNormWaves; ++w) all += red[w];
+        part[blockIdx.x] = all;
+    }
 }
 
 // X = U / (|U| + eps), zeros where no block is stored and past the edges; a thread
@@ -562,9 +565,10 @@ OrthogonalPlan orthogonal_plan(const BlockIndex& w, bool split)
     // other dies have just written, and few workgroups wait for that, while small tiles read
     // their operands more often.  us by 64 and 128 rows: bf16 512 x 1792 137 and 195, 1000 x
     // 2500 227 and 275, 2048 x 2048 434 and 452, fp32 1000 x 2500 334 and 362; by 128 and
-    // 256: bf16 1536 x 4096 410 and 440, 2048 x 5632 706 and 661, fp32 1536 x 4096 757 and 726.
+    // 256: bf16 1536 x 4096 410 and 440, 2048 x 5632 706 and 661.  With operands in two halves
+    // there is no size for 128 (fp32 1536 x 4096 757, by 256 726).
     auto count = [&](int64_t side) { return (rows + side - 1) / side * ((columns + side - 1) / side); };
-    p.tile = count(64) <= 1024 ? 64 : count(128) <= (p.split ? 256 : 512) ? 128 : 256;
+    p.tile = count(64) <= 1024 ? 64 : !p.split && count(128) <= 512 ? 128 : 256;
     const int64_t tj = tile_columns(p.tile);
     p.m = (rows + p.tile - 1) / p.tile * p.tile;
     p.k = (columns + tj - 1) / tj * tj;
@@ -648,7 +652,7 @@ void orthogonal_steps(const BlockIndex& w, const T* update, T* out, const Orthog
     f.Kb = (int32_t)w.Kb;
     f.transposed = p.transposed;
     double* norm = reinterpret_cast<double*>(at + p.norm);
-    hipLaunchKernelGGL((ff_square_sum_kernel<T>), dim3(kNormShares), dim3(256), 0, s, update, w.row, w.col, w.nnzb,
+    hipLaunchKernelGGL((ff_square_sum_kernel<T>), dim3(kNormShares), dim3(64 * kNormWaves), 0, s, update, w.row, w.col, w.nnzb,
                        (int32_t)w.M, (int32_t)w.K, norm);
     f.out = x[0];
     f.ld = p.k;
@@ -705,12 +709,13 @@ void orthogonalize(const BlockIndex& w, const T* update, T* out, const Orthogona
 {
     if (w.nnzb == 0) return;
     const ff::OrthogonalPlan p = ff::orthogonal_plan(w, ff::is_split<T>);
-    if (p.tile == 256)
-        ff::orthogonal_steps<T, 256>(w, update, out, o, p, static_cast<char*>(scratch), s);
-    else if (p.tile == 64)
-        ff::orthogonal_steps<T, 64>(w, update, out, o, p, static_cast<char*>(scratch), s);
-    else
-        ff::orthogonal_steps<T, 128>(w, update, out, o, p, static_cast<char*>(scratch), s);
+    char* at = static_cast<char*>(scratch);
+    if (p.tile == 64)
+        ff::orthogonal_steps<T, 64>(w, update, out, o, p, at, s);
+    else if (p.tile == 256)
+        ff::orthogonal_steps<T, 256>(w, update, out, o, p, at, s);
+    else if constexpr (!ff::is_split<T>)
+        ff::orthogonal_steps<T, 128>(w, update, out, o, p, at, s);
 }
 
 #define XSPMM_ORTHOGONAL(T)                                     \
