@@ -11,7 +11,8 @@ the Tier-2 pipeline ``spmm_pipeline`` and ``unpermute_dense_matrix`` -- with
 torch tensors as device buffers.  Beside it stands the feed-forward layer of a
 language model on block-sparse weights (``feed_forward``): ``SparseWeight``,
 ``sparse_linear``, ``sparse_gated``, ``layer_norm``, their gradients and the
-``FeedForward`` module.  Every call goes to the HIP library; there is no CPU
+``FeedForward`` module, its serving in 8-bit integers (``int8``) and orthogonalised
+updates for its training (``orthogonal``).  Every call goes to the HIP library; there is no CPU
 fallback, and importing the library fails loudly when it has not
 been built.
 """
