@@ -99,6 +99,24 @@ def test_infinities_stay_in_their_token(kind, N):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("K", [16383, 16384, 16385, 32768, 32769, 100003])
+def test_one_long_token(kind, K):
+    """In one workgroup's registers or, past 16384 features, in slices; a product rounds
+    up to 32768 itself.  The largest value stands last, in the last slice."""
+    dtype = TYPES[kind][0]
+    x = normal((K, 1), dtype, K)
+    x[-1] = 9
+    same_tokens(X.quantize_tokens(x), x)
+    W, A, _ = weight(40, K, 0.05, dtype, K)
+    check_linear(W, A, x, None, None, None, kind)
+    bad = x.clone()
+    bad[K // 2] = math.inf
+    t = X.quantize_tokens(bad)
+    assert t.scale.isnan().all() and not t.values.any()
+    assert X.int8_linear(X.Int8Weight(W), bad).isnan().all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("M,K", [(1, 1), (16, 16), (17, 15), (85, 150), (16, 3000), (200, 33)])
 def test_weights(kind, M, K):
     dtype = TYPES[kind][0]

@@ -1,8 +1,8 @@
-"""Loads straight into LDS of the 8-bit products' tiles and of the products behind
+"""Loads straight into LDS of the 8-bit products' tiles and lists and of the products behind
 orthogonalised updates, in the assembly that the sources compile to.
 
 The wait states before each such load, as in test_lds_load_hazards.  And the count
-behind the tiles' wait for a window of x: it lets the loads of the last steps' blocks
+behind the waits of tiles and lists for a window of x: it lets the loads of the last steps' blocks
 be under way, so at least as many loads of blocks have to stand between the window's
 last load into LDS and the wait, wherever the compiler put them.
 """
@@ -80,6 +80,27 @@ def test_tiles_wait_for_their_window(tmp_path):
         found = [fewest_blocks_since(code, before, w) for w in waits]
         assert any(f is not None for f in found) and all(f is None or f >= 12 for f in found), (name, found)
     assert kernels == 6
+
+
+@pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc")
+def test_lists_wait_for_their_window(tmp_path):
+    text = assembly(tmp_path, "ff_int8_list")
+    loads, bad = violations(text)
+    assert loads >= 18 * 8 and not bad, (len(bad), bad[:3])
+    kernels = 0
+    for name, code, before in functions(text):
+        found = re.search(r"ff_int8_list_kernelI.*Lb[01]ELi([123])EE", name)
+        if not found:
+            continue
+        kernels += 1
+        # two rows' blocks may be under way: vmcnt(2 Q) next to a barrier
+        most = 2 * int(found.group(1))
+        waits = [i for i, line in enumerate(code) if line == f"s_waitcnt vmcnt({most})"
+                 and any("s_barrier" in c for c in code[i:i + 12])]
+        assert waits, name
+        fewest = [fewest_blocks_since(code, before, w) for w in waits]
+        assert any(f is not None for f in fewest) and all(f is None or f >= most for f in fewest), (name, fewest)
+    assert kernels == 18
 
 
 @pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc")
