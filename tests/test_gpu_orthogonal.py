@@ -356,6 +356,19 @@ def test_optimiser(kind, nesterov):
         velocity = [opt.state[p]["momentum"].clone() for p in params]
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_optimiser_of_a_weight_without_blocks(kind):
+    dtype = TYPES[kind][0]
+    sides = ((144, 96, 0.4), (144, 96, 0.0), (96, 144, 0.4))
+    L = X.FeedForward(*(weight(m, k, d, dtype, 1)[0].matrix for m, k, d in sides))
+    opt = X.OrthogonalMomentum(L, lr=0.1, weight_decay=0.5)
+    was = L.down.detach().clone()
+    L(normal((96, 64), dtype, 1)).float().square().mean().backward()
+    opt.step()
+    # up gives zeros: the others' gradients are zero, and so are their updates
+    assert L.up.numel() == 0 and torch.equal(L.down, (was.float() * (1 - 0.1 * 0.5)).to(dtype))
+
+
 def test_optimiser_resumes():
     """State saved and loaded gives the same next step, bit for bit."""
     x = normal((96, 64), torch.bfloat16, 1)

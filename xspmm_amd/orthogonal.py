@@ -124,7 +124,7 @@ class OrthogonalMomentum(torch.optim.Optimizer):
             lr, momentum = group["lr"], group["momentum"]
             for p in group["params"]:
                 W = next(weights)
-                if p.grad is None:
+                if p.grad is None or not p.numel():  # a weight without blocks
                     continue
                 state = self.state[p]
                 if not state:
