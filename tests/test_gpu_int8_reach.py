@@ -80,6 +80,29 @@ def test_kernels(kind, M, K, N, density, gated):
     check(kind, M, K, N, density, gated)
 
 
+# one weight without blocks; lists of rows with more blocks than are fetched ahead, which
+# is chosen by both weights' blocks together
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,K,N,gate,up", [(300, 500, 1, 0.3, 0.0), (300, 500, 9, 0.0, 0.3), (300, 500, 40, 0.3, 0.0),
+                                           (2048, 1000, 1030, 0.0, 0.5), (4096, 2048, 1030, 0.9, 0.02),
+                                           (4096, 2000, 2048, 0.02, 0.6), (4096, 2000, 2048, 0.1, 0.0)])
+def test_weights_of_two_densities(kind, M, K, N, gate, up):
+    dtype, u = TYPES[kind]
+    (G, g, gs), (U, w, us) = weight(M, K, gate, dtype, 1), weight(M, K, up, dtype, 2)
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn((K, N), generator=gen, device=DEV).to(dtype)
+    b = torch.randn(M, generator=gen, device=DEV).to(dtype)
+    most = x.double().abs().amax(0)
+    q = (x.double() * 127 / most).round()
+    z = [(d @ q) * s * (most / 127) + b.double()[:, None] for d, s in ((g, gs), (w, us))]
+    err = [EPS32 * (8 * v.abs() + 8 * b.double().abs()[:, None]) for v in z]
+    want = z[0].clamp(min=0) * z[1]
+    bound = err[0] * (z[1].abs() + err[1]) + z[0].abs() * err[1]
+    y = X.int8_gated(G, U, x, bias_gate=b, bias_up=b, activation="relu")
+    bad = (y.double() - want).abs() > bound + u * want.abs() * 1.01 + TINY
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
 def units(shape, seed, dtype):
     g = torch.Generator(device=DEV).manual_seed(seed)
     t = torch.randint(-1, 2, shape, generator=g, device=DEV, dtype=torch.int8).to(dtype)
