@@ -1,0 +1,95 @@
+"""OrthogonalMomentum: copies of it, a captured step."""
+from __future__ import annotations
+
+import copy
+import io
+
+import pytest
+import torch
+
+import xspmm_amd as X
+from test_gpu_feed_forward import TYPES, normal, weight
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def layer(dtype, features=96, hidden=144, density=0.4):
+    sides = ((hidden, features, 1), (hidden, features, 2), (features, hidden, 3))
+    return X.FeedForward(*(weight(m, k, density, dtype, s)[0].matrix for m, k, s in sides))
+
+
+def weights(L):
+    return [L.gate, L.up, L.down]
+
+
+def gradients(L, seed, scale=1.0):
+    """Whole numbers of at most 8 times `scale`, which every type holds."""
+    g = torch.Generator().manual_seed(seed)
+    for p in weights(L):
+        p.grad = (torch.randint(-8, 9, p.shape, generator=g).double() * scale).to(p.dtype).to(DEV)
+
+
+def same(A, B):
+    return all(torch.equal(p, q) for p, q in zip(weights(A), weights(B)))
+
+
+def pickled(t):
+    f = io.BytesIO()
+    torch.save(t, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("duplicate", [copy.deepcopy, pickled])
+@pytest.mark.parametrize("before", [0, 2])
+def test_copies(kind, duplicate, before):
+    """A layer copied with its optimiser goes on as the first ones do, apart from them."""
+    A = layer(TYPES[kind][0])
+    a = X.OrthogonalMomentum(A, lr=0.01, weight_decay=0.1)
+    for i in range(before):
+        gradients(A, i)
+        a.step()
+    B, b = duplicate((A, a))
+    assert all(p is q for p, q in zip(weights(B), b.param_groups[0]["params"]))
+    assert same(A, B)
+    was = [p.detach().clone() for p in weights(A)]
+    gradients(B, 9)
+    b.step()
+    assert all(torch.equal(p, w) for p, w in zip(weights(A), was)) and not same(A, B)
+    gradients(A, 9)
+    a.step()
+    assert same(A, B)
+    for o in (a, b):
+        with pytest.raises(RuntimeError, match="layers' weights"):
+            o.add_param_group({"params": [A.norm_weight]})
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("sides", [(96, 144), (1024, 4096)])
+def test_captured(kind, sides):
+    """A step in a graph, replayed with other gradients and eager work between."""
+    A, B = layer(TYPES[kind][0], *sides), layer(TYPES[kind][0], *sides)
+    a, b = (X.OrthogonalMomentum(L, lr=0.01) for L in (A, B))
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        gradients(A, 0)
+        a.step()
+    torch.cuda.synchronize()
+    gradients(B, 0)
+    b.step()
+    assert same(A, B)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        a.step()
+    for i in range(1, 6):
+        gradients(B, i)
+        for p, q in zip(weights(A), weights(B)):
+            p.grad.copy_(q.grad)
+        graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        assert same(A, B), i

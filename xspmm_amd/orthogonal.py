@@ -100,6 +100,10 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                                       steps=steps))
         self._weights = [W for layer in layers for W in layer._weights]
 
+    def __getstate__(self):
+        # copies and pickles: torch's own state leaves the weights out
+        return {**super().__getstate__(), "_weights": self._weights}
+
     def add_param_group(self, group):
         if getattr(self, "_weights", None) is not None:
             raise RuntimeError("the parameters of OrthogonalMomentum are its layers' weights")
