@@ -1,4 +1,4 @@
-"""OrthogonalMomentum: copies of it, a captured step."""
+"""OrthogonalMomentum: copies of it, gradients of any size, a captured step."""
 from __future__ import annotations
 
 import copy
@@ -65,6 +65,32 @@ def test_copies(kind, duplicate, before):
     for o in (a, b):
         with pytest.raises(RuntimeError, match="layers' weights"):
             o.add_param_group({"params": [A.norm_weight]})
+
+
+# (fp16's smallest number is 2^-24)
+@pytest.mark.parametrize("kind,scale", [("f16", 2.0 ** -24), ("bf16", 2.0 ** -60), ("bf16", 2.0 ** -115), ("f32", 2.0 ** -24),
+                                        ("f32", 2.0 ** -60), ("f32", 2.0 ** -115), ("f32", 2.0 ** 100)])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_gradients_of_any_size(kind, scale, nesterov):
+    """The size of the gradients does not matter: powers of two, so that nothing but the size differs."""
+    A, B = layer(TYPES[kind][0]), layer(TYPES[kind][0])
+    a, b = (X.OrthogonalMomentum(L, lr=0.01, nesterov=nesterov) for L in (A, B))
+    for i in range(2):
+        gradients(A, i)
+        gradients(B, i, scale)
+        a.step()
+        b.step()
+        assert same(A, B)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_gradients_of_zero(kind):
+    A = layer(TYPES[kind][0])
+    was = [p.detach().clone() for p in weights(A)]
+    a = X.OrthogonalMomentum(A, lr=0.5)
+    gradients(A, 0, 0.0)
+    a.step()
+    assert all(torch.equal(p, w) for p, w in zip(weights(A), was))
 
 
 @pytest.mark.parametrize("kind", list(TYPES))

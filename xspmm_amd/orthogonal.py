@@ -85,7 +85,8 @@ class OrthogonalMomentum(torch.optim.Optimizer):
       v <- momentum v + g,   u = g + momentum v (nesterov) or v
       w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / columns)) orthogonalize(u)
 
-    v and, for 16-bit weights, a master copy of w are kept in fp32."""
+    The size of u does not matter, however small.  v and, for 16-bit weights, a master
+    copy of w are kept in fp32."""
 
     def __init__(self, layers, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
         layers = [layers] if isinstance(layers, torch.nn.Module) else list(layers)
@@ -138,11 +139,14 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                 g, v = p.grad.float(), state["momentum"]
                 v.mul_(momentum).add_(g)
                 u = g.add(v, alpha=momentum) if group["nesterov"] else v
-                if W.dtype is not torch.float32:  # its scale does not matter, but has to fit the type
-                    u = u / u.abs().amax().clamp_min(1e-30)
+                # The size of u does not matter, nor may eps damp it: beside a 16-bit u, scaled to fit
+                # its type with a largest element of 1, it is nothing, in fp32 it is left out.
+                eps = 0.0
+                if W.dtype is not torch.float32:
+                    u, eps = u / u.abs().amax().clamp_min(torch.finfo(torch.float32).tiny), 1e-7
                 # a copy in W's type: the result goes where it stood
                 u = u.to(W.dtype, copy=True)
-                orthogonalize(W, u, steps=group["steps"], out=u)
+                orthogonalize(W, u, steps=group["steps"], eps=eps, out=u)
                 master = state.get("master", p)
                 if group["weight_decay"]:
                     master.mul_(1 - lr * group["weight_decay"])
