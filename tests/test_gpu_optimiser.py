@@ -1,4 +1,5 @@
-"""OrthogonalMomentum: copies of it, gradients of any size, a captured step."""
+"""OrthogonalMomentum: copies of it, gradients of any size, values that come from elsewhere,
+a captured step."""
 from __future__ import annotations
 
 import copy
@@ -91,6 +92,43 @@ def test_gradients_of_zero(kind):
     gradients(A, 0, 0.0)
     a.step()
     assert all(torch.equal(p, w) for p, w in zip(weights(A), was))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_values_from_elsewhere(kind):
+    """Values that a layer is given between two steps are what the next one moves."""
+    A, B = layer(TYPES[kind][0]), layer(TYPES[kind][0])
+    a = X.OrthogonalMomentum(A, lr=0.01)
+    gradients(A, 0)
+    a.step()
+    with torch.no_grad():
+        for p in weights(B):
+            p.mul_(3)
+    A.load_state_dict(B.state_dict())
+    A.up.data.mul_(2)  # past torch's count of changes
+    B.up.data.mul_(2)
+    for group in a.param_groups:
+        group["lr"] = 0.0
+    gradients(A, 1)
+    a.step()
+    assert same(A, B)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_small_steps_add_up(kind):
+    """What a 16-bit weight cannot show of a step is kept for the next ones."""
+    dtype, u = TYPES[kind]
+    A = layer(dtype)
+    was = A.gate.detach().float()
+    # an element of an update is at most 1.3 and some 0.08, of a weight some 1, whose neighbours are 2 u away:
+    # one step moves hardly any, 64 most
+    a = X.OrthogonalMomentum(A, lr=u / 4, momentum=0.0, nesterov=False)
+    for _ in range(64):
+        gradients(A, 0)
+        a.step()
+        assert torch.equal(a.state[A.gate]["master"].to(dtype), A.gate.detach())
+    moved = A.gate.detach().float() - was
+    assert (moved != 0).float().mean() > 0.5
 
 
 @pytest.mark.parametrize("kind", list(TYPES))

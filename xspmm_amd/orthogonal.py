@@ -86,7 +86,8 @@ class OrthogonalMomentum(torch.optim.Optimizer):
       w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / columns)) orthogonalize(u)
 
     The size of u does not matter, however small.  v and, for 16-bit weights, a master
-    copy of w are kept in fp32."""
+    copy of w are kept in fp32; where a weight is not what its copy rounds to, as after
+    loading another, the weight counts."""
 
     def __init__(self, layers, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
         layers = [layers] if isinstance(layers, torch.nn.Module) else list(layers)
@@ -148,6 +149,8 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                 u = u.to(W.dtype, copy=True)
                 orthogonalize(W, u, steps=group["steps"], eps=eps, out=u)
                 master = state.get("master", p)
+                if master is not p:  # values that the weight has been given since the last step count
+                    master.copy_(torch.where(master.to(p.dtype) == p, master, p.float()))
                 if group["weight_decay"]:
                     master.mul_(1 - lr * group["weight_decay"])
                 rows, columns = W.shape
