@@ -137,6 +137,37 @@ def _scratch(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
+class _Positions:
+    """Where a weight's blocks stand, as the library holds it, for all that use it: the
+    handle ``h`` lasts until the last of them goes or one is closed (None from then on)."""
+
+    def __init__(self, shape, grid, row_ptr, col_ind):
+        self.h = None
+        self.made_of = shape, grid, row_ptr, col_ind
+        self._L = _load()
+        h = C.c_void_p()
+        with torch.cuda.device(row_ptr.device):
+            X._check(self._L.xspmm_weight_create(X.icode(row_ptr.dtype), *shape, *grid, int(col_ind.numel()),
+                                                 X._ptr(row_ptr), X._ptr(col_ind), _raw_stream(row_ptr.device.index),
+                                                 C.byref(h)))
+        self.h = h
+
+    def close(self):
+        if self.h is not None:
+            self._L.xspmm_weight_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __reduce__(self):
+        # copies lay the blocks out again: two that held one handle would free it twice
+        return _Positions, self.made_of
+
+
 class SparseWeight:
     """Where the 16x16 blocks of a BCSR matrix stand, laid out once for products
     with the matrix and with its transpose.  The positions are read once, here,
@@ -146,7 +177,7 @@ class SparseWeight:
     is; and a call can bring its own (``values=``)."""
 
     def __init__(self, A):
-        self._h = self._own = None
+        self._h = self._own = self._positions = None
         if A.r_block != 16 or A.c_block != 16:
             raise ValueError("a weight has 16x16 blocks")
         if A.values.dtype not in _TYPES:
@@ -166,13 +197,9 @@ class SparseWeight:
         self.matrix = A
         self._flat = (self.num_blocks * 256,)
         _check(A.values, "values", (self.num_blocks * 256,), self.dtype, device)
-        h = C.c_void_p()
         self._L = _load()
-        with torch.cuda.device(device):
-            X._check(self._L.xspmm_weight_create(X.icode(rp.dtype), *self.shape, int(A.num_block_rows),
-                                                 int(A.num_block_cols), self.num_blocks, X._ptr(rp), X._ptr(ci),
-                                                 _raw_stream(device.index), C.byref(h)))
-        self._h = h
+        self._positions = _Positions(self.shape, (int(A.num_block_rows), int(A.num_block_cols)), rp, ci)
+        self._h = self._positions.h
 
     @property
     def values(self):
@@ -194,18 +221,12 @@ class SparseWeight:
         return v, _check(v, "values", self._flat, self.dtype, self.device)
 
     def close(self):
-        if self._h is not None:
-            self._L.xspmm_weight_destroy(self._h)
-            self._h = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+        self._h = None
+        if self._positions is not None:
+            self._positions.close()
 
     def __reduce__(self):
-        # copies lay their matrix out again: two that held one handle would free it twice
+        # copies lay their matrix out again
         return SparseWeight, (self.matrix,), {"_own": self._own}
 
 

@@ -73,14 +73,16 @@ class Int8Weight:
     """The block values of a SparseWeight in 8 bits, with a scale for each row:
     ``values`` (num_blocks * 256 whole numbers, where the weight's values stand) and
     ``scale`` (fp32, one for each row).  Made once from the weight's values or from
-    others (``values=``), which are not kept; the weight is, for its positions."""
+    others (``values=``).  Neither they nor the weight are kept, only where its blocks
+    stand: the values' memory is free when the weight goes.  Closing the weight closes
+    what was made from it."""
 
     def __init__(self, W, values=None):
         if not isinstance(W, SparseWeight):
             raise TypeError("W must be a SparseWeight")
         _, vals = W._values(None if values is None else values.detach())
-        self.weight = W
         self.shape, self.dtype, self.device, self.num_blocks = W.shape, W.dtype, W.device, W.num_blocks
+        self._positions, self._code = W._positions, W.code
         self.values = torch.empty(W.num_blocks * 256, dtype=torch.int8, device=W.device)
         self.scale = torch.empty(W.shape[0], dtype=torch.float32, device=W.device)
         self._flat, self._rows = (W.num_blocks * 256,), (W.shape[0],)
@@ -88,9 +90,10 @@ class Int8Weight:
               self.scale.data_ptr() or None)
 
     def _operands(self):
-        if self.weight._h is None:
+        h = self._positions.h
+        if h is None:
             raise RuntimeError("SparseWeight is closed")
-        return (_check(self.values, "values", self._flat, torch.int8, self.device),
+        return (h, _check(self.values, "values", self._flat, torch.int8, self.device),
                 _check(self.scale, "scale", self._rows, torch.float32, self.device, 3))
 
 
@@ -178,14 +181,14 @@ def int8_linear(W, x, bias=None, activation=None, residual=None, out=None):
     from every operand, or the residual itself."""
     act = _activation(activation)
     (M, K), dt, dev = W.shape, W.dtype, W.device
-    vals, scale = W._operands()
+    h, vals, scale = W._operands()
     N, xp, q, s, ws, n, held = _tokens(x, 1, M, K, dt, dev)
     bp = None if bias is None else _check(bias, "bias", (M,), dt, dev, 0)
     rp = None if residual is None else _check(residual, "residual", (M, N), dt, dev)
     _no_gradients(None if held is x else x, bias, residual)
     y, yp = _result(out, M, N, dt, dev, **({} if out is None else dict(
         residual=residual, bias=bias, values=W.values, scale=W.scale, **_parts(x))))
-    _call(dev.index, _load().xspmm_int8_linear, W.weight._h, W.weight.code, act, vals, scale, xp, q, s, bp, rp, yp, N,
+    _call(dev.index, _load().xspmm_int8_linear, h, W._code, act, vals, scale, xp, q, s, bp, rp, yp, N,
           ws, n)
     return y
 
@@ -196,7 +199,7 @@ def int8_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", out=Non
     operand."""
     act = _activation(activation)
     (M, K), dt, dev = _pair(G, U), G.dtype, G.device
-    (gv, gs), (uv, us) = G._operands(), U._operands()
+    (gh, gv, gs), (uh, uv, us) = G._operands(), U._operands()
     N, xp, q, s, ws, n, held = _tokens(x, 2, M, K, dt, dev)
     gb = None if bias_gate is None else _check(bias_gate, "bias_gate", (M,), dt, dev, 0)
     ub = None if bias_up is None else _check(bias_up, "bias_up", (M,), dt, dev, 0)
@@ -204,7 +207,7 @@ def int8_gated(G, U, x, bias_gate=None, bias_up=None, activation="silu", out=Non
     h, hp = _result(out, M, N, dt, dev, **({} if out is None else dict(
         bias_gate=bias_gate, bias_up=bias_up, gate=G.values, gate_scale=G.scale, up=U.values, up_scale=U.scale,
         **_parts(x))))
-    _call(dev.index, _load().xspmm_int8_gated, G.weight._h, U.weight._h, G.weight.code, act, gv, gs, uv, us, xp, q, s,
+    _call(dev.index, _load().xspmm_int8_gated, gh, uh, G._code, act, gv, gs, uv, us, xp, q, s,
           gb, ub, hp, N, ws, n)
     return h
 
