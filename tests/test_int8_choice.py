@@ -1,0 +1,83 @@
+"""Which kernel a product in 8-bit integers takes, asked of the library (no GPU is)."""
+from __future__ import annotations
+
+import ctypes as C
+import itertools
+import re
+import shutil
+import subprocess
+
+import pytest
+
+import xspmm_amd as X
+from test_feed_forward_capi import refused
+
+FEW, WALK, LISTS, TILES = range(4)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from xspmm_amd import int8
+
+    return int8._load()
+
+
+def blocks(M, K, density):
+    return round(-(-M // 16) * -(-K // 16) * density)
+
+
+def chosen(lib, weights, M, K, N, density, up=None, quantized=False):
+    """(kernel, its two numbers) of a product of weights with that share of their blocks."""
+    k = (C.c_int32 * 3)(-1, -1, -1)
+    up = blocks(M, K, density if up is None else up) if weights == 2 else 0
+    X._check(lib.xspmm_int8_kernel(weights, M, K, N, blocks(M, K, density), up, int(quantized), k))
+    return tuple(k)
+
+
+SIDES = (16, 200, 1000, 2048, 4096, 7000, 9000, 14336, 20000, 33000, 70000)
+NS = (1, 2, 5, 16, 17, 31, 33, 64, 100, 256, 700, 1100, 2048, 9000)
+
+
+def test_every_kernel_that_is_built_can_be_chosen(lib):
+    """And no other is chosen."""
+    if not shutil.which("nm"):
+        pytest.skip("needs nm")
+    names = subprocess.run(["nm", X.LIB_PATH], check=True, capture_output=True, text=True).stdout
+    built = {}
+    for kernel, value, rest in re.findall(r"__device_stub__ff_int8_(few|walk|list|tile)_kernelI(f|DF16_|DF16b)((?:L[ib]\d+E)+)E",
+                                          names):
+        built.setdefault(value, set()).add((kernel, *(int(n) for n in re.findall(r"\d+", rest))))
+    assert len(built) == 3
+    wanted = set()
+    for weights, M, K, N, density, quantized in itertools.product(
+            (1, 2), SIDES, SIDES, NS, (0.01, 0.03, 0.1, 0.3, 0.7, 1.0), (False, True)):
+        kernel, a, b = chosen(lib, weights, M, K, N, density, quantized=quantized)
+        wanted.add({FEW: ("few", weights, a, b, N == 1), WALK: ("walk", a, weights, b), LISTS: ("list", weights - 1, a),
+                    TILES: ("tile", weights - 1)}[kernel])
+    for of in built.values():
+        assert of == wanted, (sorted(of - wanted), sorted(wanted - of))
+
+
+def test_what_windows_need(lib):
+    """Lists and tiles take weights with a map of their grid, and at most 2^21 tokens."""
+    windows = lambda *a, **k: chosen(lib, *a, **k)[0] in (LISTS, TILES)
+    assert windows(1, 14336, 4096, 2048, 0.2) and windows(1, 14336, 4096, 2048, 1.0)
+    # a weight without blocks, or with hardly any, has none
+    assert not windows(2, 14336, 4096, 2048, 0.2, up=0.0) and not windows(2, 14336, 4096, 2048, 0.01, up=0.5)
+    for density in (0.2, 1.0):
+        assert windows(1, 64, 48, 1 << 21, density) and not windows(1, 64, 48, (1 << 21) + 1, density)
+    # 2^31 bytes of blocks, 2^24 blocks of a grid
+    assert not windows(1, 16 * 2900, 16 * 2900, 2048, 1.0) and windows(1, 16 * 2800, 16 * 2800, 2048, 1.0)
+    assert windows(1, 16 * 4096, 16 * 4096, 2048, 0.3) and not windows(1, 16 * 4097, 16 * 4096, 2048, 0.3)
+
+
+def test_refusals(lib):
+    k = (C.c_int32 * 3)()
+    call = lambda weights, M, K, N, a, b, out=k: lambda: lib.xspmm_int8_kernel(weights, M, K, N, a, b, 0, out)
+    assert "null" in refused(lib, call(1, 64, 64, 1, 4, 0, None))
+    assert "one weight or two" in refused(lib, call(0, 64, 64, 1, 4, 0))
+    assert "one weight or two" in refused(lib, call(3, 64, 64, 1, 4, 4))
+    for M, K, N in ((0, 64, 1), (64, 64, 0), (-1, 64, 1), (64, -1, 1), (64, 133137, 1), (1 << 30, 64, 1), (64, 64, 1 << 31)):
+        assert "size" in refused(lib, call(1, M, K, N, 0, 0))
+    for a, b in ((17, 0), (-1, 0), (4, 17), (4, -1)):
+        assert "blocks" in refused(lib, call(2, 64, 64, 1, a, b))

@@ -874,6 +874,24 @@ int xspmm_int8_scratch(int weights, int64_t M, int64_t K, int64_t N, int64_t* by
     });
 }
 
+int xspmm_int8_kernel(int weights, int64_t M, int64_t K, int64_t N, int64_t blocks, int64_t up_blocks, int quantized,
+                      int32_t* kernel)
+{
+    return guarded([&] {
+        require(kernel != nullptr, "xspmm_int8_kernel: kernel is null.");
+        require(weights == 1 || weights == 2, "xspmm_int8_kernel: a product has one weight or two.");
+        require_tokens(K, N);
+        require(M > 0 && N > 0 && K <= kInt8MostFeatures && M <= (int64_t(1) << 30) - 64, "xSpMM: bad size of a weight.");
+        const int64_t most = ((M + 15) / 16) * ((K + 15) / 16), both[2] = {blocks, up_blocks};
+        require(blocks >= 0 && blocks <= most && (weights == 1 || (up_blocks >= 0 && up_blocks <= most)),
+                "xspmm_int8_kernel: more blocks than the grid has.");
+        const Int8Choice c = int8_choice(weights, M, K, both, N, !quantized && int8_rounds_itself(weights, M, K, N));
+        kernel[0] = (int32_t)c.kernel;
+        kernel[1] = c.a;
+        kernel[2] = c.b;
+    });
+}
+
 int xspmm_int8_linear(xspmm_weight_t weight, int vtype, int act, const int8_t* q, const float* scale, const void* x,
                       const int8_t* xq, const float* x_scale, const void* bias, const void* residual, void* y, int64_t N,
                       void* scratch, int64_t scratch_bytes, void* stream)

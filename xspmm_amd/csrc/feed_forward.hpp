@@ -103,6 +103,9 @@ inline dim3 launch_grid(int64_t groups, int threads, unsigned sides = 1)
     return dim3((unsigned)groups, sides);
 }
 
+// Whether a weight has a map of its grid of blocks.
+bool has_block_map(int64_t Mb, int64_t Kb, int64_t nnzb);
+
 // Bytes of `rows` rows of N elements where those of whole blocks of rows stay
 // below 2^31, else -1.
 inline int64_t narrow_bytes(int64_t rows, int64_t N, int64_t size)

@@ -21,12 +21,13 @@ namespace xspmm {
 namespace detail {
 namespace ff {
 
-constexpr int kListWide = 64;  // tokens of a workgroup
+constexpr int kListWide = kInt8ListTokens;  // of a workgroup
 constexpr int kListTiles = kListWide / 16;
 constexpr int kListWaves = 8, kListThreads = 64 * kListWaves;
 constexpr int kListRows = 4;     // a wave's block-rows, of both weights
 constexpr int kListSlots = kListRows * kListWaves;
-constexpr int kListWindow = 32;  // block-columns
+static_assert(kListSlots == kInt8ListRows);
+constexpr int kListWindow = kInt8ListColumns;
 constexpr int kListStage = kListWindow * kListWide * 16;
 constexpr int kListAhead = 2;    // rows whose blocks are on their way
 constexpr int kListLanes = 64 / kListRows, kListColumns = kListWindow / kListLanes;  // of a row's list
@@ -226,41 +227,20 @@ void launch_list(const Int8Product<T>& a, int weights, int64_t items, hipStream_
 
 }  // namespace ff
 
-// us, measured at 14336 x 4096, 4096 x 14336 and 2048 x 2048 with 64 to 2048 tokens and 5 to
-// 40 % stored (within a tenth): a window's loads, one after the other, and its blocks, in
-// rounds of two workgroups a CU, a last one of one.
 template <typename T>
-double int8_lists_us(const ff::Int8Product<T>& a, int weights, int64_t blocks)
-{
-    if (!a.side[0].map || (weights == 2 && !a.side[1].map) || a.N > (1 << 21)) return 1e30;
-    if (a.vals_bytes[0] == 0 || (weights == 2 && a.vals_bytes[1] == 0)) return 1e30;
-    const int rows = ff::kListSlots / weights;
-    const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + ff::kListWide - 1) / ff::kListWide);
-    const double share = (double)blocks / ((double)weights * a.block_rows * a.in_blocks);
-    const int64_t rest = items % 512;
-    const double full = 2.7 + 7.5 * share, last = rest == 0 ? 0.0 : rest <= 256 ? 1.75 + 5.5 * share : full;
-    const int64_t windows = (a.in_blocks + ff::kListWindow - 1) / ff::kListWindow;
-    return 6.0 + (double)windows * ((double)(items / 512) * full + last);
-}
-
-template <typename T>
-void int8_lists(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s)
+void int8_lists(const ff::Int8Product<T>& a, int weights, int fours, hipStream_t s)
 {
     const int rows = ff::kListSlots / weights;
     const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + ff::kListWide - 1) / ff::kListWide);
-    // so that four times Q blocks are more than a row has in most windows
-    const double share = (double)blocks / ((double)weights * a.block_rows * a.in_blocks);
-    if (share < 0.06)
+    if (fours == 1)
         ff::launch_list<T, 1>(a, weights, items, s);
-    else if (share < 0.15)
+    else if (fours == 2)
         ff::launch_list<T, 2>(a, weights, items, s);
     else
         ff::launch_list<T, 3>(a, weights, items, s);
 }
 
-#define XSPMM_INT8_LIST(T)                                                       \
-    template double int8_lists_us<T>(const ff::Int8Product<T>&, int, int64_t);     \
-    template void int8_lists<T>(const ff::Int8Product<T>&, int, int64_t, hipStream_t);
+#define XSPMM_INT8_LIST(T) template void int8_lists<T>(const ff::Int8Product<T>&, int, int, hipStream_t);
 XSPMM_INT8_LIST(float)
 XSPMM_INT8_LIST(_Float16)
 XSPMM_INT8_LIST(__bf16)

@@ -118,7 +118,8 @@ __global__ __launch_bounds__(64 * (SPLIT > 4 ? SPLIT : 4)) void ff_int8_walk_ker
 // Few tokens and few features: a workgroup rounds its (up to 16) tokens itself, into LDS,
 // with its first blocks on their way meanwhile, and then walks ROWS block-rows, 16 /
 // ROWS waves to each.
-constexpr int kFewTokens = 16, kFewThreads = 1024;
+constexpr int kFewTokens = kInt8FewTokens, kFewThreads = 1024;
+static_assert(kInt8FewPieces == kFewThreads);
 
 // KEPT: such blocks of a thread
 template <typename T, int NACC, int ROWS, int KEPT, bool ONE>
@@ -257,17 +258,12 @@ __global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_ke
     a.y[row * a.N + n0 + li] = (T)int8_finish<T, NACC>(a, sum, row, n0 + li, scales[li]);
 }
 
-template <typename T, int NACC, int ROWS>
+template <typename T, int NACC, int ROWS, int KEPT, bool ONE>
 void launch_few(const Int8Product<T>& a, hipStream_t s)
 {
     const int64_t items = (int64_t)((a.block_rows + ROWS - 1) / ROWS) * ((a.N + kFewTokens - 1) / kFewTokens);
-    const dim3 grid = launch_grid(items, kFewThreads), threads(kFewThreads);
-    if (a.N > 1)
-        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, 1, false>), grid, threads, 0, s, a);
-    else if (a.in_blocks <= kFewThreads)
-        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, 1, true>), grid, threads, 0, s, a);
-    else
-        hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, 2, true>), grid, threads, 0, s, a);
+    hipLaunchKernelGGL((ff_int8_few_kernel<T, NACC, ROWS, KEPT, ONE>), launch_grid(items, kFewThreads), dim3(kFewThreads), 0, s,
+                       a);
     XSPMM_LAUNCH_CHECK();
 }
 
@@ -281,31 +277,37 @@ void launch_walk(const Int8Product<T>& a, hipStream_t s)
     XSPMM_LAUNCH_CHECK();
 }
 
+// What int8_choice has chosen: no other kernels are built.
 template <typename T, int NACC>
-void launch_int8(const Int8Product<T>& a, int64_t blocks, hipStream_t s)
+void launch_few(const Int8Product<T>& a, const Int8Choice& c, hipStream_t s)
 {
-    if (a.raw) {
-        // Sixteen waves to a block-row while there are no more than two workgroups a CU
-        // (16 waves each), half and a quarter of them beyond (us of one and two rows a
-        // workgroup: fp16 4096 x 14336, 25 % stored, one token 6.7 and 7.8; bf16 gate and
-        // up of 14336 x 4096 13.0 and 10.1, of four rows 10.3).
-        const int64_t groups = a.block_rows * ((a.N + kFewTokens - 1) / kFewTokens);
-        if (groups <= 512)
-            launch_few<T, NACC, 1>(a, s);
-        else if (groups <= 1024)
-            launch_few<T, NACC, 2>(a, s);
+    auto one = [&](auto rows) {
+        constexpr int R = decltype(rows)::value;
+        c.b == 1 ? launch_few<T, NACC, R, 1, true>(a, s) : launch_few<T, NACC, R, 2, true>(a, s);
+    };
+    if (a.N == 1) {
+        if (c.a == 1)
+            one(std::integral_constant<int, 1>{});
+        else if (c.a == 2)
+            one(std::integral_constant<int, 2>{});
         else
-            launch_few<T, NACC, 4>(a, s);
-        return;
+            one(std::integral_constant<int, 4>{});
+    } else if (NACC == 2 || c.a == 1) {
+        launch_few<T, NACC, 1, 1, false>(a, s);
+    } else if constexpr (NACC == 1) {
+        launch_few<T, NACC, 2, 1, false>(a, s);
     }
-    auto waves = [&](int v) { return (int64_t)a.block_rows * ((a.N + 16 * v - 1) / (16 * v)); };
-    const int64_t each = blocks / a.block_rows;
-    if (a.N > 32 && waves(4) >= 256) {
-        if (waves(4) < 4096 && each >= 16)
+}
+
+template <typename T, int NACC>
+void launch_walk(const Int8Product<T>& a, const Int8Choice& c, hipStream_t s)
+{
+    if (c.a == 4) {
+        if (c.b == 4)
             launch_walk<T, 4, NACC, 4>(a, s);
         else
             launch_walk<T, 4, NACC, 1>(a, s);
-    } else if (waves(1) <= 512 && each >= 64) {
+    } else if (c.b == 16) {
         launch_walk<T, 1, NACC, 16>(a, s);
     } else {
         launch_walk<T, 1, NACC, 4>(a, s);
@@ -314,31 +316,19 @@ void launch_int8(const Int8Product<T>& a, int64_t blocks, hipStream_t s)
 
 }  // namespace ff
 
-// One token, and more where every workgroup's rounding them anew costs less than a launch:
-// us with and without, bf16, 16384 x 1024 30 % stored 16 tokens 10.4 and 11.1, 48 tokens 15.7
-// and 10.9; gate and up of 14336 x 4096 25 % stored one token 10.0 and 12.6, two 16.9 and
-// 13.6; 4096 x 4096 10 % stored four tokens 8.5 and 11.1.
-bool int8_rounds_itself(int weights, int64_t M, int64_t K, int64_t N)
-{
-    const int64_t Mb = (M + 15) / 16, Kb = (K + 15) / 16;
-    if (N == 1) return Kb <= 2 * ff::kFewThreads;
-    const int64_t tokens = N < ff::kFewTokens ? N : ff::kFewTokens, tiles = (N + ff::kFewTokens - 1) / ff::kFewTokens;
-    return Kb * tokens <= ff::kFewThreads && weights * Mb * tiles <= 1024;
-}
-
 template <typename T>
 void int8_product(const Int8Args<T>& f, int weights, hipStream_t s)
 {
     const BlockIndex& w = *f.weight[0];
     if (w.Mb == 0 || f.N == 0) return;
     ff::Int8Product<T> a{};
-    int64_t blocks = 0;
+    int64_t blocks[2] = {};
     for (int l = 0; l < weights; ++l) {
         const BlockIndex& wl = *f.weight[l];
         a.side[l] = {wl.ptr, wl.col, wl.map, f.vals[l], f.scale[l], f.bias[l]};
         const int64_t vb = narrow_bytes(wl.nnzb, 256, 1);
         a.vals_bytes[l] = vb < 0 ? 0u : (uint32_t)vb;
-        blocks += wl.nnzb;
+        blocks[l] = wl.nnzb;
     }
     a.raw = f.raw;
     a.x = f.x;
@@ -351,27 +341,21 @@ void int8_product(const Int8Args<T>& f, int weights, hipStream_t s)
     a.block_rows = (int32_t)w.Mb;
     a.N = f.N;
     a.act = f.act;
-    if (!a.raw) {
-        // The walk by blocks, whose x comes through L1, and results: 14336 x 4096 and 2048
-        // tokens 48 us at 5 % stored, 117 at 25 %, 370 with all.  The others have a chain of
-        // loads for every window of x: they pay where there are tokens enough, lists up to
-        // some 45 % stored (90 us at 40 %, tiles 103), tiles from there on (119; lists
-        // of 4096 x 14336 114 at 40 %, tiles 118).
-        const double walk = 5.0 + 7.4e-7 * (double)blocks * (double)a.N + 7e-7 * (double)weights * (double)w.M * (double)a.N;
-        const double lists = int8_lists_us<T>(a, weights, blocks), tiles = int8_tiles_us<T>(a, weights, blocks);
-        if (lists < walk && lists <= tiles) {
-            int8_lists<T>(a, weights, blocks, s);
-            return;
-        }
-        if (tiles < walk) {
-            int8_tiles<T>(a, weights, s);
-            return;
-        }
+    const Int8Choice c = int8_choice(weights, w.M, w.K, blocks, f.N, a.raw != nullptr);
+    switch (c.kernel) {
+    case Int8Kernel::kLists:
+        int8_lists<T>(a, weights, c.a, s);
+        break;
+    case Int8Kernel::kTiles:
+        int8_tiles<T>(a, weights, s);
+        break;
+    case Int8Kernel::kFew:
+        weights == 2 ? ff::launch_few<T, 2>(a, c, s) : ff::launch_few<T, 1>(a, c, s);
+        break;
+    case Int8Kernel::kWalk:
+        weights == 2 ? ff::launch_walk<T, 2>(a, c, s) : ff::launch_walk<T, 1>(a, c, s);
+        break;
     }
-    if (weights == 2)
-        ff::launch_int8<T, 2>(a, blocks, s);
-    else
-        ff::launch_int8<T, 1>(a, blocks, s);
 }
 
 #define XSPMM_INT8_PRODUCT(T) template void int8_product<T>(const Int8Args<T>&, int, hipStream_t);

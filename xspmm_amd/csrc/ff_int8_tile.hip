@@ -21,10 +21,11 @@ namespace xspmm {
 namespace detail {
 namespace ff {
 
-constexpr int kI8Wide = 128;               // tokens of a workgroup
+constexpr int kI8Wide = kInt8TileTokens;   // of a workgroup
 constexpr int kI8Waves = 4, kI8Threads = 64 * kI8Waves;
 constexpr int kI8Rows = 4;                 // a wave's block-rows, of both weights
 constexpr int kI8Slots = kI8Rows * kI8Waves;
+static_assert(kI8Slots == kInt8TileRows);
 constexpr int kI8Tiles = kI8Wide / 16;
 constexpr int kI8Window = 16;              // block-columns
 constexpr int kI8Stage = kI8Window * kI8Wide * 16;
@@ -209,21 +210,6 @@ __global__ __launch_bounds__(kI8Threads, 2) void ff_int8_tile_kernel(const Int8P
 
 }  // namespace ff
 
-// us, as int8_lists_us: a step of four block-columns, whose loads take most of it whatever
-// is stored.
-template <typename T>
-double int8_tiles_us(const ff::Int8Product<T>& a, int weights, int64_t blocks)
-{
-    if (!a.side[0].map || (weights == 2 && !a.side[1].map) || a.N > (1 << 21)) return 1e30;
-    if (a.vals_bytes[0] == 0 || (weights == 2 && a.vals_bytes[1] == 0)) return 1e30;
-    const int rows = ff::kI8Slots / weights;
-    const int64_t items = (int64_t)((a.block_rows + rows - 1) / rows) * ((a.N + ff::kI8Wide - 1) / ff::kI8Wide);
-    const double share = (double)blocks / ((double)weights * a.block_rows * a.in_blocks);
-    const int64_t rest = items % 512;
-    const double full = 0.6 + 0.3 * share, last = rest == 0 ? 0.0 : rest <= 256 ? 0.42 + 0.2 * share : full;
-    return 8.0 + (double)((a.in_blocks + 3) / 4) * ((double)(items / 512) * full + last);
-}
-
 template <typename T>
 void int8_tiles(const ff::Int8Product<T>& a, int weights, hipStream_t s)
 {
@@ -237,9 +223,7 @@ void int8_tiles(const ff::Int8Product<T>& a, int weights, hipStream_t s)
     XSPMM_LAUNCH_CHECK();
 }
 
-#define XSPMM_INT8_TILE(T)                                                       \
-    template double int8_tiles_us<T>(const ff::Int8Product<T>&, int, int64_t);     \
-    template void int8_tiles<T>(const ff::Int8Product<T>&, int, hipStream_t);
+#define XSPMM_INT8_TILE(T) template void int8_tiles<T>(const ff::Int8Product<T>&, int, hipStream_t);
 XSPMM_INT8_TILE(float)
 XSPMM_INT8_TILE(_Float16)
 XSPMM_INT8_TILE(__bf16)

@@ -136,11 +136,14 @@ __global__ __launch_bounds__(256) void ff_fill_kernel(int32_t* __restrict__ p, i
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = v;
 }
 
+}  // namespace
+
 // The tile kernels' map costs 4 bytes for every block of the grid, stored or
 // not: worth it up to 64 MB where at least one block in 64 is stored.
-bool wants_map(int64_t Mb, int64_t Kb, int64_t nnzb) { return Mb * Kb <= (1 << 24) && nnzb * 64 >= Mb * Kb && nnzb > 0; }
-
-}  // namespace
+bool has_block_map(int64_t Mb, int64_t Kb, int64_t nnzb)
+{
+    return Mb * Kb <= (1 << 24) && nnzb * 64 >= Mb * Kb && nnzb > 0;
+}
 
 template <typename I>
 void build_block_index(BlockIndex& out, int64_t M, int64_t K, int64_t Mb, int64_t Kb, int64_t nnzb, const I* brp,
@@ -167,7 +170,7 @@ void build_block_index(BlockIndex& out, int64_t M, int64_t K, int64_t Mb, int64_
     const size_t o_bad = c.take(4);
     const size_t o_gptr = c.take((size_t)(Mb + 1) * 4);
     const size_t o_group = c.take((size_t)(nnzb / kGroupBlocks + (Mb < nnzb ? Mb : nnzb)) * 4);
-    const bool map = wants_map(Mb, Kb, nnzb);
+    const bool map = has_block_map(Mb, Kb, nnzb);
     const size_t o_map = c.take(map ? (size_t)(Mb * Kb) * 4 : 0);
     XSPMM_HIP_CHECK(hipMalloc(&out.memory, c.end));
     char* p = static_cast<char*>(out.memory);

@@ -40,6 +40,26 @@ struct Int8Args {
 };
 // Whether a product of N tokens rounds them itself, without memory for the result.
 bool int8_rounds_itself(int weights, int64_t M, int64_t K, int64_t N);
+
+// What the kernels take at a time: few tokens' workgroups 16 tokens and 1024 pieces of 16
+// features; lists and tiles some block-rows (of both weights), tokens and block-columns.
+constexpr int kInt8FewTokens = 16, kInt8FewPieces = 1024;
+constexpr int kInt8ListRows = 32, kInt8ListTokens = 64, kInt8ListColumns = 32;
+constexpr int kInt8TileRows = 16, kInt8TileTokens = 128, kInt8TileColumns = 4;
+
+// Which kernel a product takes, by its sizes alone.
+enum class Int8Kernel {
+    kFew,    // tokens rounded within: `a` block-rows a workgroup, `b` pieces of a token a thread
+    kWalk,   // `a` tiles of 16 tokens a wave, `b` waves to a block-row
+    kLists,  // the first `a` fours of blocks of a row are fetched ahead
+    kTiles
+};
+struct Int8Choice {
+    Int8Kernel kernel;
+    int a, b;
+};
+// M x K, blocks of each weight, N tokens; whether the product rounds them
+Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks, int64_t N, bool rounds);
 template <typename T>
 void int8_product(const Int8Args<T>& a, int weights, hipStream_t s);
 

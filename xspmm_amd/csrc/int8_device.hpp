@@ -274,14 +274,10 @@ __device__ __forceinline__ void int8_rows(const Int8Product<T>& a, const float* 
 
 }  // namespace ff
 
-// The product by lists of blocks, and by tiles, both with x in LDS: the time to expect (us;
-// past any other where it does not apply) and the launch.
+// The products by lists of blocks (the first `fours` of a row fetched ahead) and by tiles,
+// both with x in LDS.
 template <typename T>
-double int8_lists_us(const ff::Int8Product<T>& a, int weights, int64_t blocks);
-template <typename T>
-void int8_lists(const ff::Int8Product<T>& a, int weights, int64_t blocks, hipStream_t s);
-template <typename T>
-double int8_tiles_us(const ff::Int8Product<T>& a, int weights, int64_t blocks);
+void int8_lists(const ff::Int8Product<T>& a, int weights, int fours, hipStream_t s);
 template <typename T>
 void int8_tiles(const ff::Int8Product<T>& a, int weights, hipStream_t s);
 
