@@ -188,20 +188,40 @@ struct TokenPlan {
     int32_t slices;
 };
 
-TokenPlan token_plan(int64_t K, int64_t N)
+// size: bytes of a value.  us, bf16 and fp32, of whole tokens by four lanes (4) and sixteen
+// (16), and in slices by sixteen (s16), by 64 (s64) and by 64 of four tokens (s64x4):
+//   4999 x 31      8.6 and 8.1 (4), 12.3 and 10.6 (s16)
+//   2048 x 128     7.3 and 5.7 (4), 9.8 and 6.8 (16), 10.8 and 9.0 (s64)
+//   4096 x 128     8.2 (4), 11.1 (s64); 4096 x 512 13.5 and 16.9 (4), 11.0 and 9.9 (s64)
+//   6000 x 63      9.4 and 13.5 (4), 11.1 and 9.6 (s16)
+//   1024 x 1500    11.7 and 11.9 (4), 8.2 and 8.0 (16), 10.9 and 9.9 (s64)
+//   1024 x 16384   32.7 and 27.0 (16), 25.3 and 27.7 (s64)
+//   14336 x 512    15.5 and 15.8 (s16), 14.5 and 14.9 (s64), 18.2 and 22.0 (s64x4)
+//   14336 x 8192   152 and 216 (s64), 139 and 222 (s64x4)
+// Whole tokens read x once, as long as there are workgroups enough and a thread's segments of
+// a row, eight bytes with four lanes, come from L1 again.
+TokenPlan token_plan(int64_t K, int64_t N, int size)
 {
     TokenPlan p{};
     const int64_t Kb = (K + 15) / 16;
     auto tiles = [&](int lanes, int vec) { return (N + lanes * vec - 1) / (lanes * vec); };
     p.vec = 1;
-    p.lanes = N < 64 ? 4 : 16;
-    p.whole = (N == 1 && K <= kOneMost) || (N > 1 && N <= 1024 && Kb * p.lanes <= kKept * 1024);
+    if (N == 1) {
+        p.lanes = 1;
+        p.whole = K <= kOneMost;
+    } else if (Kb * 4 <= kKept * 1024 && N <= 1024 && K * N * size <= 5 << 18) {
+        p.lanes = 4;
+        p.whole = true;
+    } else if (Kb <= 96 && N <= 8192) {  // (Kb * 16 <= kKept * 1024)
+        p.lanes = 16;
+        p.whole = true;
+    }
     if (p.whole) {
         p.tiles = tiles(p.lanes, 1);
         return p;
     }
-    p.lanes = N == 1 ? 1 : N < 64 ? 16 : 64;
-    if (N >= 512) p.vec = 4;
+    if (N > 1) p.lanes = N < 64 ? 16 : 64;
+    if (N >= 256 && size == 2 && K * N > 1 << 24) p.vec = 4;
     p.tiles = tiles(p.lanes, p.vec);
     const int each = kSliceThreads / p.lanes;
     const int64_t want = (256 + p.tiles - 1) / p.tiles, most = (Kb + each - 1) / each;
@@ -235,8 +255,12 @@ void int8_weight(const BlockIndex& w, const T* vals, int8_t* q, float* scale, hi
 int64_t quantize_tokens_scratch(int64_t K, int64_t N)
 {
     if (K == 0 || N == 0) return 0;
-    const ff::TokenPlan p = ff::token_plan(K, N);
-    return p.whole ? 0 : (int64_t)p.slices * N * 4;
+    int64_t most = 0;  // of any type
+    for (int size : {2, 4}) {
+        const ff::TokenPlan p = ff::token_plan(K, N, size);
+        if (!p.whole && p.slices * N * 4 > most) most = p.slices * N * 4;
+    }
+    return most;
 }
 
 namespace ff {
@@ -256,7 +280,7 @@ void quantize_tokens(const T* x, int8_t* q, float* scale, int64_t K, int64_t N, 
         XSPMM_LAUNCH_CHECK();
         return;
     }
-    const ff::TokenPlan p = ff::token_plan(K, N);
+    const ff::TokenPlan p = ff::token_plan(K, N, (int)sizeof(T));
     if (p.whole) {
         const dim3 grid = launch_grid(p.tiles, 1024);
         if (N == 1)
@@ -268,14 +292,18 @@ void quantize_tokens(const T* x, int8_t* q, float* scale, int64_t K, int64_t N, 
         XSPMM_LAUNCH_CHECK();
         return;
     }
-    if (p.vec == 4)
-        ff::launch_tokens<T, 4, 64>(x, q, scale, K, N, scratch, p, s);
-    else if (p.lanes == 64)
+    if (p.lanes == 64) {
+        if constexpr (sizeof(T) == 2)
+            if (p.vec == 4) {
+                ff::launch_tokens<T, 4, 64>(x, q, scale, K, N, scratch, p, s);
+                return;
+            }
         ff::launch_tokens<T, 1, 64>(x, q, scale, K, N, scratch, p, s);
-    else if (p.lanes == 16)
+    } else if (p.lanes == 16) {
         ff::launch_tokens<T, 1, 16>(x, q, scale, K, N, scratch, p, s);
-    else
+    } else {
         ff::launch_tokens<T, 1, 1>(x, q, scale, K, N, scratch, p, s);
+    }
 }
 
 #define XSPMM_INT8(T)                                                                            \
