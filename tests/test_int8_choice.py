@@ -92,3 +92,23 @@ def test_tokens_launches(lib, K, N, launches):
     n = C.c_int64(-1)
     assert lib.xspmm_quantize_tokens_scratch(K, N, C.byref(n)) == X.OK
     assert (n.value > 0) == (launches == 2)
+
+
+# the walk's widths and splits at sizes where it is chosen: us of 1 tile and 4 waves, 1 and 16, 4 and 1, 4 and 4
+WALKS = [
+    (1, 14336, 4096, 64, 0.03, (5.65, 13.28, 7.31, 4.55)), (2, 14336, 4096, 64, 0.03, (7.01, 18.07, 10.15, 5.8)),
+    (1, 5003, 4999, 31, 0.8, (12.83, 11.91, 21.14, 8.67)), (1, 4096, 14336, 31, 0.3, (12.96, 9.35, 23.93, 8.51)),
+    (2, 2048, 2048, 96, 0.06, (3.93, 6.17, 9.71, 4.87)), (2, 512, 8192, 512, 0.015, (4.08, 6.95, 9.63, 4.87)),
+    (1, 512, 8192, 300, 0.8, (16.44, 12.11, 55.87, 17.18)), (2, 1024, 1024, 300, 0.1, (4.35, 8.25, 9.69, 5.16)),
+    (1, 16384, 1024, 96, 0.1, (7.61, 20.72, 7.83, 6.69)), (1, 14336, 4096, 2, 0.8, (12.14, 11.52, 27.25, 13.35)),
+    (1, 4096, 14336, 33, 0.2, (11.07, 10.81, 18.54, 7.1)), (2, 4096, 14336, 24, 0.3, (21.85, 14.39, 72.98, 21.98)),
+    (2, 50000, 300, 24, 0.06, (9.14, 28.01, 7.14, 10.83)),
+]
+
+
+@pytest.mark.parametrize("weights,M,K,N,density,times", WALKS)
+def test_walks(lib, weights, M, K, N, density, times):
+    """The fastest or, of ways that are near to each other, one within a quarter of it."""
+    kernel, a, b = chosen(lib, weights, M, K, N, density, quantized=True)
+    assert kernel == WALK
+    assert times[[(1, 4), (1, 16), (4, 1), (4, 4)].index((a, b))] <= 1.25 * min(times)

@@ -72,10 +72,27 @@ Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks,
         if (lists < walk && lists <= tiles) return {Int8Kernel::kLists, share < 0.06 ? 1 : share < 0.15 ? 2 : 3, 0};
         if (tiles < walk) return {Int8Kernel::kTiles, 0, 0};
     }
-    auto waves = [&](int v) { return Mb * groups_of(N, 16 * v); };
-    const int64_t each = Mb > 0 ? all / Mb : 0;
-    if (N > 32 && waves(4) >= 256) return {Int8Kernel::kWalk, 4, waves(4) < 4096 && each >= 16 ? 4 : 1};
-    return {Int8Kernel::kWalk, 1, waves(1) <= 512 && each >= 64 ? 16 : 4};
+    // us by (tiles of 16 tokens a wave, waves to a block-row):
+    //   sizes, stored, tokens              1, 4   1, 16   4, 1   4, 4
+    //   14336 x 4096,  3 %, 64              5.7   13.3     7.3    4.6
+    //   2048 x 2048,   6 %, 96, gated       3.9    6.2     9.7    4.9
+    //   1024 x 1024,  10 %, 300, gated      4.4    8.3     9.7    5.2
+    //   4096 x 14336, 20 %, 33             11.1   10.8    18.5    7.1
+    //   4096 x 14336, 30 %, 24, gated      21.9   14.4    73.0   22.0
+    //   512 x 8192,   80 %, 300            16.4   12.1    55.9   17.2
+    //   4096 x 14336, 10 %, 1100, gated   124    152      80.3   65.1
+    //   14336 x 4096,  3 %, 2048           93.4  365      42.0   54.4
+    //   50000 x 300,   6 %, 24, gated       9.1   28.0     7.1   10.8
+    // Four tiles of tokens read a block and its column once for 64, and pay as soon as there
+    // are two workgroups of them a CU, with long rows one.  Four waves to a row have a
+    // quarter of the chain of loads, and sums to join: they pay until there are waves enough
+    // without that, the sooner the shorter the rows.  Where there are few workgroups of
+    // one tile, long rows are split over sixteen waves.
+    auto waves = [&](int tiles) { return Mb * groups_of(N, 16 * tiles); };
+    const int64_t each = Mb > 0 ? all / Mb : 0, four = waves(4), one = waves(1);
+    if (N > 16 && (four >= 512 || (each >= 128 && four >= (N > 32 ? 256 : 257))))
+        return {Int8Kernel::kWalk, 4, four < 8192 && four < 2048 + 64 * each ? 4 : 1};
+    return {Int8Kernel::kWalk, 1, (one <= 512 && each >= 64) || (one <= 1024 && each >= 192) ? 16 : 4};
 }
 
 }  // namespace detail
