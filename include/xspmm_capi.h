@@ -525,7 +525,7 @@ int xspmm_int8_linear(xspmm_weight_t weight, int vtype, int act, const int8_t* q
                       void* scratch, int64_t scratch_bytes, void* stream);
 
 /*
- * Which kernel such a product of N tokens runs, by its sizes alone, for reports: of one
+ * Which kernel such a product of N tokens runs, by type and sizes alone, for reports: of one
  * weight of `blocks` blocks, or of two (the other's up_blocks), of tokens that come
  * quantized or not.  kernel[0] is XSPMM_INT8_FEW (tokens rounded within; kernel[1]
  * block-rows a workgroup, kernel[2] pieces of 16 features a thread), XSPMM_INT8_WALK
@@ -533,8 +533,8 @@ int xspmm_int8_linear(xspmm_weight_t weight, int vtype, int act, const int8_t* q
  * fetched ahead) or XSPMM_INT8_TILES.
  */
 enum { XSPMM_INT8_FEW = 0, XSPMM_INT8_WALK = 1, XSPMM_INT8_LISTS = 2, XSPMM_INT8_TILES = 3 };
-int xspmm_int8_kernel(int weights, int64_t M, int64_t K, int64_t N, int64_t blocks, int64_t up_blocks, int quantized,
-                      int32_t* kernel);
+int xspmm_int8_kernel(int weights, int vtype, int64_t M, int64_t K, int64_t N, int64_t blocks, int64_t up_blocks,
+                      int quantized, int32_t* kernel);
 
 /* h = act(G x + gate_bias) * (U x + up_bias) in 8 bits, likewise. */
 int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act, const int8_t* gate_q,

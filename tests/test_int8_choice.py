@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import ctypes as C
 import itertools
+import math
+import os
 import re
 import shutil
 import subprocess
@@ -10,9 +12,10 @@ import subprocess
 import pytest
 
 import xspmm_amd as X
-from test_feed_forward_capi import refused
+from test_feed_forward_capi import BAD, BF16, refused
 
 FEW, WALK, LISTS, TILES = range(4)
+CODES = {"f16": X.F16, "bf16": BF16, "f32": X.F32}
 
 
 @pytest.fixture(scope="module")
@@ -26,11 +29,11 @@ def blocks(M, K, density):
     return round(-(-M // 16) * -(-K // 16) * density)
 
 
-def chosen(lib, weights, M, K, N, density, up=None, quantized=False):
+def chosen(lib, weights, M, K, N, density, up=None, quantized=False, kind="bf16"):
     """(kernel, its two numbers) of a product of weights with that share of their blocks."""
     k = (C.c_int32 * 3)(-1, -1, -1)
     up = blocks(M, K, density if up is None else up) if weights == 2 else 0
-    X._check(lib.xspmm_int8_kernel(weights, M, K, N, blocks(M, K, density), up, int(quantized), k))
+    X._check(lib.xspmm_int8_kernel(weights, CODES[kind], M, K, N, blocks(M, K, density), up, int(quantized), k))
     return tuple(k)
 
 
@@ -73,7 +76,9 @@ def test_what_windows_need(lib):
 
 def test_refusals(lib):
     k = (C.c_int32 * 3)()
-    call = lambda weights, M, K, N, a, b, out=k: lambda: lib.xspmm_int8_kernel(weights, M, K, N, a, b, 0, out)
+    call = lambda weights, M, K, N, a, b, out=k, vtype=X.F16: (
+        lambda: lib.xspmm_int8_kernel(weights, vtype, M, K, N, a, b, 0, out))
+    assert "type" in refused(lib, call(1, 64, 64, 1, 4, 0, vtype=BAD))
     assert "null" in refused(lib, call(1, 64, 64, 1, 4, 0, None))
     assert "one weight or two" in refused(lib, call(0, 64, 64, 1, 4, 0))
     assert "one weight or two" in refused(lib, call(3, 64, 64, 1, 4, 4))
@@ -112,3 +117,26 @@ def test_walks(lib, weights, M, K, N, density, times):
     kernel, a, b = chosen(lib, weights, M, K, N, density, quantized=True)
     assert kernel == WALK
     assert times[[(1, 4), (1, 16), (4, 1), (4, 4)].index((a, b))] <= 1.25 * min(times)
+
+
+def timed():
+    """(weights, type, M, K, N, stored, us of the walk, lists and tiles) of products that were timed."""
+    with open(os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "profiles", "int8_kernel_choice.txt")) as f:
+        for line in f:
+            v = line.split()
+            if len(v) == 9 and v[1] in CODES:
+                yield int(v[0]), v[1], *(int(t) for t in v[2:5]), *(float(t) for t in v[5:])
+
+
+def test_kernels_go_by_their_times(lib):
+    """What is chosen is the fastest, or near to it, at sizes where all three kernels were timed."""
+    ratios = []
+    for weights, kind, M, K, N, density, *us in timed():
+        kernel = chosen(lib, weights, M, K, N, density, quantized=True, kind=kind)[0]
+        ratios.append((us[[WALK, LISTS, TILES].index(kernel)] / min(us), weights, kind, M, K, N, density))
+    assert len(ratios) > 300
+    assert math.prod(r[0] ** (1 / len(ratios)) for r in ratios) < 1.01
+    assert max(ratios)[0] < 1.3, max(ratios)
+    # lists from a tenth on, at the size whose times stand beside the kernels
+    assert [chosen(lib, 1, 14336, 4096, 2048, d, quantized=True)[0] for d in (0.04, 0.1, 0.25, 0.4, 1.0)] == [
+        WALK, LISTS, LISTS, LISTS, TILES]

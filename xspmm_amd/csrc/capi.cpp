@@ -874,7 +874,7 @@ int xspmm_int8_scratch(int weights, int64_t M, int64_t K, int64_t N, int64_t* by
     });
 }
 
-int xspmm_int8_kernel(int weights, int64_t M, int64_t K, int64_t N, int64_t blocks, int64_t up_blocks, int quantized,
+int xspmm_int8_kernel(int weights, int vtype, int64_t M, int64_t K, int64_t N, int64_t blocks, int64_t up_blocks, int quantized,
                       int32_t* kernel)
 {
     return guarded([&] {
@@ -885,7 +885,9 @@ int xspmm_int8_kernel(int weights, int64_t M, int64_t K, int64_t N, int64_t bloc
         const int64_t most = ((M + 15) / 16) * ((K + 15) / 16), both[2] = {blocks, up_blocks};
         require(blocks >= 0 && blocks <= most && (weights == 1 || (up_blocks >= 0 && up_blocks <= most)),
                 "xspmm_int8_kernel: more blocks than the grid has.");
-        const Int8Choice c = int8_choice(weights, M, K, both, N, !quantized && int8_rounds_itself(weights, M, K, N));
+        int size = 0;
+        with_layer_type(vtype, [&](auto tv) { size = (int)sizeof(typename decltype(tv)::type); });
+        const Int8Choice c = int8_choice(weights, M, K, both, N, size, !quantized && int8_rounds_itself(weights, M, K, N));
         kernel[0] = (int32_t)c.kernel;
         kernel[1] = c.a;
         kernel[2] = c.b;

@@ -341,7 +341,7 @@ void int8_product(const Int8Args<T>& f, int weights, hipStream_t s)
     a.block_rows = (int32_t)w.Mb;
     a.N = f.N;
     a.act = f.act;
-    const Int8Choice c = int8_choice(weights, w.M, w.K, blocks, f.N, a.raw != nullptr);
+    const Int8Choice c = int8_choice(weights, w.M, w.K, blocks, f.N, (int)sizeof(T), a.raw != nullptr);
     switch (c.kernel) {
     case Int8Kernel::kLists:
         int8_lists<T>(a, weights, c.a, s);

@@ -58,8 +58,8 @@ struct Int8Choice {
     Int8Kernel kernel;
     int a, b;
 };
-// M x K, blocks of each weight, N tokens; whether the product rounds them
-Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks, int64_t N, bool rounds);
+// M x K, blocks of each weight, N tokens, bytes of a result; whether the product rounds them
+Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks, int64_t N, int size, bool rounds);
 template <typename T>
 void int8_product(const Int8Args<T>& a, int weights, hipStream_t s);
 

@@ -11,22 +11,18 @@ namespace {
 
 int64_t groups_of(int64_t n, int64_t each) { return (n + each - 1) / each; }
 
-// us of lists, measured at 14336 x 4096, 4096 x 14336 and 2048 x 2048 with 64 to 2048 tokens
-// and 5 to 40 % stored (within a tenth): a window's loads, one after the other, and its
-// blocks, in rounds of two workgroups a CU, a last one of one.
-double lists_us(int weights, int64_t Mb, int64_t Kb, int64_t N, double share)
+// us of a kernel with x in LDS: `steps` of a workgroup's windows one after the other, in rounds
+// of two workgroups a CU, of which the last may be one or less; what is stored adds to a
+// step; results in fp32 are written at 3 TB/s more of them.
+struct Steps {
+    double launch, two[2], one[2];  // of a step: none stored, and what all stored adds
+};
+double steps_us(const Steps& t, int64_t items, int64_t steps, double share, double more_bytes)
 {
-    const int64_t items = groups_of(Mb, kInt8ListRows / weights) * groups_of(N, kInt8ListTokens), rest = items % 512;
-    const double full = 2.7 + 7.5 * share, last = rest == 0 ? 0.0 : rest <= 256 ? 1.75 + 5.5 * share : full;
-    return 6.0 + (double)groups_of(Kb, kInt8ListColumns) * ((double)(items / 512) * full + last);
-}
-
-// us of tiles: a step of four block-columns, whose loads take most of it whatever is stored.
-double tiles_us(int weights, int64_t Mb, int64_t Kb, int64_t N, double share)
-{
-    const int64_t items = groups_of(Mb, kInt8TileRows / weights) * groups_of(N, kInt8TileTokens), rest = items % 512;
-    const double full = 0.6 + 0.3 * share, last = rest == 0 ? 0.0 : rest <= 256 ? 0.42 + 0.2 * share : full;
-    return 8.0 + (double)groups_of(Kb, kInt8TileColumns) * ((double)(items / 512) * full + last);
+    const int64_t rest = items % 512;
+    const double two = t.two[0] + t.two[1] * share, one = t.one[0] + t.one[1] * share;
+    const double last = rest == 0 ? 0.0 : rest <= 256 ? one : one + (two - one) * (double)(rest - 256) / 256.0;
+    return t.launch + (double)steps * ((double)(items / 512) * two + last) + more_bytes * 3e-7;
 }
 
 }  // namespace
@@ -43,7 +39,7 @@ bool int8_rounds_itself(int weights, int64_t M, int64_t K, int64_t N)
     return Kb * tokens <= kInt8FewPieces && weights * Mb * groups_of(N, kInt8FewTokens) <= 1024;
 }
 
-Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks, int64_t N, bool rounds)
+Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks, int64_t N, int size, bool rounds)
 {
     const int64_t Mb = (M + 15) / 16, Kb = (K + 15) / 16, all = blocks[0] + (weights == 2 ? blocks[1] : 0);
     if (rounds) {
@@ -55,21 +51,38 @@ Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks,
         return {Int8Kernel::kFew, groups <= 512 ? 1 : groups <= 1024 ? 2 : 4, N > 1 || Kb <= kInt8FewPieces ? 1 : 2};
     }
     // Lists and tiles look their blocks up in a map of the grid, and load them, and their
-    // windows of x, by offsets of 31 bits.
-    bool windows = N <= (1 << 21);
+    // windows of x, by offsets of 31 bits.  Few tokens leave most of a workgroup's without work
+    // (70000 x 1024, 70 % stored, 31 tokens: walk 17.4 us, lists 26.0, tiles 28.9).
+    bool windows = N > 32 && N <= (1 << 21);
     for (int l = 0; l < weights; ++l)
         windows = windows && has_block_map(Mb, Kb, blocks[l]) && narrow_bytes(blocks[l], 256, 1) >= 0;
     if (windows) {
-        // The walk by blocks, whose x comes through L1, and results: 14336 x 4096 and 2048
-        // tokens 48 us at 5 % stored, 117 at 25 %, 370 with all.  The others have a chain of
-        // loads for every window of x: they pay where there are tokens enough, lists up to
-        // some 45 % stored (90 us at 40 %, tiles 103), tiles from there on (119; lists
-        // of 4096 x 14336 114 at 40 %, tiles 118).
+        // Times (us) fitted to 1584 measured products of eight shapes, 2 to 100 % stored, 64 to
+        // 2048 tokens, one weight and two, 16 and 32 bits, of a sample in
+        // profiles/int8_kernel_choice.txt: within 14 % of them (one standard deviation), and
+        // what they choose is 0.4 % slower than the fastest in the mean.  Measured at 14336
+        // x 4096, 2048 tokens, bf16:
+        //   stored      4 %    10 %   18 %   25 %   35 %   50 %   100 %
+        //   walk        45     69     97     126    160    216    378
+        //   lists       50     58     62      75     90    110    178
+        //   tiles       78     83     91     100    106    111    123
+        // The walk goes by blocks, whose x comes through L1, and results; lists and tiles have a
+        // chain of loads for every window of x.
+        const int64_t rows = groups_of(N, 64) * 64;
         const double share = (double)all / ((double)weights * (double)Mb * (double)Kb);
-        const double walk = 5.0 + 7.4e-7 * (double)all * (double)N + 7e-7 * (double)weights * (double)M * (double)N;
-        const double lists = lists_us(weights, Mb, Kb, N, share), tiles = tiles_us(weights, Mb, Kb, N, share);
-        // so that four times as many blocks are more than a row has in most windows
-        if (lists < walk && lists <= tiles) return {Int8Kernel::kLists, share < 0.06 ? 1 : share < 0.15 ? 2 : 3, 0};
+        const double more = size == 4 ? 2.0 * (double)M * (double)N : 0.0;
+        const double walk = 4.5 + 9.8e-7 * (double)all * (double)rows + 9e-7 * (double)weights * (double)M * (double)rows;
+        const double lists = steps_us({7.3, {2.65, 8.4}, {1.3, 7.7}},
+                                      groups_of(Mb, kInt8ListRows / weights) * groups_of(N, kInt8ListTokens),
+                                      groups_of(Kb, kInt8ListColumns), share, more);
+        const double tiles = steps_us({11.0, {0.6, 0.47}, {0.41, 0.21}},
+                                      groups_of(Mb, kInt8TileRows / weights) * groups_of(N, kInt8TileTokens),
+                                      groups_of(Kb, kInt8TileColumns), share, more);
+        // Four times as many blocks are more than a row has in most windows (us of one, two
+        // and three fours, 14336 x 4096, gate and up, 2048 tokens: 6 % stored 84, 92 and
+        // 122, 10 % 96, 97 and 126, 22 % 135, 118 and 135, 40 % 202, 171 and 171; 4096 x
+        // 14336 at 30 % 131, 102 and 93).
+        if (lists < walk && lists <= tiles) return {Int8Kernel::kLists, share < 0.08 ? 1 : share < 0.26 ? 2 : 3, 0};
         if (tiles < walk) return {Int8Kernel::kTiles, 0, 0};
     }
     // us by (tiles of 16 tokens a wave, waves to a block-row):

@@ -47,7 +47,7 @@ def _load():
             "xspmm_quantize_tokens_scratch": [i64, i64, out],
             "xspmm_quantize_tokens": [i32, i64, i64, p, p, p, p, i64, p],
             "xspmm_int8_scratch": [i32, i64, i64, i64, out],
-            "xspmm_int8_kernel": [i32, i64, i64, i64, i64, i64, i32, C.POINTER(C.c_int32)],
+            "xspmm_int8_kernel": [i32, i32, i64, i64, i64, i64, i64, i32, C.POINTER(C.c_int32)],
             "xspmm_int8_linear": [p, i32, i32, p, p, p, p, p, p, p, p, i64, p, i64, p],
             "xspmm_int8_gated": [p, p, i32, i32, p, p, p, p, p, p, p, p, p, p, i64, p, i64, p],
         }.items():
