@@ -119,6 +119,34 @@ def test_walks(lib, weights, M, K, N, density, times):
     assert times[[(1, 4), (1, 16), (4, 1), (4, 4)].index((a, b))] <= 1.25 * min(times)
 
 
+# tokens rounded within: us of one, two and four block-rows a workgroup, and rounded ahead
+FEWS = [
+    (1, 14336, 4096, 2, 0.05, (22.3, 12.9, 9.4, 9.2)),
+    (1, 14336, 4096, 4, 0.05, (19.8, 11.9, 8.7, 10.2)),
+    (2, 14336, 4096, 1, 0.25, (14.6, 9.8, 10.9, 11.8)),
+    (2, 14336, 4096, 2, 0.25, (26.4, 16.6, 13.9, 13.2)),
+    (2, 14336, 4096, 4, 0.25, (22.7, 14.7, 13.0, 14.1)),
+    (2, 14336, 4096, 4, 0.8, (30.4, 21.4, 23.1, 25.6)),
+    (1, 4096, 14336, 1, 0.25, (7.6, 8.2, 9.7, 9.3)),
+    (2, 16384, 1024, 8, 0.25, (14.5, 8.6, 7.2, 9.3)),
+    (2, 16384, 1024, 16, 0.25, (19.1, 10.8, 8.2, 9.5)),
+    (2, 16384, 1024, 32, 0.25, (34.7, 19.0, 11.1, 11.2)),
+    (2, 16384, 1024, 64, 0.25, (72.9, 39.3, 23.5, 12.5)),
+    (2, 16384, 1024, 2, 0.8, (16.1, 10.6, 10.5, 9.9)),
+    (1, 9000, 20000, 1, 0.05, (17.9, 13.9, 8.7, 19.4)),
+    (1, 5120, 4096, 4, 0.05, (11.9, 8.5, 8.7, 9.9)),
+    (1, 8192, 4096, 4, 0.05, (12.3, 8.7, 8.6, 9.9)),
+    (1, 5000, 30000, 1, 0.8, (39.1, 31.0, 49.8, 41.8)),
+]
+
+
+@pytest.mark.parametrize("weights,M,K,N,density,times", FEWS)
+def test_few_tokens(lib, weights, M, K, N, density, times):
+    """The fastest way or, of those that are near to each other, one within a sixth of it."""
+    kernel, rows, _ = chosen(lib, weights, M, K, N, density)
+    assert times[[1, 2, 4].index(rows) if kernel == FEW else 3] <= 7 / 6 * min(times)
+
+
 def timed():
     """(weights, type, M, K, N, stored, us of the walk, lists and tiles) of products that were timed."""
     with open(os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "profiles", "int8_kernel_choice.txt")) as f:

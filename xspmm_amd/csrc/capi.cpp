@@ -158,7 +158,7 @@ TokenMemory token_memory(int64_t K, int64_t N)
 
 // The tokens of a product: as they come, or quantized into its scratch.
 template <typename T>
-void int8_tokens(Int8Args<T>& a, const BlockIndex& w, int weights, bool any, const void* x, const int8_t* xq, const float* x_scale,
+void int8_tokens(Int8Args<T>& a, const BlockIndex& w, bool any, const void* x, const int8_t* xq, const float* x_scale,
                  void* scratch, int64_t scratch_bytes, hipStream_t s)
 {
     require(w.K <= kInt8MostFeatures, "xSpMM: a weight in 8 bits has at most 133136 columns.");
@@ -169,7 +169,7 @@ void int8_tokens(Int8Args<T>& a, const BlockIndex& w, int weights, bool any, con
         require(x_scale != nullptr, "xSpMM: x_scale is null.");
         return;
     }
-    if (int8_rounds_itself(weights, w.M, w.K, a.N)) {
+    if (int8_rounds_itself(w.M, w.K, a.N)) {
         a.raw = operand<T>(x, false, "x");
         return;
     }
@@ -870,7 +870,7 @@ int xspmm_int8_scratch(int weights, int64_t M, int64_t K, int64_t N, int64_t* by
         require(weights == 1 || weights == 2, "xspmm_int8_scratch: a product has one weight or two.");
         require(M >= 0, "xSpMM: bad size of a weight.");
         require_tokens(K, N);
-        *bytes = int8_rounds_itself(weights, M, K, N) ? 0 : (int64_t)token_memory(K, N).end;
+        *bytes = int8_rounds_itself(M, K, N) ? 0 : (int64_t)token_memory(K, N).end;
     });
 }
 
@@ -887,7 +887,7 @@ int xspmm_int8_kernel(int weights, int vtype, int64_t M, int64_t K, int64_t N, i
                 "xspmm_int8_kernel: more blocks than the grid has.");
         int size = 0;
         with_layer_type(vtype, [&](auto tv) { size = (int)sizeof(typename decltype(tv)::type); });
-        const Int8Choice c = int8_choice(weights, M, K, both, N, size, !quantized && int8_rounds_itself(weights, M, K, N));
+        const Int8Choice c = int8_choice(weights, M, K, both, N, size, !quantized && int8_rounds_itself(M, K, N));
         kernel[0] = (int32_t)c.kernel;
         kernel[1] = c.a;
         kernel[2] = c.b;
@@ -915,7 +915,7 @@ int xspmm_int8_linear(xspmm_weight_t weight, int vtype, int act, const int8_t* q
             a.y = result<T>(y, any, "y");
             a.N = N;
             a.act = act;
-            int8_tokens<T>(a, w, 1, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
+            int8_tokens<T>(a, w, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
             if (any) int8_product<T>(a, 1, as_stream(stream));
         });
     });
@@ -947,7 +947,7 @@ int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act,
             a.y = result<T>(h, any, "h");
             a.N = N;
             a.act = act;
-            int8_tokens<T>(a, g, 2, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
+            int8_tokens<T>(a, g, any, x, xq, x_scale, scratch, scratch_bytes, as_stream(stream));
             if (any) int8_product<T>(a, 2, as_stream(stream));
         });
     });

@@ -281,22 +281,21 @@ void launch_walk(const Int8Product<T>& a, hipStream_t s)
 template <typename T, int NACC>
 void launch_few(const Int8Product<T>& a, const Int8Choice& c, hipStream_t s)
 {
-    auto one = [&](auto rows) {
+    auto with = [&](auto rows) {
         constexpr int R = decltype(rows)::value;
-        c.b == 1 ? launch_few<T, NACC, R, 1, true>(a, s) : launch_few<T, NACC, R, 2, true>(a, s);
-    };
-    if (a.N == 1) {
-        if (c.a == 1)
-            one(std::integral_constant<int, 1>{});
-        else if (c.a == 2)
-            one(std::integral_constant<int, 2>{});
+        if (a.N > 1)
+            launch_few<T, NACC, R, 1, false>(a, s);
+        else if (c.b == 1)
+            launch_few<T, NACC, R, 1, true>(a, s);
         else
-            one(std::integral_constant<int, 4>{});
-    } else if (NACC == 2 || c.a == 1) {
-        launch_few<T, NACC, 1, 1, false>(a, s);
-    } else if constexpr (NACC == 1) {
-        launch_few<T, NACC, 2, 1, false>(a, s);
-    }
+            launch_few<T, NACC, R, 2, true>(a, s);
+    };
+    if (c.a == 1)
+        with(std::integral_constant<int, 1>{});
+    else if (c.a == 2)
+        with(std::integral_constant<int, 2>{});
+    else
+        with(std::integral_constant<int, 4>{});
 }
 
 template <typename T, int NACC>

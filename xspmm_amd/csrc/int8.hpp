@@ -39,7 +39,7 @@ struct Int8Args {
     int act;
 };
 // Whether a product of N tokens rounds them itself, without memory for the result.
-bool int8_rounds_itself(int weights, int64_t M, int64_t K, int64_t N);
+bool int8_rounds_itself(int64_t M, int64_t K, int64_t N);
 
 // What the kernels take at a time: few tokens' workgroups 16 tokens and 1024 pieces of 16
 // features; lists and tiles some block-rows (of both weights), tokens and block-columns.

@@ -27,28 +27,39 @@ double steps_us(const Steps& t, int64_t items, int64_t steps, double share, doub
 
 }  // namespace
 
-// One token, and more where every workgroup's rounding them anew costs less than a launch:
-// us with and without, bf16, 16384 x 1024 30 % stored 16 tokens 10.4 and 11.1, 48 tokens 15.7
-// and 10.9; gate and up of 14336 x 4096 25 % stored one token 10.0 and 12.6, two 16.9 and
-// 13.6; 4096 x 4096 10 % stored four tokens 8.5 and 11.1.
-bool int8_rounds_itself(int weights, int64_t M, int64_t K, int64_t N)
+// One token, and more where every workgroup's rounding them anew costs less than a launch
+// and the walk behind it: us with (its fastest) and without, bf16, 14336 x 4096 25 % stored, gate and
+// up, one token 9.8 and 11.8, two 13.9 and 13.2, four 13.0 and 14.1; 5 % stored, one
+// weight, four tokens 8.7 and 10.2; 16384 x 1024 25 % stored, gate and up, eight tokens 7.2
+// and 9.3, sixteen 8.2 and 9.5, 32 11.1 and 11.2, 64 23.5 and 12.5.
+bool int8_rounds_itself(int64_t M, int64_t K, int64_t N)
 {
     const int64_t Mb = (M + 15) / 16, Kb = (K + 15) / 16;
     if (N == 1) return Kb <= 2 * kInt8FewPieces;
     const int64_t tokens = N < kInt8FewTokens ? N : kInt8FewTokens;
-    return Kb * tokens <= kInt8FewPieces && weights * Mb * groups_of(N, kInt8FewTokens) <= 1024;
+    return Kb * tokens <= kInt8FewPieces && Mb * groups_of(N, kInt8FewTokens) <= 1024;
 }
 
 Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks, int64_t N, int size, bool rounds)
 {
     const int64_t Mb = (M + 15) / 16, Kb = (K + 15) / 16, all = blocks[0] + (weights == 2 ? blocks[1] : 0);
     if (rounds) {
-        // Sixteen waves to a block-row while there are no more than two workgroups a CU
-        // (16 waves each), half and a quarter of them beyond (us of one and two rows a
-        // workgroup: fp16 4096 x 14336, 25 % stored, one token 6.7 and 7.8; bf16 gate and
-        // up of 14336 x 4096 13.0 and 10.1, of four rows 10.3).
-        const int64_t groups = Mb * groups_of(N, kInt8FewTokens);
-        return {Int8Kernel::kFew, groups <= 512 ? 1 : groups <= 1024 ? 2 : 4, N > 1 || Kb <= kInt8FewPieces ? 1 : 2};
+        // Sixteen waves to a block-row while all workgroups run at once, two a CU of one token
+        // and one a CU of more, half of them up to twice that.  Beyond, half or a quarter: by
+        // how much the blocks of a row take beside rounding the tokens once more.  us of one,
+        // two and four rows a workgroup, bf16:
+        //   4096 x 14336,  25 %, 1 token            8.1    8.9   10.4
+        //   8192 x 4096,    5 %, 4                 12.2    8.7    8.6
+        //   14336 x 4096,  25 %, 1, gate and up    14.5    9.7   11.0
+        //   14336 x 4096,   5 %, 2                 22.5   13.0    9.5
+        //   16384 x 1024,  25 %, 16, gate and up   19.8   11.2    8.4
+        //   16384 x 1024,  80 %, 2, gate and up    15.7   10.3   10.3
+        //   5000 x 30000,  80 %, 1                 39.1   31.0   49.8
+        const int64_t groups = Mb * groups_of(N, kInt8FewTokens), pieces = Kb * (N < kInt8FewTokens ? N : kInt8FewTokens);
+        const int kept = N > 1 || Kb <= kInt8FewPieces ? 1 : 2;
+        const bool two = N == 1 && kept == 1;
+        const int rows = groups <= (two ? 512 : 256) ? 1 : groups <= 512 ? 2 : 4 * all <= (128 + pieces) * Mb ? 4 : 2;
+        return {Int8Kernel::kFew, rows, kept};
     }
     // Lists and tiles look their blocks up in a map of the grid, and load them, and their
     // windows of x, by offsets of 31 bits.  Few tokens leave most of a workgroup's without work
