@@ -91,8 +91,10 @@ __global__ __launch_bounds__(kListThreads, 4) void ff_int8_list_kernel(const Int
     // fours: of every row how many fours of blocks it has, 4 bits each
     auto list = [&](uint32_t* to, const int32_t (&p)[kListColumns]) -> uint32_t {
         constexpr int kEach = kListRows * kListWindow / 64;
+        lanes_in_order();
 #pragma unroll
         for (int j = 0; j < kEach; ++j) to[kEach * lane + j] = kNone;
+        lanes_in_order();
         constexpr uint32_t kRow = (uint32_t)((1ull << kListLanes) - 1);
         int at = mine * kListWindow;
         uint64_t there[kListColumns];
@@ -104,6 +106,7 @@ __global__ __launch_bounds__(kListThreads, 4) void ff_int8_list_kernel(const Int
                 to[at + __popc(row & ((1u << (lane % kListLanes)) - 1u))] = (uint32_t)p[j] * 256u + (uint32_t)(at_c + j);
             at += __popc(row);
         }
+        lanes_in_order();
         uint32_t fours = 0;
 #pragma unroll
         for (int s = 0; s < kListRows; ++s) {

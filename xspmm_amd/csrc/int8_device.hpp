@@ -152,6 +152,14 @@ __device__ __forceinline__ void join(uint32_t (&m)[VEC], uint32_t* red)
     }
 }
 
+// Between what lanes of a wave leave in LDS and what others of it read or write there.  LDS
+// takes a wave's operations in their order, so nothing waits; the compiler has to keep it.
+__device__ __forceinline__ void lanes_in_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 struct Int8Side {
     const int32_t* ptr;
     const int32_t* col;
