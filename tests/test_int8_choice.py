@@ -41,8 +41,13 @@ SIDES = (16, 200, 1000, 2048, 4096, 7000, 9000, 14336, 20000, 33000, 70000)
 NS = (1, 2, 5, 16, 17, 31, 33, 64, 100, 256, 700, 1100, 2048, 9000)
 
 
-def test_every_kernel_that_is_built_can_be_chosen(lib):
-    """And no other is chosen."""
+def instance(weights, N, kernel, a, b):
+    """The template's arguments that a choice stands for."""
+    return {FEW: ("few", weights, a, b, N == 1), WALK: ("walk", a, weights, b), LISTS: ("list", weights - 1, a),
+            TILES: ("tile", weights - 1)}[kernel]
+
+
+def instances_built():
     if not shutil.which("nm"):
         pytest.skip("needs nm")
     names = subprocess.run(["nm", X.LIB_PATH], check=True, capture_output=True, text=True).stdout
@@ -51,14 +56,25 @@ def test_every_kernel_that_is_built_can_be_chosen(lib):
                                           names):
         built.setdefault(value, set()).add((kernel, *(int(n) for n in re.findall(r"\d+", rest))))
     assert len(built) == 3
-    wanted = set()
+    return built
+
+
+def test_every_kernel_that_is_built_can_be_chosen(lib):
+    """And no other is chosen."""
+    built, wanted = instances_built(), set()
     for weights, M, K, N, density, quantized in itertools.product(
             (1, 2), SIDES, SIDES, NS, (0.01, 0.03, 0.1, 0.3, 0.7, 1.0), (False, True)):
-        kernel, a, b = chosen(lib, weights, M, K, N, density, quantized=quantized)
-        wanted.add({FEW: ("few", weights, a, b, N == 1), WALK: ("walk", a, weights, b), LISTS: ("list", weights - 1, a),
-                    TILES: ("tile", weights - 1)}[kernel])
+        wanted.add(instance(weights, N, *chosen(lib, weights, M, K, N, density, quantized=quantized)))
     for of in built.values():
         assert of == wanted, (sorted(of - wanted), sorted(wanted - of))
+
+
+def test_every_kernel_that_is_built_has_a_test_on_the_gpu():
+    from test_gpu_int8_kernels import CASES
+
+    tested = {instance(weights, N, *which) for which, weights, _, _, N, _ in CASES}
+    for of in instances_built().values():
+        assert of == tested, (sorted(of - tested), sorted(tested - of))
 
 
 def test_what_windows_need(lib):
