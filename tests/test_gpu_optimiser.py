@@ -157,3 +157,22 @@ def test_captured(kind, sides):
         b.step()
         torch.cuda.synchronize()
         assert same(A, B), i
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_state_of_a_layer_in_fp32(kind):
+    """It holds no copy of the weights in fp32: a 16-bit layer that takes it up has one of its own."""
+    dtype, u = TYPES[kind]
+    A, B = layer(torch.float32), layer(dtype)
+    a, b = X.OrthogonalMomentum(A), X.OrthogonalMomentum(B)
+    gradients(A, 0)
+    a.step()
+    b.load_state_dict(a.state_dict())
+    for group in b.param_groups:
+        group.update(lr=u / 4, momentum=0.0, nesterov=False)
+    was = B.gate.detach().clone()
+    for _ in range(64):
+        gradients(B, 0)
+        b.step()
+    # steps that a 16-bit weight cannot show one by one
+    assert (B.gate != was).float().mean() > 0.5

@@ -133,10 +133,10 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                 if p.grad is None or not p.numel():  # a weight without blocks
                     continue
                 state = self.state[p]
-                if not state:
+                if "momentum" not in state:
                     state["momentum"] = torch.zeros_like(p, dtype=torch.float32)
-                    if p.dtype is not torch.float32:
-                        state["master"] = p.detach().float()
+                if "master" not in state and p.dtype is not torch.float32:  # nor in the state of an fp32 layer
+                    state["master"] = p.detach().float()
                 g, v = p.grad.float(), state["momentum"]
                 v.mul_(momentum).add_(g)
                 u = g.add(v, alpha=momentum) if group["nesterov"] else v
