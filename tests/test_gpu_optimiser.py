@@ -176,3 +176,9 @@ def test_state_of_a_layer_in_fp32(kind):
         b.step()
     # steps that a 16-bit weight cannot show one by one
     assert (B.gate != was).float().mean() > 0.5
+
+
+def test_a_layer_given_twice():
+    A = layer(torch.float16)
+    with pytest.raises(ValueError, match="twice"):
+        X.OrthogonalMomentum([A, A])

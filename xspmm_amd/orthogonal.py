@@ -97,6 +97,8 @@ class OrthogonalMomentum(torch.optim.Optimizer):
         if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1:
             raise ValueError("lr and weight_decay must not be negative, momentum lies in [0, 1)")
         params = [p for layer in layers for p in (layer.gate, layer.up, layer.down)]
+        if len(set(map(id, params))) < len(params):
+            raise ValueError("a layer's weights are given twice")
         self._weights = None
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       steps=steps))
