@@ -549,11 +549,12 @@ int xspmm_int8_gated(xspmm_weight_t gate, xspmm_weight_t up, int vtype, int act,
  * rows); out receives X at the stored blocks, zero past the edges of the weight.
  * Products take fp16 operands, of fp16 and fp32 updates two halves of each: the elements
  * of X, S and b S + c S S must stay below 16 (with the usual 3.4445, -4.775, 2.0315 they are
- * below 3).  An update that holds an infinity or
- * a NaN gives NaN.  steps >= 1, eps >= 0, finite coefficients, weights of at most 2^20
- * rows and columns.  out may be the update.  scratch (256-byte aligned) has as many
- * bytes as xspmm_orthogonalize_scratch says: several dense matrices of the weight's
- * size.  Asynchronous on `stream`; nothing is allocated.
+ * below 3).  X is held to 2^-37, which leaves fewer digits of an update whose norm is
+ * less than a hundredth of eps.  An update that holds an infinity or a NaN gives NaN.
+ * steps >= 1, eps >= 0, finite coefficients, weights of at most 2^20 rows and columns.
+ * out may be the update.  scratch (256-byte aligned) has as many bytes as
+ * xspmm_orthogonalize_scratch says: several dense matrices of the weight's size.
+ * Asynchronous on `stream`; nothing is allocated.
  */
 int xspmm_orthogonalize_scratch(xspmm_weight_t weight, int vtype, int64_t* bytes);
 int xspmm_orthogonalize(xspmm_weight_t weight, int vtype, const void* update, void* out, int steps, float a, float b,

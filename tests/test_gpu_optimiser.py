@@ -182,3 +182,24 @@ def test_a_layer_given_twice():
     A = layer(torch.float16)
     with pytest.raises(ValueError, match="twice"):
         X.OrthogonalMomentum([A, A])
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("share", [1.0, 0.1, 0.01])
+def test_updates_as_small_as_eps(kind, share):
+    """orthogonalize itself adds eps to the norm: down to a hundredth of it as many digits are right."""
+    dtype, u = TYPES[kind]
+    W, A, (rows, cols, inside) = weight(200, 333, 1.0, dtype, 3)
+    norm = A.norm()
+    eps = float(norm) / share  # (an fp16 update of a size that the type holds)
+    x = A / (norm + eps)
+    for _ in range(5):
+        s = x @ x.t()
+        x = 3.4445 * x + (-4.775 * s + 2.0315 * (s @ s)) @ x
+    got = X.orthogonalize(W, W.values, eps=eps).double().cpu().view(-1, 16, 16)
+    full = torch.zeros((13 * 16, 21 * 16), dtype=torch.float64)
+    full[:200, :333] = x
+    want = full.view(13, 16, 21, 16).permute(0, 2, 1, 3)[rows, cols]
+    rms = lambda t: float(t.square().mean().sqrt())
+    # 1e-5 of the rms as stated, and the result's rounding (below 2^-14 by up to 2^-25 in fp16)
+    assert rms(got - want) <= (1e-5 + u) * rms(want) + (2.0 ** -25 if kind == "f16" else 0.0)

@@ -13,8 +13,9 @@
 // What bounds it is latency, of a window's x, lists and first blocks one after the other
 // (at 5 % stored a window takes 2 us, its instructions a quarter of that): waves of eight
 // block-rows with twice the registers, two a SIMD, take 163 us for gate and up of 14336 x
-// 4096, 2048 tokens, 25 % stored, bf16; of four, four a SIMD, 147.  One product 76 (by
-// tiles 95, by the walk 117), 10 % stored 56 (83, 68).
+// 4096, 2048 tokens, 25 % stored, bf16, where waves of four, four a SIMD, took 147; those
+// take 126 to 135 now, with two fours fetched ahead in place of three.  One product 75 (by
+// tiles 100, by the walk 126), 10 % stored 58 (83, 69).
 #include "int8_device.hpp"
 
 namespace xspmm {

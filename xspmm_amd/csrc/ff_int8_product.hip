@@ -10,9 +10,9 @@
 // order; a result is float(sum) * row's scale * token's scale, then as in fp32.
 //
 // Few tokens are bound by latency and the weight's bytes: one token of fp16 4096 x 14336,
-// 25 % stored, 7.0 us for 15 MB; gate and up of bf16 14336 x 4096 10.1 us for 29 MB
+// 25 % stored, 6.9 us for 15 MB; gate and up of bf16 14336 x 4096 10.0 us for 29 MB
 // (3.1 and 6.0 at the rate of a copy), rounding the token ahead of the blocks.  The walk is
-// bound by x, of which L1 brings every stored block its tokens: 48 us at 5 % stored, 14336
+// bound by x, of which L1 brings every stored block its tokens: 45 us at 4 % stored, 14336
 // x 4096 and 2048 tokens; 4.4 us at fp32 5003 x 4999, 10 %, 31 tokens.
 #include "int8_device.hpp"
 

@@ -19,7 +19,8 @@ The products take activations in the weight's value type, features x tokens as
 ``sparse_linear`` does, and round them themselves, or an ``Int8Tokens`` that several
 products share.  A token or a weight's row that holds an infinity or a NaN has the
 scale NaN, and so NaN results.  They run on torch's current stream, allocate with
-torch, and have no gradients: an operand that wants one is refused.
+torch, and have no gradients: an operand that wants one is refused.  An
+``Int8Weight`` does not keep the wide values that it was made from.
 """
 from __future__ import annotations
 

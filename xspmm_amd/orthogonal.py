@@ -45,10 +45,11 @@ def orthogonalize(W, update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=N
     read), orthogonalised: values as W's, num_blocks * 256 in its value type, zeros past
     the weight's edges.  Products take fp16 operands, of fp16 and fp32 updates two halves of
     each; the result is off by its own rounding and up to 1e-3 (bf16), 1e-5 (fp16, fp32)
-    of its rms.  With coefficients of one's own, the elements of X, S and b S + c S S have
-    to stay below 16.  An update that holds an infinity or a NaN gives NaN.  out: memory
-    for the result, apart from the update or the update itself.  Scratch of several dense
-    matrices of W's size is allocated for the call.  No gradients."""
+    of its rms.  (X is held to 2^-37, which leaves fewer digits of an update whose norm is
+    less than a hundredth of eps.)  With coefficients of one's own, the elements of X, S and
+    b S + c S S have to stay below 16.  An update that holds an infinity or a NaN gives NaN.
+    out: memory for the result, apart from the update or the update itself.  Scratch of
+    several dense matrices of W's size is allocated for the call.  No gradients."""
     if not isinstance(W, SparseWeight):
         raise TypeError("W must be a SparseWeight")
     if W._h is None:
