@@ -61,15 +61,14 @@ __global__ __launch_bounds__(64 * kWeightWaves) void ff_int8_weight_kernel(const
     }
 }
 
-// Tiles of LT * VEC tokens, LT threads along them; the others take blocks of 16
-// features in turn.
+// Tiles of LT tokens, LT threads along them; the others take blocks of 16 features in
+// turn.
 
-// The first token of a thread; the last tile moves back into the matrix.
-template <int LT, int VEC>
-__device__ __forceinline__ int64_t first_token(int64_t tile, int64_t N)
+// The token of a thread; past the last one that again.
+template <int LT>
+__device__ __forceinline__ int64_t token_of(int64_t tile, int64_t N)
 {
-    const int64_t n = (tile * LT + threadIdx.x % LT) * VEC;
-    return n + VEC <= N ? n : N - VEC;
+    return min(tile * LT + threadIdx.x % LT, N - 1);
 }
 
 // Few tokens: a workgroup to a tile, whose features stay in registers.
@@ -79,24 +78,24 @@ __global__ __launch_bounds__(1024) void ff_tokens_whole_kernel(const T* __restri
                                                                float* __restrict__ scale, int64_t K, int64_t N)
 {
     __shared__ uint32_t red[16 * LT];
-    const int64_t n = first_token<LT, 1>(blockIdx.x, N), Kb = (K + 15) / 16;
-    float v[kKept][16][1];
+    const int64_t n = token_of<LT>(blockIdx.x, N), Kb = (K + 15) / 16;
+    float v[kKept][16];
 #pragma unroll
     for (int u = 0; u < kKept; ++u) {
         const int64_t kb = threadIdx.x / LT + u * (1024 / LT);
         if (kb < Kb)
-            load_features<T, 1>(x, K, N, kb, n, v[u]);
+            load_features<T>(x, K, N, kb, n, v[u]);
         else
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[u][i][0] = 0.f;
+            for (int i = 0; i < 16; ++i) v[u][i] = 0.f;
     }
-    uint32_t m[1] = {};
+    uint32_t m = 0;
 #pragma unroll
     for (int u = 0; u < kKept; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) m[0] = max(m[0], magnitude(v[u][i][0]));
-    join<1024, LT, 1>(m, red);
-    const Rounding round(m[0]);
+        for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[u][i]));
+    join<1024, LT>(m, red);
+    const Rounding round(m);
     if (threadIdx.x < LT) scale[n] = round.scale;
 #pragma unroll
     for (int u = 0; u < kKept; ++u) {
@@ -122,38 +121,34 @@ __global__ __launch_bounds__(1024) void ff_token_kernel(const T* __restrict__ x,
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = k + i < K ? (float)x[k + i] : 0.f;
     }
-    uint32_t m[1] = {0u};
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m[0] = max(m[0], magnitude(v[i]));
-    join<1024, 1, 1>(m, red);
-    const Rounding round(m[0]);
+    for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[i]));
+    join<1024, 1>(m, red);
+    const Rounding round(m);
     if (threadIdx.x == 0) scale[0] = round.scale;
     if (k < K) *reinterpret_cast<u32x4_t*>(q + k) = round_features(v, round);
 }
 
 // part[slice][n]: bits of the largest magnitude of a slice of the features
 constexpr int kSliceThreads = 1024;
-template <typename T, int VEC, int LT>
+template <typename T, int LT>
 __global__ __launch_bounds__(kSliceThreads) void ff_tokens_most_kernel(const T* __restrict__ x, uint32_t* __restrict__ part,
                                                              int64_t K, int64_t N, int32_t slices)
 {
-    __shared__ uint32_t red[kSliceThreads / 64 * LT * VEC];
+    __shared__ uint32_t red[kSliceThreads / 64 * LT];
     const int64_t tile = blockIdx.x / slices, s = blockIdx.x % slices, Kb = (K + 15) / 16;
-    const int64_t n = first_token<LT, VEC>(tile, N);
-    float v[16][VEC];
-    uint32_t m[VEC] = {};
+    const int64_t n = token_of<LT>(tile, N);
+    float v[16];
+    uint32_t m = 0;
     const int64_t end = Kb * (s + 1) / slices;
     for (int64_t kb = Kb * s / slices + threadIdx.x / LT; kb < end; kb += kSliceThreads / LT) {
-        load_features<T, VEC>(x, K, N, kb, n, v);
+        load_features<T>(x, K, N, kb, n, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) m[c] = max(m[c], magnitude(v[i][c]));
+        for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[i]));
     }
-    join<kSliceThreads, LT, VEC>(m, red);
-    if (threadIdx.x < LT)
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) part[s * N + n + c] = m[c];
+    join<kSliceThreads, LT>(m, red);
+    if (threadIdx.x < LT) part[s * N + n] = m;
 }
 
 // A thread takes one token at a time: 64 of them store 1 KB side by side (with four
@@ -167,45 +162,42 @@ __global__ __launch_bounds__(kSliceThreads) void ff_tokens_round_kernel(const T*
 {
     __shared__ uint32_t red[kSliceThreads / 64 * LT];
     const int64_t tile = blockIdx.x / slices, s = blockIdx.x % slices, Kb = (K + 15) / 16;
-    const int64_t n = first_token<LT, 1>(tile, N);
-    uint32_t m[1] = {};
-    for (int32_t p = threadIdx.x / LT; p < slices; p += kSliceThreads / LT) m[0] = max(m[0], part[p * N + n]);
-    join<kSliceThreads, LT, 1>(m, red);
-    const Rounding round(m[0]);
+    const int64_t n = token_of<LT>(tile, N);
+    uint32_t m = 0;
+    for (int32_t p = threadIdx.x / LT; p < slices; p += kSliceThreads / LT) m = max(m, part[p * N + n]);
+    join<kSliceThreads, LT>(m, red);
+    const Rounding round(m);
     if (s == 0 && threadIdx.x < LT) scale[n] = round.scale;
     const int64_t end = Kb * (s + 1) / slices;
     for (int64_t kb = Kb * s / slices + threadIdx.x / LT; kb < end; kb += kSliceThreads / LT) {
-        float v[16][1];
-        load_features<T, 1>(x, K, N, kb, n, v);
+        float v[16];
+        load_features<T>(x, K, N, kb, n, v);
         store_features(q, N, kb, n, v, round);
     }
 }
 
 struct TokenPlan {
     bool whole;  // one launch, a workgroup to a tile
-    int vec, lanes;
+    int lanes;
     int64_t tiles;
     int32_t slices;
 };
 
 // size: bytes of a value.  us, bf16 and fp32, of whole tokens by four lanes (4) and sixteen
-// (16), and in slices by sixteen (s16), by 64 (s64) and by 64 of four tokens (s64x4):
+// (16), and in slices by sixteen (s16) and by 64 (s64):
 //   4999 x 31      8.6 and 8.1 (4), 12.3 and 10.6 (s16)
 //   2048 x 128     7.3 and 5.7 (4), 9.8 and 6.8 (16), 10.8 and 9.0 (s64)
 //   4096 x 128     8.2 (4), 11.1 (s64); 4096 x 512 13.5 and 16.9 (4), 11.0 and 9.9 (s64)
 //   6000 x 63      9.4 and 13.5 (4), 11.1 and 9.6 (s16)
 //   1024 x 1500    11.7 and 11.9 (4), 8.2 and 8.0 (16), 10.9 and 9.9 (s64)
 //   1024 x 16384   32.7 and 27.0 (16), 25.3 and 27.7 (s64)
-//   14336 x 512    15.5 and 15.8 (s16), 14.5 and 14.9 (s64), 18.2 and 22.0 (s64x4)
-//   14336 x 8192   152 and 216 (s64), 139 and 222 (s64x4)
+//   14336 x 512    15.5 and 15.8 (s16), 14.5 and 14.9 (s64)
 // Whole tokens read x once, as long as there are workgroups enough and a thread's segments of
 // a row, eight bytes with four lanes, come from L1 again.
 TokenPlan token_plan(int64_t K, int64_t N, int size)
 {
     TokenPlan p{};
     const int64_t Kb = (K + 15) / 16;
-    auto tiles = [&](int lanes, int vec) { return (N + lanes * vec - 1) / (lanes * vec); };
-    p.vec = 1;
     if (N == 1) {
         p.lanes = 1;
         p.whole = K <= kOneMost;
@@ -215,29 +207,38 @@ TokenPlan token_plan(int64_t K, int64_t N, int size)
     } else if (Kb <= 96 && N <= 8192) {  // (Kb * 16 <= kKept * 1024)
         p.lanes = 16;
         p.whole = true;
+    } else {
+        p.lanes = N < 64 ? 16 : 64;
     }
-    if (p.whole) {
-        p.tiles = tiles(p.lanes, 1);
-        return p;
-    }
-    if (N > 1) p.lanes = N < 64 ? 16 : 64;
-    if (N >= 256 && size == 2 && K * N > 1 << 24) p.vec = 4;
-    p.tiles = tiles(p.lanes, p.vec);
+    p.tiles = (N + p.lanes - 1) / p.lanes;
+    if (p.whole) return p;
+    // Rounds of a workgroup a CU, filled as far as they can be, in the time of 16 features of a
+    // tile, of which a workgroup costs some 24 beside its own (us, bf16): at 5350 x 1385 22
+    // tiles by twelve slices, eight workgroups more than CUs, 26.0, by eleven 21.0; at 6661 x
+    // 8893 139 tiles by one slice 125, by three 95; at 537 x 9362 147 by one 18.9, by three 21.7.
     const int each = kSliceThreads / p.lanes;
-    const int64_t want = (256 + p.tiles - 1) / p.tiles, most = (Kb + each - 1) / each;
-    p.slices = (int32_t)(want < most ? want : most);
+    const int64_t most = (Kb + each - 1) / each;
+    double least = 0.0;
+    for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+        int64_t s = 256 * rounds / p.tiles;
+        s = s < 1 ? 1 : s < most ? s : most;
+        const double time = (double)((p.tiles * s + 255) / 256) * ((double)Kb / (double)s + 24.0);
+        if (rounds == 1 || time < least) {
+            least = time;
+            p.slices = (int32_t)s;
+        }
+    }
     return p;
 }
 
-template <typename T, int VEC, int LT>
+template <typename T, int LT>
 void launch_tokens(const T* x, int8_t* q, float* scale, int64_t K, int64_t N, void* scratch, const TokenPlan& p,
                    hipStream_t s)
 {
     uint32_t* part = static_cast<uint32_t*>(scratch);
     const dim3 grid = launch_grid(p.tiles * p.slices, kSliceThreads), threads(kSliceThreads);
-    const dim3 narrow = launch_grid((N + LT - 1) / LT * p.slices, kSliceThreads);
-    hipLaunchKernelGGL((ff_tokens_most_kernel<T, VEC, LT>), grid, threads, 0, s, x, part, K, N, p.slices);
-    hipLaunchKernelGGL((ff_tokens_round_kernel<T, LT>), narrow, threads, 0, s, x, part, q, scale, K, N, p.slices);
+    hipLaunchKernelGGL((ff_tokens_most_kernel<T, LT>), grid, threads, 0, s, x, part, K, N, p.slices);
+    hipLaunchKernelGGL((ff_tokens_round_kernel<T, LT>), grid, threads, 0, s, x, part, q, scale, K, N, p.slices);
     XSPMM_LAUNCH_CHECK();
 }
 
@@ -292,18 +293,12 @@ void quantize_tokens(const T* x, int8_t* q, float* scale, int64_t K, int64_t N, 
         XSPMM_LAUNCH_CHECK();
         return;
     }
-    if (p.lanes == 64) {
-        if constexpr (sizeof(T) == 2)
-            if (p.vec == 4) {
-                ff::launch_tokens<T, 4, 64>(x, q, scale, K, N, scratch, p, s);
-                return;
-            }
-        ff::launch_tokens<T, 1, 64>(x, q, scale, K, N, scratch, p, s);
-    } else if (p.lanes == 16) {
-        ff::launch_tokens<T, 1, 16>(x, q, scale, K, N, scratch, p, s);
-    } else {
-        ff::launch_tokens<T, 1, 1>(x, q, scale, K, N, scratch, p, s);
-    }
+    if (p.lanes == 64)
+        ff::launch_tokens<T, 64>(x, q, scale, K, N, scratch, p, s);
+    else if (p.lanes == 16)
+        ff::launch_tokens<T, 16>(x, q, scale, K, N, scratch, p, s);
+    else
+        ff::launch_tokens<T, 1>(x, q, scale, K, N, scratch, p, s);
 }
 
 #define XSPMM_INT8(T)                                                                            \

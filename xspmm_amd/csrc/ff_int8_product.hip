@@ -139,7 +139,7 @@ __global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_ke
     const int nt = ONE ? 1 : (int)min((int64_t)kFewTokens, a.N - n0);
     const int blocks = a.in_blocks * nt;
 
-    float v[KEPT][16][1];
+    float v[KEPT][16];
 #pragma unroll
     for (int u = 0; u < KEPT; ++u) {
         const int e = t + kFewThreads * u;
@@ -149,17 +149,17 @@ __global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_ke
                 if (k + 16 <= a.in_rows) {
                     const Pack<T, 16> p = *reinterpret_cast<const Pack<T, 16>*>(a.raw + k);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[u][i][0] = (float)p.v[i];
+                    for (int i = 0; i < 16; ++i) v[u][i] = (float)p.v[i];
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[u][i][0] = k + i < a.in_rows ? (float)a.raw[k + i] : 0.f;
+                    for (int i = 0; i < 16; ++i) v[u][i] = k + i < a.in_rows ? (float)a.raw[k + i] : 0.f;
                 }
             } else {
-                load_features<T, 1>(a.raw, a.in_rows, a.N, e / nt, n0 + e % nt, v[u]);
+                load_features<T>(a.raw, a.in_rows, a.N, e / nt, n0 + e % nt, v[u]);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[u][i][0] = 0.f;
+            for (int i = 0; i < 16; ++i) v[u][i] = 0.f;
         }
     }
 
@@ -188,22 +188,17 @@ __global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_ke
 
     // the tokens' scales
     if constexpr (ONE) {
-        uint32_t m[1] = {0u};
+        uint32_t m = 0u;
 #pragma unroll
         for (int u = 0; u < KEPT; ++u)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) m[0] = max(m[0], magnitude(v[u][i][0]));
-        join<kFewThreads, 1, 1>(m, most);
-        const Rounding round(m[0]);
+            for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[u][i]));
+        join<kFewThreads, 1>(m, most);
+        const Rounding round(m);
         if (t == 0) scales[0] = round.scale;
 #pragma unroll
         for (int u = 0; u < KEPT; ++u)
-            if (t + kFewThreads * u < blocks) {
-                float w[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = v[u][i][0];
-                xs[t + kFewThreads * u] = round_features(w, round);
-            }
+            if (t + kFewThreads * u < blocks) xs[t + kFewThreads * u] = round_features(v[u], round);
     } else {
         if (t < kFewTokens) most[t] = 0u;
         __syncthreads();
@@ -212,19 +207,15 @@ __global__ __launch_bounds__(kFewThreads, KEPT == 1 ? 8 : 4) void ff_int8_few_ke
             if (t + kFewThreads * u < blocks) {
                 uint32_t m = 0u;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[u][i][0]));
+                for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[u][i]));
                 atomicMax(&most[(t + kFewThreads * u) % nt], m);
             }
         __syncthreads();
         if (t < nt) scales[t] = Rounding(most[t]).scale;
 #pragma unroll
         for (int u = 0; u < KEPT; ++u)
-            if (t + kFewThreads * u < blocks) {
-                float w[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = v[u][i][0];
-                xs[t + kFewThreads * u] = round_features(w, Rounding(most[(t + kFewThreads * u) % nt]));
-            }
+            if (t + kFewThreads * u < blocks)
+                xs[t + kFewThreads * u] = round_features(v[u], Rounding(most[(t + kFewThreads * u) % nt]));
     }
     __syncthreads();
 

@@ -95,61 +95,46 @@ __device__ __forceinline__ u32x4_t round_features(const float (&v)[16], const Ro
     return w;
 }
 
-// The 16 features of block kb of tokens n .. + VEC - 1, zeros past the last.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_features(const T* x, int64_t K, int64_t N, int64_t kb, int64_t n,
-                                              float (&v)[16][VEC])
+// The 16 features of block kb of token n, zeros past the last.
+template <typename T>
+__device__ __forceinline__ void load_features(const T* x, int64_t K, int64_t N, int64_t kb, int64_t n, float (&v)[16])
 {
-    using P = Pack<T, VEC>;
     if (16 * kb + 16 <= K) {
-        P p[16];
+        T p[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = *reinterpret_cast<const P*>(x + (16 * kb + i) * N + n);
+        for (int i = 0; i < 16; ++i) p[i] = x[(16 * kb + i) * N + n];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) v[i][c] = (float)p[i].v[c];
+        for (int i = 0; i < 16; ++i) v[i] = (float)p[i];
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const bool in = 16 * kb + i < K;
-            const P p = *reinterpret_cast<const P*>(x + (in ? 16 * kb + i : K - 1) * N + n);
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) v[i][c] = in ? (float)p.v[c] : 0.f;
+            const T p = x[(in ? 16 * kb + i : K - 1) * N + n];
+            v[i] = in ? (float)p : 0.f;
         }
     }
 }
 
-__device__ __forceinline__ void store_features(int8_t* q, int64_t N, int64_t kb, int64_t n, const float (&v)[16][1],
+__device__ __forceinline__ void store_features(int8_t* q, int64_t N, int64_t kb, int64_t n, const float (&v)[16],
                                                const Rounding& round)
 {
-    float w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = v[i][0];
-    *reinterpret_cast<u32x4_t*>(q + (kb * N + n) * 16) = round_features(w, round);
+    *reinterpret_cast<u32x4_t*>(q + (kb * N + n) * 16) = round_features(v, round);
 }
 
-// The largest of `m` over the threads of a column tile that have the same tokens.
-template <int THREADS, int LT, int VEC>
-__device__ __forceinline__ void join(uint32_t (&m)[VEC], uint32_t* red)
+// The largest of `m` over the threads of a column tile that have the same token.
+template <int THREADS, int LT>
+__device__ __forceinline__ void join(uint32_t& m, uint32_t* red)
 {
     const int t = threadIdx.x;
 #pragma unroll
-    for (int c = 0; c < VEC; ++c)
-#pragma unroll
-        for (int d = LT; d < 64; d *= 2) m[c] = max(m[c], (uint32_t)__shfl_xor((int)m[c], d));
+    for (int d = LT; d < 64; d *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, d));
     constexpr int kWaves = THREADS / 64;
     const int lane = t & 63, wave = t >> 6;
-    if (lane < LT)
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) red[(wave * LT + lane) * VEC + c] = m[c];
+    if (lane < LT) red[wave * LT + lane] = m;
     __syncthreads();
+    m = 0;
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) {
-        m[c] = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) m[c] = max(m[c], red[(w * LT + (t % LT)) * VEC + c]);
-    }
+    for (int w = 0; w < kWaves; ++w) m = max(m, red[w * LT + (t % LT)]);
 }
 
 // Between what lanes of a wave leave in LDS and what others of it read or write there.  LDS
