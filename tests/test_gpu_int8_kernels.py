@@ -28,7 +28,7 @@ def kernel(parts, kind, N):
 
 CASES = [
     # one token: one, two and four block-rows a workgroup, one piece of the token a thread and two
-    ((FEW, 1, 1), 1, 8190, 1030, 1, 0.3), ((FEW, 2, 1), 1, 9000, 2047, 1, 0.9), ((FEW, 4, 1), 1, 9001, 2047, 1, 0.05),
+    ((FEW, 1, 1), 1, 4090, 1030, 1, 0.3), ((FEW, 2, 1), 1, 8190, 1030, 1, 0.3), ((FEW, 2, 1), 1, 9000, 2047, 1, 0.9), ((FEW, 4, 1), 1, 9001, 2047, 1, 0.05),
     ((FEW, 4, 1), 1, 20000, 64, 1, 0.5), ((FEW, 1, 2), 1, 700, 20000, 1, 0.2), ((FEW, 2, 2), 1, 5000, 17000, 1, 0.1),
     ((FEW, 4, 2), 1, 9000, 20000, 1, 0.05), ((FEW, 2, 2), 1, 8300, 16500, 1, 0.5),
     ((FEW, 1, 1), 2, 300, 1024, 1, 0.5), ((FEW, 2, 1), 2, 9000, 500, 1, 0.7), ((FEW, 4, 1), 2, 9001, 2047, 1, 0.03),

@@ -15,12 +15,12 @@ DEV = "cuda:0"
 
 SIZES = [
     # whole tokens by four lanes, one and two pieces of 16 features a thread, around its bounds
-    (4096, 2), (4096, 79), (4097, 70), (5000, 33), (8192, 39), (8191, 40), (640, 1024),
+    (4096, 2), (3520, 1023), (3521, 112), (4097, 70), (5000, 33), (8192, 23), (8191, 48), (640, 1024), (8180, 5),
     # by sixteen lanes
-    (641, 1024), (1023, 1025), (1536, 500), (1521, 8191), (64, 8192), (17, 4001),
-    # slices of features: by sixteen lanes, by 64, by 64 of four 16-bit tokens
-    (8208, 63), (14336, 17), (20000, 5), (100003, 3), (1537, 900), (4999, 301), (14336, 515), (16, 8193), (300, 20000),
-    (14336, 1171), (65537, 257), (66001, 259), (2048, 8200), (16400, 1024)]
+    (641, 1024), (1023, 1025), (1536, 1500), (1521, 8191), (2048, 1025), (2033, 200), (64, 8192), (17, 4001),
+    # slices of features: by sixteen lanes and by 64, one of them and several rounds of workgroups
+    (8208, 63), (14336, 17), (20000, 5), (100003, 3), (2049, 1025), (4999, 301), (14336, 515), (16, 8193), (300, 20000),
+    (14336, 1171), (65537, 257), (2048, 8200), (16400, 1024), (3000, 9001), (40, 70000)]
 
 
 @pytest.mark.parametrize("kind", list(TYPES))

@@ -183,17 +183,24 @@ struct TokenPlan {
     int32_t slices;
 };
 
-// size: bytes of a value.  us, bf16 and fp32, of whole tokens by four lanes (4) and sixteen
-// (16), and in slices by sixteen (s16) and by 64 (s64):
-//   4999 x 31      8.6 and 8.1 (4), 12.3 and 10.6 (s16)
-//   2048 x 128     7.3 and 5.7 (4), 9.8 and 6.8 (16), 10.8 and 9.0 (s64)
-//   4096 x 128     8.2 (4), 11.1 (s64); 4096 x 512 13.5 and 16.9 (4), 11.0 and 9.9 (s64)
-//   6000 x 63      9.4 and 13.5 (4), 11.1 and 9.6 (s16)
-//   1024 x 1500    11.7 and 11.9 (4), 8.2 and 8.0 (16), 10.9 and 9.9 (s64)
-//   1024 x 16384   32.7 and 27.0 (16), 25.3 and 27.7 (s64)
-//   14336 x 512    15.5 and 15.8 (s16), 14.5 and 14.9 (s64)
-// Whole tokens read x once, as long as there are workgroups enough and a thread's segments of
-// a row, eight bytes with four lanes, come from L1 again.
+// size: bytes of a value.  us of whole tokens by four lanes (4) and sixteen (16), and in slices by
+// sixteen (s16) and by 64 (s64), of x that has left L2:
+//   bf16   1000 x 2288   15.3 (4), 8.5 (16), 13.9 (s16), 11.7 (s64)
+//          1695 x 936     8.7,    13.6,      15.3,       14.7
+//          3453 x 414    10.8,                15.2,       14.6
+//          5163 x 791    17.7,                21.3,       15.3
+//          4705 x 96     12.0,                12.3,       11.1
+//          1298 x 5245   31.6,    21.9,      34.0,       17.0
+//          862 x 11664   46.5,    23.4,      47.8,       25.8
+//   fp32   1936 x 163     7.0 (4), 8.1 (16),  9.5 (s16),   8.5 (s64)
+//          788 x 675      8.0,     7.7,      11.8,        9.7
+//          1733 x 994    13.5,    10.3,      13.6,       11.0
+//          5007 x 89     14.1,               13.6,       12.6
+//          6706 x 33     13.9,               10.0
+// and of x that stays there: bf16 4999 x 31 8.6 (4), 12.3 (s16), 4096 x 512 13.5 (4), 11.0 (s64).
+// Whole tokens read x once; a workgroup then reads every row, of which four lanes use 8 or 16
+// bytes, in a time that goes by the features.  Over 862 drawn sizes the rule is 1.5 % slower
+// than the fastest way in the mean, 1.1 % where x stays in L2.
 TokenPlan token_plan(int64_t K, int64_t N, int size)
 {
     TokenPlan p{};
@@ -201,10 +208,11 @@ TokenPlan token_plan(int64_t K, int64_t N, int size)
     if (N == 1) {
         p.lanes = 1;
         p.whole = K <= kOneMost;
-    } else if (Kb * 4 <= kKept * 1024 && N <= 1024 && K * N * size <= 5 << 18) {
+    } else if (Kb * 4 <= kKept * 1024 && N <= 1024 && (K * N * size <= 3 << 18 || (size == 2 && Kb <= 220))) {
         p.lanes = 4;
         p.whole = true;
-    } else if (Kb <= 96 && N <= 8192) {  // (Kb * 16 <= kKept * 1024)
+    } else if (Kb <= (size == 4 ? 128 : 96) && N <= 8192) {
+        static_assert(128 * 16 <= kKept * 1024);
         p.lanes = 16;
         p.whole = true;
     } else {

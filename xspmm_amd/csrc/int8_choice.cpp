@@ -44,22 +44,20 @@ Int8Choice int8_choice(int weights, int64_t M, int64_t K, const int64_t* blocks,
 {
     const int64_t Mb = (M + 15) / 16, Kb = (K + 15) / 16, all = blocks[0] + (weights == 2 ? blocks[1] : 0);
     if (rounds) {
-        // Sixteen waves to a block-row while all workgroups run at once, two a CU of one token
-        // and one a CU of more, half of them up to twice that.  Beyond, half or a quarter: by
-        // how much the blocks of a row take beside rounding the tokens once more.  us of one,
-        // two and four rows a workgroup, bf16:
+        // Sixteen waves to a block-row while there is a workgroup a CU, half of them up to twice
+        // that.  Beyond, half or a quarter: by how much the blocks of a row take beside
+        // rounding the tokens once more.  us of one, two and four rows a workgroup, bf16:
         //   4096 x 14336,  25 %, 1 token            8.1    8.9   10.4
-        //   8192 x 4096,    5 %, 4                 12.2    8.7    8.6
+        //   8192 x 4096,    5 %, 1                  6.8    6.1    6.2
+        //   8192 x 4096,    5 %, 4                 12.3    8.7    8.6
         //   14336 x 4096,  25 %, 1, gate and up    14.5    9.7   11.0
         //   14336 x 4096,   5 %, 2                 22.5   13.0    9.5
         //   16384 x 1024,  25 %, 16, gate and up   19.8   11.2    8.4
         //   16384 x 1024,  80 %, 2, gate and up    15.7   10.3   10.3
         //   5000 x 30000,  80 %, 1                 39.1   31.0   49.8
         const int64_t groups = Mb * groups_of(N, kInt8FewTokens), pieces = Kb * (N < kInt8FewTokens ? N : kInt8FewTokens);
-        const int kept = N > 1 || Kb <= kInt8FewPieces ? 1 : 2;
-        const bool two = N == 1 && kept == 1;
-        const int rows = groups <= (two ? 512 : 256) ? 1 : groups <= 512 ? 2 : 4 * all <= (128 + pieces) * Mb ? 4 : 2;
-        return {Int8Kernel::kFew, rows, kept};
+        const int rows = groups <= 256 ? 1 : groups <= 512 ? 2 : 4 * all <= (128 + pieces) * Mb ? 4 : 2;
+        return {Int8Kernel::kFew, rows, N > 1 || Kb <= kInt8FewPieces ? 1 : 2};
     }
     // Lists and tiles look their blocks up in a map of the grid, and load them, and their
     // windows of x, by offsets of 31 bits.  Few tokens leave most of a workgroup's without work
