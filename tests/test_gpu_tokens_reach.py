@@ -20,7 +20,9 @@ SIZES = [
     (641, 1024), (1023, 1025), (1536, 1500), (1521, 8191), (2048, 1025), (2033, 200), (64, 8192), (17, 4001),
     # slices of features: by sixteen lanes and by 64, one of them and several rounds of workgroups
     (8208, 63), (14336, 17), (20000, 5), (100003, 3), (2049, 1025), (4999, 301), (14336, 515), (16, 8193), (300, 20000),
-    (14336, 1171), (65537, 257), (2048, 8200), (16400, 1024), (3000, 9001), (40, 70000)]
+    (14336, 1171), (65537, 257), (2048, 8200), (16400, 1024), (3000, 9001), (40, 70000),
+    # more than 48 MB of 16-bit values: four tokens a thread for the maxima
+    (14336, 1771), (98500, 257), (2999, 8401), (12290, 2049)]
 
 
 @pytest.mark.parametrize("kind", list(TYPES))

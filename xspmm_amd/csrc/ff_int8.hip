@@ -130,25 +130,32 @@ __global__ __launch_bounds__(1024) void ff_token_kernel(const T* __restrict__ x,
     if (k < K) *reinterpret_cast<u32x4_t*>(q + k) = round_features(v, round);
 }
 
-// part[slice][n]: bits of the largest magnitude of a slice of the features
+// part[slice][n]: bits of the largest magnitude of a slice of the features, of VEC tokens a
+// thread (the last of them move back into the matrix)
 constexpr int kSliceThreads = 1024;
-template <typename T, int LT>
+template <typename T, int VEC, int LT>
 __global__ __launch_bounds__(kSliceThreads) void ff_tokens_most_kernel(const T* __restrict__ x, uint32_t* __restrict__ part,
                                                              int64_t K, int64_t N, int32_t slices)
 {
-    __shared__ uint32_t red[kSliceThreads / 64 * LT];
+    __shared__ uint32_t red[VEC][kSliceThreads / 64 * LT];
     const int64_t tile = blockIdx.x / slices, s = blockIdx.x % slices, Kb = (K + 15) / 16;
-    const int64_t n = token_of<LT>(tile, N);
-    float v[16];
-    uint32_t m = 0;
+    const int64_t n = min((tile * LT + threadIdx.x % LT) * VEC, N - VEC);
+    uint32_t m[VEC] = {};
     const int64_t end = Kb * (s + 1) / slices;
     for (int64_t kb = Kb * s / slices + threadIdx.x / LT; kb < end; kb += kSliceThreads / LT) {
-        load_features<T>(x, K, N, kb, n, v);
+        Pack<T, VEC> p[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[i]));
+        for (int i = 0; i < 16; ++i) p[i] = *reinterpret_cast<const Pack<T, VEC>*>(x + min(16 * kb + i, K - 1) * N + n);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) m[c] = max(m[c], magnitude((float)p[i].v[c]));
     }
-    join<kSliceThreads, LT>(m, red);
-    if (threadIdx.x < LT) part[s * N + n] = m;
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+        join<kSliceThreads, LT>(m[c], red[c]);
+        if (threadIdx.x < LT) part[s * N + n + c] = m[c];
+    }
 }
 
 // A thread takes one token at a time: 64 of them store 1 KB side by side (with four
@@ -178,7 +185,7 @@ __global__ __launch_bounds__(kSliceThreads) void ff_tokens_round_kernel(const T*
 
 struct TokenPlan {
     bool whole;  // one launch, a workgroup to a tile
-    int lanes;
+    int lanes, vec;   // a tile's threads along the tokens, and a thread's tokens (for the maxima)
     int64_t tiles;
     int32_t slices;
 };
@@ -200,7 +207,10 @@ struct TokenPlan {
 // and of x that stays there: bf16 4999 x 31 8.6 (4), 12.3 (s16), 4096 x 512 13.5 (4), 11.0 (s64).
 // Whole tokens read x once; a workgroup then reads every row, of which four lanes use 8 or 16
 // bytes, in a time that goes by the features.  Over 862 drawn sizes the rule is 1.5 % slower
-// than the fastest way in the mean, 1.1 % where x stays in L2.
+// than the fastest way in the mean, 1.1 % where x stays in L2.  Four 16-bit tokens a thread read
+// the maxima of more than 48 MB faster (us of one and four: 14336 x 2048 38.2 and 35.7, 10958 x
+// 4237 80.4 and 76.1, 15936 x 3067 74.1 and 72.4), of less slower (6991 x 3663 49.8 and 49.9, 5783 x
+// 3598 37.9 and 40.9, 9174 x 1943 27.2 and 34.9).
 TokenPlan token_plan(int64_t K, int64_t N, int size)
 {
     TokenPlan p{};
@@ -218,7 +228,8 @@ TokenPlan token_plan(int64_t K, int64_t N, int size)
     } else {
         p.lanes = N < 64 ? 16 : 64;
     }
-    p.tiles = (N + p.lanes - 1) / p.lanes;
+    p.vec = p.lanes == 64 && size == 2 && N >= 256 && K * N > 3 << 23 ? 4 : 1;
+    p.tiles = (N + p.lanes * p.vec - 1) / (p.lanes * p.vec);
     if (p.whole) return p;
     // Rounds of a workgroup a CU, filled as far as they can be, in the time of 16 features of a
     // tile, of which a workgroup costs some 24 beside its own (us, bf16): at 5350 x 1385 22
@@ -239,14 +250,15 @@ TokenPlan token_plan(int64_t K, int64_t N, int size)
     return p;
 }
 
-template <typename T, int LT>
+template <typename T, int VEC, int LT>
 void launch_tokens(const T* x, int8_t* q, float* scale, int64_t K, int64_t N, void* scratch, const TokenPlan& p,
                    hipStream_t s)
 {
     uint32_t* part = static_cast<uint32_t*>(scratch);
     const dim3 grid = launch_grid(p.tiles * p.slices, kSliceThreads), threads(kSliceThreads);
-    hipLaunchKernelGGL((ff_tokens_most_kernel<T, LT>), grid, threads, 0, s, x, part, K, N, p.slices);
-    hipLaunchKernelGGL((ff_tokens_round_kernel<T, LT>), grid, threads, 0, s, x, part, q, scale, K, N, p.slices);
+    const dim3 narrow = launch_grid((N + LT - 1) / LT * p.slices, kSliceThreads);
+    hipLaunchKernelGGL((ff_tokens_most_kernel<T, VEC, LT>), grid, threads, 0, s, x, part, K, N, p.slices);
+    hipLaunchKernelGGL((ff_tokens_round_kernel<T, LT>), narrow, threads, 0, s, x, part, q, scale, K, N, p.slices);
     XSPMM_LAUNCH_CHECK();
 }
 
@@ -301,12 +313,18 @@ void quantize_tokens(const T* x, int8_t* q, float* scale, int64_t K, int64_t N, 
         XSPMM_LAUNCH_CHECK();
         return;
     }
-    if (p.lanes == 64)
-        ff::launch_tokens<T, 64>(x, q, scale, K, N, scratch, p, s);
-    else if (p.lanes == 16)
-        ff::launch_tokens<T, 16>(x, q, scale, K, N, scratch, p, s);
-    else
-        ff::launch_tokens<T, 1>(x, q, scale, K, N, scratch, p, s);
+    if (p.lanes == 64) {
+        if constexpr (sizeof(T) == 2)
+            if (p.vec == 4) {
+                ff::launch_tokens<T, 4, 64>(x, q, scale, K, N, scratch, p, s);
+                return;
+            }
+        ff::launch_tokens<T, 1, 64>(x, q, scale, K, N, scratch, p, s);
+    } else if (p.lanes == 16) {
+        ff::launch_tokens<T, 1, 16>(x, q, scale, K, N, scratch, p, s);
+    } else {
+        ff::launch_tokens<T, 1, 1>(x, q, scale, K, N, scratch, p, s);
+    }
 }
 
 #define XSPMM_INT8(T)                                                                            \
