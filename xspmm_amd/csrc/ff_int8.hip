@@ -10,7 +10,7 @@
 //
 // Tokens are bound by memory: x is read for the maxima and once more for the
 // quotients, where it fits in the caches behind the first pass: bf16 14336 x 2048 (59 MB)
-// 10.8 us (5.4 TB/s) for the maxima and 27.1 (3.3 TB/s with what it writes) for the
+// 10.9 us (5.4 TB/s) for the maxima and 27 (3.3 TB/s with what it writes) for the
 // rounding.  One token of 14336 takes 2.6 us; a weight of 14336 x 4096, 25 % stored, 21.
 #include "int8_device.hpp"
 

@@ -9,8 +9,8 @@
 // stored.  A value of x is read from LDS once for four block-rows; a block is read
 // from memory by the one wave that needs it, three steps ahead, its position two windows.
 //
-// 14336 x 4096, all stored, 2048 tokens, fp16, bias and gelu: 140 to 162 us by the clock that
-// power leaves, 144 in the mean, 1.7 Pop/s.  The matrix units are busy for 57 us of that at 2
+// 14336 x 4096, all stored, 2048 tokens, fp16, bias and gelu: 140 to 170 us by the clock that
+// power leaves, 144 to 150 in the mean, 1.6 to 1.7 Pop/s.  The matrix units are busy for 57 us of that at 2
 // GHz; a step's loads, 24 KB a workgroup through the 64 bytes a clock of a CU's L1, take
 // three quarters of the matrix instructions' time beside them, and the gelus and the results
 // 25 us, of which the other workgroup hides a part (one workgroup of eight waves: 142 where
